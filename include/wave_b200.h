@@ -446,6 +446,46 @@ int wb200_multi_gpu_synchronize(wb200_multi_gpu_t* h);
 int wb200_multi_gpu_time_begin(wb200_multi_gpu_t* h);
 int wb200_multi_gpu_time_end(wb200_multi_gpu_t* h, float* max_ms);
 
+/* ---- beside frozen weights: low-rank adapters, input gradient, router ------------------------- */
+/* Low-rank adapters of many requests: out[t] = y[t] + scale[l] * B_l (A_l x[t]) with l = ids[t]; rows whose id is outside
+ * [0, num_adapters) have no adapter and keep y. x [rows, K] bf16 (pitch ldx), a [num_adapters, rank, K] and b [num_adapters, N, rank]
+ * bf16, contiguous; ids int32 or int64; scale f32 [num_adapters], or null for ones; y and out [rows, N] of `dtype`, out may be y (in
+ * place), otherwise they do not overlap. K is a multiple of 8, rank at most 256, N any. hidden: wb200_adapters_hidden_bytes(rows, K, rank)
+ * bytes, 16-byte aligned, left with A_l x[t] in f32, which the backward call reads. Two launches, no order of the ids needed. */
+size_t wb200_adapters_hidden_bytes(int rows, int K, int rank);
+int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,
+                           const void* ids, int ids_are_int64, const float* scale, const void* y, long long ldy, void* out, long long ldo,
+                           int dtype, void* hidden, size_t hidden_bytes, void* stream);
+/* Its gradients for g = the gradient of out [rows, N] bf16: dx [rows, K] (the adapters' part), da and db laid out as a and b (zeros for an
+ * adapter without rows), all bf16; each may be null. hidden: as the forward call left it (read for db). At most 256 adapters. Sums over rows are
+ * made in a fixed order. workspace: wb200_adapters_backward_workspace_bytes, 256-byte aligned. */
+size_t wb200_adapters_backward_workspace_bytes(int rows, int K, int N, int rank, int num_adapters);
+int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,
+                            const void* ids, int ids_are_int64, const float* scale, const void* g, long long ldg, const void* hidden,
+                            size_t hidden_bytes, void* dx, long long ldd, void* da, void* db, void* workspace, size_t workspace_bytes,
+                            void* stream);
+/* Input gradient of a linear layer with MXFP4 weights: dx [M, K] = g [M, N] * dequant(b, b_scale) [N, K], g and dx bf16, f32 accumulation.
+ * b and b_scale as wb200_mxfp4_gemm's, the scales row-major with a pitch. Rows of g and dx start on 16 bytes. */
+int wb200_mxfp4_input_grad(int M, int N, int K, const void* g, long long ldg, const void* b, const void* b_scale, long long b_scale_stride,
+                           void* dx, long long ldd, void* stream);
+/* Router: weight [rows, top_k] and ids [rows, top_k] of the top_k largest of num_experts (at most 256) logits, f32 or bf16 with row pitch
+ * ld: softmax over all experts, over the chosen ones with renormalize != 0; in descending order, the lower expert first among equals, NaN
+ * above all. counts [num_experts]: how often each was chosen; tokens: rows that count; loss = num_experts * sum_e counts[e] / (top_k tokens) *
+ * mean_t p[t, e]. mask (or null): one byte a row, 0 = padding: ids -1, weight 0, in no sum. given_ids (or null): int32 or int64 [rows, top_k]
+ * choices made elsewhere; weight and ids are then not written, and ids out of range do not count. top_k at most 32 where it is chosen here. */
+size_t wb200_router_workspace_bytes(int rows, int num_experts);
+int wb200_router(int rows, int num_experts, int top_k, const void* logits, int dtype, long long ld, const void* mask, const void* given_ids,
+                 int given_are_int64, int renormalize, float* weight, int* ids, int* counts, int* tokens, float* loss, void* workspace,
+                 size_t workspace_bytes, void* stream);
+/* Gradient of the router: g_logits [rows, num_experts] (the type of logits, pitch ldg) from g_weight [rows, top_k] (or null) and the device
+ * scalar g_loss (or null); ids, counts and tokens as the forward call wrote them. Rows of padding get zeros. */
+int wb200_router_grad(int rows, int num_experts, int top_k, const void* logits, int dtype, long long ld, const void* mask, const int* ids,
+                      const float* g_weight, const float* g_loss, int renormalize, const int* counts, const int* tokens, void* g_logits,
+                      long long ldg, void* stream);
+/* Gradient of wb200_moe_combine by its weights: g_weight[t, j] = sum_c g[t, c] * y[row_of[t, j], c], f32; 0 for pairs with row_of < 0. */
+int wb200_moe_combine_grad(const void* g, long long ldg, const void* y, long long ldy, int dtype, const int* row_of, int tokens, int top_k,
+                           int cols, float* g_weight, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

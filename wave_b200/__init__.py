@@ -25,6 +25,8 @@ from .templates import (get_broadcasted_scale_gemm_mxfp4, get_scaled_gemm_kernel
                         get_tagged_splitk_mxfp4_gemm_preshuffle_b, get_tagged_splitk_mxfp4_gemm_preshuffle_scales)
 
 from .nn import MXFP4Linear  # noqa: F401,E402
-from .moe import (MXFP4ExpertMLP, get_silu_and_mul_kernel, moe_align_block_size, silu_and_mul)  # noqa: F401,E402
+from .moe import (MXFP4ExpertMLP, Routing, balance_loss, combine_rows, get_silu_and_mul_kernel, moe_align_block_size, router, silu_and_mul)  # noqa: F401,E402
+from .adapters import LowRankAdapters, apply_adapters  # noqa: F401,E402
+from .ops import mxfp4_input_grad  # noqa: F401,E402
 
 __version__ = "0.1.0"

@@ -94,6 +94,15 @@ EXPORTED_SYMBOLS = (
     "wb200_silu_and_mul",
     "wb200_moe_quantize_scatter",
     "wb200_moe_combine",
+    "wb200_adapters_hidden_bytes",
+    "wb200_adapters_forward",
+    "wb200_adapters_backward_workspace_bytes",
+    "wb200_adapters_backward",
+    "wb200_mxfp4_input_grad",
+    "wb200_router_workspace_bytes",
+    "wb200_router",
+    "wb200_router_grad",
+    "wb200_moe_combine_grad",
     "wb200_mxfp4_gemm_scatter_rows",
     "wb200_peer_buffer_create",
     "wb200_peer_buffer_open",
@@ -229,6 +238,27 @@ def load() -> ctypes.CDLL:
     lib.wb200_moe_combine.restype = c_int
     lib.wb200_moe_combine.argtypes = [c_void_p, c_ll, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_ll,
                                       c_void_p]
+    lib.wb200_adapters_hidden_bytes.restype = c_size_t
+    lib.wb200_adapters_hidden_bytes.argtypes = [c_int] * 3
+    lib.wb200_adapters_forward.restype = c_int
+    lib.wb200_adapters_forward.argtypes = [c_int] * 5 + [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_ll, c_void_p,
+                                                         c_ll, c_int, c_void_p, c_size_t, c_void_p]
+    lib.wb200_adapters_backward_workspace_bytes.restype = c_size_t
+    lib.wb200_adapters_backward_workspace_bytes.argtypes = [c_int] * 5
+    lib.wb200_adapters_backward.restype = c_int
+    lib.wb200_adapters_backward.argtypes = [c_int] * 5 + [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_ll, c_void_p,
+                                                          c_size_t, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.wb200_mxfp4_input_grad.restype = c_int
+    lib.wb200_mxfp4_input_grad.argtypes = [c_int, c_int, c_int, c_void_p, c_ll, c_void_p, c_void_p, c_ll, c_void_p, c_ll, c_void_p]
+    lib.wb200_router_workspace_bytes.restype = c_size_t
+    lib.wb200_router_workspace_bytes.argtypes = [c_int, c_int]
+    lib.wb200_router.restype = c_int
+    lib.wb200_router.argtypes = [c_int, c_int, c_int, c_void_p, c_int, c_ll, c_void_p, c_void_p, c_int, c_int] + [c_void_p] * 6 + [c_size_t, c_void_p]
+    lib.wb200_router_grad.restype = c_int
+    lib.wb200_router_grad.argtypes = [c_int, c_int, c_int, c_void_p, c_int, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                      c_void_p, c_ll, c_void_p]
+    lib.wb200_moe_combine_grad.restype = c_int
+    lib.wb200_moe_combine_grad.argtypes = [c_void_p, c_ll, c_void_p, c_ll, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]
     lib.wb200_mxfp4_gemm_scatter_rows.restype = c_int
     lib.wb200_mxfp4_gemm_scatter_rows.argtypes = [c_int, ctypes.POINTER(c_int), c_int, c_int, c_void_p, c_void_p, c_void_p,
                                                   c_void_p, ctypes.POINTER(c_void_p), c_int, c_ll, c_uint, c_void_p]

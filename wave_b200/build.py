@@ -5,18 +5,19 @@ from __future__ import annotations
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OUT = PKG / "libwave_b200.so"
-SOURCES = [CSRC / "api.cu"]
+SOURCES = [CSRC / "api.cu", CSRC / "adapt.cu"]
 HEADERS = sorted(CSRC.glob("*.cuh")) + [PKG.parent / "include" / "wave_b200.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -52,17 +53,35 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False, check
         return out
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     variant = ["-DWB200_TRACE"] if trace else ["-DWB200_CHECKS"] if checks else ["-DWB200_MMA_CEILING"] if mma_ceiling else []
-    cmd = [nvcc, *NVCC_FLAGS, *variant, "-o", str(out), *map(str, SOURCES)]
-    if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-        print(" ".join(cmd))
+    objects = PKG / "build" / out.stem
+    objects.mkdir(parents=True, exist_ok=True)
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        units = list(pool.map(lambda source: _compile(nvcc, source, objects, variant, force, verbose), SOURCES))
+    _run([nvcc, *NVCC_FLAGS, "-shared", "-o", str(out), *map(str, units)])
+    return out
+
+
+def _run(cmd: list[str]) -> str:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    return res.stderr
+
+
+def _compile(nvcc: str, source: Path, objects: Path, variant: list[str], force: bool, verbose: bool) -> Path:
+    """One source to an object, unless that is newer than all it was compiled from (nvcc writes them down beside it)."""
+    unit, made_from = objects / f"{source.stem}.o", objects / f"{source.stem}.d"
+    if not force and not verbose and unit.exists() and made_from.exists():
+        deps = [Path(d) for d in made_from.read_text().replace("\\\n", " ").split(":", 1)[1].split()]
+        if all(d.exists() and d.stat().st_mtime <= unit.stat().st_mtime for d in deps):
+            return unit
+    cmd = [nvcc, *NVCC_FLAGS, *variant, *(["-Xptxas", "-v"] if verbose else []), "-MD", "-MF", str(made_from), "-c", "-o", str(unit), str(source)]
     if verbose:
-        print(res.stderr)
-    return out
+        print(" ".join(cmd))
+    said = _run(cmd)
+    if verbose:
+        print(said)
+    return unit
 
 
 FAST_OUT = PKG / "_fast.so"

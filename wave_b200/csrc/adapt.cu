@@ -1,0 +1,422 @@
+// C entry points of what is trained and served beside frozen MXFP4 weights: low-rank adapters, the input gradient of a linear layer,
+// the router of an expert MLP with its balance loss, and the gradient of the weighted combine.
+#include "../../include/wave_b200.h"
+#include "host.cuh"
+
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "adapters.cuh"
+#include "input_grad_sm100.cuh"
+#include "router.cuh"
+
+namespace {
+
+using wbhost::fail;
+
+constexpr int kTargetCtas = 296;  // two per SM of a B200
+
+bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+int div_up(long long a, long long b) { return int((a + b - 1) / b); }
+int rank_pad(int R) { return (R + 15) / 16 * 16; }
+int chunks_of(int rows) { return div_up(rows, wb::kChunkRows); }
+
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
+// Lets a kernel have up to 200 KB of dynamic shared memory, once per device.
+template <auto Kernel>
+int allow_smem() {
+  static bool done[wbhost::kMaxDevices] = {};
+  int dev = 0;
+  WB_HOST_CUDA(cudaGetDevice(&dev));
+  if (!done[dev]) {
+    WB_HOST_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    done[dev] = true;
+  }
+  return WB200_OK;
+}
+
+// ------------------------------------------------------------------------------------------
+// adapters
+// ------------------------------------------------------------------------------------------
+// K is cut where there are few chunks of rows; a split has at least one block of each warp.
+int shrink_splits(int rows, int K) {
+  const int most = std::max(1, std::min(16, K / 512));
+  return std::max(1, std::min(most, div_up(kTargetCtas, chunks_of(rows))));
+}
+
+template <int RT, int MT, int KU, bool TRANS>
+cudaError_t launch_shrink(const wb::ShrinkParams& p, bool wide_ids, dim3 grid, cudaStream_t s) {
+  return wide_ids ? launch(wb::adapter_shrink_kernel<long long, RT, MT, KU, TRANS>, grid, wb::kAdapterThreads, 0, s, p)
+                  : launch(wb::adapter_shrink_kernel<int, RT, MT, KU, TRANS>, grid, wb::kAdapterThreads, 0, s, p);
+}
+
+// hidden [splits][rows][Rp] = rows of x onto the ranks. trans: w is [L][K][R].
+int run_shrink(const __nv_bfloat16* x, long long ldx, const __nv_bfloat16* w, bool trans, const void* ids, bool wide_ids, float* hidden, int rows,
+               int K, int R, int L, cudaStream_t s) {
+  wb::ShrinkParams p;
+  p.x = x; p.w = w; p.ids = ids; p.hidden = hidden; p.ldx = ldx;
+  p.rows = rows; p.K = K; p.R = R; p.Rp = rank_pad(R); p.L = L;
+  const int splits = shrink_splits(rows, K), chunks = chunks_of(rows);
+  p.split_k = div_up(div_up(K, splits), 64) * 64;
+  const int rt = p.Rp <= 16 ? 2 : p.Rp <= 32 ? 4 : 8;
+  p.x_vec = aligned_to(x, 16) && ldx % 8 == 0 && K % 8 == 0;
+  p.w_vec = trans ? aligned_to(w, 2 * rt) && R % rt == 0 : aligned_to(w, 16) && K % 8 == 0;
+  const int lanes = rows <= wb::kChunkRows ? std::min(rows, L) : std::max(1, std::min(std::min(wb::kChunkRows, L), kTargetCtas / (chunks * splits)));
+  const dim3 grid(splits, chunks, lanes);
+  const bool few = rows <= wb::kChunkRows;
+#define WB_SHRINK(RT, KU)                                                                                            \
+  (trans ? (few ? launch_shrink<RT, 1, 2, true>(p, wide_ids, grid, s) : launch_shrink<RT, 4, KU, true>(p, wide_ids, grid, s)) \
+         : (few ? launch_shrink<RT, 1, 2, false>(p, wide_ids, grid, s) : launch_shrink<RT, 4, KU, false>(p, wide_ids, grid, s)))
+  WB_HOST_CUDA(rt == 2 ? WB_SHRINK(2, 2) : rt == 4 ? WB_SHRINK(4, 1) : WB_SHRINK(8, 1));
+#undef WB_SHRINK
+  return WB200_OK;
+}
+
+template <typename IdT, typename T, int P, int QN, bool TRANS>
+int launch_expand(const wb::ExpandParams& p, dim3 grid, cudaStream_t s) {
+  constexpr auto kernel = wb::adapter_expand_kernel<IdT, T, P, QN, TRANS>;
+  const size_t smem = size_t(P) * wb::kChunkRows * (p.Rp + 8) * 2;
+  if (int rc = smem > 40 * 1024 ? allow_smem<kernel>() : WB200_OK) return rc;
+  WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, smem, s, p));
+  return WB200_OK;
+}
+template <typename T, int P, bool TRANS>
+int launch_expand_ranks(const wb::ExpandParams& p, bool wide_ids, dim3 grid, cudaStream_t s) {
+  const int steps = p.Rp / 16;
+  if (wide_ids) return steps == 1 ? launch_expand<long long, T, P, 1, TRANS>(p, grid, s) : steps == 2 ? launch_expand<long long, T, P, 2, TRANS>(p, grid, s) : launch_expand<long long, T, P, 4, TRANS>(p, grid, s);
+  return steps == 1 ? launch_expand<int, T, P, 1, TRANS>(p, grid, s) : steps == 2 ? launch_expand<int, T, P, 2, TRANS>(p, grid, s) : launch_expand<int, T, P, 4, TRANS>(p, grid, s);
+}
+
+// out = y + scale * (ranks onto C columns); contraction: that of the product that made `hidden`, which says how often it was split.
+int run_expand(const __nv_bfloat16* w, bool trans, const void* ids, bool wide_ids, const float* scale, const float* hidden, int contraction,
+               const void* y, long long ldy, void* out, long long ldo, bool f32, int rows, int C, int R, int L, cudaStream_t s) {
+  wb::ExpandParams p;
+  p.w = w; p.ids = ids; p.scale = scale; p.hidden = hidden; p.y = y; p.out = out; p.ldy = ldy; p.ldo = ldo;
+  p.rows = rows; p.C = C; p.R = R; p.Rp = rank_pad(R); p.L = L;
+  p.splits = shrink_splits(rows, contraction);
+  const int chunks = chunks_of(rows);
+  p.cols_per_cta = 1024;
+  while (p.cols_per_cta > 256 && (long long)chunks * div_up(C, p.cols_per_cta) < kTargetCtas) p.cols_per_cta /= 2;
+  const size_t esz = f32 ? 4 : 2;
+  p.io_vec = aligned_to(out, 16) && ldo * esz % 16 == 0 && (!y || (aligned_to(y, 16) && ldy * esz % 16 == 0));
+  p.w_vec = trans ? aligned_to(w, 8) && C % 4 == 0 : aligned_to(w, 8) && R % 4 == 0;
+  const int slices = div_up(C, p.cols_per_cta);
+  const int lanes = rows <= wb::kChunkRows ? std::min(rows, L)
+                                           : std::max(1, std::min(std::min(wb::kChunkRows, L), int(kTargetCtas / ((long long)chunks * slices))));
+  const dim3 grid(slices, chunks, lanes);
+  if (trans) return launch_expand_ranks<__nv_bfloat16, 2, true>(p, wide_ids, grid, s);
+  return f32 ? launch_expand_ranks<float, 3, false>(p, wide_ids, grid, s) : launch_expand_ranks<__nv_bfloat16, 2, false>(p, wide_ids, grid, s);
+}
+
+int check_adapters(const char* what, int rows, int K, int N, int R, int L) {
+  if (rows <= 0 || K <= 0 || N <= 0 || R <= 0 || L <= 0)
+    return fail(WB200_ERR_INVALID_ARG, "%s: rows = %d, K = %d, N = %d, rank = %d, adapters = %d", what, rows, K, N, R, L);
+  if (K % 8) return fail(WB200_ERR_INVALID_ARG, "%s: K = %d is not a multiple of 8", what, K);
+  if (R > 256) return fail(WB200_ERR_UNSUPPORTED, "%s: rank %d is above 256", what, R);
+  if (rows > 4000000) return fail(WB200_ERR_UNSUPPORTED, "%s: %d rows in one call", what, rows);
+  return WB200_OK;
+}
+
+struct BackwardPlan {
+  int splits_a, splits_b;  // of the rows, in the sums over them
+  size_t list, owner, listed, u, part_a, part_b, total;
+};
+int outer_splits(int rows, int C, int L) { return std::max(1, std::min({16, chunks_of(rows), int(kTargetCtas / std::max(1ll, (long long)div_up(C, 256) * L))})); }
+BackwardPlan plan_backward(int rows, int K, int N, int R, int L) {
+  BackwardPlan p;
+  const size_t Rp = rank_pad(R);
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  p.splits_a = outer_splits(rows, K, L);
+  p.splits_b = outer_splits(rows, N, L);
+  p.list = 0;
+  p.owner = up(size_t(rows) * 4);
+  p.listed = p.owner + up(size_t(rows) * 4);
+  p.u = p.listed + 256;
+  p.part_a = p.u + up(size_t(shrink_splits(rows, N)) * rows * Rp * 4);
+  p.part_b = p.part_a + up(size_t(p.splits_a) * L * K * Rp * 4);
+  p.total = p.part_b + up(size_t(p.splits_b) * L * N * Rp * 4);
+  return p;
+}
+
+template <bool RANK_MAJOR>
+int run_outer(const __nv_bfloat16* z, long long ldz, const float* hidden, int contraction, const float* scale, const int* list, const int* owner,
+              const int* listed, float* part, int row_splits, __nv_bfloat16* out, int rows, int C, int R, int L, cudaStream_t s) {
+  wb::OuterParams p;
+  p.z = z; p.hidden = hidden; p.scale = scale; p.list = list; p.owner = owner; p.listed = listed; p.part = part; p.ldz = ldz;
+  p.rows = rows; p.C = C; p.R = R; p.Rp = rank_pad(R); p.L = L;
+  p.splits = shrink_splits(rows, contraction);
+  p.z_vec = aligned_to(z, 8) && ldz % 4 == 0;
+  const dim3 grid(div_up(C, 256), L, row_splits);
+  WB_HOST_CUDA(p.Rp <= 16   ? launch(wb::adapter_outer_kernel<2, RANK_MAJOR>, grid, wb::kAdapterThreads, 0, s, p)
+               : p.Rp <= 32 ? launch(wb::adapter_outer_kernel<4, RANK_MAJOR>, grid, wb::kAdapterThreads, 0, s, p)
+                            : launch(wb::adapter_outer_kernel<8, RANK_MAJOR>, grid, wb::kAdapterThreads, 0, s, p));
+  const long long total = (long long)L * R * C;
+  const int blocks = int(std::min<long long>(div_up(total, 256), 148 * 8));
+  if (RANK_MAJOR) WB_HOST_CUDA(launch(wb::adapter_reduce_kernel, dim3(blocks), 256, 0, s, (const float*)part, row_splits, L, R, p.Rp, C, C, out));
+  else WB_HOST_CUDA(launch(wb::adapter_reduce_kernel, dim3(blocks), 256, 0, s, (const float*)part, row_splits, L, C, C, R, p.Rp, out));
+  return WB200_OK;
+}
+
+// ------------------------------------------------------------------------------------------
+// input gradient
+// ------------------------------------------------------------------------------------------
+template <int CG>
+int launch_input_grad(const CUtensorMap& map, wb::InputGradParams p, int sms, cudaStream_t stream) {
+  using Cfg = wb::InputGradCfg<CG>;
+  p.tiles_m = div_up(p.M, Cfg::BM * CG);
+  p.tiles_k = div_up(p.K, Cfg::TILE_K);
+  p.group_k = std::min(8, p.tiles_k);
+  auto kernel = wb::input_grad_kernel<CG>;
+  static bool done[wbhost::kMaxDevices] = {};
+  int dev = 0;
+  WB_HOST_CUDA(cudaGetDevice(&dev));
+  if (!done[dev]) {
+    WB_HOST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+    done[dev] = true;
+  }
+  const long long tiles = (long long)p.tiles_m * p.tiles_k;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(std::min<long long>(tiles, sms / CG)) * CG, 1, 1);
+  cfg.blockDim = dim3(Cfg::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  WB_HOST_CUDA(cudaLaunchKernelEx(&cfg, kernel, map, p));
+  return WB200_OK;
+}
+
+// ------------------------------------------------------------------------------------------
+// router
+// ------------------------------------------------------------------------------------------
+int router_ctas(int rows) { return rows <= wb::kRouterOneCta ? 1 : std::min(wb::kRouterMaxCtas, div_up(rows, wb::kRouterWarps)); }
+
+int check_router(const char* what, int rows, int E, int top_k, int dtype, const void* logits, long long ld) {
+  if (rows <= 0 || E <= 0 || top_k <= 0) return fail(WB200_ERR_INVALID_ARG, "%s: rows = %d, experts = %d, top_k = %d", what, rows, E, top_k);
+  if (E > wb::kRouterMaxExperts) return fail(WB200_ERR_UNSUPPORTED, "%s: at most %d experts (got %d)", what, wb::kRouterMaxExperts, E);
+  if (dtype != WB200_F32 && dtype != WB200_BF16) return fail(WB200_ERR_INVALID_ARG, "%s: unknown dtype %d", what, dtype);
+  if (!logits) return fail(WB200_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (ld < E && rows > 1) return fail(WB200_ERR_INVALID_ARG, "%s: row pitch %lld is smaller than %d experts", what, ld, E);
+  if (!aligned_to(logits, dtype == WB200_F32 ? 4 : 2)) return fail(WB200_ERR_ALIGNMENT, "%s: logits are not aligned to their element size", what);
+  return WB200_OK;
+}
+
+#define WB_BY_EXPERTS(KERNEL, T, E)                                                                          \
+  ((E) <= 32 ? KERNEL<T, 1> : (E) <= 64 ? KERNEL<T, 2> : (E) <= 128 ? KERNEL<T, 4> : KERNEL<T, 8>)
+
+template <typename T, bool VEC>
+cudaError_t launch_combine_grad(const void* g, long long ldg, const void* y, long long ldy, const int* row_of, int tokens, int top_k, int cols,
+                                float* g_weight, cudaStream_t s) {
+  return launch(wb::combine_grad_kernel<T, VEC>, dim3(tokens), 128, 0, s, static_cast<const T*>(g), ldg, static_cast<const T*>(y), ldy, row_of,
+                top_k, cols, g_weight);
+}
+
+}  // namespace
+
+namespace wbhost {
+cudaError_t adapt_check_record(unsigned long long (&record)[3], bool reset) {
+#ifdef WB200_CHECKS
+  cudaError_t e = cudaMemcpyFromSymbol(record, wb::g_check_record, sizeof(record));
+  const unsigned long long zero[3] = {};
+  if (e == cudaSuccess && reset) e = cudaMemcpyToSymbol(wb::g_check_record, zero, sizeof(zero));
+  return e;
+#else
+  record[0] = record[1] = record[2] = 0;
+  (void)reset;
+  return cudaSuccess;
+#endif
+}
+}  // namespace wbhost
+
+extern "C" {
+
+size_t wb200_adapters_hidden_bytes(int rows, int K, int rank) {
+  if (rows <= 0 || K <= 0 || rank <= 0) return 0;
+  return size_t(shrink_splits(rows, K)) * rows * rank_pad(rank) * sizeof(float);
+}
+
+int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,
+                           const void* ids, int ids_are_int64, const float* scale, const void* y, long long ldy, void* out, long long ldo, int dtype,
+                           void* hidden, size_t hidden_bytes, void* stream) {
+  if (int rc = check_adapters("adapters", rows, K, N, rank, num_adapters)) return rc;
+  if (!x || !a || !b || !ids || !y || !out || !hidden) return fail(WB200_ERR_INVALID_ARG, "adapters: null pointer");
+  if (dtype != WB200_F32 && dtype != WB200_BF16) return fail(WB200_ERR_INVALID_ARG, "adapters: unknown output dtype %d", dtype);
+  if (rows > 1 && (ldx < K || ldy < N || ldo < N)) return fail(WB200_ERR_INVALID_ARG, "adapters: a row pitch is smaller than a row");
+  if (!aligned_to(x, 2) || !aligned_to(a, 2) || !aligned_to(b, 2) || !aligned_to(y, dtype == WB200_F32 ? 4 : 2) || !aligned_to(out, dtype == WB200_F32 ? 4 : 2) ||
+      !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(hidden, 16))
+    return fail(WB200_ERR_ALIGNMENT, "adapters: a tensor is not aligned to its element size, or hidden not to 16 bytes");
+  const size_t need = wb200_adapters_hidden_bytes(rows, K, rank);
+  if (hidden_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters: hidden of %zu bytes needed (got %zu)", need, hidden_bytes);
+  if (int rc = wbhost::device(nullptr, nullptr)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  float* h = static_cast<float*>(hidden);
+  if (int rc = run_shrink(static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(a), false, ids, ids_are_int64 != 0, h, rows, K, rank,
+                          num_adapters, s))
+    return rc;
+  return run_expand(static_cast<const __nv_bfloat16*>(b), false, ids, ids_are_int64 != 0, scale, h, K, y, ldy, out, ldo, dtype == WB200_F32, rows, N, rank,
+                    num_adapters, s);
+}
+
+size_t wb200_adapters_backward_workspace_bytes(int rows, int K, int N, int rank, int num_adapters) {
+  if (rows <= 0 || K <= 0 || N <= 0 || rank <= 0 || num_adapters <= 0) return 0;
+  return plan_backward(rows, K, N, rank, num_adapters).total;
+}
+
+int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,
+                            const void* ids, int ids_are_int64, const float* scale, const void* g, long long ldg, const void* hidden,
+                            size_t hidden_bytes, void* dx, long long ldd, void* da, void* db, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  if (int rc = check_adapters("adapters backward", rows, K, N, rank, num_adapters)) return rc;
+  if (num_adapters > 256) return fail(WB200_ERR_UNSUPPORTED, "adapters backward: at most 256 adapters (got %d)", num_adapters);
+  if (!dx && !da && !db) return fail(WB200_ERR_INVALID_ARG, "adapters backward: no gradient is asked for");
+  if (!ids || !g || !workspace || ((dx || da) && (!b || !a)) || (da && !x) || (db && !hidden))
+    return fail(WB200_ERR_INVALID_ARG, "adapters backward: null pointer");
+  if (rows > 1 && (ldg < N || (da && ldx < K) || (dx && ldd < K))) return fail(WB200_ERR_INVALID_ARG, "adapters backward: a row pitch is smaller than a row");
+  if (!aligned_to(x, 2) || !aligned_to(a, 2) || !aligned_to(b, 2) || !aligned_to(g, 2) || !aligned_to(dx, 2) || !aligned_to(da, 2) || !aligned_to(db, 2) ||
+      !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(hidden, 16) || !aligned_to(workspace, 256))
+    return fail(WB200_ERR_ALIGNMENT, "adapters backward: a tensor is not aligned to its element size, or the workspace not to 256 bytes");
+  const BackwardPlan plan = plan_backward(rows, K, N, rank, num_adapters);
+  if (workspace_bytes < plan.total) return fail(WB200_ERR_WORKSPACE, "adapters backward: workspace of %zu bytes needed (got %zu)", plan.total, workspace_bytes);
+  if (db && hidden_bytes < wb200_adapters_hidden_bytes(rows, K, rank)) return fail(WB200_ERR_WORKSPACE, "adapters backward: hidden of %zu bytes needed", wb200_adapters_hidden_bytes(rows, K, rank));
+  if (int rc = wbhost::device(nullptr, nullptr)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  int *list = reinterpret_cast<int*>(ws + plan.list), *owner = reinterpret_cast<int*>(ws + plan.owner), *listed = reinterpret_cast<int*>(ws + plan.listed);
+  float* u = reinterpret_cast<float*>(ws + plan.u);
+  const auto* gp = static_cast<const __nv_bfloat16*>(g);
+  const bool wide = ids_are_int64 != 0;
+  if (da || db)
+    if (int rc = wb200_moe_align_block_size(ids, ids_are_int64, rows, num_adapters, 1, list, rows, owner, rows, listed, nullptr, stream)) return rc;
+  if (dx || da)
+    if (int rc = run_shrink(gp, ldg, static_cast<const __nv_bfloat16*>(b), true, ids, wide, u, rows, N, rank, num_adapters, s)) return rc;
+  if (dx)
+    if (int rc = run_expand(static_cast<const __nv_bfloat16*>(a), true, ids, wide, scale, u, N, nullptr, 0, dx, ldd, false, rows, K, rank, num_adapters, s))
+      return rc;
+  if (db)
+    if (int rc = run_outer<false>(gp, ldg, static_cast<const float*>(hidden), K, scale, list, owner, listed, reinterpret_cast<float*>(ws + plan.part_b),
+                                  plan.splits_b, static_cast<__nv_bfloat16*>(db), rows, N, rank, num_adapters, s))
+      return rc;
+  if (da)
+    if (int rc = run_outer<true>(static_cast<const __nv_bfloat16*>(x), ldx, u, N, scale, list, owner, listed, reinterpret_cast<float*>(ws + plan.part_a),
+                                 plan.splits_a, static_cast<__nv_bfloat16*>(da), rows, K, rank, num_adapters, s))
+      return rc;
+  return WB200_OK;
+}
+
+int wb200_mxfp4_input_grad(int M, int N, int K, const void* g, long long ldg, const void* b, const void* b_scale, long long b_scale_stride, void* dx,
+                           long long ldd, void* stream) {
+  if (M <= 0 || N <= 0 || K <= 0) return fail(WB200_ERR_INVALID_ARG, "input_grad: M, N, K must be positive (got %d, %d, %d)", M, N, K);
+  if (K % 32) return fail(WB200_ERR_INVALID_ARG, "input_grad: K = %d is not a multiple of the scale group size 32", K);
+  if (!g || !b || !b_scale || !dx) return fail(WB200_ERR_INVALID_ARG, "input_grad: null tensor pointer");
+  if (M > 1 && (ldg < N || ldd < K)) return fail(WB200_ERR_INVALID_ARG, "input_grad: a row pitch is smaller than a row");
+  if (N > 1 && b_scale_stride < K / 32) return fail(WB200_ERR_INVALID_ARG, "input_grad: the pitch of the scales is smaller than a row");
+  if (M == 1) { ldg = (N + 7) / 8 * 8; ldd = K; }
+  if (!aligned_to(g, 16) || ldg % 8 || !aligned_to(b, 16) || !aligned_to(dx, 16) || ldd % 8)
+    return fail(WB200_ERR_ALIGNMENT, "input_grad: rows of g and dx and the codes must be 16-byte aligned");
+  int sms = 0;
+  wb::InputGradParams p;
+  if (int rc = wbhost::device(&sms, &p.status)) return rc;
+  p.codes = static_cast<const uint8_t*>(b);
+  p.scales = static_cast<const uint8_t*>(b_scale);
+  p.dx = static_cast<__nv_bfloat16*>(dx);
+  p.ld_scales = b_scale_stride; p.ldd = ldd;
+  p.M = M; p.N = N; p.K = K;
+  CUtensorMap map;
+  if (int rc = wbhost::tensor_map(&map, g, N, M, (unsigned long long)ldg * 2, 64, 128, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const long long pair_tiles = (long long)div_up(M, 256) * div_up(K, 256);
+  return pair_tiles * 2 >= sms / 2 ? launch_input_grad<2>(map, p, sms, s) : launch_input_grad<1>(map, p, sms, s);
+}
+
+size_t wb200_router_workspace_bytes(int rows, int num_experts) {
+  if (rows <= 0 || num_experts <= 0) return 0;
+  return size_t(router_ctas(rows)) * (2 * num_experts + 1) * 4;
+}
+
+int wb200_router(int rows, int num_experts, int top_k, const void* logits, int dtype, long long ld, const void* mask, const void* given_ids,
+                 int given_are_int64, int renormalize, float* weight, int* ids, int* counts, int* tokens, float* loss, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+  if (int rc = check_router("router", rows, num_experts, top_k, dtype, logits, ld)) return rc;
+  if (!given_ids && (top_k > num_experts || top_k > wb::kRouterMaxTopK))
+    return fail(WB200_ERR_INVALID_ARG, "router: top_k = %d with %d experts (at most %d)", top_k, num_experts, wb::kRouterMaxTopK);
+  if ((!given_ids && (!weight || !ids)) || !counts || !tokens || !loss || !workspace) return fail(WB200_ERR_INVALID_ARG, "router: null pointer");
+  const size_t need = wb200_router_workspace_bytes(rows, num_experts);
+  if (workspace_bytes < need) return fail(WB200_ERR_WORKSPACE, "router: workspace of %zu bytes needed (got %zu)", need, workspace_bytes);
+  if (!aligned_to(workspace, 4)) return fail(WB200_ERR_ALIGNMENT, "router: the workspace must be 4-byte aligned");
+  if (int rc = wbhost::device(nullptr, nullptr)) return rc;
+  wb::RouterParams p;
+  p.logits = logits; p.mask = static_cast<const uint8_t*>(mask); p.given = given_ids; p.ld = ld;
+  p.rows = rows; p.E = num_experts; p.top_k = top_k; p.renormalize = renormalize; p.given_i64 = given_are_int64;
+  p.weight = weight; p.ids = ids; p.counts = counts; p.tokens = tokens; p.loss = loss;
+  const int ctas = router_ctas(rows);
+  p.part_p = static_cast<float*>(workspace);
+  p.part_n = reinterpret_cast<int*>(p.part_p + size_t(ctas) * num_experts);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  void (*kernel)(wb::RouterParams) = dtype == WB200_F32 ? WB_BY_EXPERTS(wb::router_kernel, float, num_experts) : WB_BY_EXPERTS(wb::router_kernel, __nv_bfloat16, num_experts);
+  WB_HOST_CUDA(launch(kernel, dim3(ctas), wb::kRouterWarps * 32, 0, s, p));
+  if (ctas > 1) WB_HOST_CUDA(launch(wb::router_finish_kernel, dim3(1), wb::kRouterWarps * 32, 0, s, p, ctas));
+  return WB200_OK;
+}
+
+int wb200_router_grad(int rows, int num_experts, int top_k, const void* logits, int dtype, long long ld, const void* mask, const int* ids,
+                      const float* g_weight, const float* g_loss, int renormalize, const int* counts, const int* tokens, void* g_logits,
+                      long long ldg, void* stream) {
+  if (int rc = check_router("router gradient", rows, num_experts, top_k, dtype, logits, ld)) return rc;
+  if (!counts || !tokens || !g_logits || (g_weight && !ids)) return fail(WB200_ERR_INVALID_ARG, "router gradient: null pointer");
+  if (g_weight && (top_k > num_experts || top_k > wb::kRouterMaxTopK))
+    return fail(WB200_ERR_INVALID_ARG, "router gradient: top_k = %d with %d experts (at most %d)", top_k, num_experts, wb::kRouterMaxTopK);
+  if (rows > 1 && ldg < num_experts) return fail(WB200_ERR_INVALID_ARG, "router gradient: row pitch %lld is smaller than %d experts", ldg, num_experts);
+  if (int rc = wbhost::device(nullptr, nullptr)) return rc;
+  wb::RouterGradParams p;
+  p.logits = logits; p.mask = static_cast<const uint8_t*>(mask); p.ids = ids; p.g_weight = g_weight; p.g_loss = g_loss; p.counts = counts;
+  p.tokens = tokens; p.g_logits = g_logits; p.ld = ld; p.ldg = ldg;
+  p.rows = rows; p.E = num_experts; p.top_k = top_k; p.renormalize = renormalize;
+  void (*kernel)(wb::RouterGradParams) =
+      dtype == WB200_F32 ? WB_BY_EXPERTS(wb::router_grad_kernel, float, num_experts) : WB_BY_EXPERTS(wb::router_grad_kernel, __nv_bfloat16, num_experts);
+  WB_HOST_CUDA(launch(kernel, dim3(std::min(1184, div_up(rows, wb::kRouterWarps))), wb::kRouterWarps * 32, 0, static_cast<cudaStream_t>(stream), p));
+  return WB200_OK;
+}
+
+int wb200_moe_combine_grad(const void* g, long long ldg, const void* y, long long ldy, int dtype, const int* row_of, int tokens, int top_k, int cols,
+                           float* g_weight, void* stream) {
+  if (tokens <= 0 || top_k <= 0 || cols <= 0)
+    return fail(WB200_ERR_INVALID_ARG, "moe_combine_grad: tokens = %d, top_k = %d, cols = %d", tokens, top_k, cols);
+  if (!g || !y || !row_of || !g_weight) return fail(WB200_ERR_INVALID_ARG, "moe_combine_grad: null pointer");
+  if (dtype != WB200_F32 && dtype != WB200_BF16) return fail(WB200_ERR_INVALID_ARG, "moe_combine_grad: unknown dtype %d", dtype);
+  if (ldy < cols || (tokens > 1 && ldg < cols)) return fail(WB200_ERR_INVALID_ARG, "moe_combine_grad: a row pitch is smaller than cols = %d", cols);
+  if (int rc = wbhost::device(nullptr, nullptr)) return rc;
+  const size_t esz = dtype == WB200_F32 ? 4 : 2;
+  const bool vec = cols % 8 == 0 && aligned_to(g, 16) && aligned_to(y, 16) && ldg * esz % 16 == 0 && ldy * esz % 16 == 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == WB200_F32)
+    WB_HOST_CUDA(vec ? launch_combine_grad<float, true>(g, ldg, y, ldy, row_of, tokens, top_k, cols, g_weight, s)
+                     : launch_combine_grad<float, false>(g, ldg, y, ldy, row_of, tokens, top_k, cols, g_weight, s));
+  else
+    WB_HOST_CUDA(vec ? launch_combine_grad<__nv_bfloat16, true>(g, ldg, y, ldy, row_of, tokens, top_k, cols, g_weight, s)
+                     : launch_combine_grad<__nv_bfloat16, false>(g, ldg, y, ldy, row_of, tokens, top_k, cols, g_weight, s));
+  return WB200_OK;
+}
+
+}  // extern "C"

@@ -2,6 +2,7 @@
 // launches. Plays the role of the reference's native launch shim
 // (wave_lang/kernel/wave/runtime/runtime.cpp:123-263) for the MXFP4 scaled-GEMM kernels.
 #include "../../include/wave_b200.h"
+#include "host.cuh"
 #include "gemm_cluster_splitk_sm100.cuh"
 #include "gemm_sm100.cuh"
 #include "mixed_decode_sm100.cuh"
@@ -115,9 +116,16 @@ CUresult encode_2d(CUtensorMap* map, const MapKey& k) {
   cuuint64_t strides[1] = {k.stride};
   cuuint32_t box[2] = {k.box0, k.box1};
   cuuint32_t estr[2] = {1u, 1u};
-  CUresult r = g_encode(map, CUtensorMapDataType(k.dtype), 2, const_cast<void*>(k.base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CUtensorMapSwizzle(k.swizzle), CUtensorMapL2promotion(k.promo),
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return g_encode(map, CUtensorMapDataType(k.dtype), 2, const_cast<void*>(k.base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CUtensorMapSwizzle(k.swizzle), CUtensorMapL2promotion(k.promo),
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a thread that has made no CUDA call yet, as autograd's: the runtime binds the context
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
   if (r == CUDA_SUCCESS) {
     const int slot = (c.used < kMapCacheSize) ? c.used++ : (c.next = (c.next + 1) % kMapCacheSize);
     c.keys[slot] = k;
@@ -1270,6 +1278,30 @@ __global__ void selftest_wait_timeout_kernel(int* status, long long limit_cycles
 
 }  // namespace
 
+namespace wbhost {
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+int device(int* sm_count, int** status) {
+  DeviceInfo* dev;
+  if (int rc = get_device(&dev)) return rc;
+  if (sm_count) *sm_count = dev->sm_count;
+  if (status) *status = dev->status_ptr;
+  return WB200_OK;
+}
+int tensor_map(CUtensorMap* map, const void* base, unsigned long long d0, unsigned long long d1, unsigned long long stride, unsigned box0,
+               unsigned box1, CUtensorMapDataType dtype, CUtensorMapSwizzle swizzle) {
+  const MapKey k{base, d0, d1, stride, box0, box1, int(dtype), int(swizzle), int(CU_TENSOR_MAP_L2_PROMOTION_NONE)};
+  const CUresult r = encode_2d(map, k);
+  if (r != CUDA_SUCCESS) return ::fail(WB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (%llu x %llu)", int(r), d0, d1);
+  return WB200_OK;
+}
+}  // namespace wbhost
+
 extern "C" {
 
 int wb200_version(void) { return 1000; }
@@ -2266,6 +2298,10 @@ int wb200_debug_checks(unsigned long long* record, int reset) {
     const unsigned long long zero[3] = {0, 0, 0};
     WB_CUDA(cudaMemcpyToSymbol(wb::g_check_record, zero, sizeof(zero)));
   }
+  unsigned long long other[3];  // of the kernels in adapt.cu
+  WB_CUDA(wbhost::adapt_check_record(other, reset != 0));
+  if (!record[0]) { record[0] = other[0]; record[1] = other[1]; }
+  record[2] += other[2];
   return WB200_OK;
 #else
   (void)record; (void)reset;

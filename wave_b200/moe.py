@@ -133,6 +133,175 @@ def combine(y: torch.Tensor, row_of: torch.Tensor, weight: torch.Tensor, top_k: 
                                          weight.data_ptr(), tokens, top_k, cols, out.data_ptr(), out.stride(0), _stream()))
 
 
+class _CombineRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, row_of, weight):
+        out = torch.empty(row_of.shape[0], y.shape[1], dtype=y.dtype, device=y.device)
+        combine(y, row_of, weight, row_of.shape[1], out)
+        ctx.save_for_backward(y, row_of)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        y, row_of = ctx.saved_tensors
+        if g.stride(1) != 1 or g.shape[0] > 1 and g.stride(0) < g.shape[1]:
+            g = g.contiguous()
+        tokens, top_k = row_of.shape
+        grad = torch.empty(tokens, top_k, dtype=torch.float32, device=y.device)
+        lib = _lib.load()
+        with torch.cuda.device(y.device):
+            _lib.check(lib.wb200_moe_combine_grad(g.data_ptr(), g.stride(0) if tokens > 1 else y.shape[1], y.data_ptr(), y.stride(0), ops._DTYPE_CODE[y.dtype],
+                                                  row_of.data_ptr(), tokens, top_k, y.shape[1], grad.data_ptr(), _stream()))
+        return None, None, grad
+
+
+def combine_rows(y: torch.Tensor, row_of: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """out[t] = sum_j weight[t, j] * y[row_of[t, j]] in f32, slot order, rounded once to y's type: `combine` with a new output, differentiable
+    in the weights (the rows of y are those of frozen experts: a y that requires a gradient is refused). y [R, N] f32 or bf16, row_of [tokens, k]
+    int32, negative for a dropped pair, weight [tokens, k] f32. Rows at or past R are not checked for."""
+    if not y.is_cuda or y.dtype not in ops._DTYPE_CODE or y.dim() != 2:
+        raise ValueError(f"y must be a 2-D float32 or bfloat16 CUDA tensor, got {y.dtype} {tuple(y.shape)}")
+    if row_of.dtype != torch.int32 or weight.dtype != torch.float32 or row_of.dim() != 2 or weight.shape != row_of.shape or row_of.shape[1] == 0:
+        raise ValueError(f"row_of (int32) and weight (float32) must be [tokens, k], got {row_of.dtype} {tuple(row_of.shape)} and {weight.dtype} {tuple(weight.shape)}")
+    if row_of.device != y.device or weight.device != y.device:
+        raise ValueError("y, row_of and weight must be on one device")
+    if torch.is_grad_enabled() and y.requires_grad:
+        raise ValueError("the gradient of y is not computed: pass y.detach()")
+    if y.shape[1] == 0 or y.stride(1) != 1 and y.shape[1] > 1 or y.shape[0] > 1 and y.stride(0) < y.shape[1]:
+        y = y.contiguous()
+    if row_of.shape[0] == 0 or y.shape[1] == 0:
+        return torch.zeros(row_of.shape[0], y.shape[1], dtype=y.dtype, device=y.device) + 0 * weight.sum().to(y.dtype)
+    return _CombineRows.apply(y, row_of.contiguous(), weight.contiguous())
+
+
+@dataclass
+class Routing:
+    """What `router` gives: weight [rows, k] f32 and balance_loss (f32 scalar), both differentiable in the logits; ids [rows, k] int32 (-1 in
+    padded rows) and counts [experts] int32, how often each expert was chosen."""
+    weight: torch.Tensor
+    ids: torch.Tensor
+    counts: torch.Tensor
+    balance_loss: torch.Tensor
+
+
+def _check_router(logits, mask) -> tuple[torch.Tensor, torch.Tensor | None]:
+    if not logits.is_cuda or logits.dtype not in ops._DTYPE_CODE or logits.dim() != 2:
+        raise ValueError(f"logits must be a 2-D float32 or bfloat16 CUDA tensor, got {logits.dtype} {tuple(logits.shape)} on {logits.device}")
+    rows, E = logits.shape
+    if not 1 <= E <= ROUTER_MAX_EXPERTS:
+        raise ValueError(f"{E} experts (1 .. {ROUTER_MAX_EXPERTS})")
+    if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != (rows,) or mask.device != logits.device):
+        raise ValueError(f"mask must be bool [{rows}] on {logits.device}, got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
+    if logits.stride(1) != 1 and E > 1 or rows > 1 and logits.stride(0) < E:  # overlapping rows too, as of an expanded bias
+        logits = logits.contiguous()
+    return logits, mask.contiguous() if mask is not None else None
+
+
+ROUTER_MAX_EXPERTS = 256
+ROUTER_MAX_TOP_K = 32
+
+
+def _run_router(logits, mask, top_k, renormalize, given):
+    lib = _lib.load()
+    rows, E = logits.shape
+    dev = logits.device
+    nbytes = int(lib.wb200_router_workspace_bytes(rows, E))
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    small = torch.empty(1 + E + nbytes // 4, dtype=torch.int32, device=dev)  # tokens, counts, then the partial sums
+    weight = ids = None
+    if given is None:
+        weight = torch.empty(rows, top_k, dtype=torch.float32, device=dev)
+        ids = torch.empty(rows, top_k, dtype=torch.int32, device=dev)
+    base = small.data_ptr()
+    with torch.cuda.device(dev):
+        _lib.check(lib.wb200_router(rows, E, top_k, logits.data_ptr(), ops._DTYPE_CODE[logits.dtype], logits.stride(0) if rows > 1 else E,
+                                    mask.data_ptr() if mask is not None else None, given.data_ptr() if given is not None else None,
+                                    int(given is not None and given.dtype == torch.int64), int(renormalize),
+                                    weight.data_ptr() if weight is not None else None, ids.data_ptr() if ids is not None else None, base + 4,
+                                    base, loss.data_ptr(), base + 4 * (1 + E), nbytes, _stream()))
+    return weight, ids, small[1:1 + E], loss, small[:1]
+
+
+def _run_router_grad(logits, mask, top_k, renormalize, ids, g_weight, g_loss, counts, tokens):
+    lib = _lib.load()
+    rows, E = logits.shape
+    grad = torch.empty(rows, E, dtype=logits.dtype, device=logits.device)
+    with torch.cuda.device(logits.device):
+        _lib.check(lib.wb200_router_grad(rows, E, top_k, logits.data_ptr(), ops._DTYPE_CODE[logits.dtype], logits.stride(0) if rows > 1 else E,
+                                         mask.data_ptr() if mask is not None else None, ids.data_ptr() if ids is not None else None,
+                                         g_weight.data_ptr() if g_weight is not None else None, g_loss.data_ptr() if g_loss is not None else None,
+                                         int(renormalize), counts.data_ptr(), tokens.data_ptr(), grad.data_ptr(), E, _stream()))
+    return grad
+
+
+class _Router(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, mask, top_k, renormalize):
+        weight, ids, counts, loss, tokens = _run_router(logits, mask, top_k, renormalize, None)
+        ctx.save_for_backward(logits, mask, ids, counts, tokens)
+        ctx.options = top_k, renormalize
+        ctx.mark_non_differentiable(ids, counts)
+        ctx.set_materialize_grads(False)
+        return weight, ids, counts, loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_weight, _ids, _counts, g_loss):
+        logits, mask, ids, counts, tokens = ctx.saved_tensors
+        top_k, renormalize = ctx.options
+        if g_weight is None and g_loss is None:
+            return None, None, None, None
+        g_weight = g_weight.contiguous() if g_weight is not None else None
+        return _run_router_grad(logits, mask, top_k, renormalize, ids, g_weight, g_loss, counts, tokens), None, None, None
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, mask, ids):
+        _, _, counts, loss, tokens = _run_router(logits, mask, ids.shape[1], False, ids)
+        ctx.save_for_backward(logits, mask, counts, tokens)
+        ctx.top_k = ids.shape[1]
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_loss, _counts):
+        logits, mask, counts, tokens = ctx.saved_tensors
+        return _run_router_grad(logits, mask, ctx.top_k, False, None, None, g_loss, counts, tokens), None, None
+
+
+def router(logits: torch.Tensor, top_k: int, mask: torch.Tensor | None = None, renormalize: bool = False) -> Routing:
+    """Routing of rows to experts with what its training needs, in one pass over the logits [rows, experts] (f32 or bf16, at most 256 experts).
+
+    ids: the top_k (at most 32) largest logits of a row, the lower expert first among equals, NaN above all; weight: softmax(logits)[ids], over
+    the chosen ones alone with renormalize. balance_loss = E sum_e f_e P_e, f_e = counts[e] / (top_k n), P_e = the mean of softmax(logits)[:, e]
+    over the n rows that count; 0 where none does. Its gradient takes f as a constant. mask: bool [rows], False for padding: ids -1, weight
+    0, in no sum, gradient 0."""
+    if not 1 <= top_k <= min(logits.shape[-1], ROUTER_MAX_TOP_K):
+        raise ValueError(f"top_k = {top_k} of {logits.shape[-1]} experts (at most {ROUTER_MAX_TOP_K})")
+    logits, mask = _check_router(logits, mask)
+    if logits.shape[0] == 0:
+        zero = logits.float().sum()
+        return Routing(logits.new_zeros(0, top_k, dtype=torch.float32) + zero, torch.zeros(0, top_k, dtype=torch.int32, device=logits.device),
+                       torch.zeros(logits.shape[1], dtype=torch.int32, device=logits.device), zero)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return Routing(*_Router.apply(logits, mask, top_k, renormalize))
+    return Routing(*_run_router(logits, mask, top_k, renormalize, None)[:4])
+
+
+def balance_loss(logits: torch.Tensor, ids: torch.Tensor, mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(balance loss, counts) as in `router`, for choices ids [rows, k] (int32 or int64) that were made elsewhere (limited to groups, biased).
+    Ids outside [0, experts) do not count; an expert chosen twice by a row counts twice."""
+    logits, mask = _check_router(logits, mask)
+    if ids.dtype not in (torch.int32, torch.int64) or ids.dim() != 2 or ids.shape[0] != logits.shape[0] or ids.shape[1] == 0 or ids.device != logits.device:
+        raise ValueError(f"ids must be int32 or int64 [{logits.shape[0]}, k] on {logits.device}, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
+    if logits.shape[0] == 0:
+        return logits.float().sum(), torch.zeros(logits.shape[1], dtype=torch.int32, device=logits.device)
+    return _BalanceLoss.apply(logits, mask, ids.contiguous())
+
+
 @dataclass
 class SiluAndMulTemplate:
     """What get_silu_and_mul_kernel returns in place of the reference's traced kernel."""
@@ -222,10 +391,33 @@ class MXFP4ExpertMLP:
     def _forward_steps(self, x: torch.Tensor, router_logits: torch.Tensor) -> torch.Tensor:
         """Everything is sized by the worst case of the routing (tokens * top_k + E * 255 rows) and driven by the
         device outputs of the block alignment, so the call never waits for the GPU."""
+        weight, ids = self.route(router_logits)
+        y, inverse = self._expert_rows(x, ids)
+        out = torch.empty(x.shape[0], self.w2.N, dtype=torch.bfloat16, device=x.device)
+        combine(y, inverse, weight.reshape(-1), self.top_k, out)
+        return out
+
+    def forward_routed(self, x: torch.Tensor, routing: Routing) -> torch.Tensor:
+        """The expert MLP on choices and weights made by `router` (or put together by the caller): bf16 [tokens, K_out], differentiable in
+        routing.weight. The experts are frozen and have no input gradient: an x that requires one is refused. Pairs with an id of -1 (padding)
+        add nothing. Never waits for the GPU."""
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise ValueError("frozen experts give no gradient for x: pass x.detach()")
+        ids, weight = routing.ids, routing.weight
+        if not x.is_cuda or x.dim() != 2 or x.shape[1] != self.K or x.dtype not in ops._DTYPE_CODE:
+            raise ValueError(f"x must be an f32 or bf16 CUDA tensor [tokens, {self.K}], got {x.dtype} {tuple(x.shape)}")
+        if tuple(ids.shape) != (x.shape[0], self.top_k) or tuple(weight.shape) != tuple(ids.shape) or weight.dtype != torch.float32:
+            raise ValueError(f"routing must hold ids and f32 weights [{x.shape[0]}, {self.top_k}], got {tuple(ids.shape)} and {weight.dtype} {tuple(weight.shape)}")
+        if x.shape[0] == 0:
+            return torch.zeros(0, self.w2.N, dtype=torch.bfloat16, device=x.device) + 0 * weight.sum().to(torch.bfloat16)
+        y, inverse = self._expert_rows(x, ids)
+        return combine_rows(y, inverse.reshape(ids.shape), weight)
+
+    def _expert_rows(self, x: torch.Tensor, ids: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """Every expert's output for its rows, and the row of every (token, slot) pair (-1 for an id that is no expert)."""
         T, dev = x.shape[0], x.device
         n = T * self.top_k
         B = self.BLOCK
-        weight, ids = self.route(router_logits)
         cap = (n + self.E * (B - 1) + B - 1) // B * B
         sorted_ids = torch.empty(cap, dtype=torch.int32, device=dev)
         expert_ids = torch.empty(cap // B, dtype=torch.int32, device=dev)
@@ -243,9 +435,7 @@ class MXFP4ExpertMLP:
         _, hq, hs = silu_and_mul(h[:, :self.I], h[:, self.I:], quantize=True, num_rows=post_pad)
         y = torch.empty(cap, self.w2.N, dtype=torch.bfloat16, device=dev)
         moe_scaled_gemm(hq, hs, self.w2, expert_ids, post_pad, y)
-        out = torch.empty(T, self.w2.N, dtype=torch.bfloat16, device=dev)
-        combine(y, inverse, weight.reshape(-1), self.top_k, out)
-        return out
+        return y, inverse
 
     __call__ = forward
 

@@ -28,18 +28,41 @@ def _native():
     return _lib._fast
 
 
+class _FrozenLinear(torch.autograd.Function):
+    """A layer's output with the gradient of its input; the rounding of the activations to MXFP4 counts as the identity."""
+
+    @staticmethod
+    def forward(ctx, x, layer):
+        ctx.save_for_backward(layer.weight_codes, layer.weight_scales)
+        return layer._base(x)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        codes, scales = ctx.saved_tensors
+        dx = ops.mxfp4_input_grad(g.reshape(-1, g.shape[-1]), codes, scales)
+        return dx.reshape(*g.shape[:-1], dx.shape[1]), None
+
+
 class MXFP4Linear(torch.nn.Module):
-    def __init__(self, weight_codes: torch.Tensor, weight_scales: torch.Tensor, output_dtype=torch.bfloat16):
+    def __init__(self, weight_codes: torch.Tensor, weight_scales: torch.Tensor, output_dtype=torch.bfloat16, input_grad: bool = False):
         """weight_codes [N, K/2] uint8, weight_scales [N, K/32] uint8 (row-major E8M0), both on the GPU. The GEMM reads the scales in
-        packings that are made here, on the current stream, and anew when a state dict is loaded."""
+        packings that are made here, on the current stream, and anew when a state dict is loaded.
+        input_grad: gradients flow through the frozen weight to an x that requires one (bf16 x and output); without it the output
+        is detached from x."""
         super().__init__()
         ops._as_u8(weight_codes, "weight_codes")
         self.out_features, half_k = weight_codes.shape
         self.in_features = half_k * 2
         self.output_dtype = as_output_dtype(output_dtype).torch_dtype
+        if input_grad and self.output_dtype != torch.bfloat16:
+            raise ValueError("the input gradient is taken from a bfloat16 output")
+        self.input_grad = input_grad
         self.register_buffer("weight_codes", weight_codes.contiguous())
         self.register_buffer("weight_scales", weight_scales.contiguous())
         self._pack()
+
+    input_grad = False
 
     # Decode calls (at most 128 rows) may read a second packing, per tile of the height h that gives every SM the same number of
     # weight tiles: one height per layer, as it follows from out_features, and 128 / h times the bytes of the usual packing. Made with that one, not
@@ -82,12 +105,37 @@ class MXFP4Linear(torch.nn.Module):
         return self._packed if self._packed_low is None else self._packed_low
 
     @classmethod
-    def from_float(cls, weight: torch.Tensor, output_dtype=torch.bfloat16) -> "MXFP4Linear":
+    def from_float(cls, weight: torch.Tensor, output_dtype=torch.bfloat16, input_grad: bool = False) -> "MXFP4Linear":
         """Quantise an f32 / bf16 [N, K] weight on the GPU."""
         q, s, _ = ops.quantize_mxfp4(weight, want_rowmajor=True, want_packed=False)
-        return cls(q, s, output_dtype)
+        return cls(q, s, output_dtype, input_grad)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, adapters=None, ids: torch.Tensor | None = None) -> torch.Tensor:
+        """x [..., K] -> [..., N]. adapters: a `LowRankAdapters` pool, ids [...]: the adapter of every row (outside the pool: none); what they
+        add is rounded onto the layer's rounded output. They take a bf16 x."""
+        if adapters is None and not self.input_grad:
+            return self._base(x)
+        return self._forward_trained(x, adapters, ids)
+
+    def _forward_trained(self, x: torch.Tensor, adapters, ids) -> torch.Tensor:
+        if torch.is_grad_enabled() and x.requires_grad:
+            if not self.input_grad:
+                raise ValueError("the gradient of x needs the layer's part: make the layer with input_grad=True, or pass x.detach()")
+            if x.dtype != torch.bfloat16:
+                raise ValueError(f"the gradient of x needs a bfloat16 x, got {x.dtype}")
+            y = _FrozenLinear.apply(x, self)
+        else:
+            y = self._base(x)
+        if adapters is None:
+            return y
+        if ids is None or ids.shape != x.shape[:-1]:
+            raise ValueError(f"ids must hold the adapter of every row of x, {tuple(x.shape[:-1])}")
+        trained = torch.is_grad_enabled() and (y.requires_grad or adapters.a.requires_grad or adapters.b.requires_grad)
+        y2 = y.reshape(-1, self.out_features)
+        z = adapters(y2, x.reshape(-1, self.in_features), ids.reshape(-1), out=None if trained else y2)
+        return z.reshape(y.shape)
+
+    def _base(self, x: torch.Tensor) -> torch.Tensor:
         # a call whose tensors need no preparation; anything else comes back unhandled
         native, scales = _native(), self._native_scales
         if native is None or scales is None:

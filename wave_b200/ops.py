@@ -335,6 +335,52 @@ def quantized_gemm(x: torch.Tensor, b: torch.Tensor, b_sf: PackedScales, c: torc
         _lib.check(rc)
 
 
+def mxfp4_input_grad(g: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of a linear layer with MXFP4 weights by its input: g [M, N] @ dequant(b, b_scale) [N, K], f32 accumulation, rounded once to
+    bf16. g bf16, b uint8 [N, K/2] and b_scale uint8 [N, K/32] row-major as the layer's forward takes them. Rows of g that do not start on
+    16 bytes (odd N) are copied first. out: bf16 [M, K] whose rows start on 16 bytes."""
+    lib = _lib.load()
+    if not g.is_cuda or g.dtype != torch.bfloat16 or g.dim() != 2:
+        raise ValueError(f"g must be a 2-D bfloat16 CUDA tensor, got {g.dtype} {tuple(g.shape)} on {g.device}")
+    _as_u8(b, "b")
+    _as_u8(b_scale, "b_scale")
+    (M, N), K = g.shape, b.shape[-1] * 2
+    if b.dim() != 2 or b.shape[0] != N or K % SCALE_GROUP_SIZE or tuple(b_scale.shape) != (N, K // SCALE_GROUP_SIZE) or N == 0 or K == 0:
+        raise ValueError(f"b must be [{N}, K/2] and b_scale [{N}, K/32] for K a multiple of 32, got {tuple(b.shape)} and {tuple(b_scale.shape)}")
+    if b.device != g.device or b_scale.device != g.device:
+        raise ValueError("g, b and b_scale must be on one device")
+    if not b.is_contiguous() or b.data_ptr() % 16:
+        b = b.contiguous() if not b.is_contiguous() else b.clone()
+    if b_scale.stride(1) != 1 and K > SCALE_GROUP_SIZE or N > 1 and b_scale.stride(0) < K // SCALE_GROUP_SIZE:
+        b_scale = b_scale.contiguous()
+    if out is None:
+        out = torch.empty(M, K, dtype=torch.bfloat16, device=g.device)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (M, K) or out.device != g.device or out.stride(1) != 1 or not rows_aligned(out) or \
+            (M > 1 and out.stride(0) < K):
+        raise ValueError(f"out must be bfloat16 [{M}, {K}] on {g.device} with rows that start on 16 bytes")
+    if M == 0:
+        return out
+    if g.stride(1) != 1 and N > 1 or not rows_aligned(g) or M > 1 and g.stride(0) < N:
+        padded = torch.empty(M, (N + 7) // 8 * 8, dtype=torch.bfloat16, device=g.device)
+        padded[:, :N].copy_(g)
+        g = padded[:, :N]
+    ldg = g.stride(0) if M > 1 else (N + 7) // 8 * 8
+    ldd = out.stride(0) if M > 1 else K
+
+    def run():
+        return lib.wb200_mxfp4_input_grad(M, N, K, g.data_ptr(), ldg, b.data_ptr(), b_scale.data_ptr(), b_scale.stride(0) if N > 1 else K // SCALE_GROUP_SIZE,
+                                          out.data_ptr(), ldd, _stream())
+
+    if g.device.index == torch.cuda.current_device():
+        rc = run()
+    else:
+        with torch.cuda.device(g.device):
+            rc = run()
+    if rc:
+        _lib.check(rc)
+    return out
+
+
 _FP8_FORMATS = {torch.float8_e5m2: _lib.E5M2, torch.float8_e4m3fn: _lib.E4M3}
 
 
