@@ -470,17 +470,17 @@ int wb200_mxfp4_input_grad(int M, int N, int K, const void* g, long long ldg, co
                            void* dx, long long ldd, void* stream);
 /* Router: weight [rows, top_k] and ids [rows, top_k] of the top_k largest of num_experts (at most 256) logits, f32 or bf16 with row pitch
  * ld: softmax over all experts, over the chosen ones with renormalize != 0; in descending order, the lower expert first among equals, NaN
- * above all. counts [num_experts]: how often each was chosen; tokens: rows that count; loss = num_experts * sum_e counts[e] / (top_k tokens) *
- * mean_t p[t, e]. mask (or null): one byte a row, 0 = padding: ids -1, weight 0, in no sum. given_ids (or null): int32 or int64 [rows, top_k]
+ * above all. counts [num_experts]: how often each was chosen; loss = num_experts * sum_e counts[e] / (top_k n) *
+ * mean_t p[t, e] over the n rows that count; unit = num_experts / (top_k n^2), for the gradient. mask (or null): one byte a row, 0 = padding: ids -1, weight 0, in no sum. given_ids (or null): int32 or int64 [rows, top_k]
  * choices made elsewhere; weight and ids are then not written, and ids out of range do not count. top_k at most 32 where it is chosen here. */
 size_t wb200_router_workspace_bytes(int rows, int num_experts);
 int wb200_router(int rows, int num_experts, int top_k, const void* logits, int dtype, long long ld, const void* mask, const void* given_ids,
-                 int given_are_int64, int renormalize, float* weight, int* ids, int* counts, int* tokens, float* loss, void* workspace,
+                 int given_are_int64, int renormalize, float* weight, int* ids, int* counts, float* unit, float* loss, void* workspace,
                  size_t workspace_bytes, void* stream);
 /* Gradient of the router: g_logits [rows, num_experts] (the type of logits, pitch ldg) from g_weight [rows, top_k] (or null) and the device
- * scalar g_loss (or null); ids, counts and tokens as the forward call wrote them. Rows of padding get zeros. */
+ * scalar g_loss (or null); ids, counts and unit as the forward call wrote them. Rows of padding get zeros. */
 int wb200_router_grad(int rows, int num_experts, int top_k, const void* logits, int dtype, long long ld, const void* mask, const int* ids,
-                      const float* g_weight, const float* g_loss, int renormalize, const int* counts, const int* tokens, void* g_logits,
+                      const float* g_weight, const float* g_loss, int renormalize, const int* counts, const float* unit, void* g_logits,
                       long long ldg, void* stream);
 /* Gradient of wb200_moe_combine by its weights: g_weight[t, j] = sum_c g[t, c] * y[row_of[t, j], c], f32; 0 for pairs with row_of < 0. */
 int wb200_moe_combine_grad(const void* g, long long ldg, const void* y, long long ldy, int dtype, const int* row_of, int tokens, int top_k,

@@ -176,7 +176,7 @@ int run_outer(const __nv_bfloat16* z, long long ldz, const float* hidden, int co
 // input gradient
 // ------------------------------------------------------------------------------------------
 template <int CG>
-int launch_input_grad(const CUtensorMap& map, wb::InputGradParams p, int sms, cudaStream_t stream) {
+int launch_input_grad(const CUtensorMap& map, const CUtensorMap& codes, wb::InputGradParams p, int sms, cudaStream_t stream) {
   using Cfg = wb::InputGradCfg<CG>;
   p.tiles_m = div_up(p.M, Cfg::BM * CG);
   p.tiles_k = div_up(p.K, Cfg::TILE_K);
@@ -204,7 +204,7 @@ int launch_input_grad(const CUtensorMap& map, wb::InputGradParams p, int sms, cu
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  WB_HOST_CUDA(cudaLaunchKernelEx(&cfg, kernel, map, p));
+  WB_HOST_CUDA(cudaLaunchKernelEx(&cfg, kernel, map, codes, p));
   return WB200_OK;
 }
 
@@ -338,16 +338,17 @@ int wb200_mxfp4_input_grad(int M, int N, int K, const void* g, long long ldg, co
   int sms = 0;
   wb::InputGradParams p;
   if (int rc = wbhost::device(&sms, &p.status)) return rc;
-  p.codes = static_cast<const uint8_t*>(b);
   p.scales = static_cast<const uint8_t*>(b_scale);
   p.dx = static_cast<__nv_bfloat16*>(dx);
   p.ld_scales = b_scale_stride; p.ldd = ldd;
   p.M = M; p.N = N; p.K = K;
-  CUtensorMap map;
+  p.scale_words = aligned_to(b_scale, 4) && b_scale_stride % 4 == 0 && K % 128 == 0;
+  CUtensorMap map, codes;
+  if (int rc = wbhost::tensor_map(&codes, b, K / 2, N, K / 2, 64, 64, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
   if (int rc = wbhost::tensor_map(&map, g, N, M, (unsigned long long)ldg * 2, 64, 128, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const long long pair_tiles = (long long)div_up(M, 256) * div_up(K, 256);
-  return pair_tiles * 2 >= sms / 2 ? launch_input_grad<2>(map, p, sms, s) : launch_input_grad<1>(map, p, sms, s);
+  return pair_tiles * 2 >= sms / 2 ? launch_input_grad<2>(map, codes, p, sms, s) : launch_input_grad<1>(map, codes, p, sms, s);
 }
 
 size_t wb200_router_workspace_bytes(int rows, int num_experts) {
@@ -356,12 +357,12 @@ size_t wb200_router_workspace_bytes(int rows, int num_experts) {
 }
 
 int wb200_router(int rows, int num_experts, int top_k, const void* logits, int dtype, long long ld, const void* mask, const void* given_ids,
-                 int given_are_int64, int renormalize, float* weight, int* ids, int* counts, int* tokens, float* loss, void* workspace,
+                 int given_are_int64, int renormalize, float* weight, int* ids, int* counts, float* unit, float* loss, void* workspace,
                  size_t workspace_bytes, void* stream) {
   if (int rc = check_router("router", rows, num_experts, top_k, dtype, logits, ld)) return rc;
   if (!given_ids && (top_k > num_experts || top_k > wb::kRouterMaxTopK))
     return fail(WB200_ERR_INVALID_ARG, "router: top_k = %d with %d experts (at most %d)", top_k, num_experts, wb::kRouterMaxTopK);
-  if ((!given_ids && (!weight || !ids)) || !counts || !tokens || !loss || !workspace) return fail(WB200_ERR_INVALID_ARG, "router: null pointer");
+  if ((!given_ids && (!weight || !ids)) || !counts || !unit || !loss || !workspace) return fail(WB200_ERR_INVALID_ARG, "router: null pointer");
   const size_t need = wb200_router_workspace_bytes(rows, num_experts);
   if (workspace_bytes < need) return fail(WB200_ERR_WORKSPACE, "router: workspace of %zu bytes needed (got %zu)", need, workspace_bytes);
   if (!aligned_to(workspace, 4)) return fail(WB200_ERR_ALIGNMENT, "router: the workspace must be 4-byte aligned");
@@ -369,29 +370,29 @@ int wb200_router(int rows, int num_experts, int top_k, const void* logits, int d
   wb::RouterParams p;
   p.logits = logits; p.mask = static_cast<const uint8_t*>(mask); p.given = given_ids; p.ld = ld;
   p.rows = rows; p.E = num_experts; p.top_k = top_k; p.renormalize = renormalize; p.given_i64 = given_are_int64;
-  p.weight = weight; p.ids = ids; p.counts = counts; p.tokens = tokens; p.loss = loss;
+  p.weight = weight; p.ids = ids; p.counts = counts; p.unit = unit; p.loss = loss;
   const int ctas = router_ctas(rows);
   p.part_p = static_cast<float*>(workspace);
   p.part_n = reinterpret_cast<int*>(p.part_p + size_t(ctas) * num_experts);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   void (*kernel)(wb::RouterParams) = dtype == WB200_F32 ? WB_BY_EXPERTS(wb::router_kernel, float, num_experts) : WB_BY_EXPERTS(wb::router_kernel, __nv_bfloat16, num_experts);
   WB_HOST_CUDA(launch(kernel, dim3(ctas), wb::kRouterWarps * 32, 0, s, p));
-  if (ctas > 1) WB_HOST_CUDA(launch(wb::router_finish_kernel, dim3(1), wb::kRouterWarps * 32, 0, s, p, ctas));
+  if (ctas > 1) WB_HOST_CUDA(launch(wb::router_finish_kernel, dim3(1), 1024, 0, s, p, ctas));
   return WB200_OK;
 }
 
 int wb200_router_grad(int rows, int num_experts, int top_k, const void* logits, int dtype, long long ld, const void* mask, const int* ids,
-                      const float* g_weight, const float* g_loss, int renormalize, const int* counts, const int* tokens, void* g_logits,
+                      const float* g_weight, const float* g_loss, int renormalize, const int* counts, const float* unit, void* g_logits,
                       long long ldg, void* stream) {
   if (int rc = check_router("router gradient", rows, num_experts, top_k, dtype, logits, ld)) return rc;
-  if (!counts || !tokens || !g_logits || (g_weight && !ids)) return fail(WB200_ERR_INVALID_ARG, "router gradient: null pointer");
+  if (!counts || !unit || !g_logits || (g_weight && !ids)) return fail(WB200_ERR_INVALID_ARG, "router gradient: null pointer");
   if (g_weight && (top_k > num_experts || top_k > wb::kRouterMaxTopK))
     return fail(WB200_ERR_INVALID_ARG, "router gradient: top_k = %d with %d experts (at most %d)", top_k, num_experts, wb::kRouterMaxTopK);
   if (rows > 1 && ldg < num_experts) return fail(WB200_ERR_INVALID_ARG, "router gradient: row pitch %lld is smaller than %d experts", ldg, num_experts);
   if (int rc = wbhost::device(nullptr, nullptr)) return rc;
   wb::RouterGradParams p;
   p.logits = logits; p.mask = static_cast<const uint8_t*>(mask); p.ids = ids; p.g_weight = g_weight; p.g_loss = g_loss; p.counts = counts;
-  p.tokens = tokens; p.g_logits = g_logits; p.ld = ld; p.ldg = ldg;
+  p.unit = unit; p.g_logits = g_logits; p.ld = ld; p.ldg = ldg;
   p.rows = rows; p.E = num_experts; p.top_k = top_k; p.renormalize = renormalize;
   void (*kernel)(wb::RouterGradParams) =
       dtype == WB200_F32 ? WB_BY_EXPERTS(wb::router_grad_kernel, float, num_experts) : WB_BY_EXPERTS(wb::router_grad_kernel, __nv_bfloat16, num_experts);

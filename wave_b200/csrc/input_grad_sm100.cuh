@@ -8,9 +8,14 @@
 //   warp 0       TMA: g tiles, 128 rows x 64 N, K-major with the 128-byte swizzle
 //   warp 1       tcgen05.mma (leader CTA of a pair)
 //   warps 2..5   epilogue: accumulator -> bf16 -> dx
-//   warps 6..13  expansion: 64 N x 128 K codes a stage, from global memory (three stages ahead, in registers) to shared memory. A thread
-//                takes 32 codes with their one scale. W's rows are contiguous in K, the MMA's N dimension: the tile is an MN-major
-//                operand of 64-column groups, rows of 128 bytes per n, swizzled as a TMA load would leave them.
+//   warps 6..21  expansion of 64 N x 128 K codes a stage within shared memory. A thread takes 32 codes with their one scale. W's rows are
+//                contiguous in K, the MMA's N dimension: the tile is an MN-major operand of 64-column groups, rows of 128 bytes per n,
+//                swizzled as a TMA load would leave them.
+//   warp 22      scales of a stage (four to a row of codes, at any alignment), from global to shared memory
+//
+// The codes come by TMA, and the scales by a warp of their own, because the expanding threads fence their stores for the tensor core
+// (fence.proxy.async), and that fence waits for every load that the thread has in flight: with codes prefetched into registers the kernel
+// stood at 480 TFLOP/s, each stage waiting a whole memory latency.
 //
 // CG = 2: 256 x 256 tiles, each CTA holds 128 rows of g and expands 128 columns of W; CG = 1: 128 x 128 tiles. Both accumulators of
 // neighbouring tiles are in tensor memory, so an epilogue runs under the next tile's products.
@@ -27,21 +32,33 @@ struct InputGradCfg {
   static constexpr int TILE_K = COLS * CG;
   static constexpr int A_BYTES = BM * BN * 2;
   static constexpr int B_BYTES = COLS * BN * 2;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 6;
+  static constexpr int A_STAGES = 6;                 // deeper than B's: a load from memory takes longer than an expansion
+  static constexpr int B_STAGES = 6;
+  static constexpr int CODE_BYTES = COLS / 2 * BN;   // of a stage
+  static constexpr int SCALE_BYTES = COLS / 32 * BN;
+  static constexpr int CODE_STAGES = 6;
+  static constexpr int SCALE_BATCH = 8;              // stages whose scales are loaded together; two batches in shared memory
   static constexpr int TMEM_COLS = 2 * TILE_K;
-  static constexpr int NUM_BARRIERS = 3 * STAGES + 4;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + NUM_BARRIERS * 8 + 16 + 1024;
-  static constexpr int EXPAND_WARPS = 8;
-  static constexpr int THREADS = (6 + EXPAND_WARPS) * 32;
+  static constexpr int NUM_BARRIERS = 2 * (A_STAGES + B_STAGES + CODE_STAGES) + 8;
+  static constexpr int B_BASE = A_STAGES * A_BYTES;
+  static constexpr int CODE_BASE = B_BASE + B_STAGES * B_BYTES;
+  static constexpr int SCALE_BASE = CODE_BASE + CODE_STAGES * CODE_BYTES;
+  static constexpr int BAR_BASE = SCALE_BASE + 2 * SCALE_BATCH * SCALE_BYTES;
+  static constexpr int SMEM_BYTES = BAR_BASE + NUM_BARRIERS * 8 + 16 + 1024;
+  static constexpr int EXPAND_WARPS = 16;
+  static constexpr int GROUPS = 4;                   // of the expanding warps, each on a stage of its own
+  static constexpr int GROUP_WARPS = EXPAND_WARPS / GROUPS;
+  static_assert(GROUPS <= B_STAGES && GROUPS <= SCALE_BATCH && EXPAND_WARPS % GROUPS == 0, "a group moves on by less than a ring");
+  static constexpr int THREADS = (7 + EXPAND_WARPS) * 32;
+  static_assert(CODE_BASE % 1024 == 0 && CODE_BYTES % 1024 == 0 && BAR_BASE % 8 == 0 && SMEM_BYTES <= 227 * 1024, "shared memory");
 };
 
 struct InputGradParams {
-  const uint8_t* codes;   // [N, K/2]
   const uint8_t* scales;  // [N, K/32], pitch ld_scales
   __nv_bfloat16* dx;
   long long ld_scales, ldd;
   int M, N, K, tiles_m, tiles_k, group_k;
+  int scale_words;  // four scales of a row are an aligned word (K % 128 == 0)
   int* status;
 };
 
@@ -78,6 +95,24 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64
         : "memory");
 }
 
+// Arrival on the leader's barrier for operand bytes that lie in THIS CTA's shared memory: the pair's MMA reads them through this SM's own tensor
+// core, so the stores have to be complete here before the signal leaves (every writer has executed fence.proxy.async, the warp has met), which a
+// release at CTA scope orders. At cluster scope the release waits for a round trip through the memory system, about 2 us a stage under
+// load: 8192 x 4096 x 4096 275 against 208 us.
+__device__ __forceinline__ void mbar_arrive_own_operand(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// The barrier at this offset in every CTA of the pair completes once the MMAs issued so far have.
+template <int CG>
+__device__ __forceinline__ void tc_commit_all(uint32_t bar) {
+  if constexpr (CG == 1)
+    tc_commit<1>(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(uint16_t(3))
+                 : "memory");
+}
+
 // 2^(s - 127) twice as a bf16 pair; exact for every E8M0 value (2^-127 is a bf16 subnormal), NaN for 255.
 __device__ __forceinline__ uint32_t e8m0_bf16x2(uint32_t s) {
   const uint32_t h = s == 255u ? 0x7fffu : s == 0u ? 0x0040u : s << 7;
@@ -102,9 +137,8 @@ __device__ __forceinline__ void expand4(uint32_t w, uint32_t scale, uint32_t& lo
 
 template <int CG>
 __global__ void __launch_bounds__(InputGradCfg<CG>::THREADS, 1)
-input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const InputGradParams p) {
+input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_codes, const InputGradParams p) {
   using Cfg = InputGradCfg<CG>;
-  constexpr int STAGES = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -112,25 +146,42 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const InputGradPara
   const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
   const bool leader = rank == 0;
 
-  const uint32_t bar_base = smem_base + STAGES * Cfg::STAGE_BYTES;
+  const uint32_t bar_base = smem_base + Cfg::BAR_BASE;
   auto a_full = [&](int s) { return bar_base + 8u * s; };
-  auto b_full = [&](int s) { return bar_base + 8u * (STAGES + s); };
-  auto empty_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };
-  auto acc_full = [&](int s) { return bar_base + 8u * (3 * STAGES + s); };
-  auto acc_empty = [&](int s) { return bar_base + 8u * (3 * STAGES + 2 + s); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + STAGES * Cfg::STAGE_BYTES + Cfg::NUM_BARRIERS * 8);
+  auto a_empty = [&](int s) { return bar_base + 8u * (Cfg::A_STAGES + s); };
+  constexpr int B0 = 2 * Cfg::A_STAGES, C0 = B0 + 2 * Cfg::B_STAGES, D0 = C0 + 2 * Cfg::CODE_STAGES;
+  auto b_full = [&](int s) { return bar_base + 8u * (B0 + s); };
+  auto b_empty = [&](int s) { return bar_base + 8u * (B0 + Cfg::B_STAGES + s); };
+  auto code_full = [&](int s) { return bar_base + 8u * (C0 + s); };
+  auto code_empty = [&](int s) { return bar_base + 8u * (C0 + Cfg::CODE_STAGES + s); };
+  auto acc_full = [&](int s) { return bar_base + 8u * (D0 + s); };
+  auto acc_empty = [&](int s) { return bar_base + 8u * (D0 + 2 + s); };
+  auto scale_full = [&](int s) { return bar_base + 8u * (D0 + 4 + s); };
+  auto scale_empty = [&](int s) { return bar_base + 8u * (D0 + 6 + s); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + Cfg::BAR_BASE + Cfg::NUM_BARRIERS * 8);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   WaitCtx ctx{abort_flag, p.status};
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < Cfg::A_STAGES; ++s) {
       mbar_init(a_full(s), 1);
-      mbar_init(b_full(s), Cfg::EXPAND_WARPS * CG);
-      mbar_init(empty_bar(s), 1);
+      mbar_init(a_empty(s), 1);
+    }
+    for (int s = 0; s < Cfg::B_STAGES; ++s) {
+      mbar_init(b_full(s), Cfg::GROUP_WARPS * CG);
+      mbar_init(b_empty(s), 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(acc_full(s), 1);
       mbar_init(acc_empty(s), 4 * CG);
+    }
+    for (int s = 0; s < Cfg::CODE_STAGES; ++s) {
+      mbar_init(code_full(s), 1);
+      mbar_init(code_empty(s), Cfg::GROUP_WARPS);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(scale_full(s), 1);
+      mbar_init(scale_empty(s), Cfg::EXPAND_WARPS);
     }
     *abort_flag = 0u;
     fence_mbar_init();
@@ -139,7 +190,10 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const InputGradPara
     tmem_alloc<CG>(smem_u32(tmem_slot), Cfg::TMEM_COLS);
     tmem_relinquish<CG>();
   }
-  if (warp == 0 && lane == 0) prefetch_tensormap(&map_g);
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&map_g);
+    prefetch_tensormap(&map_codes);
+  }
   tc_fence_before_sync();
   __syncthreads();
   if constexpr (CG == 2) {
@@ -163,55 +217,58 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const InputGradPara
   };
 
   if (warp == 0) {
-    uint32_t stage = 0, phase = 0;
+    uint32_t stage = 0, phase = 0, cs = 0, cphase = 0;
     for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
       int mt, kt;
       tile_at(tile, mt, kt);
       const int row = (mt * CG + int(rank)) * Cfg::BM;
+      const int col = kt * Cfg::TILE_K + int(rank) * Cfg::COLS;
       for (int s = 0; s < steps; ++s) {
-        if (!mbar_wait(empty_bar(stage), phase ^ 1u, ctx, WB_DEV_TIMEOUT_PRODUCER)) continue;  // given up: nothing more is issued
+        if (!mbar_wait(code_empty(cs), cphase ^ 1u, ctx, WB_DEV_TIMEOUT_PRODUCER)) continue;  // given up: nothing more is issued
+        if (elect_one()) {
+          mbar_expect_tx(code_full(cs), Cfg::CODE_BYTES);
+          tma_load_2d<CG>(smem_base + Cfg::CODE_BASE + cs * Cfg::CODE_BYTES, &map_codes, col / 2, s * Cfg::BN, code_full(cs));
+        }
+        __syncwarp();
+        if (++cs == Cfg::CODE_STAGES) { cs = 0; cphase ^= 1u; }
+        if (!mbar_wait(a_empty(stage), phase ^ 1u, ctx, WB_DEV_TIMEOUT_PRODUCER)) continue;
         const uint32_t bar = CG == 2 ? mapa_shared(a_full(stage), 0) : a_full(stage);
         if (elect_one()) {
           if (leader) mbar_expect_tx(a_full(stage), Cfg::A_BYTES * CG);
-          tma_load_2d<CG>(smem_base + stage * Cfg::STAGE_BYTES, &map_g, s * Cfg::BN, row, bar);
+          tma_load_2d<CG>(smem_base + stage * Cfg::A_BYTES, &map_g, s * Cfg::BN, row, bar);
         }
         __syncwarp();
-        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        if (++stage == Cfg::A_STAGES) { stage = 0; phase ^= 1u; }
       }
     }
     pdl_launch_dependents();
   } else if (warp == 1) {
     if (leader) {
       const uint32_t idesc = make_idesc_bf16_bt(Cfg::BM * CG, Cfg::TILE_K);
-      const uint32_t peer_empty = CG == 2 ? mapa_shared(empty_bar(0), 1) : 0u;
-      const uint32_t peer_acc_full = CG == 2 ? mapa_shared(acc_full(0), 1) : 0u;
-      uint32_t stage = 0, phase = 0;
+      uint32_t as = 0, aphase = 0, bs = 0, bphase = 0;
       int it = 0;
       for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++it) {
-        const int as = it & 1;
-        if (it >= 2) mbar_wait<CG == 2>(acc_empty(as), uint32_t((it - 2) >> 1) & 1u, ctx, WB_DEV_TIMEOUT_MMA_ACC);
+        const int acc = it & 1;
+        if (it >= 2) mbar_wait<CG == 2>(acc_empty(acc), uint32_t((it - 2) >> 1) & 1u, ctx, WB_DEV_TIMEOUT_MMA_ACC);
         tc_fence_after_sync();
-        const uint32_t d = tmem_base + as * Cfg::TILE_K;
+        const uint32_t d = tmem_base + acc * Cfg::TILE_K;
         for (int s = 0; s < steps; ++s) {
-          mbar_wait(a_full(stage), phase, ctx, WB_DEV_TIMEOUT_MMA_FULL);
-          mbar_wait<CG == 2>(b_full(stage), phase, ctx, WB_DEV_TIMEOUT_MMA_FULL);
+          mbar_wait(a_full(as), aphase, ctx, WB_DEV_TIMEOUT_MMA_FULL);
+          mbar_wait<CG == 2>(b_full(bs), bphase, ctx, WB_DEV_TIMEOUT_MMA_FULL);
           tc_fence_after_sync();
-          const uint32_t sA = smem_base + stage * Cfg::STAGE_BYTES;
-          const uint64_t a_desc = make_desc_k_sw128(sA);
-          const uint64_t b_desc = make_desc_mn_sw128(sA + Cfg::A_BYTES, Cfg::BN * 128);
+          const uint64_t a_desc = make_desc_k_sw128(smem_base + as * Cfg::A_BYTES);
+          const uint64_t b_desc = make_desc_mn_sw128(smem_base + Cfg::B_BASE + bs * Cfg::B_BYTES, Cfg::BN * 128);
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < Cfg::BN / 16; ++k)  // 16 n: 32 bytes along A's rows, two groups of eight rows of B
               mma_f16<CG>(d, a_desc + uint64_t(k * 2), b_desc + uint64_t(k * (2048 >> 4)), idesc, (s > 0 || k > 0) ? 1u : 0u);
-            tc_commit<CG>(empty_bar(stage));
-            if constexpr (CG == 2) tc_commit<CG>(peer_empty + 8u * stage);
-            if (s == steps - 1) {
-              tc_commit<CG>(acc_full(as));
-              if constexpr (CG == 2) tc_commit<CG>(peer_acc_full + 8u * as);
-            }
+            tc_commit_all<CG>(b_empty(bs));
+            tc_commit_all<CG>(a_empty(as));
+            if (s == steps - 1) tc_commit_all<CG>(acc_full(acc));
           }
           __syncwarp();
-          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          if (++as == Cfg::A_STAGES) { as = 0; aphase ^= 1u; }
+          if (++bs == Cfg::B_STAGES) { bs = 0; bphase ^= 1u; }
         }
       }
     }
@@ -245,65 +302,109 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const InputGradPara
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CG == 2) mbar_arrive_cluster(mapa_shared(acc_empty(as), 0));
+        if constexpr (CG == 2) mbar_arrive_cluster_relaxed(mapa_shared(acc_empty(as), 0));  // publishes no data: the reads are complete
         else mbar_arrive(acc_empty(as));
       }
     }
-  } else {
-    // a thread's 32 codes: row n of the stage, block of 32 columns
-    const int id = (warp - 6) * 32 + lane;
-    const int n = (id & 7) + 8 * (id >> 5), blk = (id >> 3) & 3;
-    const uint32_t row_at = uint32_t((blk >> 1) * (Cfg::BN * 128) + n * 128);
-    const uint32_t chunk0 = uint32_t((blk & 1) * 4), flip = uint32_t(n & 7);
-    uint32_t stage = 0, phase = 0;
-    int tile = first_tile, s = 0;  // of the next load
-    uint4 codes[3];
-    uint32_t scale[3];
-    int col = 0;
-    auto fetch = [&](uint4& c, uint32_t& e) {
-      c = make_uint4(0u, 0u, 0u, 0u);
-      e = 127u;
-      if (tile >= num_tiles) return;
-      if (s == 0) {
-        int mt, kt;
-        tile_at(tile, mt, kt);
-        col = kt * Cfg::TILE_K + int(rank) * Cfg::COLS + blk * 32;
-      }
-      const int row = s * Cfg::BN + n;
-      if (row < p.N && col < p.K) {
-        c = *reinterpret_cast<const uint4*>(p.codes + (long long)row * (p.K / 2) + col / 2);
-        e = p.scales[row * p.ld_scales + col / 32];
-      }
-      if (++s == steps) { s = 0; tile += tile_step; }
-    };
+  } else if (warp < 6 + Cfg::EXPAND_WARPS) {
+    // 32 codes at a time: row n of the stage, block of 32 columns. Eight lanes of neighbouring n read and write at a time: the swizzles (64 bytes
+    // of the codes, 128 of the operand) put their 16-byte pieces into different banks. A stage is a chain of waits, so that the warps work
+    // in groups, each on every GROUPS-th stage.
+    const int group = (warp - 6) / Cfg::GROUP_WARPS;
+    const int id0 = ((warp - 6) % Cfg::GROUP_WARPS) * 32 + lane;
     const int my_tiles = first_tile < num_tiles ? (num_tiles - first_tile + tile_step - 1) / tile_step : 0;
     const long long total = (long long)my_tiles * steps;
+    uint32_t stage = group, phase = 0;
+    for (long long i = group; i < total; i += Cfg::GROUPS) {
+      const int at = int(i & (2 * Cfg::SCALE_BATCH - 1)), half = at / Cfg::SCALE_BATCH, in_batch = at & (Cfg::SCALE_BATCH - 1);
+      const int cs = int(i % Cfg::CODE_STAGES);
+      if (in_batch < Cfg::GROUPS) mbar_wait(scale_full(half), uint32_t(i / (2 * Cfg::SCALE_BATCH)) & 1u, ctx, WB_DEV_TIMEOUT_MMA_FULL);
+      mbar_wait(code_full(cs), uint32_t(i / Cfg::CODE_STAGES) & 1u, ctx, WB_DEV_TIMEOUT_MMA_FULL);
+      constexpr int ITEMS = Cfg::BN * 4 / (Cfg::GROUP_WARPS * 32);
+      uint32_t v[ITEMS][16];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) fetch(codes[i], scale[i]);
-    for (long long i = 0; i < total; ++i) {
-      const uint4 c = codes[0];
-      const uint32_t f = e8m0_bf16x2(scale[0]);
-      codes[0] = codes[1]; scale[0] = scale[1];
-      codes[1] = codes[2]; scale[1] = scale[2];
-      fetch(codes[2], scale[2]);
-      mbar_wait(empty_bar(stage), phase ^ 1u, ctx, WB_DEV_TIMEOUT_PRODUCER);
-      const uint32_t sB = smem_base + stage * Cfg::STAGE_BYTES + Cfg::A_BYTES + row_at;
-      const uint32_t word[4] = {c.x, c.y, c.z, c.w};
+      for (int u = 0; u < ITEMS; ++u) {
+        const int id = id0 + u * Cfg::GROUP_WARPS * 32;
+        const int n = (id & 7) + 8 * (id >> 5), blk = (id >> 3) & 3;
+        uint32_t word[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(word[0]), "=r"(word[1]), "=r"(word[2]), "=r"(word[3])
+                     : "r"(smem_base + Cfg::CODE_BASE + cs * Cfg::CODE_BYTES + n * 64 + ((blk ^ ((n >> 1) & 3)) << 4)));
+        const uint32_t f = e8m0_bf16x2(smem_gen[Cfg::SCALE_BASE + at * Cfg::SCALE_BYTES + n * 4 + blk]);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t v[4];
-        expand4(word[q], f, v[0], v[1]);
-        expand4(word[q] >> 16, f, v[2], v[3]);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sB + (((chunk0 + q) ^ flip) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
-                     : "memory");
+        for (int q = 0; q < 4; ++q) {
+          expand4(word[q], f, v[u][4 * q], v[u][4 * q + 1]);
+          expand4(word[q] >> 16, f, v[u][4 * q + 2], v[u][4 * q + 3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(code_empty(cs));
+        if (in_batch >= Cfg::SCALE_BATCH - Cfg::GROUPS) mbar_arrive(scale_empty(half));
+      }
+      mbar_wait(b_empty(stage), phase ^ 1u, ctx, WB_DEV_TIMEOUT_PRODUCER);  // only now: a stage is held for the stores alone
+#pragma unroll
+      for (int u = 0; u < ITEMS; ++u) {
+        const int id = id0 + u * Cfg::GROUP_WARPS * 32;
+        const int n = (id & 7) + 8 * (id >> 5), blk = (id >> 3) & 3;
+        const uint32_t to = smem_base + Cfg::B_BASE + stage * Cfg::B_BYTES + (blk >> 1) * (Cfg::BN * 128) + n * 128;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((((blk & 1) * 4 + q) ^ (n & 7)) << 4)), "r"(v[u][4 * q]),
+                       "r"(v[u][4 * q + 1]), "r"(v[u][4 * q + 2]), "r"(v[u][4 * q + 3])
+                       : "memory");
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CG == 2) mbar_arrive_cluster(mapa_shared(b_full(stage), 0));
+        if constexpr (CG == 2) mbar_arrive_own_operand(mapa_shared(b_full(stage), 0));
         else mbar_arrive(b_full(stage));
       }
-      if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+      stage += Cfg::GROUPS;
+      if (stage >= Cfg::B_STAGES) { stage -= Cfg::B_STAGES; phase ^= 1u; }
+    }
+  } else {
+    // scales of rows `lane` and `lane + 32` of a stage, four to a row: the loads of a batch of stages are in flight together, while the batch before
+    // is being read
+    const int my_tiles = first_tile < num_tiles ? (num_tiles - first_tile + tile_step - 1) / tile_step : 0;
+    const long long total = (long long)my_tiles * steps;
+    int tile = first_tile, s = 0, col = 0;
+    for (long long i = 0; i < total; i += Cfg::SCALE_BATCH) {
+      uint32_t word[Cfg::SCALE_BATCH][2];
+#pragma unroll
+      for (int j = 0; j < Cfg::SCALE_BATCH; ++j) {
+        if (s == 0 && i + j < total) {
+          int mt, kt;
+          tile_at(tile, mt, kt);
+          col = (kt * Cfg::TILE_K + int(rank) * Cfg::COLS) / 32;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = s * Cfg::BN + lane + 32 * h;
+          const bool real = i + j < total && row < p.N;
+          const uint8_t* at = p.scales + row * p.ld_scales + col;
+          word[j][h] = 0x7f7f7f7fu;
+          if (p.scale_words) {
+            if (real && col * 32 < p.K) word[j][h] = *reinterpret_cast<const uint32_t*>(at);
+          } else {
+            uint32_t w = 0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) w |= uint32_t(real && (col + b) * 32 < p.K ? at[b] : 0x7fu) << (8 * b);
+            word[j][h] = w;
+          }
+        }
+        if (++s == steps) { s = 0; tile += tile_step; }
+      }
+      const int half = int(i / Cfg::SCALE_BATCH) & 1;
+      mbar_wait(scale_empty(half), (uint32_t(i / (2 * Cfg::SCALE_BATCH)) & 1u) ^ 1u, ctx, WB_DEV_TIMEOUT_PRODUCER);
+      uint32_t* dst = reinterpret_cast<uint32_t*>(smem_gen + Cfg::SCALE_BASE + half * Cfg::SCALE_BATCH * Cfg::SCALE_BYTES);
+#pragma unroll
+      for (int j = 0; j < Cfg::SCALE_BATCH; ++j) {
+        dst[j * Cfg::BN + lane] = word[j][0];
+        dst[j * Cfg::BN + lane + 32] = word[j][1];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(scale_full(half));
     }
   }
 

@@ -32,7 +32,7 @@ struct RouterParams {
   float* part_p;         // [CTAs][E]
   int* part_n;           // [CTAs][E + 1]: counts, rows
   int* counts;           // [E]
-  int* tokens;           // rows that are not masked
+  float* unit;           // E / (k n^2): what a count adds to the gradient of p; 0 where no row counts
   float* loss;
 };
 
@@ -80,31 +80,56 @@ __device__ __forceinline__ float softmax_row(const T* row, int E, int lane, floa
   return 1.f / warp_sum(sum);
 }
 
-// What the partial sums become; E threads at least.
-__device__ __forceinline__ void router_finish(const RouterParams& p, int ctas, double* share) {
-  int n = 0;
-  for (int c = 0; c < ctas; ++c) n += p.part_n[c * (p.E + 1) + p.E];
-  double mine = 0.0;
-  const int e = threadIdx.x;
-  if (e < p.E) {
-    double sum = 0.0;
-    int count = 0;
-    for (int c = 0; c < ctas; ++c) {
+// What the partial sums become, by a CTA: thread (e, q) of THREADS / EP slices adds up every so-manieth CTA's sums of expert e, then the
+// slices are added in order.
+template <int THREADS>
+__device__ __forceinline__ void router_finish(const RouterParams& p, int ctas, double (*sums)[THREADS], int (*counts)[THREADS]) {
+  const int EP = (p.E + 31) / 32 * 32, slices = THREADS / EP;
+  const int e = threadIdx.x % EP, q = threadIdx.x / EP;
+  double sum = 0.0;
+  int count = 0;
+  if (q < slices && e < p.E) {
+#pragma unroll 8
+    for (int c = q; c < ctas; c += slices) {
       sum += p.part_p[c * p.E + e];
       count += p.part_n[c * (p.E + 1) + e];
     }
-    p.counts[e] = count;
+  }
+  int n = 0;
+  for (int c = threadIdx.x; c < ctas; c += THREADS) n += p.part_n[c * (p.E + 1) + p.E];
+  (*sums)[threadIdx.x] = sum;
+  (*counts)[threadIdx.x] = count;
+  __syncthreads();
+  double mine = 0.0;
+  if (threadIdx.x < p.E) {
+    for (int i = 1; i < slices; ++i) {
+      sum += (*sums)[i * EP + threadIdx.x];
+      count += (*counts)[i * EP + threadIdx.x];
+    }
+    p.counts[threadIdx.x] = count;
     mine = sum * count;
   }
+  __syncthreads();
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if ((threadIdx.x & 31) == 0) share[threadIdx.x >> 5] = mine;
+  for (int o = 16; o > 0; o >>= 1) {
+    mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    n += __shfl_xor_sync(0xffffffffu, n, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    (*sums)[threadIdx.x >> 5] = mine;
+    (*counts)[threadIdx.x >> 5] = n;
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
     double total = 0.0;
-    for (int w = 0; w < kRouterWarps; ++w) total += share[w];
-    *p.tokens = n;
-    *p.loss = n > 0 ? float(total * p.E / (double(p.top_k) * n * n)) : 0.f;
+    n = 0;
+    for (int w = 0; w < THREADS / 32; ++w) {
+      total += (*sums)[w];
+      n += (*counts)[w];
+    }
+    const double unit = n > 0 ? p.E / (double(p.top_k) * n * n) : 0.0;
+    *p.unit = float(unit);
+    *p.loss = float(total * unit);
   }
 }
 
@@ -113,7 +138,8 @@ __global__ void __launch_bounds__(kRouterWarps * 32)
 router_kernel(const RouterParams p) {
   __shared__ float sum_p[kRouterWarps][EV * 32];
   __shared__ int sum_n[EV * 32 + 1];
-  __shared__ double share[kRouterWarps];
+  __shared__ double sums[kRouterWarps * 32];
+  __shared__ int counts[kRouterWarps * 32];
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -189,15 +215,16 @@ router_kernel(const RouterParams p) {
   if (threadIdx.x == 0) p.part_n[blockIdx.x * (p.E + 1) + p.E] = sum_n[EV * 32];
   if (gridDim.x == 1) {
     __syncthreads();
-    router_finish(p, 1, share);
+    router_finish<kRouterWarps * 32>(p, 1, &sums, &counts);
   }
 }
 
-__global__ void __launch_bounds__(kRouterWarps * 32) router_finish_kernel(const RouterParams p, int ctas) {
-  __shared__ double share[kRouterWarps];
+__global__ void __launch_bounds__(1024) router_finish_kernel(const RouterParams p, int ctas) {
+  __shared__ double sums[1024];
+  __shared__ int counts[1024];
   pdl_launch_dependents();
   pdl_wait();
-  router_finish(p, ctas, share);
+  router_finish<1024>(p, ctas, &sums, &counts);
 }
 
 struct RouterGradParams {
@@ -207,7 +234,7 @@ struct RouterGradParams {
   const float* g_weight;   // [rows, top_k], or null
   const float* g_loss;     // device scalar, or null
   const int* counts;
-  const int* tokens;
+  const float* unit;
   void* g_logits;          // [rows, E], pitch ldg
   long long ld, ldg;
   int rows, E, top_k, renormalize;
@@ -219,8 +246,7 @@ router_grad_kernel(const RouterGradParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = *p.tokens;
-  const float unit = p.g_loss && n > 0 ? float(double(*p.g_loss) * p.E / (double(p.top_k) * n * n)) : 0.f;
+  const float unit = p.g_loss ? *p.g_loss * *p.unit : 0.f;
   float loss_dp[EV];
 #pragma unroll
   for (int i = 0; i < EV; ++i) loss_dp[i] = lane + 32 * i < p.E ? unit * p.counts[lane + 32 * i] : 0.f;

@@ -208,7 +208,7 @@ def _run_router(logits, mask, top_k, renormalize, given):
     dev = logits.device
     nbytes = int(lib.wb200_router_workspace_bytes(rows, E))
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    small = torch.empty(1 + E + nbytes // 4, dtype=torch.int32, device=dev)  # tokens, counts, then the partial sums
+    small = torch.empty(1 + E + nbytes // 4, dtype=torch.int32, device=dev)  # unit, counts, then the partial sums
     weight = ids = None
     if given is None:
         weight = torch.empty(rows, top_k, dtype=torch.float32, device=dev)
@@ -220,10 +220,10 @@ def _run_router(logits, mask, top_k, renormalize, given):
                                     int(given is not None and given.dtype == torch.int64), int(renormalize),
                                     weight.data_ptr() if weight is not None else None, ids.data_ptr() if ids is not None else None, base + 4,
                                     base, loss.data_ptr(), base + 4 * (1 + E), nbytes, _stream()))
-    return weight, ids, small[1:1 + E], loss, small[:1]
+    return weight, ids, small[1:1 + E], loss, small[:1].view(torch.float32)
 
 
-def _run_router_grad(logits, mask, top_k, renormalize, ids, g_weight, g_loss, counts, tokens):
+def _run_router_grad(logits, mask, top_k, renormalize, ids, g_weight, g_loss, counts, unit):
     lib = _lib.load()
     rows, E = logits.shape
     grad = torch.empty(rows, E, dtype=logits.dtype, device=logits.device)
@@ -231,15 +231,15 @@ def _run_router_grad(logits, mask, top_k, renormalize, ids, g_weight, g_loss, co
         _lib.check(lib.wb200_router_grad(rows, E, top_k, logits.data_ptr(), ops._DTYPE_CODE[logits.dtype], logits.stride(0) if rows > 1 else E,
                                          mask.data_ptr() if mask is not None else None, ids.data_ptr() if ids is not None else None,
                                          g_weight.data_ptr() if g_weight is not None else None, g_loss.data_ptr() if g_loss is not None else None,
-                                         int(renormalize), counts.data_ptr(), tokens.data_ptr(), grad.data_ptr(), E, _stream()))
+                                         int(renormalize), counts.data_ptr(), unit.data_ptr(), grad.data_ptr(), E, _stream()))
     return grad
 
 
 class _Router(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, mask, top_k, renormalize):
-        weight, ids, counts, loss, tokens = _run_router(logits, mask, top_k, renormalize, None)
-        ctx.save_for_backward(logits, mask, ids, counts, tokens)
+        weight, ids, counts, loss, unit = _run_router(logits, mask, top_k, renormalize, None)
+        ctx.save_for_backward(logits, mask, ids, counts, unit)
         ctx.options = top_k, renormalize
         ctx.mark_non_differentiable(ids, counts)
         ctx.set_materialize_grads(False)
@@ -248,19 +248,19 @@ class _Router(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_weight, _ids, _counts, g_loss):
-        logits, mask, ids, counts, tokens = ctx.saved_tensors
+        logits, mask, ids, counts, unit = ctx.saved_tensors
         top_k, renormalize = ctx.options
         if g_weight is None and g_loss is None:
             return None, None, None, None
         g_weight = g_weight.contiguous() if g_weight is not None else None
-        return _run_router_grad(logits, mask, top_k, renormalize, ids, g_weight, g_loss, counts, tokens), None, None, None
+        return _run_router_grad(logits, mask, top_k, renormalize, ids, g_weight, g_loss, counts, unit), None, None, None
 
 
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, mask, ids):
-        _, _, counts, loss, tokens = _run_router(logits, mask, ids.shape[1], False, ids)
-        ctx.save_for_backward(logits, mask, counts, tokens)
+        _, _, counts, loss, unit = _run_router(logits, mask, ids.shape[1], False, ids)
+        ctx.save_for_backward(logits, mask, counts, unit)
         ctx.top_k = ids.shape[1]
         ctx.mark_non_differentiable(counts)
         return loss, counts
@@ -268,8 +268,8 @@ class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, _counts):
-        logits, mask, counts, tokens = ctx.saved_tensors
-        return _run_router_grad(logits, mask, ctx.top_k, False, None, None, g_loss, counts, tokens), None, None
+        logits, mask, counts, unit = ctx.saved_tensors
+        return _run_router_grad(logits, mask, ctx.top_k, False, None, None, g_loss, counts, unit), None, None
 
 
 def router(logits: torch.Tensor, top_k: int, mask: torch.Tensor | None = None, renormalize: bool = False) -> Routing:
