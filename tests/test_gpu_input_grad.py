@@ -54,7 +54,8 @@ def test_large_tiles(M, N, K):
     check(*make(M, N, K, seed=1))
 
 
-@pytest.mark.parametrize("M,N,K", [(600, 4000, 2048), (16, 14336, 4096), (1, 8192, 1024), (333, 2048, 96)])
+@pytest.mark.parametrize("M,N,K", [(600, 4000, 2048), (16, 14336, 4096), (1, 8192, 1024), (333, 2048, 96), (128, 4096, 4096), (1024, 8192, 1024), (16, 8192, 512),
+                                   (100, 8200, 2560), (250, 4096, 4064), (130, 700, 2048)])
 def test_few_tiles_and_long_sums(M, N, K):
     check(*make(M, N, K, seed=2))
 

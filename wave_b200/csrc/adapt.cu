@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <iterator>
+#include <mutex>
 
 #include "adapters.cuh"
 #include "input_grad_sm100.cuh"
@@ -175,36 +177,91 @@ int run_outer(const __nv_bfloat16* z, long long ldz, const float* hidden, int co
 // ------------------------------------------------------------------------------------------
 // input gradient
 // ------------------------------------------------------------------------------------------
+// CTAs to a tile (1: 128 x 128, a pair: 256 x 256) and slices of the sum over N (a cluster of cg * slices CTAs to a tile).
+struct InputGradLayout {
+  int cg, slices;
+};
+constexpr InputGradLayout kInputGradLayouts[] = {{2, 1}, {1, 1}, {2, 2}, {1, 2}, {2, 3}, {1, 3}, {2, 4}, {1, 4}, {1, 6}, {1, 8}};
+
+template <int CG>
+int input_grad_config(int slices, cudaStream_t stream, cudaLaunchConfig_t* cfg, cudaLaunchAttribute (&attr)[2]) {
+  using Cfg = wb::InputGradCfg<CG>;
+  static bool done[wbhost::kMaxDevices] = {};
+  int dev = 0;
+  WB_HOST_CUDA(cudaGetDevice(&dev));
+  if (!done[dev]) {
+    WB_HOST_CUDA(cudaFuncSetAttribute(wb::input_grad_kernel<CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+    done[dev] = true;
+  }
+  *cfg = {};
+  cfg->gridDim = dim3(CG * slices, 1, 1);
+  cfg->blockDim = dim3(Cfg::THREADS, 1, 1);
+  cfg->dynamicSmemBytes = Cfg::SMEM_BYTES;
+  cfg->stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG * slices;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg->attrs = attr;
+  cfg->numAttrs = 2;
+  return WB200_OK;
+}
+
+// How many clusters of every layout run at one time on the current device.
+int input_grad_resident(const int** out) {
+  static int resident[wbhost::kMaxDevices][std::size(kInputGradLayouts)] = {};
+  static std::mutex mu;
+  int dev = 0;
+  WB_HOST_CUDA(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lk(mu);
+  if (!resident[dev][0])
+    for (int i = int(std::size(kInputGradLayouts)) - 1; i >= 0; --i) {
+      cudaLaunchConfig_t cfg;
+      cudaLaunchAttribute attr[2];
+      const InputGradLayout l = kInputGradLayouts[i];
+      if (int rc = l.cg == 2 ? input_grad_config<2>(l.slices, nullptr, &cfg, attr) : input_grad_config<1>(l.slices, nullptr, &cfg, attr)) return rc;
+      int n = 0;
+      cfg.numAttrs = 1;
+      WB_HOST_CUDA(l.cg == 2 ? cudaOccupancyMaxActiveClusters(&n, wb::input_grad_kernel<2>, &cfg) : cudaOccupancyMaxActiveClusters(&n, wb::input_grad_kernel<1>, &cfg));
+      resident[dev][i] = n > 0 ? n : -1;
+    }
+  *out = resident[dev];
+  return WB200_OK;
+}
+
+// The layout of least estimated time. Measured (us): a step of 64 N takes 0.42 with either tile, a launch 4 on top of its steps, and each round
+// of sliced tiles 10.5, for filling the ring, reading the accumulators and adding them up. 16 x 14336 x 4096: one CTA a tile 88, four slices
+// 30; 600 x 4000 x 2048: pairs 31, two slices 25; 2048^3: pairs 21, two slices 38.
+int input_grad_layout(int M, int N, int K, InputGradLayout* best) {
+  const int* resident;
+  if (int rc = input_grad_resident(&resident)) return rc;
+  const int steps = div_up(N, 64);
+  double least = 1e30;
+  for (size_t i = 0; i < std::size(kInputGradLayouts); ++i) {
+    const InputGradLayout l = kInputGradLayouts[i];
+    if (l.slices > steps || resident[i] <= 0) continue;
+    const long long tiles = (long long)div_up(M, 128 * l.cg) * div_up(K, 128 * l.cg);
+    const double rounds = div_up(tiles, resident[i]);
+    const double us = l.slices == 1 ? rounds * steps * 0.42 + 4 : rounds * (div_up(steps, l.slices) * 0.42 + 10.5);
+    if (us < least) { least = us; *best = l; }
+  }
+  return WB200_OK;
+}
+
 template <int CG>
 int launch_input_grad(const CUtensorMap& map, const CUtensorMap& codes, wb::InputGradParams p, int sms, cudaStream_t stream) {
   using Cfg = wb::InputGradCfg<CG>;
   p.tiles_m = div_up(p.M, Cfg::BM * CG);
   p.tiles_k = div_up(p.K, Cfg::TILE_K);
   p.group_k = std::min(8, p.tiles_k);
-  auto kernel = wb::input_grad_kernel<CG>;
-  static bool done[wbhost::kMaxDevices] = {};
-  int dev = 0;
-  WB_HOST_CUDA(cudaGetDevice(&dev));
-  if (!done[dev]) {
-    WB_HOST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
-    done[dev] = true;
-  }
-  const long long tiles = (long long)p.tiles_m * p.tiles_k;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(std::min<long long>(tiles, sms / CG)) * CG, 1, 1);
-  cfg.blockDim = dim3(Cfg::THREADS, 1, 1);
-  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
-  cfg.stream = stream;
+  cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  WB_HOST_CUDA(cudaLaunchKernelEx(&cfg, kernel, map, codes, p));
+  if (int rc = input_grad_config<CG>(p.slices, stream, &cfg, attr)) return rc;
+  const long long tiles = (long long)p.tiles_m * p.tiles_k;
+  cfg.gridDim.x = unsigned((p.slices > 1 ? tiles : std::min<long long>(tiles, sms / CG)) * CG * p.slices);
+  WB_HOST_CUDA(cudaLaunchKernelEx(&cfg, wb::input_grad_kernel<CG>, map, codes, p));
   return WB200_OK;
 }
 
@@ -347,8 +404,10 @@ int wb200_mxfp4_input_grad(int M, int N, int K, const void* g, long long ldg, co
   if (int rc = wbhost::tensor_map(&codes, b, K / 2, N, K / 2, 64, 64, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
   if (int rc = wbhost::tensor_map(&map, g, N, M, (unsigned long long)ldg * 2, 64, 128, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const long long pair_tiles = (long long)div_up(M, 256) * div_up(K, 256);
-  return pair_tiles * 2 >= sms / 2 ? launch_input_grad<2>(map, codes, p, sms, s) : launch_input_grad<1>(map, codes, p, sms, s);
+  InputGradLayout layout{2, 1};
+  if (int rc = input_grad_layout(M, N, K, &layout)) return rc;
+  p.slices = layout.slices;
+  return layout.cg == 2 ? launch_input_grad<2>(map, codes, p, sms, s) : launch_input_grad<1>(map, codes, p, sms, s);
 }
 
 size_t wb200_router_workspace_bytes(int rows, int num_experts) {

@@ -17,6 +17,9 @@
 // (fence.proxy.async), and that fence waits for every load that the thread has in flight: with codes prefetched into registers the kernel
 // stood at 480 TFLOP/s, each stage waiting a whole memory latency.
 //
+// With few tiles the sum over N is cut into slices: one cluster of `slices` pairs (or CTAs) to a tile, which then add their f32 accumulators
+// through distributed shared memory, in slice order, each its share of the rows. No workspace, no second launch, the same bits on every run.
+//
 // CG = 2: 256 x 256 tiles, each CTA holds 128 rows of g and expands 128 columns of W; CG = 1: 128 x 128 tiles. Both accumulators of
 // neighbouring tiles are in tensor memory, so an epilogue runs under the next tile's products.
 #pragma once
@@ -38,6 +41,7 @@ struct InputGradCfg {
   static constexpr int SCALE_BYTES = COLS / 32 * BN;
   static constexpr int CODE_STAGES = 6;
   static constexpr int SCALE_BATCH = 8;              // stages whose scales are loaded together; two batches in shared memory
+  static constexpr int SUM_PITCH = TILE_K * 4 + 16;  // rows of f32 accumulators in shared memory; 16 bytes spread the lanes over the banks
   static constexpr int TMEM_COLS = 2 * TILE_K;
   static constexpr int NUM_BARRIERS = 2 * (A_STAGES + B_STAGES + CODE_STAGES) + 8;
   static constexpr int B_BASE = A_STAGES * A_BYTES;
@@ -50,14 +54,14 @@ struct InputGradCfg {
   static constexpr int GROUP_WARPS = EXPAND_WARPS / GROUPS;
   static_assert(GROUPS <= B_STAGES && GROUPS <= SCALE_BATCH && EXPAND_WARPS % GROUPS == 0, "a group moves on by less than a ring");
   static constexpr int THREADS = (7 + EXPAND_WARPS) * 32;
-  static_assert(CODE_BASE % 1024 == 0 && CODE_BYTES % 1024 == 0 && BAR_BASE % 8 == 0 && SMEM_BYTES <= 227 * 1024, "shared memory");
+  static_assert(CODE_BASE % 1024 == 0 && CODE_BYTES % 1024 == 0 && BAR_BASE % 8 == 0 && BM * SUM_PITCH <= CODE_BASE && SMEM_BYTES <= 227 * 1024, "shared memory");
 };
 
 struct InputGradParams {
   const uint8_t* scales;  // [N, K/32], pitch ld_scales
   __nv_bfloat16* dx;
   long long ld_scales, ldd;
-  int M, N, K, tiles_m, tiles_k, group_k;
+  int M, N, K, tiles_m, tiles_k, group_k, slices;
   int scale_words;  // four scales of a row are an aligned word (K % 128 == 0)
   int* status;
 };
@@ -105,11 +109,11 @@ __device__ __forceinline__ void mbar_arrive_own_operand(uint32_t cluster_bar) {
 
 // The barrier at this offset in every CTA of the pair completes once the MMAs issued so far have.
 template <int CG>
-__device__ __forceinline__ void tc_commit_all(uint32_t bar) {
+__device__ __forceinline__ void tc_commit_all(uint32_t bar, uint16_t pair_mask) {
   if constexpr (CG == 1)
     tc_commit<1>(bar);
   else
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(uint16_t(3))
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(pair_mask)
                  : "memory");
 }
 
@@ -135,6 +139,37 @@ __device__ __forceinline__ void expand4(uint32_t w, uint32_t scale, uint32_t& lo
   hi_pair = mul_bf16x2(p1, scale);
 }
 
+// A CTA's share of the rows of a tile, added up over the slices: eight columns a thread, the loads of all slices in flight together.
+template <int CG, int S>
+__device__ __forceinline__ void sum_slices(const InputGradParams& p, uint32_t smem_base, int mt, int kt, int rank, int slice) {
+  using Cfg = InputGradCfg<CG>;
+  const int first = Cfg::BM * slice / S, rows = Cfg::BM * (slice + 1) / S - first;
+  for (int e = threadIdx.x; e < rows * (Cfg::TILE_K / 8); e += Cfg::THREADS) {
+    const int in = first + e / (Cfg::TILE_K / 8), c = e % (Cfg::TILE_K / 8) * 8;
+    const int row = (mt * CG + rank) * Cfg::BM + in, col = kt * Cfg::TILE_K + c;
+    if (row >= p.M || col >= p.K) continue;
+    float v[S][8];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const uint32_t at = mapa_shared(smem_base + uint32_t(in) * Cfg::SUM_PITCH + c * 4, uint32_t(s * CG + rank));
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[s][4 * h]), "=f"(v[s][4 * h + 1]), "=f"(v[s][4 * h + 2]), "=f"(v[s][4 * h + 3])
+                     : "r"(at + 16 * h));
+    }
+    float sum[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      sum[j] = v[0][j];
+#pragma unroll
+      for (int s = 1; s < S; ++s) sum[j] += v[s][j];
+    }
+    *reinterpret_cast<uint4*>(p.dx + (long long)row * p.ldd + col) = make_uint4(pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]),
+                                                                                pack_bf16x2(sum[4], sum[5]), pack_bf16x2(sum[6], sum[7]));
+  }
+}
+
 template <int CG>
 __global__ void __launch_bounds__(InputGradCfg<CG>::THREADS, 1)
 input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_codes, const InputGradParams p) {
@@ -143,8 +178,11 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
+  const uint32_t cluster_rank = (CG == 2 || p.slices > 1) ? cluster_ctarank() : 0u;
+  const uint32_t rank = cluster_rank % CG;         // in the pair
+  const uint32_t leader_rank = cluster_rank - rank;  // of the pair's leader in the cluster
   const bool leader = rank == 0;
+  const int slice = int(cluster_rank) / CG;
 
   const uint32_t bar_base = smem_base + Cfg::BAR_BASE;
   auto a_full = [&](int s) { return bar_base + 8u * s; };
@@ -196,7 +234,7 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
   }
   tc_fence_before_sync();
   __syncthreads();
-  if constexpr (CG == 2) {
+  if (CG == 2 || p.slices > 1) {
     cluster_arrive();
     cluster_wait();
   }
@@ -205,8 +243,10 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
   pdl_wait();
 
   const int num_tiles = p.tiles_m * p.tiles_k;
-  const int first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
-  const int steps = (p.N + Cfg::BN - 1) / Cfg::BN;
+  const int first_tile = blockIdx.x / (CG * p.slices), tile_step = gridDim.x / (CG * p.slices);  // with slices: one tile per cluster
+  const int all_steps = (p.N + Cfg::BN - 1) / Cfg::BN;
+  const int step0 = int((long long)all_steps * slice / p.slices);
+  const int steps = int((long long)all_steps * (slice + 1) / p.slices) - step0;  // at least one
   // tiles in groups of group_k columns of tiles, each swept down the rows
   auto tile_at = [&](int tile, int& mt, int& kt) {
     const int per = p.group_k * p.tiles_m;
@@ -227,15 +267,15 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
         if (!mbar_wait(code_empty(cs), cphase ^ 1u, ctx, WB_DEV_TIMEOUT_PRODUCER)) continue;  // given up: nothing more is issued
         if (elect_one()) {
           mbar_expect_tx(code_full(cs), Cfg::CODE_BYTES);
-          tma_load_2d<CG>(smem_base + Cfg::CODE_BASE + cs * Cfg::CODE_BYTES, &map_codes, col / 2, s * Cfg::BN, code_full(cs));
+          tma_load_2d<CG>(smem_base + Cfg::CODE_BASE + cs * Cfg::CODE_BYTES, &map_codes, col / 2, (step0 + s) * Cfg::BN, code_full(cs));
         }
         __syncwarp();
         if (++cs == Cfg::CODE_STAGES) { cs = 0; cphase ^= 1u; }
         if (!mbar_wait(a_empty(stage), phase ^ 1u, ctx, WB_DEV_TIMEOUT_PRODUCER)) continue;
-        const uint32_t bar = CG == 2 ? mapa_shared(a_full(stage), 0) : a_full(stage);
+        const uint32_t bar = CG == 2 ? mapa_shared(a_full(stage), leader_rank) : a_full(stage);
         if (elect_one()) {
           if (leader) mbar_expect_tx(a_full(stage), Cfg::A_BYTES * CG);
-          tma_load_2d<CG>(smem_base + stage * Cfg::A_BYTES, &map_g, s * Cfg::BN, row, bar);
+          tma_load_2d<CG>(smem_base + stage * Cfg::A_BYTES, &map_g, (step0 + s) * Cfg::BN, row, bar);
         }
         __syncwarp();
         if (++stage == Cfg::A_STAGES) { stage = 0; phase ^= 1u; }
@@ -245,6 +285,7 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
   } else if (warp == 1) {
     if (leader) {
       const uint32_t idesc = make_idesc_bf16_bt(Cfg::BM * CG, Cfg::TILE_K);
+      const uint16_t pair_mask = uint16_t(3u << leader_rank);
       uint32_t as = 0, aphase = 0, bs = 0, bphase = 0;
       int it = 0;
       for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++it) {
@@ -262,9 +303,9 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
 #pragma unroll
             for (int k = 0; k < Cfg::BN / 16; ++k)  // 16 n: 32 bytes along A's rows, two groups of eight rows of B
               mma_f16<CG>(d, a_desc + uint64_t(k * 2), b_desc + uint64_t(k * (2048 >> 4)), idesc, (s > 0 || k > 0) ? 1u : 0u);
-            tc_commit_all<CG>(b_empty(bs));
-            tc_commit_all<CG>(a_empty(as));
-            if (s == steps - 1) tc_commit_all<CG>(acc_full(acc));
+            tc_commit_all<CG>(b_empty(bs), pair_mask);
+            tc_commit_all<CG>(a_empty(as), pair_mask);
+            if (s == steps - 1) tc_commit_all<CG>(acc_full(acc), pair_mask);
           }
           __syncwarp();
           if (++as == Cfg::A_STAGES) { as = 0; aphase ^= 1u; }
@@ -288,6 +329,14 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
         uint32_t r[32];
         tmem_ld_32x32(tmem_base + (uint32_t(quad * 32) << 16) + as * Cfg::TILE_K + c, r);
         tmem_ld_wait();
+        if (p.slices > 1) {  // into this CTA's shared memory, whose stages are all read
+          const uint32_t at = smem_base + uint32_t(quad * 32 + lane) * Cfg::SUM_PITCH + c * 4;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + 16 * j), "r"(r[4 * j]), "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3])
+                         : "memory");
+          continue;
+        }
         const int col = kt * Cfg::TILE_K + c;
         if (row < p.M && col < p.K) {  // K is a multiple of 32
           uint4* q = reinterpret_cast<uint4*>(dst + col);
@@ -302,7 +351,7 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CG == 2) mbar_arrive_cluster_relaxed(mapa_shared(acc_empty(as), 0));  // publishes no data: the reads are complete
+        if constexpr (CG == 2) mbar_arrive_cluster_relaxed(mapa_shared(acc_empty(as), leader_rank));  // publishes no data: the reads are complete
         else mbar_arrive(acc_empty(as));
       }
     }
@@ -357,7 +406,7 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CG == 2) mbar_arrive_own_operand(mapa_shared(b_full(stage), 0));
+        if constexpr (CG == 2) mbar_arrive_own_operand(mapa_shared(b_full(stage), leader_rank));
         else mbar_arrive(b_full(stage));
       }
       stage += Cfg::GROUPS;
@@ -380,7 +429,7 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int row = s * Cfg::BN + lane + 32 * h;
+          const int row = (step0 + s) * Cfg::BN + lane + 32 * h;
           const bool real = i + j < total && row < p.N;
           const uint8_t* at = p.scales + row * p.ld_scales + col;
           word[j][h] = 0x7f7f7f7fu;
@@ -408,10 +457,28 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
     }
   }
 
+  if (p.slices > 1) {
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    int mt, kt;
+    tile_at(first_tile, mt, kt);
+    switch (p.slices) {
+      case 2: sum_slices<CG, 2>(p, smem_base, mt, kt, int(rank), slice); break;
+      case 3: sum_slices<CG, 3>(p, smem_base, mt, kt, int(rank), slice); break;
+      case 4: sum_slices<CG, 4>(p, smem_base, mt, kt, int(rank), slice); break;
+      default:
+        if constexpr (CG == 1) {
+          if (p.slices == 8) sum_slices<CG, 8>(p, smem_base, mt, kt, int(rank), slice);
+          else sum_slices<CG, 6>(p, smem_base, mt, kt, int(rank), slice);
+        }
+    }
+  }
+
   // nobody leaves while the other CTA's barriers may still be signalled or its operands read
   tc_fence_before_sync();
   __syncthreads();
-  if constexpr (CG == 2) {
+  if (CG == 2 || p.slices > 1) {
     cluster_arrive();
     cluster_wait();
   }
