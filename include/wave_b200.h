@@ -450,20 +450,21 @@ int wb200_multi_gpu_time_end(wb200_multi_gpu_t* h, float* max_ms);
 /* Low-rank adapters of many requests: out[t] = y[t] + scale[l] * B_l (A_l x[t]) with l = ids[t]; rows whose id is outside
  * [0, num_adapters) have no adapter and keep y. x [rows, K] bf16 (pitch ldx), a [num_adapters, rank, K] and b [num_adapters, N, rank]
  * bf16, contiguous; ids int32 or int64; scale f32 [num_adapters], or null for ones; y and out [rows, N] of `dtype`, out may be y (in
- * place), otherwise they do not overlap. K is a multiple of 8, rank at most 256, N any. hidden: wb200_adapters_hidden_bytes(rows, K, rank)
- * bytes, 16-byte aligned, left with A_l x[t] in f32, which the backward call reads. Two launches, no order of the ids needed. */
-size_t wb200_adapters_hidden_bytes(int rows, int K, int rank);
+ * place), otherwise they do not overlap. K is a multiple of 8, rank at most 256, N any. hidden: wb200_adapters_hidden_bytes(rows, rank, dtype)
+ * bytes, 16-byte aligned, left with scale[l] * A_l x[t] as sums of bf16 parts, which the backward call reads. Two launches, no order of the
+ * ids needed. */
+size_t wb200_adapters_hidden_bytes(int rows, int rank, int dtype);
 int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,
                            const void* ids, int ids_are_int64, const float* scale, const void* y, long long ldy, void* out, long long ldo,
                            int dtype, void* hidden, size_t hidden_bytes, void* stream);
-/* Its gradients for g = the gradient of out [rows, N] bf16: dx [rows, K] (the adapters' part), da and db laid out as a and b (zeros for an
- * adapter without rows), all bf16; each may be null. hidden: as the forward call left it (read for db). At most 256 adapters. Sums over rows are
- * made in a fixed order. workspace: wb200_adapters_backward_workspace_bytes, 256-byte aligned. */
-size_t wb200_adapters_backward_workspace_bytes(int rows, int K, int N, int rank, int num_adapters);
+/* Its gradients for g = the gradient of a bf16 out [rows, N]: dx [rows, K] (the adapters' part, or with accumulate_dx != 0 added to what dx
+ * holds), da and db laid out as a and b (zeros for an adapter without rows), all bf16; each may be null. hidden: as the forward call left it
+ * (read for db). Sums over rows are made in a fixed order. At most 65535 adapters. workspace (for dx and da): as many bytes as hidden, 16-byte
+ * aligned. */
 int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,
                             const void* ids, int ids_are_int64, const float* scale, const void* g, long long ldg, const void* hidden,
-                            size_t hidden_bytes, void* dx, long long ldd, void* da, void* db, void* workspace, size_t workspace_bytes,
-                            void* stream);
+                            size_t hidden_bytes, void* dx, long long ldd, int accumulate_dx, void* da, void* db, void* workspace,
+                            size_t workspace_bytes, void* stream);
 /* Input gradient of a linear layer with MXFP4 weights: dx [M, K] = g [M, N] * dequant(b, b_scale) [N, K], g and dx bf16, f32 accumulation.
  * b and b_scale as wb200_mxfp4_gemm's, the scales row-major with a pitch. Rows of g and dx start on 16 bytes. */
 int wb200_mxfp4_input_grad(int M, int N, int K, const void* g, long long ldg, const void* b, const void* b_scale, long long b_scale_stride,

@@ -284,7 +284,7 @@ def test_refusals():
     with pytest.raises(ValueError):
         apply(y.float(), x, a, b, ids, s)
     with pytest.raises(ValueError):
-        apply(y, x, a.repeat(100, 1, 1), b.repeat(100, 1, 1), ids, s.repeat(100))
+        apply(y, x, a[:, :, :8].repeat(22000, 1, 1)[:, :1].repeat(1, 1, 8), b.repeat(22000, 1, 1)[:, :, :1], ids)
     with pytest.raises(ValueError):
         apply(y, x, a, b, ids, s.requires_grad_())
 

@@ -96,7 +96,6 @@ EXPORTED_SYMBOLS = (
     "wb200_moe_combine",
     "wb200_adapters_hidden_bytes",
     "wb200_adapters_forward",
-    "wb200_adapters_backward_workspace_bytes",
     "wb200_adapters_backward",
     "wb200_mxfp4_input_grad",
     "wb200_router_workspace_bytes",
@@ -243,11 +242,9 @@ def load() -> ctypes.CDLL:
     lib.wb200_adapters_forward.restype = c_int
     lib.wb200_adapters_forward.argtypes = [c_int] * 5 + [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_ll, c_void_p,
                                                          c_ll, c_int, c_void_p, c_size_t, c_void_p]
-    lib.wb200_adapters_backward_workspace_bytes.restype = c_size_t
-    lib.wb200_adapters_backward_workspace_bytes.argtypes = [c_int] * 5
     lib.wb200_adapters_backward.restype = c_int
     lib.wb200_adapters_backward.argtypes = [c_int] * 5 + [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_ll, c_void_p,
-                                                          c_size_t, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+                                                          c_size_t, c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
     lib.wb200_mxfp4_input_grad.restype = c_int
     lib.wb200_mxfp4_input_grad.argtypes = [c_int, c_int, c_int, c_void_p, c_ll, c_void_p, c_void_p, c_ll, c_void_p, c_ll, c_void_p]
     lib.wb200_router_workspace_bytes.restype = c_size_t

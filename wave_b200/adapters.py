@@ -15,7 +15,7 @@ from . import _lib, ops
 
 _OUT_CODE = ops._DTYPE_CODE
 MAX_RANK = 256
-MAX_TRAINED = 256  # adapters of a pool whose gradients are asked for
+MAX_TRAINED = 65535  # adapters of a pool whose gradients are asked for
 
 
 def _check(y, x, a, b, ids, scale, out) -> tuple[int, int, int, int, int]:
@@ -72,12 +72,11 @@ def _forward(sizes, y, x, a, b, ids, scale, out) -> torch.Tensor:
     """Writes out, returns the hidden vectors."""
     rows, K, N, rank, pool = sizes
     lib = _lib.load()
-    nbytes = int(lib.wb200_adapters_hidden_bytes(rows, K, rank))
-    hidden = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device)
+    hidden = torch.empty(rows, 2 if y.dtype == torch.bfloat16 else 3, (rank + 15) // 16 * 16, dtype=torch.bfloat16, device=x.device)
     _launch(x.device, lambda stream: lib.wb200_adapters_forward(
         rows, K, N, rank, pool, x.data_ptr(), _pitch(x), a.data_ptr(), b.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64),
         scale.data_ptr() if scale is not None else None, y.data_ptr(), _pitch(y), out.data_ptr(), _pitch(out), _OUT_CODE[out.dtype],
-        hidden.data_ptr(), nbytes, stream))
+        hidden.data_ptr(), 2 * hidden.numel(), stream))
     return hidden
 
 
@@ -104,13 +103,12 @@ class _Adapters(torch.autograd.Function):
         if need_x or need_a or need_b:
             lib = _lib.load()
             rows_g = _rows(g)
-            nbytes = int(lib.wb200_adapters_backward_workspace_bytes(*ctx.sizes))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            ws = torch.empty_like(hidden)
             ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
             _launch(x.device, lambda stream: lib.wb200_adapters_backward(
                 rows, K, N, rank, pool, x.data_ptr(), _pitch(x), a.data_ptr(), b.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64),
-                ptr(scale), rows_g.data_ptr(), _pitch(rows_g), hidden.data_ptr(), hidden.numel() * 4, ptr(dx), K, ptr(da), ptr(db),
-                ws.data_ptr(), nbytes, stream))
+                ptr(scale), rows_g.data_ptr(), _pitch(rows_g), hidden.data_ptr(), 2 * hidden.numel(), ptr(dx), K, 0, ptr(da), ptr(db),
+                ws.data_ptr(), 2 * ws.numel(), stream))
         return (g if need_y else None), dx, da, db, None, None, None
 
 
@@ -121,7 +119,7 @@ def apply_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.T
     y [rows, N] f32 or bf16, x [rows, K] bf16, a [adapters, rank, K] and b [adapters, N, rank] bf16 (adapters of a lower rank are padded
     with zeros), ids [rows] int32 or int64, scale [adapters] f32 or None for ones. A row whose id is outside [0, adapters) has no adapter:
     its y comes back. The sum is made in f32 and rounded once to y's type. out: where to write (may be y), not together with gradients.
-    Differentiable in y, x, a and b for a bf16 y and pools of at most 256 adapters; sums over rows are made in a fixed order.
+    Differentiable in y, x, a and b for a bf16 y and pools of at most 65535 adapters; sums over rows are made in a fixed order.
     """
     sizes = _check(y, x, a, b, ids, scale, out)
     rows = sizes[0]

@@ -55,74 +55,142 @@ int allow_smem() {
 // ------------------------------------------------------------------------------------------
 // adapters
 // ------------------------------------------------------------------------------------------
-// K is cut where there are few chunks of rows; a split has at least one block of each warp.
-int shrink_splits(int rows, int K) {
-  const int most = std::max(1, std::min(16, K / 512));
-  return std::max(1, std::min(most, div_up(kTargetCtas, chunks_of(rows))));
+// A launch whose grid.x is one cluster.
+template <typename... P, typename... A>
+cudaError_t launch_clusters(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = grid.x;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = grid.x > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
-template <int RT, int MT, int KU, bool TRANS>
-cudaError_t launch_shrink(const wb::ShrinkParams& p, bool wide_ids, dim3 grid, cudaStream_t s) {
-  return wide_ids ? launch(wb::adapter_shrink_kernel<long long, RT, MT, KU, TRANS>, grid, wb::kAdapterThreads, 0, s, p)
-                  : launch(wb::adapter_shrink_kernel<int, RT, MT, KU, TRANS>, grid, wb::kAdapterThreads, 0, s, p);
+// The smallest power of two, at most `most` and 8 (a cluster), with which `units` come to two CTAs per SM.
+int splits_for(long long units, int most) {
+  int s = 1;
+  while (s < 8 && 2 * s <= most && units * s < kTargetCtas * 2 / 3) s *= 2;
+  return s;
+}
+int group_lanes(int rows, int L, long long others) {
+  return rows <= wb::kChunkRows ? std::min(rows, L) : int(std::max(1ll, std::min<long long>(std::min(wb::kChunkRows, L), kTargetCtas / others)));
 }
 
-// hidden [splits][rows][Rp] = rows of x onto the ranks. trans: w is [L][K][R].
-int run_shrink(const __nv_bfloat16* x, long long ldx, const __nv_bfloat16* w, bool trans, const void* ids, bool wide_ids, float* hidden, int rows,
-               int K, int R, int L, cudaStream_t s) {
-  wb::ShrinkParams p;
-  p.x = x; p.w = w; p.ids = ids; p.hidden = hidden; p.ldx = ldx;
-  p.rows = rows; p.K = K; p.R = R; p.Rp = rank_pad(R); p.L = L;
-  const int splits = shrink_splits(rows, K), chunks = chunks_of(rows);
-  p.split_k = div_up(div_up(K, splits), 64) * 64;
-  const int rt = p.Rp <= 16 ? 2 : p.Rp <= 32 ? 4 : 8;
-  p.x_vec = aligned_to(x, 16) && ldx % 8 == 0 && K % 8 == 0;
-  p.w_vec = trans ? aligned_to(w, 2 * rt) && R % rt == 0 : aligned_to(w, 16) && K % 8 == 0;
-  const int lanes = rows <= wb::kChunkRows ? std::min(rows, L) : std::max(1, std::min(std::min(wb::kChunkRows, L), kTargetCtas / (chunks * splits)));
-  const dim3 grid(splits, chunks, lanes);
-  const bool few = rows <= wb::kChunkRows;
-#define WB_SHRINK(RT, KU)                                                                                            \
-  (trans ? (few ? launch_shrink<RT, 1, 2, true>(p, wide_ids, grid, s) : launch_shrink<RT, 4, KU, true>(p, wide_ids, grid, s)) \
-         : (few ? launch_shrink<RT, 1, 2, false>(p, wide_ids, grid, s) : launch_shrink<RT, 4, KU, false>(p, wide_ids, grid, s)))
-  WB_HOST_CUDA(rt == 2 ? WB_SHRINK(2, 2) : rt == 4 ? WB_SHRINK(4, 1) : WB_SHRINK(8, 1));
-#undef WB_SHRINK
+struct AdapterCall {
+  const void* ids;
+  bool wide_ids;
+  int rows, R, Rp, L, parts;
+  cudaStream_t stream;
+};
+
+template <typename IdT, int RT, bool TRANS>
+int launch_shrink(const wb::ShrinkParams& p, bool few, dim3 grid, cudaStream_t s) {
+  if (few) {
+    WB_HOST_CUDA(launch_clusters(wb::adapter_shrink_few_kernel<IdT, RT, TRANS>, grid, wb::kAdapterThreads, 0, s, p));
+    return WB200_OK;
+  }
+  constexpr auto kernel = wb::adapter_shrink_tile_kernel<IdT, RT, TRANS>;
+  if (int rc = allow_smem<kernel>()) return rc;
+  WB_HOST_CUDA(launch_clusters(kernel, grid, wb::kAdapterThreads, wb::ShrinkTile<RT>::SMEM_BYTES, s, p));
   return WB200_OK;
+}
+template <typename IdT, bool TRANS>
+int launch_shrink_ranks(const wb::ShrinkParams& p, bool few, dim3 grid, cudaStream_t s) {
+  return p.Rp <= 16 ? launch_shrink<IdT, 2, TRANS>(p, few, grid, s) : p.Rp <= 32 ? launch_shrink<IdT, 4, TRANS>(p, few, grid, s) : launch_shrink<IdT, 8, TRANS>(p, few, grid, s);
+}
+
+// hidden [rows][parts][Rp] = rows of x onto the ranks, scaled. trans: w is [L][K][R].
+int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int K, const __nv_bfloat16* w, bool trans, const float* scale, __nv_bfloat16* hidden) {
+  wb::ShrinkParams p;
+  p.x = x; p.w = w; p.ids = c.ids; p.scale = scale; p.hidden = hidden; p.ldx = ldx;
+  p.rows = c.rows; p.K = K; p.R = c.R; p.Rp = c.Rp; p.L = c.L; p.parts = c.parts;
+  const bool few = c.rows <= wb::kChunkRows;
+  const int chunks = chunks_of(c.rows);
+  const int splits = few ? splits_for(1, std::max(1, K / 512)) : splits_for(chunks, std::max(1, K / 256));
+  p.split_k = div_up(div_up(K, splits), 64) * 64;
+  const int vec = !trans ? 8 : !few ? 8 : c.Rp <= 16 ? 2 : c.Rp <= 32 ? 4 : 8;  // elements of a load of w
+  p.x_vec = aligned_to(x, 16) && ldx % 8 == 0 && K % 8 == 0;
+  p.w_vec = aligned_to(w, 2 * vec) && (trans ? c.R : K) % vec == 0;
+  const dim3 grid(splits, chunks, group_lanes(c.rows, c.L, (long long)chunks * splits));
+  if (c.wide_ids) return trans ? launch_shrink_ranks<long long, true>(p, few, grid, c.stream) : launch_shrink_ranks<long long, false>(p, few, grid, c.stream);
+  return trans ? launch_shrink_ranks<int, true>(p, few, grid, c.stream) : launch_shrink_ranks<int, false>(p, few, grid, c.stream);
 }
 
 template <typename IdT, typename T, int P, int QN, bool TRANS>
-int launch_expand(const wb::ExpandParams& p, dim3 grid, cudaStream_t s) {
-  constexpr auto kernel = wb::adapter_expand_kernel<IdT, T, P, QN, TRANS>;
-  const size_t smem = size_t(P) * wb::kChunkRows * (p.Rp + 8) * 2;
+int launch_expand_tile(const wb::ExpandParams& p, dim3 grid, cudaStream_t s) {
+  constexpr auto kernel = wb::adapter_expand_tile_kernel<IdT, T, P, QN, TRANS>;
+  const size_t smem = size_t(wb::kChunkRows) * (P * p.Rp + 8) * 2;
   if (int rc = smem > 40 * 1024 ? allow_smem<kernel>() : WB200_OK) return rc;
   WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, smem, s, p));
   return WB200_OK;
 }
-template <typename T, int P, bool TRANS>
-int launch_expand_ranks(const wb::ExpandParams& p, bool wide_ids, dim3 grid, cudaStream_t s) {
+template <typename IdT, typename T, int P, bool TRANS>
+int launch_expand(const wb::ExpandParams& p, bool few, dim3 grid, cudaStream_t s) {
+  if (few) {
+    WB_HOST_CUDA(launch(wb::adapter_expand_few_kernel<IdT, T, P, TRANS>, grid, wb::kAdapterThreads, size_t(8) * p.Rp * 4, s, p));
+    return WB200_OK;
+  }
   const int steps = p.Rp / 16;
-  if (wide_ids) return steps == 1 ? launch_expand<long long, T, P, 1, TRANS>(p, grid, s) : steps == 2 ? launch_expand<long long, T, P, 2, TRANS>(p, grid, s) : launch_expand<long long, T, P, 4, TRANS>(p, grid, s);
-  return steps == 1 ? launch_expand<int, T, P, 1, TRANS>(p, grid, s) : steps == 2 ? launch_expand<int, T, P, 2, TRANS>(p, grid, s) : launch_expand<int, T, P, 4, TRANS>(p, grid, s);
+  return steps == 1 ? launch_expand_tile<IdT, T, P, 1, TRANS>(p, grid, s) : steps == 2 ? launch_expand_tile<IdT, T, P, 2, TRANS>(p, grid, s) : launch_expand_tile<IdT, T, P, 4, TRANS>(p, grid, s);
 }
 
-// out = y + scale * (ranks onto C columns); contraction: that of the product that made `hidden`, which says how often it was split.
-int run_expand(const __nv_bfloat16* w, bool trans, const void* ids, bool wide_ids, const float* scale, const float* hidden, int contraction,
-               const void* y, long long ldy, void* out, long long ldo, bool f32, int rows, int C, int R, int L, cudaStream_t s) {
+// out = y + ranks onto C columns.
+int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const __nv_bfloat16* hidden, const void* y, long long ldy, void* out, long long ldo, bool f32, int C) {
   wb::ExpandParams p;
-  p.w = w; p.ids = ids; p.scale = scale; p.hidden = hidden; p.y = y; p.out = out; p.ldy = ldy; p.ldo = ldo;
-  p.rows = rows; p.C = C; p.R = R; p.Rp = rank_pad(R); p.L = L;
-  p.splits = shrink_splits(rows, contraction);
-  const int chunks = chunks_of(rows);
-  p.cols_per_cta = 1024;
-  while (p.cols_per_cta > 256 && (long long)chunks * div_up(C, p.cols_per_cta) < kTargetCtas) p.cols_per_cta /= 2;
+  p.w = w; p.ids = c.ids; p.hidden = hidden; p.y = y; p.out = out; p.ldy = ldy; p.ldo = ldo;
+  p.rows = c.rows; p.C = C; p.R = c.R; p.Rp = c.Rp; p.L = c.L;
+  const bool few = c.rows <= wb::kChunkRows;
+  const int chunks = chunks_of(c.rows);
+  p.cols_per_cta = few ? 2 * wb::kAdapterThreads : 2048;
+  if (!few)
+    while (p.cols_per_cta > 256 && (long long)chunks * div_up(C, p.cols_per_cta) < kTargetCtas * 3 / 2) p.cols_per_cta /= 2;
   const size_t esz = f32 ? 4 : 2;
   p.io_vec = aligned_to(out, 16) && ldo * esz % 16 == 0 && (!y || (aligned_to(y, 16) && ldy * esz % 16 == 0));
-  p.w_vec = trans ? aligned_to(w, 8) && C % 4 == 0 : aligned_to(w, 8) && R % 4 == 0;
+  const int vec = few ? (trans ? 2 : 8) : 4;  // elements of a load of w
+  p.w_vec = aligned_to(w, 2 * vec) && (trans ? C : c.R) % (trans && few ? 4 : vec) == 0;
   const int slices = div_up(C, p.cols_per_cta);
-  const int lanes = rows <= wb::kChunkRows ? std::min(rows, L)
-                                           : std::max(1, std::min(std::min(wb::kChunkRows, L), int(kTargetCtas / ((long long)chunks * slices))));
-  const dim3 grid(slices, chunks, lanes);
-  if (trans) return launch_expand_ranks<__nv_bfloat16, 2, true>(p, wide_ids, grid, s);
-  return f32 ? launch_expand_ranks<float, 3, false>(p, wide_ids, grid, s) : launch_expand_ranks<__nv_bfloat16, 2, false>(p, wide_ids, grid, s);
+  const dim3 grid(slices, chunks, group_lanes(c.rows, c.L, (long long)chunks * slices));
+  using bf16 = __nv_bfloat16;
+  if (c.wide_ids)
+    return trans ? launch_expand<long long, bf16, 2, true>(p, few, grid, c.stream)
+           : f32 ? launch_expand<long long, float, 3, false>(p, few, grid, c.stream) : launch_expand<long long, bf16, 2, false>(p, few, grid, c.stream);
+  return trans ? launch_expand<int, bf16, 2, true>(p, few, grid, c.stream)
+         : f32 ? launch_expand<int, float, 3, false>(p, few, grid, c.stream) : launch_expand<int, bf16, 2, false>(p, few, grid, c.stream);
+}
+
+template <typename IdT, int RT>
+int launch_outer(const wb::OuterParams& p, dim3 grid, cudaStream_t s) {
+  constexpr auto kernel = wb::adapter_outer_kernel<IdT, RT>;
+  if (int rc = allow_smem<kernel>()) return rc;
+  WB_HOST_CUDA(launch_clusters(kernel, grid, wb::kAdapterThreads, wb::OuterTile<RT>::SMEM_BYTES, s, p));
+  return WB200_OK;
+}
+
+// Either side may be left out (out null); the splits, and with them the order of the sums, do not depend on that.
+int run_outer(const AdapterCall& c, wb::OuterSide first, wb::OuterSide second) {
+  wb::OuterParams p;
+  p.side[0] = first;
+  p.side[1] = second;
+  for (wb::OuterSide& side : p.side) {
+    side.blocks = side.out ? div_up(side.C, wb::kOuterCols) : 0;
+    side.vec = aligned_to(side.z, 16) && side.ldz % 8 == 0 && side.C % 8 == 0;
+  }
+  p.ids = c.ids;
+  p.rows = c.rows; p.R = c.R; p.Rp = c.Rp; p.L = c.L;
+  const int blocks = p.side[0].blocks + p.side[1].blocks;
+  const long long both = (long long)div_up(first.C, wb::kOuterCols) + div_up(second.C, wb::kOuterCols);
+  const dim3 grid(splits_for(both * c.L, chunks_of(c.rows)), blocks, c.L);
+  if (c.wide_ids) return c.Rp <= 16 ? launch_outer<long long, 2>(p, grid, c.stream) : c.Rp <= 32 ? launch_outer<long long, 4>(p, grid, c.stream) : launch_outer<long long, 8>(p, grid, c.stream);
+  return c.Rp <= 16 ? launch_outer<int, 2>(p, grid, c.stream) : c.Rp <= 32 ? launch_outer<int, 4>(p, grid, c.stream) : launch_outer<int, 8>(p, grid, c.stream);
 }
 
 int check_adapters(const char* what, int rows, int K, int N, int R, int L) {
@@ -131,46 +199,7 @@ int check_adapters(const char* what, int rows, int K, int N, int R, int L) {
   if (K % 8) return fail(WB200_ERR_INVALID_ARG, "%s: K = %d is not a multiple of 8", what, K);
   if (R > 256) return fail(WB200_ERR_UNSUPPORTED, "%s: rank %d is above 256", what, R);
   if (rows > 4000000) return fail(WB200_ERR_UNSUPPORTED, "%s: %d rows in one call", what, rows);
-  return WB200_OK;
-}
-
-struct BackwardPlan {
-  int splits_a, splits_b;  // of the rows, in the sums over them
-  size_t list, owner, listed, u, part_a, part_b, total;
-};
-int outer_splits(int rows, int C, int L) { return std::max(1, std::min({16, chunks_of(rows), int(kTargetCtas / std::max(1ll, (long long)div_up(C, 256) * L))})); }
-BackwardPlan plan_backward(int rows, int K, int N, int R, int L) {
-  BackwardPlan p;
-  const size_t Rp = rank_pad(R);
-  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  p.splits_a = outer_splits(rows, K, L);
-  p.splits_b = outer_splits(rows, N, L);
-  p.list = 0;
-  p.owner = up(size_t(rows) * 4);
-  p.listed = p.owner + up(size_t(rows) * 4);
-  p.u = p.listed + 256;
-  p.part_a = p.u + up(size_t(shrink_splits(rows, N)) * rows * Rp * 4);
-  p.part_b = p.part_a + up(size_t(p.splits_a) * L * K * Rp * 4);
-  p.total = p.part_b + up(size_t(p.splits_b) * L * N * Rp * 4);
-  return p;
-}
-
-template <bool RANK_MAJOR>
-int run_outer(const __nv_bfloat16* z, long long ldz, const float* hidden, int contraction, const float* scale, const int* list, const int* owner,
-              const int* listed, float* part, int row_splits, __nv_bfloat16* out, int rows, int C, int R, int L, cudaStream_t s) {
-  wb::OuterParams p;
-  p.z = z; p.hidden = hidden; p.scale = scale; p.list = list; p.owner = owner; p.listed = listed; p.part = part; p.ldz = ldz;
-  p.rows = rows; p.C = C; p.R = R; p.Rp = rank_pad(R); p.L = L;
-  p.splits = shrink_splits(rows, contraction);
-  p.z_vec = aligned_to(z, 8) && ldz % 4 == 0;
-  const dim3 grid(div_up(C, 256), L, row_splits);
-  WB_HOST_CUDA(p.Rp <= 16   ? launch(wb::adapter_outer_kernel<2, RANK_MAJOR>, grid, wb::kAdapterThreads, 0, s, p)
-               : p.Rp <= 32 ? launch(wb::adapter_outer_kernel<4, RANK_MAJOR>, grid, wb::kAdapterThreads, 0, s, p)
-                            : launch(wb::adapter_outer_kernel<8, RANK_MAJOR>, grid, wb::kAdapterThreads, 0, s, p));
-  const long long total = (long long)L * R * C;
-  const int blocks = int(std::min<long long>(div_up(total, 256), 148 * 8));
-  if (RANK_MAJOR) WB_HOST_CUDA(launch(wb::adapter_reduce_kernel, dim3(blocks), 256, 0, s, (const float*)part, row_splits, L, R, p.Rp, C, C, out));
-  else WB_HOST_CUDA(launch(wb::adapter_reduce_kernel, dim3(blocks), 256, 0, s, (const float*)part, row_splits, L, C, C, R, p.Rp, out));
+  if ((long long)div_up(N, 128) + div_up(K, 128) > 65535) return fail(WB200_ERR_UNSUPPORTED, "%s: K = %d and N = %d are too wide", what, K, N);
   return WB200_OK;
 }
 
@@ -309,9 +338,9 @@ cudaError_t adapt_check_record(unsigned long long (&record)[3], bool reset) {
 
 extern "C" {
 
-size_t wb200_adapters_hidden_bytes(int rows, int K, int rank) {
-  if (rows <= 0 || K <= 0 || rank <= 0) return 0;
-  return size_t(shrink_splits(rows, K)) * rows * rank_pad(rank) * sizeof(float);
+size_t wb200_adapters_hidden_bytes(int rows, int rank, int dtype) {
+  if (rows <= 0 || rank <= 0) return 0;
+  return size_t(rows) * (dtype == WB200_F32 ? 3 : 2) * rank_pad(rank) * sizeof(__nv_bfloat16);
 }
 
 int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,
@@ -324,61 +353,44 @@ int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, c
   if (!aligned_to(x, 2) || !aligned_to(a, 2) || !aligned_to(b, 2) || !aligned_to(y, dtype == WB200_F32 ? 4 : 2) || !aligned_to(out, dtype == WB200_F32 ? 4 : 2) ||
       !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(hidden, 16))
     return fail(WB200_ERR_ALIGNMENT, "adapters: a tensor is not aligned to its element size, or hidden not to 16 bytes");
-  const size_t need = wb200_adapters_hidden_bytes(rows, K, rank);
+  const size_t need = wb200_adapters_hidden_bytes(rows, rank, dtype);
   if (hidden_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters: hidden of %zu bytes needed (got %zu)", need, hidden_bytes);
   if (int rc = wbhost::device(nullptr, nullptr)) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  float* h = static_cast<float*>(hidden);
-  if (int rc = run_shrink(static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(a), false, ids, ids_are_int64 != 0, h, rows, K, rank,
-                          num_adapters, s))
-    return rc;
-  return run_expand(static_cast<const __nv_bfloat16*>(b), false, ids, ids_are_int64 != 0, scale, h, K, y, ldy, out, ldo, dtype == WB200_F32, rows, N, rank,
-                    num_adapters, s);
-}
-
-size_t wb200_adapters_backward_workspace_bytes(int rows, int K, int N, int rank, int num_adapters) {
-  if (rows <= 0 || K <= 0 || N <= 0 || rank <= 0 || num_adapters <= 0) return 0;
-  return plan_backward(rows, K, N, rank, num_adapters).total;
+  const AdapterCall c{ids, ids_are_int64 != 0, rows, rank, rank_pad(rank), num_adapters, dtype == WB200_F32 ? 3 : 2, static_cast<cudaStream_t>(stream)};
+  auto* h = static_cast<__nv_bfloat16*>(hidden);
+  if (int rc = run_shrink(c, static_cast<const __nv_bfloat16*>(x), ldx, K, static_cast<const __nv_bfloat16*>(a), false, scale, h)) return rc;
+  return run_expand(c, static_cast<const __nv_bfloat16*>(b), false, h, y, ldy, out, ldo, dtype == WB200_F32, N);
 }
 
 int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,
                             const void* ids, int ids_are_int64, const float* scale, const void* g, long long ldg, const void* hidden,
-                            size_t hidden_bytes, void* dx, long long ldd, void* da, void* db, void* workspace, size_t workspace_bytes,
-                            void* stream) {
+                            size_t hidden_bytes, void* dx, long long ldd, int accumulate_dx, void* da, void* db, void* workspace,
+                            size_t workspace_bytes, void* stream) {
   if (int rc = check_adapters("adapters backward", rows, K, N, rank, num_adapters)) return rc;
-  if (num_adapters > 256) return fail(WB200_ERR_UNSUPPORTED, "adapters backward: at most 256 adapters (got %d)", num_adapters);
+  if (num_adapters > 65535) return fail(WB200_ERR_UNSUPPORTED, "adapters backward: at most 65535 adapters (got %d)", num_adapters);
   if (!dx && !da && !db) return fail(WB200_ERR_INVALID_ARG, "adapters backward: no gradient is asked for");
-  if (!ids || !g || !workspace || ((dx || da) && (!b || !a)) || (da && !x) || (db && !hidden))
+  if (!ids || !g || ((dx || da) && (!b || !workspace)) || (dx && !a) || (da && !x) || (db && !hidden))
     return fail(WB200_ERR_INVALID_ARG, "adapters backward: null pointer");
   if (rows > 1 && (ldg < N || (da && ldx < K) || (dx && ldd < K))) return fail(WB200_ERR_INVALID_ARG, "adapters backward: a row pitch is smaller than a row");
   if (!aligned_to(x, 2) || !aligned_to(a, 2) || !aligned_to(b, 2) || !aligned_to(g, 2) || !aligned_to(dx, 2) || !aligned_to(da, 2) || !aligned_to(db, 2) ||
-      !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(hidden, 16) || !aligned_to(workspace, 256))
-    return fail(WB200_ERR_ALIGNMENT, "adapters backward: a tensor is not aligned to its element size, or the workspace not to 256 bytes");
-  const BackwardPlan plan = plan_backward(rows, K, N, rank, num_adapters);
-  if (workspace_bytes < plan.total) return fail(WB200_ERR_WORKSPACE, "adapters backward: workspace of %zu bytes needed (got %zu)", plan.total, workspace_bytes);
-  if (db && hidden_bytes < wb200_adapters_hidden_bytes(rows, K, rank)) return fail(WB200_ERR_WORKSPACE, "adapters backward: hidden of %zu bytes needed", wb200_adapters_hidden_bytes(rows, K, rank));
+      !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(hidden, 16) || !aligned_to(workspace, 16))
+    return fail(WB200_ERR_ALIGNMENT, "adapters backward: a tensor is not aligned to its element size, or hidden or the workspace not to 16 bytes");
+  const size_t need = wb200_adapters_hidden_bytes(rows, rank, WB200_BF16);
+  if ((dx || da) && workspace_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters backward: workspace of %zu bytes needed (got %zu)", need, workspace_bytes);
+  if (db && hidden_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters backward: hidden of %zu bytes needed (got %zu)", need, hidden_bytes);
   if (int rc = wbhost::device(nullptr, nullptr)) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  char* ws = static_cast<char*>(workspace);
-  int *list = reinterpret_cast<int*>(ws + plan.list), *owner = reinterpret_cast<int*>(ws + plan.owner), *listed = reinterpret_cast<int*>(ws + plan.listed);
-  float* u = reinterpret_cast<float*>(ws + plan.u);
+  const AdapterCall c{ids, ids_are_int64 != 0, rows, rank, rank_pad(rank), num_adapters, 2, static_cast<cudaStream_t>(stream)};
   const auto* gp = static_cast<const __nv_bfloat16*>(g);
-  const bool wide = ids_are_int64 != 0;
-  if (da || db)
-    if (int rc = wb200_moe_align_block_size(ids, ids_are_int64, rows, num_adapters, 1, list, rows, owner, rows, listed, nullptr, stream)) return rc;
+  auto* u = static_cast<__nv_bfloat16*>(workspace);
   if (dx || da)
-    if (int rc = run_shrink(gp, ldg, static_cast<const __nv_bfloat16*>(b), true, ids, wide, u, rows, N, rank, num_adapters, s)) return rc;
+    if (int rc = run_shrink(c, gp, ldg, N, static_cast<const __nv_bfloat16*>(b), true, scale, u)) return rc;
   if (dx)
-    if (int rc = run_expand(static_cast<const __nv_bfloat16*>(a), true, ids, wide, scale, u, N, nullptr, 0, dx, ldd, false, rows, K, rank, num_adapters, s))
-      return rc;
-  if (db)
-    if (int rc = run_outer<false>(gp, ldg, static_cast<const float*>(hidden), K, scale, list, owner, listed, reinterpret_cast<float*>(ws + plan.part_b),
-                                  plan.splits_b, static_cast<__nv_bfloat16*>(db), rows, N, rank, num_adapters, s))
-      return rc;
-  if (da)
-    if (int rc = run_outer<true>(static_cast<const __nv_bfloat16*>(x), ldx, u, N, scale, list, owner, listed, reinterpret_cast<float*>(ws + plan.part_a),
-                                 plan.splits_a, static_cast<__nv_bfloat16*>(da), rows, K, rank, num_adapters, s))
-      return rc;
+    if (int rc = run_expand(c, static_cast<const __nv_bfloat16*>(a), true, u, accumulate_dx ? dx : nullptr, ldd, dx, ldd, false, K)) return rc;
+  if (da || db) {
+    wb::OuterSide for_b = {gp, static_cast<const __nv_bfloat16*>(hidden), static_cast<__nv_bfloat16*>(db), ldg, N, 0, 0, 0};
+    wb::OuterSide for_a = {static_cast<const __nv_bfloat16*>(x), u, static_cast<__nv_bfloat16*>(da), ldx, K, 0, 0, 1};
+    return run_outer(c, for_b, for_a);
+  }
   return WB200_OK;
 }
 

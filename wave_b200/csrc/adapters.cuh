@@ -63,42 +63,63 @@ __device__ __forceinline__ void load_bf16(const __nv_bfloat16* p, bool whole, in
 
 // Rows of a chunk by adapter.
 struct RowGroups {
-  int id[kChunkRows];
-  int order[kChunkRows];      // rows of the chunk, those of one adapter together, in their order
-  int start[kChunkRows + 1];  // first place of a group
+  alignas(16) int id[kChunkRows];
+  alignas(16) int leader[kChunkRows];  // the adapter at its first row, elsewhere a number above all
+  int order[kChunkRows];               // rows of the chunk, those of one adapter together, in their order
+  int start[kChunkRows + 1];           // first place of a group
   int adapter[kChunkRows];
-  int leader[kChunkRows];
 };
 
-// Called by all threads of the CTA. Returns the number of groups. Ids outside [0, L) have no adapter.
+template <typename IdT>
+__device__ __forceinline__ int adapter_of(const IdT* ids, int row, int rows, int L) {  // -1: none
+  const long long id = row < rows ? (long long)ids[row] : -1;
+  return id >= 0 && id < L ? int(id) : -1;
+}
+
+// Called by all threads of the CTA, 64 at least. Returns the number of groups.
 template <typename IdT>
 __device__ __forceinline__ int group_rows(RowGroups& g, const IdT* ids, int row0, int rows, int L) {
   const int t = threadIdx.x;
-  int mine = -1;
-  if (t < kChunkRows) {
-    const long long id = row0 + t < rows ? (long long)ids[row0 + t] : -1;
-    mine = id >= 0 && id < L ? int(id) : -1;
-    g.id[t] = mine;
+  const int first_id = adapter_of(ids, row0, rows, L);
+  const int mine = t < kChunkRows ? adapter_of(ids, row0 + t, rows, L) : first_id;
+  if (t < kChunkRows) g.id[t] = mine;
+  if (__syncthreads_and(mine == first_id || (t < kChunkRows && row0 + t >= rows))) {  // one sequence: the usual chunk of a prefill
+    const int count = first_id < 0 ? 0 : min(kChunkRows, rows - row0);
+    if (t < kChunkRows) g.order[t] = t;
+    if (t == 0) {
+      g.start[0] = 0;
+      g.start[1] = count;
+      g.adapter[0] = first_id;
+    }
+    __syncthreads();
+    return count > 0 ? 1 : 0;
   }
-  const int placed = __syncthreads_count(mine >= 0);
   int before = 0;
-  bool first = mine >= 0;
-  if (mine >= 0) {
-#pragma unroll 8
-    for (int j = 0; j < kChunkRows; ++j) {
-      const int o = g.id[j];
-      const bool same_before = o == mine && j < t;
-      before += (o >= 0 && o < mine) || same_before;
-      first &= !same_before;
+  bool first = t < kChunkRows && mine >= 0;
+  if (first) {
+#pragma unroll
+    for (int j = 0; j < kChunkRows; j += 4) {
+      const int4 o = *reinterpret_cast<const int4*>(g.id + j);
+      const int v[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool same_before = v[i] == mine && j + i < t;
+        before += (v[i] >= 0 && v[i] < mine) || same_before;
+        first &= !same_before;
+      }
     }
     g.order[before] = t;
   }
   if (t < kChunkRows) g.leader[t] = first ? mine : 0x7fffffff;
+  const int placed = __syncthreads_count(t < kChunkRows && mine >= 0);
   const int groups = __syncthreads_count(first);
   if (first) {
     int at = 0;
-#pragma unroll 8
-    for (int j = 0; j < kChunkRows; ++j) at += g.leader[j] < mine;
+#pragma unroll
+    for (int j = 0; j < kChunkRows; j += 4) {
+      const int4 o = *reinterpret_cast<const int4*>(g.leader + j);
+      at += (o.x < mine) + (o.y < mine) + (o.z < mine) + (o.w < mine);
+    }
     g.start[at] = before;
     g.adapter[at] = mine;
   }
@@ -107,23 +128,115 @@ __device__ __forceinline__ int group_rows(RowGroups& g, const IdT* ids, int row0
   return groups;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {  // zeros where not real
+  const uint32_t bytes = real ? 16u : 0u;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// Eight bf16 to 16 bytes of shared memory: asynchronously where they may be loaded as one piece, otherwise one by one; zeros behind `valid`.
+__device__ __forceinline__ void copy8(uint32_t dst, const __nv_bfloat16* src, const __nv_bfloat16* fallback, bool vec, int valid) {
+  if (vec) {
+    cp_async16(dst, valid > 0 ? src : fallback, valid > 0);
+  } else {
+    uint32_t r[4] = {0u, 0u, 0u, 0u};
+    if (valid > 0) load_bf16<8>(src, false, valid, r);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+  }
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+// Place of 16-byte piece c in a row of PIECES pieces (2, 4, 8 or 16): eight neighbouring rows at one c lie in different banks.
+template <int PIECES>
+__device__ __forceinline__ uint32_t piece(int row, int c) {
+  constexpr int PER_LINE = PIECES >= 8 ? 1 : 8 / PIECES;  // rows to 128 bytes
+  return uint32_t((row * PIECES + (c ^ ((row / PER_LINE) & (PIECES >= 8 ? 7 : PIECES - 1)))) * 16);
+}
+
+// P bf16 values whose sum is v (each the rounding of what the ones before it leave).
+template <int P>
+__device__ __forceinline__ void split_bf16(float v, __nv_bfloat16 (&part)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    part[i] = __float2bfloat16_rn(v);
+    const float rest = v - __bfloat162float(part[i]);
+    v = fabsf(rest) < INFINITY ? rest : 0.f;  // an infinity or NaN is whole in its first part
+  }
+}
+
 struct ShrinkParams {
   const __nv_bfloat16* x;  // [rows, K], pitch ldx
   const __nv_bfloat16* w;  // A_l [L][R][K], or (TRANS) B_l [L][K][R]
   const void* ids;
-  float* hidden;  // [splits][rows][Rp]
+  const float* scale;      // [L], or null
+  __nv_bfloat16* hidden;   // [rows][parts][Rp]
   long long ldx;
-  int rows, K, R, Rp, L, split_k;
-  int x_vec, w_vec;  // 16-byte loads of x; vector loads of w
+  int rows, K, R, Rp, L, parts, split_k;
+  int x_vec, w_vec;        // 16-byte loads of x; vector loads of w
 };
 
-// hidden[split][t][r] = sum over the split's k of x[t, k] w_l[r, k]. Grid (splits, chunks, group lanes).
-// The 8 warps of a CTA take blocks of KU * 32 k in turn and add up through shared memory, in warp order.
-template <typename IdT, int RT, int MT, int KU, bool TRANS>
+// A split's sums of up to 64 rows and COLS ranks are in `sums` ([64][COLS + 1]) of every CTA of the cluster: this CTA adds up its share of the
+// rows over the splits, in their order, and writes the scaled bf16 parts.
+template <int COLS>
+__device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums, const RowGroups& groups, int row0, int first, int count, int n0, float scale) {
+  __syncthreads();
+  const int splits = gridDim.x, split = blockIdx.x;
+  if (splits > 1) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  const int r0 = count * split / splits, r1 = count * (split + 1) / splits;
+  for (int e = threadIdx.x; e < (r1 - r0) * COLS; e += kAdapterThreads) {
+    const int row = r0 + e / COLS, col = e % COLS;
+    if (n0 + col >= p.Rp) continue;
+    float v = 0.f;
+    if (splits == 1) {
+      v = sums[row * (COLS + 1) + col];
+    } else {
+      const uint32_t at = smem_u32(sums + row * (COLS + 1) + col);
+      float part[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) part[s] = s < splits ? ld_cluster_f32(mapa_shared(at, s)) : 0.f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) v += part[s];
+    }
+    __nv_bfloat16 part[3];
+    split_bf16<3>(v * scale, part);
+    __nv_bfloat16* dst = p.hidden + (long long)(row0 + groups.order[first + row]) * p.parts * p.Rp + n0 + col;
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < p.parts) dst[i * p.Rp] = part[i];
+  }
+  if (splits > 1) {  // nobody overwrites what others still read
+    cluster_arrive();
+    cluster_wait();
+  }
+  __syncthreads();
+}
+
+// hidden[t][r] = scale_l sum_k x[t, k] w_l[r, k]. Grid (splits of K = one cluster, chunks, group lanes).
+//
+// Few rows: operands straight from global memory to registers. The 8 warps of a CTA take blocks of 64 k in turn.
+template <typename IdT, int RT, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads)
-adapter_shrink_kernel(const ShrinkParams p) {
+adapter_shrink_few_kernel(const ShrinkParams p) {
+  constexpr int KU = 2, COLS = RT * 8;
   __shared__ RowGroups groups;
-  __shared__ float red[kAdapterWarps][16][RT * 8 + 2];
+  __shared__ float red[kAdapterWarps][16][COLS + 2];
+  __shared__ float sums[16 * (COLS + 1)];
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -132,44 +245,41 @@ adapter_shrink_kernel(const ShrinkParams p) {
   const int k0 = blockIdx.x * p.split_k, k1 = min(p.K, k0 + p.split_k);
   for (int gi = blockIdx.z; gi < ngroups; gi += gridDim.z) {
     const int end = groups.start[gi + 1];
-    const __nv_bfloat16* w = p.w + (long long)groups.adapter[gi] * p.R * p.K;
-    for (int first = groups.start[gi]; first < end; first += MT * 16) {
-      const __nv_bfloat16* src[MT][2];
+    const int l = groups.adapter[gi];
+    const __nv_bfloat16* w = p.w + (long long)l * p.R * p.K;
+    const float scale = p.scale ? p.scale[l] : 1.f;
+    for (int first = groups.start[gi]; first < end; first += 16) {
+      const __nv_bfloat16* src[2];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int at = first + m * 16 + h * 8 + g;
-          src[m][h] = at < end ? p.x + (long long)(row0 + groups.order[at]) * p.ldx : nullptr;
-        }
-      const int mtiles = min(MT, (end - first + 15) >> 4);
-      for (int n0 = 0; n0 < p.Rp; n0 += RT * 8) {
-        float acc[MT][RT][4] = {};
+      for (int h = 0; h < 2; ++h) {
+        const int at = first + h * 8 + g;
+        src[h] = at < end ? p.x + (long long)(row0 + groups.order[at]) * p.ldx : nullptr;
+      }
+      for (int n0 = 0; n0 < p.Rp; n0 += COLS) {
+        float acc[RT][4] = {};
         for (int kb = k0 + warp * (KU * 32); kb < k1; kb += kAdapterWarps * KU * 32) {
-          uint32_t xa[KU][MT][2][4];
+          uint32_t xa[KU][2][4];
 #pragma unroll
           for (int u = 0; u < KU; ++u) {
             const int k = kb + u * 32 + t * 8;
             const int valid = min(8, k1 - k);
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                if (src[m][h] && valid > 0) load_bf16<8>(src[m][h] + k, p.x_vec != 0, valid, xa[u][m][h]);
-                else xa[u][m][h][0] = xa[u][m][h][1] = xa[u][m][h][2] = xa[u][m][h][3] = 0u;
-              }
+            for (int h = 0; h < 2; ++h) {
+              if (src[h] && valid > 0) load_bf16<8>(src[h] + k, p.x_vec != 0, valid, xa[u][h]);
+              else xa[u][h][0] = xa[u][h][1] = xa[u][h][2] = xa[u][h][3] = 0u;
+            }
           }
 #pragma unroll
           for (int u = 0; u < KU; ++u) {
             const int k = kb + u * 32 + t * 8;
-            uint32_t wb_[RT][4];  // k pairs (0 1) (2 3) (4 5) (6 7) of the lane's eight
+            uint32_t wf[RT][4];  // k pairs (0 1) (2 3) (4 5) (6 7) of the lane's eight
             if constexpr (!TRANS) {
               const int valid = min(8, k1 - k);
 #pragma unroll
               for (int i = 0; i < RT; ++i) {
                 const int r = n0 + i * 8 + g;
-                if (r < p.R && valid > 0) load_bf16<8>(w + (long long)r * p.K + k, p.w_vec != 0, valid, wb_[i]);
-                else wb_[i][0] = wb_[i][1] = wb_[i][2] = wb_[i][3] = 0u;
+                if (r < p.R && valid > 0) load_bf16<8>(w + (long long)r * p.K + k, p.w_vec != 0, valid, wf[i]);
+                else wf[i][0] = wf[i][1] = wf[i][2] = wf[i][3] = 0u;
               }
             } else {
               uint32_t raw[8][RT / 2];
@@ -185,56 +295,155 @@ adapter_shrink_kernel(const ShrinkParams p) {
               for (int i = 0; i < RT; ++i)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                  wb_[i][q] = i & 1 ? high_halves(raw[2 * q][i / 2], raw[2 * q + 1][i / 2]) : low_halves(raw[2 * q][i / 2], raw[2 * q + 1][i / 2]);
+                  wf[i][q] = i & 1 ? high_halves(raw[2 * q][i / 2], raw[2 * q + 1][i / 2]) : low_halves(raw[2 * q][i / 2], raw[2 * q + 1][i / 2]);
             }
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-              if (m < mtiles)
+            for (int i = 0; i < RT; ++i)
 #pragma unroll
-                for (int i = 0; i < RT; ++i)
-#pragma unroll
-                  for (int s = 0; s < 2; ++s)
-                    mma_bf16(acc[m][i], xa[u][m][0][2 * s], xa[u][m][1][2 * s], xa[u][m][0][2 * s + 1], xa[u][m][1][2 * s + 1], wb_[i][2 * s],
-                             wb_[i][2 * s + 1]);
+              for (int s = 0; s < 2; ++s)
+                mma_bf16(acc[i], xa[u][0][2 * s], xa[u][1][2 * s], xa[u][0][2 * s + 1], xa[u][1][2 * s + 1], wf[i][2 * s], wf[i][2 * s + 1]);
           }
         }
-        for (int m = 0; m < mtiles; ++m) {
-          __syncthreads();
 #pragma unroll
-          for (int mm = 0; mm < MT; ++mm)
-            if (mm == m)
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
-              for (int i = 0; i < RT; ++i)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                  const int col = TRANS ? RT * (2 * t + (c & 1)) + i : i * 8 + 2 * t + (c & 1);
-                  red[warp][g + (c >> 1) * 8][col] = acc[mm][i][c];
-                }
-          __syncthreads();
-          for (int e = threadIdx.x; e < 16 * RT * 8; e += kAdapterThreads) {
-            const int row = e / (RT * 8), col = e % (RT * 8), at = first + m * 16 + row;
-            if (at >= end || n0 + col >= p.Rp) continue;
-            float sum = 0.f;
-#pragma unroll
-            for (int v = 0; v < kAdapterWarps; ++v) sum += red[v][row][col];
-            p.hidden[((long long)blockIdx.x * p.rows + row0 + groups.order[at]) * p.Rp + n0 + col] = sum;
+          for (int c = 0; c < 4; ++c) {
+            const int col = TRANS ? RT * (2 * t + (c & 1)) + i : i * 8 + 2 * t + (c & 1);
+            red[warp][g + (c >> 1) * 8][col] = acc[i][c];
           }
-        }
         __syncthreads();
+        for (int e = threadIdx.x; e < 16 * COLS; e += kAdapterThreads) {
+          const int row = e / COLS, col = e % COLS;
+          float v = 0.f;
+#pragma unroll
+          for (int i = 0; i < kAdapterWarps; ++i) v += red[i][row][col];
+          sums[row * (COLS + 1) + col] = v;
+        }
+        finish_hidden<COLS>(p, sums, groups, row0, first, min(16, end - first), n0, scale);
       }
     }
   }
 }
 
+// Many rows: a ring of stages of 64 k in shared memory, rows of x gathered by their place in the group. Warp (m, q) takes rows 32 m .. and the
+// q-th 16 of the 64 k. HBM-bound on x while a chunk's ranks are few; at rank 64 the MMAs (mma.sync) take about as long.
+template <int RT>
+struct ShrinkTile {
+  static constexpr int X_BYTES = kChunkRows * 128, W_BYTES = RT * 1024, STAGE_BYTES = X_BYTES + W_BYTES;
+  static constexpr int STAGES = RT == 2 ? 8 : RT == 4 ? 7 : 6;
+  static constexpr int COLS = RT * 8;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES;  // the sums reuse it
+  static_assert(4 * kChunkRows * (COLS + 1) * 4 <= SMEM_BYTES, "sums of the four k quarters");
+};
+template <typename IdT, int RT, bool TRANS>
+__global__ void __launch_bounds__(kAdapterThreads, 2)
+adapter_shrink_tile_kernel(const ShrinkParams p) {
+  using Cfg = ShrinkTile<RT>;
+  constexpr int STAGES = Cfg::STAGES, COLS = Cfg::COLS;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ RowGroups groups;
+  const uint32_t base = smem_u32(smem);
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int wm = warp & 1, wq = warp >> 1;
+  const int row0 = blockIdx.y * kChunkRows;
+  const int ngroups = group_rows(groups, static_cast<const IdT*>(p.ids), row0, p.rows, p.L);
+  const int k0 = blockIdx.x * p.split_k, k1 = min(p.K, k0 + p.split_k);
+  const int steps = max(0, (k1 - k0 + 63) / 64);
+  for (int gi = blockIdx.z; gi < ngroups; gi += gridDim.z) {
+    const int first = groups.start[gi], count = groups.start[gi + 1] - first;
+    const int l = groups.adapter[gi];
+    const __nv_bfloat16* w = p.w + (long long)l * p.R * p.K;
+    const float scale = p.scale ? p.scale[l] : 1.f;
+    // rows tid / 8 and tid / 8 + 32 of x, 16-byte piece tid % 8
+    const int xr = tid >> 3, xc = tid & 7;
+    const __nv_bfloat16* src[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) src[h] = xr + 32 * h < count ? p.x + (long long)(row0 + groups.order[first + xr + 32 * h]) * p.ldx : nullptr;
+    for (int n0 = 0; n0 < p.Rp; n0 += COLS) {
+      auto load = [&](int step) {
+        const uint32_t at = base + (step % STAGES) * Cfg::STAGE_BYTES;
+        const int kb = k0 + step * 64;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          copy8(at + piece<8>(xr + 32 * h, xc), src[h] + kb + xc * 8, p.x, p.x_vec != 0, src[h] ? min(8, k1 - kb - xc * 8) : 0);
+        if constexpr (!TRANS) {  // [rank][64 k]
+#pragma unroll
+          for (int e = tid; e < COLS * 8; e += kAdapterThreads) {
+            const int r = e >> 3, c = e & 7;
+            copy8(at + Cfg::X_BYTES + piece<8>(r, c), w + (long long)(n0 + r) * p.K + kb + c * 8, p.w, p.w_vec != 0, n0 + r < p.R ? min(8, k1 - kb - c * 8) : 0);
+          }
+        } else {  // [k][ranks]
+#pragma unroll
+          for (int e = tid; e < 64 * RT; e += kAdapterThreads) {
+            const int k = e / RT, c = e % RT;
+            copy8(at + Cfg::X_BYTES + piece<RT>(k, c), w + (long long)(kb + k) * p.R + n0 + c * 8, p.w, p.w_vec != 0, kb + k < k1 ? min(8, p.R - n0 - c * 8) : 0);
+          }
+        }
+        cp_async_commit();
+      };
+      float acc[2][RT][4] = {};
+#pragma unroll
+      for (int s = 0; s < STAGES - 1; ++s) {
+        if (s < steps) load(s);
+        else cp_async_commit();
+      }
+      for (int step = 0; step < steps; ++step) {
+        cp_async_wait<STAGES - 2>();
+        __syncthreads();
+        if (step + STAGES - 1 < steps) load(step + STAGES - 1);
+        else cp_async_commit();
+        if (32 * wm < count) {
+          const uint32_t at = base + (step % STAGES) * Cfg::STAGE_BYTES;
+          const int half = lane >> 4, in = lane & 15;
+          uint32_t xa[2][4];
+#pragma unroll
+          for (int m = 0; m < 2; ++m) ldsm4(at + piece<8>(32 * wm + 16 * m + in, 2 * wq + half), xa[m]);
+#pragma unroll
+          for (int i = 0; i < RT; i += 2) {
+            uint32_t wf[4];
+            if constexpr (!TRANS) ldsm4(at + Cfg::X_BYTES + piece<8>(i * 8 + half * 8 + (in & 7), 2 * wq + (in >> 3)), wf);
+            else ldsm4_trans(at + Cfg::X_BYTES + piece<RT>(16 * wq + in, i + half), wf);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              mma_bf16(acc[m][i], xa[m][0], xa[m][1], xa[m][2], xa[m][3], wf[0], wf[1]);
+              mma_bf16(acc[m][i + 1], xa[m][0], xa[m][1], xa[m][2], xa[m][3], wf[2], wf[3]);
+            }
+          }
+        }
+      }
+      cp_async_wait<0>();
+      __syncthreads();
+      float* sums = reinterpret_cast<float*>(smem);  // [4 quarters of k][64][COLS + 1]
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            sums[(wq * kChunkRows + 32 * wm + 16 * m + g + (c >> 1) * 8) * (COLS + 1) + i * 8 + 2 * t + (c & 1)] = acc[m][i][c];
+      __syncthreads();
+      for (int e = tid; e < count * COLS; e += kAdapterThreads) {
+        const int at = e / COLS * (COLS + 1) + e % COLS;
+        float v = sums[at];
+#pragma unroll
+        for (int q = 1; q < 4; ++q) v += sums[q * kChunkRows * (COLS + 1) + at];
+        sums[at] = v;
+      }
+      finish_hidden<COLS>(p, sums, groups, row0, first, count, n0, scale);
+    }
+  }
+}
+
 struct ExpandParams {
-  const __nv_bfloat16* w;  // B_l [L][C][R], or (TRANS) A_l [L][R][C]
+  const __nv_bfloat16* w;       // B_l [L][C][R], or (TRANS) A_l [L][R][C]
   const void* ids;
-  const float* scale;   // [L], or null
-  const float* hidden;  // [splits][rows][Rp]
-  const void* y;        // null: zeros
+  const __nv_bfloat16* hidden;  // [rows][parts][Rp]
+  const void* y;                // null: zeros
   void* out;
   long long ldy, ldo;
-  int rows, C, R, Rp, L, splits, cols_per_cta;
+  int rows, C, R, Rp, L, cols_per_cta;
   int io_vec, w_vec;
 };
 
@@ -281,26 +490,147 @@ __device__ __forceinline__ void write8(T* p, bool whole, int valid, const float 
   }
 }
 
-// `parts` bf16 values whose sum is v (each the rounding of what the ones before it leave).
-template <int P>
-__device__ __forceinline__ void split_bf16(float v, __nv_bfloat16 (&part)[P]) {
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    part[i] = __float2bfloat16_rn(v);
-    const float rest = v - __bfloat162float(part[i]);
-    v = fabsf(rest) < INFINITY ? rest : 0.f;  // an infinity or NaN is whole in its first part
+
+// Rows without an adapter: y as it is (zeros where there is no y).
+template <typename T>
+__device__ __forceinline__ void expand_rest(const ExpandParams& p, const RowGroups& groups, int row0, int c_begin, int c_end) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T* y = static_cast<const T*>(p.y);
+  T* out = static_cast<T*>(p.out);
+  if (p.out == p.y) return;
+  for (int row = warp; row < min(kChunkRows, p.rows - row0); row += kAdapterWarps) {
+    if (groups.id[row] >= 0) continue;
+    for (int c = c_begin + lane * 8; c < c_end; c += 256) {
+      const int valid = p.C - c;
+      float v[8] = {};
+      if (y) read8<T>(y + (row0 + row) * p.ldy + c, p.io_vec && valid >= 8, valid, v);
+      write8<T>(out + (row0 + row) * p.ldo + c, p.io_vec && valid >= 8, valid, v);
+    }
   }
 }
 
-// out[t, c] = y[t, c] + s_l sum_r hidden[t, r] w_l[c, r]. Grid (column slices, chunks, group lanes). A warp takes 32 columns of all the
-// rows of a group; a lane has 8 neighbouring columns of two rows. QN: steps of 16 ranks held in registers at a time.
-template <typename IdT, typename T, int P, int QN, bool TRANS>
+// out[t, c] = y[t, c] + sum_r hidden[t, r] w_l[c, r]. Grid (column slices, chunks, group lanes).
+//
+// Few rows: a thread has two columns, with 16 of their ranks in registers at a time, and walks the rows of a group. f32 FMAs: the
+// products are few, the loads of w_l (whole sectors, all of a thread's in flight) are what counts.
+template <typename IdT, typename T, int P, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads)
-adapter_expand_kernel(const ExpandParams p) {
+adapter_expand_few_kernel(const ExpandParams p) {
+  constexpr int ROWS = 8;
+  __shared__ RowGroups groups;
+  extern __shared__ __align__(16) float hs[];  // [ROWS][Rp]
+  pdl_launch_dependents();
+  const int row0 = blockIdx.y * kChunkRows;
+  const int ngroups = group_rows(groups, static_cast<const IdT*>(p.ids), row0, p.rows, p.L);
+  const int c_begin = blockIdx.x * p.cols_per_cta, c_end = min(p.C, c_begin + p.cols_per_cta);
+  const T* y = static_cast<const T*>(p.y);
+  T* out = static_cast<T*>(p.out);
+  const int c = c_begin + 2 * threadIdx.x;  // cols_per_cta is twice the number of threads
+  const bool both = c + 1 < c_end;
+  bool waited = false;
+  for (int gi = blockIdx.z; gi < ngroups; gi += gridDim.z) {
+    const __nv_bfloat16* w = p.w + (long long)groups.adapter[gi] * p.R * p.C;
+    const int end = groups.start[gi + 1];
+    for (int first = groups.start[gi]; first < end; first += ROWS) {
+      const int count = min(ROWS, end - first);
+      float acc[ROWS][2];
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        acc[i][0] = acc[i][1] = 0.f;
+        if (y && i < count && c < c_end) {
+          const T* at = y + (long long)(row0 + groups.order[first + i]) * p.ldy + c;
+          acc[i][0] = as_f32<T>(at[0]);
+          if (both) acc[i][1] = as_f32<T>(at[1]);
+        }
+      }
+      for (int r0 = 0; r0 < p.Rp; r0 += 16) {
+        uint32_t wr[2][8];  // column, pairs of ranks
+        if constexpr (!TRANS) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int r = r0 + 8 * h;
+              uint32_t v[4] = {0u, 0u, 0u, 0u};
+              if (c + j < c_end && r < p.R) load_bf16<8>(w + (long long)(c + j) * p.R + r, p.w_vec != 0, p.R - r, v);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) wr[j][4 * h + i] = v[i];
+            }
+        } else {
+          uint32_t raw[16];  // both columns of a rank
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            uint32_t v[1] = {0u};
+            if (c < c_end && r0 + i < p.R) load_bf16<2>(w + (long long)(r0 + i) * p.C + c, p.w_vec != 0, both ? 2 : 1, v);
+            raw[i] = v[0];
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            wr[0][i] = low_halves(raw[2 * i], raw[2 * i + 1]);
+            wr[1][i] = high_halves(raw[2 * i], raw[2 * i + 1]);
+          }
+        }
+        if (r0 == 0) {
+          if (!waited) pdl_wait();  // the hidden vectors are the only thing here that the kernel before this one writes
+          waited = true;
+          __syncthreads();
+          for (int e = threadIdx.x; e < count * p.Rp; e += kAdapterThreads) {
+            const int row = e / p.Rp, r = e - row * p.Rp;
+            const __nv_bfloat16* h = p.hidden + (long long)(row0 + groups.order[first + row]) * P * p.Rp + r;
+            float v = 0.f;
+#pragma unroll
+            for (int i = P - 1; i >= 0; --i) v += __bfloat162float(h[i * p.Rp]);
+            hs[e] = v;
+          }
+          __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+          if (i >= count) break;
+          const float4* h = reinterpret_cast<const float4*>(hs + i * p.Rp + r0);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4 v = h[q];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t a = wr[j][2 * q], b = wr[j][2 * q + 1];
+              acc[i][j] = fmaf(v.x, __uint_as_float(a << 16), acc[i][j]);
+              acc[i][j] = fmaf(v.y, __uint_as_float(a & 0xffff0000u), acc[i][j]);
+              acc[i][j] = fmaf(v.z, __uint_as_float(b << 16), acc[i][j]);
+              acc[i][j] = fmaf(v.w, __uint_as_float(b & 0xffff0000u), acc[i][j]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        if (i >= count || c >= c_end) break;
+        T* at = out + (long long)(row0 + groups.order[first + i]) * p.ldo + c;
+        if (p.io_vec && both) {
+          if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(at) = pack_bf16x2(acc[i][0], acc[i][1]);
+          else *reinterpret_cast<float2*>(at) = make_float2(acc[i][0], acc[i][1]);
+        } else {
+          at[0] = as_out<T>(acc[i][0]);
+          if (both) at[1] = as_out<T>(acc[i][1]);
+        }
+      }
+    }
+  }
+  if (!waited) pdl_wait();  // (out may still be in use)
+  if (blockIdx.z == 0) expand_rest<T>(p, groups, row0, c_begin, c_end);
+}
+
+// Many rows: a warp takes 32 columns of all the rows of a group; a lane has 8 neighbouring columns of two rows of an MMA tile. The rows of y
+// are loaded ahead of everything else, all of a lane's at once, those of the next 32 columns while these are worked on.
+// QN: steps of 16 ranks of w in registers at a time.
+template <typename IdT, typename T, int P, int QN, bool TRANS>
+__global__ void __launch_bounds__(kAdapterThreads, sizeof(T) == 2 ? 2 : 1)
+adapter_expand_tile_kernel(const ExpandParams p) {
+  constexpr int RAW = sizeof(T) == 2 ? 1 : 2;  // 16-byte pieces of 8 values
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ RowGroups groups;
-  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem);  // [P][64][pitch]
-  const int pitch = p.Rp + 8;
+  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem);  // [64][P][Rp] + 8 per row
+  const int pitch = P * p.Rp + 8;
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row0 = blockIdx.y * kChunkRows;
@@ -309,82 +639,100 @@ adapter_expand_kernel(const ExpandParams p) {
   const T* y = static_cast<const T*>(p.y);
   T* out = static_cast<T*>(p.out);
   const int steps = p.Rp / 16;
-  pdl_wait();
+  bool waited = false;
   for (int gi = blockIdx.z; gi < ngroups; gi += gridDim.z) {
     const int first = groups.start[gi], count = groups.start[gi + 1] - first;
-    const int l = groups.adapter[gi];
-    const float s = p.scale ? p.scale[l] : 1.f;
-    __syncthreads();
+    const __nv_bfloat16* w = p.w + (long long)groups.adapter[gi] * p.R * p.C;
     const int mtiles = (count + 15) >> 4;
-    for (int e = threadIdx.x; e < mtiles * 16 * p.Rp; e += kAdapterThreads) {
-      const int row = e / p.Rp, r = e - row * p.Rp;
-      float v = 0.f;
-      if (row < count) {
-        const float* h = p.hidden + (long long)(row0 + groups.order[first + row]) * p.Rp + r;
-        for (int i = 0; i < p.splits; ++i) v += h[(long long)i * p.rows * p.Rp];
+    int row[4][2];
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = m * 16 + h * 8 + g;
+        row[m][h] = at < count ? row0 + groups.order[first + at] : -1;
       }
-      __nv_bfloat16 part[P];
-      split_bf16<P>(v * s, part);
+    uint4 old[4][2][RAW];
+    auto load_y = [&](int col) {  // 8 values of every row, where they are whole
 #pragma unroll
-      for (int i = 0; i < P; ++i) hs[(i * kChunkRows + row) * pitch + r] = part[i];
-    }
-    __syncthreads();
-    const __nv_bfloat16* w = p.w + (long long)l * p.R * p.C;
-    for (int c0 = c_begin + warp * kExpandCols; c0 < c_end; c0 += kAdapterWarps * kExpandCols) {
-      uint32_t wf[4][QN][2];
-      auto load_w = [&](int q0) {
+      for (int m = 0; m < 4; ++m)
 #pragma unroll
-        for (int q = 0; q < QN; ++q) {
-          const int r = (q0 + q) * 16 + 4 * t;
-          if constexpr (!TRANS) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int c = c0 + 8 * (g >> 1) + 2 * i + (g & 1);
-              if (c < p.C && r < p.R) load_bf16<4>(w + (long long)c * p.R + r, p.w_vec != 0 && r + 4 <= p.R, p.R - r, wf[i][q]);
-              else wf[i][q][0] = wf[i][q][1] = 0u;
-            }
-          } else {
-            uint32_t raw[4][2];
-            const int c = c0 + 4 * g;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (c < p.C && r + i < p.R) load_bf16<4>(w + (long long)(r + i) * p.C + c, p.w_vec != 0 && c + 4 <= p.C, p.C - c, raw[i]);
-              else raw[i][0] = raw[i][1] = 0u;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                wf[i][q][h] = i & 1 ? high_halves(raw[2 * h][i / 2], raw[2 * h + 1][i / 2]) : low_halves(raw[2 * h][i / 2], raw[2 * h + 1][i / 2]);
+          for (int i = 0; i < RAW; ++i) {
+            old[m][h][i] = make_uint4(0u, 0u, 0u, 0u);
+            if (y && p.io_vec && row[m][h] >= 0 && col + 8 <= c_end) old[m][h][i] = *(reinterpret_cast<const uint4*>(y + row[m][h] * p.ldy + col) + i);
           }
+    };
+    const int c_first = c_begin + warp * kExpandCols;
+    load_y(c_first + 8 * t);
+    uint32_t wf[4][QN][2];
+    auto load_w = [&](int c0, int q0) {
+#pragma unroll
+      for (int q = 0; q < QN; ++q) {
+        const int r = (q0 + q) * 16 + 4 * t;
+        if constexpr (!TRANS) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int c = c0 + 8 * (g >> 1) + 2 * i + (g & 1);
+            if (c < p.C && r < p.R) load_bf16<4>(w + (long long)c * p.R + r, p.w_vec != 0 && r + 4 <= p.R, p.R - r, wf[i][q]);
+            else wf[i][q][0] = wf[i][q][1] = 0u;
+          }
+        } else {
+          uint32_t raw[4][2];
+          const int c = c0 + 4 * g;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (c < p.C && r + i < p.R) load_bf16<4>(w + (long long)(r + i) * p.C + c, p.w_vec != 0 && c + 4 <= p.C, p.C - c, raw[i]);
+            else raw[i][0] = raw[i][1] = 0u;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              wf[i][q][h] = i & 1 ? high_halves(raw[2 * h][i / 2], raw[2 * h + 1][i / 2]) : low_halves(raw[2 * h][i / 2], raw[2 * h + 1][i / 2]);
         }
-      };
-      if (steps <= QN) load_w(0);
+      }
+    };
+    if (!waited) pdl_wait();  // for the hidden vectors; y and w are complete before the kernel that makes those starts
+    waited = true;
+    __syncthreads();
+    const int pieces = P * p.Rp / 8;
+    for (int e = threadIdx.x; e < mtiles * 16 * pieces; e += kAdapterThreads) {
+      const int r = e / pieces, c = e - r * pieces;
+      const int in = r < count ? row0 + groups.order[first + r] : row0;
+      cp_async16(smem_u32(hs + r * pitch + c * 8), p.hidden + (long long)in * P * p.Rp + c * 8, r < count);
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncthreads();
+    for (int c0 = c_first; c0 < c_end; c0 += kAdapterWarps * kExpandCols) {
       const int col = c0 + 8 * t;
-      const int valid = p.C - col;
+      const int valid = c_end - col;
       const bool whole = p.io_vec && valid >= 8;
-      for (int m = 0; m < mtiles; ++m) {
-        int row[2];
-        float old[2][8];
+      load_w(c0, 0);
+      uint4 now[4][2][RAW];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int at = m * 16 + h * 8 + g;
-          row[h] = at < count ? row0 + groups.order[first + at] : -1;
+      for (int m = 0; m < 4; ++m)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) old[h][i] = 0.f;
-          if (y && row[h] >= 0 && valid > 0) read8<T>(y + row[h] * p.ldy + col, whole, valid, old[h]);
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < RAW; ++i) now[m][h][i] = old[m][h][i];
+      if (c0 + kAdapterWarps * kExpandCols < c_end) load_y(col + kAdapterWarps * kExpandCols);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        if (m >= mtiles) break;
         float acc[4][4] = {};
         for (int q0 = 0; q0 < steps; q0 += QN) {
-          if (steps > QN) load_w(q0);
+          if (steps > QN && (q0 > 0 || m > 0)) load_w(c0, q0);
 #pragma unroll
           for (int q = 0; q < QN; ++q) {
             if (q0 + q >= steps) break;
             const __nv_bfloat16* at = hs + (m * 16 + g) * pitch + (q0 + q) * 16 + 4 * t;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-              const uint2 lo = *reinterpret_cast<const uint2*>(at + i * kChunkRows * pitch);
-              const uint2 hi = *reinterpret_cast<const uint2*>(at + (i * kChunkRows + 8) * pitch);
+              const uint2 lo = *reinterpret_cast<const uint2*>(at + i * p.Rp);
+              const uint2 hi = *reinterpret_cast<const uint2*>(at + 8 * pitch + i * p.Rp);
 #pragma unroll
               for (int n = 0; n < 4; ++n) mma_bf16(acc[n], lo.x, hi.x, lo.y, hi.y, wf[n][q][0], wf[n][q][1]);
             }
@@ -392,160 +740,195 @@ adapter_expand_kernel(const ExpandParams p) {
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (row[h] < 0 || valid <= 0) continue;
+          if (row[m][h] < 0 || valid <= 0) continue;
           float v[8];
+          if (whole) {
+            read8<T>(reinterpret_cast<const T*>(now[m][h]), true, 8, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = y && i < valid ? as_f32<T>(y[row[m][h] * p.ldy + col + i]) : 0.f;
+          }
 #pragma unroll
           for (int n = 0; n < 4; ++n)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int at = TRANS ? 4 * j + n : 2 * n + j;
-              v[at] = old[h][at] + acc[n][2 * h + j];
-            }
-          write8<T>(out + row[h] * p.ldo + col, whole, valid, v);
+            for (int j = 0; j < 2; ++j) v[TRANS ? 4 * j + n : 2 * n + j] += acc[n][2 * h + j];
+          write8<T>(out + row[m][h] * p.ldo + col, whole, valid, v);
         }
       }
     }
   }
-  if (blockIdx.z == 0 && p.out != p.y) {  // rows without an adapter
-    for (int row = warp; row < min(kChunkRows, p.rows - row0); row += kAdapterWarps) {
-      if (groups.id[row] >= 0) continue;
-      for (int c = c_begin + lane * 8; c < c_end; c += 256) {
-        const int valid = p.C - c;
-        float v[8] = {};
-        if (y) read8<T>(y + (row0 + row) * p.ldy + c, p.io_vec && valid >= 8, valid, v);
-        write8<T>(out + (row0 + row) * p.ldo + c, p.io_vec && valid >= 8, valid, v);
-      }
-    }
-  }
+  if (!waited) pdl_wait();
+  if (blockIdx.z == 0) expand_rest<T>(p, groups, row0, c_begin, c_end);
 }
 
-struct OuterParams {
-  const __nv_bfloat16* z;  // [rows, C], pitch ldz
-  const float* hidden;     // [splits][rows][Rp]
-  const float* scale;      // [L], or null
-  const int* list;         // rows sorted by adapter
-  const int* owner;        // adapter of every entry of the list
-  const int* listed;       // entries of the list
-  float* part;             // [row splits][L][C][Rp], or (RANK_MAJOR) [row splits][L][Rp][C]
+struct OuterSide {
+  const __nv_bfloat16* z;       // [rows, C], pitch ldz
+  const __nv_bfloat16* hidden;  // [rows][2][Rp]
+  __nv_bfloat16* out;           // [L][C][R], or rank-major [L][R][C]
   long long ldz;
-  int rows, C, R, Rp, L, splits;
-  int z_vec;
+  int C, blocks, vec, rank_major;
+};
+struct OuterParams {
+  OuterSide side[2];  // blocks of columns of the first, then of the second
+  const void* ids;
+  int rows, R, Rp, L;
 };
 
-__device__ __forceinline__ int first_of(const int* owner, int n, int l) {  // first entry whose adapter is at least l
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (owner[mid] < l) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
+// out_l[c, r] = sum over the rows t of adapter l of z[t, c] hidden[t, r]: B's gradient from g and A x, A's from x and B^T g.
+// Grid (row splits = one cluster, blocks of 128 columns of both sides, adapters). A CTA picks the rows of its adapter out of its range of ids,
+// in order, and adds up their outer products with MMAs whose k runs over the rows, from a ring of 64 rows a stage. The splits are
+// added up through distributed shared memory, in their order.
+constexpr int kOuterCols = 128;
+constexpr int kOuterSegment = 4096;  // ids looked through at a time
+template <int RT>
+struct OuterTile {
+  static constexpr int P = 2, COLS = RT * 8;
+  static constexpr int Z_BYTES = kChunkRows * kOuterCols * 2, H_BYTES = kChunkRows * P * COLS * 2, STAGE_BYTES = Z_BYTES + H_BYTES;
+  static constexpr int STAGES = RT == 8 ? 3 : 4;
+  static constexpr int SUM_PITCH = COLS + 1;
+  static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int SMEM_BYTES = RING_BYTES + kOuterSegment * 4;
+  static_assert(2 * kOuterCols * SUM_PITCH * 4 <= RING_BYTES, "sums of the two halves of the rows");
+};
 
-// part[split][l][c][r] = sum over the split's rows t of adapter l of z[t, c] s_l hidden[t, r]. Grid (column blocks of 256, L, row splits).
-// A warp takes 32 columns; RT tiles of 8 ranks at a time. The hidden vectors of 64 rows are in shared memory, two rows to a word, as
-// two bf16 parts.
-template <int RT, bool RANK_MAJOR>
+template <typename IdT, int RT>
 __global__ void __launch_bounds__(kAdapterThreads)
 adapter_outer_kernel(const OuterParams p) {
-  constexpr int P = 2, PITCH = RT * 8 + 4;
-  __shared__ uint32_t hs[P][kChunkRows / 2][PITCH];
-  __shared__ int rows_of[kChunkRows];
+  using Cfg = OuterTile<RT>;
+  constexpr int STAGES = Cfg::STAGES, P = Cfg::P, COLS = Cfg::COLS;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int found[kAdapterWarps + 1];
+  int* list = reinterpret_cast<int*>(smem + Cfg::RING_BYTES);
+  const uint32_t base = smem_u32(smem);
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int l = blockIdx.y;
-  const int n = *p.listed;
-  const int seg0 = first_of(p.owner, n, l), seg1 = first_of(p.owner, n, l + 1);
-  const int blocks = (seg1 - seg0 + kChunkRows - 1) / kChunkRows;
-  const int b0 = int((long long)blocks * blockIdx.z / gridDim.z), b1 = int((long long)blocks * (blockIdx.z + 1) / gridDim.z);
-  const float s = p.scale ? p.scale[l] : 1.f;
-  const int c = blockIdx.x * (kAdapterWarps * 32) + warp * 32 + 4 * g;  // the lane's four columns
-  const bool whole = p.z_vec && c + 4 <= p.C;
-  for (int n0 = 0; n0 < p.Rp; n0 += RT * 8) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int second = int(blockIdx.y) >= p.side[0].blocks;
+  const OuterSide& side = p.side[second];
+  const int c0 = (int(blockIdx.y) - (second ? p.side[0].blocks : 0)) * kOuterCols;
+  const int l = blockIdx.z, splits = gridDim.x, split = blockIdx.x;
+  const IdT* ids = static_cast<const IdT*>(p.ids);
+  const int row_begin = int((long long)p.rows * split / splits), row_end = int((long long)p.rows * (split + 1) / splits);
+  const int wc = warp & 3, wk = warp >> 2;  // 32 columns, 32 of a stage's 64 rows
+  for (int n0 = 0; n0 < p.Rp; n0 += COLS) {
     float acc[2][RT][4] = {};
-    for (int b = b0; b < b1; ++b) {
-      const int first = seg0 + b * kChunkRows, count = min(kChunkRows, seg1 - first);
+    for (int seg = row_begin; seg < row_end; seg += kOuterSegment) {
+      // the segment's rows of this adapter, in order: a warp looks through a run of ids, then knows how many the warps before it found
+      const int seg_end = min(row_end, seg + kOuterSegment);
+      const int run = (seg_end - seg + kAdapterThreads - 1) / kAdapterThreads * 32;
+      const int w0 = seg + warp * run, w1 = min(seg_end, w0 + run);
+      int mine = 0;
       __syncthreads();
-      if (threadIdx.x < kChunkRows) rows_of[threadIdx.x] = threadIdx.x < count ? p.list[first + threadIdx.x] : -1;
+      for (int i = w0; i < w1; i += 32) mine += __popc(__ballot_sync(0xffffffffu, i + lane < w1 && adapter_of(ids, i + lane, p.rows, p.L) == l));
+      if (lane == 0) found[warp] = mine;
       __syncthreads();
-      for (int e = threadIdx.x; e < kChunkRows / 2 * RT * 8; e += kAdapterThreads) {
-        const int pair = e / (RT * 8), r = e - pair * (RT * 8);
-        uint32_t word[P] = {};
+      int at = 0, total = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = rows_of[2 * pair + h];
-          if (row < 0 || n0 + r >= p.Rp) continue;
-          float v = 0.f;
-          for (int i = 0; i < p.splits; ++i) v += p.hidden[((long long)i * p.rows + row) * p.Rp + n0 + r];
-          __nv_bfloat16 part[P];
-          split_bf16<P>(v * s, part);
-#pragma unroll
-          for (int i = 0; i < P; ++i) word[i] |= uint32_t(__bfloat16_as_ushort(part[i])) << (16 * h);
-        }
-#pragma unroll
-        for (int i = 0; i < P; ++i) hs[i][pair][r] = word[i];
+      for (int i = 0; i < kAdapterWarps; ++i) {
+        at += i < warp ? found[i] : 0;
+        total += found[i];
+      }
+      for (int i = w0; i < w1; i += 32) {
+        const bool hit = i + lane < w1 && adapter_of(ids, i + lane, p.rows, p.L) == l;
+        const unsigned hits = __ballot_sync(0xffffffffu, hit);
+        if (hit) list[at + __popc(hits & ((1u << lane) - 1u))] = i + lane;
+        at += __popc(hits);
       }
       __syncthreads();
-      if (c - 4 * g < p.C) {  // the warp's first column
+      const int steps = (total + kChunkRows - 1) / kChunkRows;
+      auto load = [&](int step) {
+        const uint32_t to = base + (step % STAGES) * Cfg::STAGE_BYTES;
 #pragma unroll
-        for (int k = 0; k < kChunkRows / 16; ++k) {
-          if (k * 16 >= count) break;
-          uint32_t raw[4][2];
+        for (int e = tid; e < kChunkRows * (kOuterCols / 8); e += kAdapterThreads) {
+          const int r = e >> 4, c = e & 15;
+          const int in = step * kChunkRows + r;
+          const int row = in < total ? list[in] : 0;
+          copy8(to + piece<16>(r, c), side.z + row * side.ldz + c0 + c * 8, side.z, side.vec != 0, in < total ? min(8, side.C - c0 - c * 8) : 0);
+        }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = rows_of[k * 16 + 4 * t + i];
-            if (row >= 0 && c < p.C) load_bf16<4>(p.z + row * p.ldz + c, whole, p.C - c, raw[i]);
-            else raw[i][0] = raw[i][1] = 0u;
-          }
-          uint32_t za[2][4];  // column tiles: columns 4 g and 4 g + 1, 4 g + 2 and 4 g + 3
+        for (int e = tid; e < kChunkRows * P * RT; e += kAdapterThreads) {
+          const int r = e / (P * RT), c = e % (P * RT);  // part c / RT, ranks 8 (c % RT) ..
+          const int in = step * kChunkRows + r;
+          const int row = in < total ? list[in] : 0;
+          const int rank = n0 + (c % RT) * 8;
+          copy8(to + Cfg::Z_BYTES + piece<P * RT>(r, c), side.hidden + ((long long)row * P + c / RT) * p.Rp + rank, side.hidden, true, in < total && rank < p.Rp ? 8 : 0);
+        }
+        cp_async_commit();
+      };
 #pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            za[m][0] = low_halves(raw[0][m], raw[1][m]);
-            za[m][1] = high_halves(raw[0][m], raw[1][m]);
-            za[m][2] = low_halves(raw[2][m], raw[3][m]);
-            za[m][3] = high_halves(raw[2][m], raw[3][m]);
-          }
+      for (int s = 0; s < STAGES - 1; ++s) {
+        if (s < steps) load(s);
+        else cp_async_commit();
+      }
+      for (int step = 0; step < steps; ++step) {
+        cp_async_wait<STAGES - 2>();
+        __syncthreads();
+        if (step + STAGES - 1 < steps) load(step + STAGES - 1);
+        else cp_async_commit();
+        const uint32_t from = base + (step % STAGES) * Cfg::STAGE_BYTES;
+        const int half = lane >> 4, in = lane & 15;
 #pragma unroll
-          for (int i = 0; i < RT; ++i)
+        for (int k = 0; k < 2; ++k) {
+          const int r = 32 * wk + 16 * k;
+          if (step * kChunkRows + r >= total) break;
+          uint32_t za[2][4];  // matrices (k 0-7, c 0-7), (k 0-7, c 8-15), (k 8-15, c 0-7), (k 8-15, c 8-15)
 #pragma unroll
-            for (int q = 0; q < P; ++q) {
-              const uint32_t h0 = hs[q][8 * k + 2 * t][i * 8 + g], h1 = hs[q][8 * k + 2 * t + 1][i * 8 + g];
+          for (int m = 0; m < 2; ++m) ldsm4_trans(from + piece<16>(r + (in & 7) + half * 8, 4 * wc + 2 * m + (in >> 3)), za[m]);
 #pragma unroll
-              for (int m = 0; m < 2; ++m) mma_bf16(acc[m][i], za[m][0], za[m][1], za[m][2], za[m][3], h0, h1);
+          for (int q = 0; q < P; ++q)
+#pragma unroll
+            for (int i = 0; i < RT; i += 2) {
+              uint32_t hf[4];
+              ldsm4_trans(from + Cfg::Z_BYTES + piece<P * RT>(r + in, q * RT + i + half), hf);
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                mma_bf16(acc[m][i], za[m][0], za[m][1], za[m][2], za[m][3], hf[0], hf[1]);
+                mma_bf16(acc[m][i + 1], za[m][0], za[m][1], za[m][2], za[m][3], hf[2], hf[3]);
+              }
             }
         }
       }
+      cp_async_wait<0>();
     }
-    float* part = p.part + ((long long)blockIdx.z * p.L + l) * p.C * p.Rp;
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(smem);  // [2 halves of the rows][128 columns][SUM_PITCH]
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int col = c + 2 * m + (e >> 1), r = n0 + i * 8 + 2 * t + (e & 1);
-          if (col < p.C && r < p.Rp) part[RANK_MAJOR ? (long long)r * p.C + col : (long long)col * p.Rp + r] = acc[m][i][e];
-        }
+        for (int e = 0; e < 4; ++e)
+          sums[(wk * kOuterCols + 32 * wc + 16 * m + g + (e >> 1) * 8) * Cfg::SUM_PITCH + i * 8 + 2 * t + (e & 1)] = acc[m][i][e];
     __syncthreads();
-  }
-}
-
-// out[l][i][j] = sum over the splits, in their order, of part[split][l][i][j]; j runs over `inner` of `pitch` entries of a row.
-__global__ void __launch_bounds__(256)
-adapter_reduce_kernel(const float* part, int splits, int L, int outer_used, int outer_n, int inner, int pitch, __nv_bfloat16* out) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const long long per = (long long)outer_used * inner, total = per * L;
-  const long long stride = (long long)L * outer_n * pitch;
-  for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (long long)gridDim.x * blockDim.x) {
-    const int l = int(e / per);
-    const long long in = e - l * per;
-    const int i = int(in / inner), j = int(in - (long long)i * inner);
-    const float* src = part + ((long long)l * outer_n + i) * pitch + j;
-    float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += src[s * stride];
-    out[e] = __float2bfloat16_rn(v);
+    if (splits > 1) {
+      cluster_arrive();
+      cluster_wait();
+    }
+    const int s0 = kOuterCols * split / splits, own = kOuterCols * (split + 1) / splits - s0;  // columns that this CTA finishes
+    for (int e = tid; e < own * COLS; e += kAdapterThreads) {
+      const int c = s0 + (side.rank_major ? e % own : e / COLS), r = side.rank_major ? e / own : e % COLS;
+      if (c0 + c >= side.C || n0 + r >= p.R) continue;
+      const int at = c * Cfg::SUM_PITCH + r;
+      float v = 0.f;
+      if (splits == 1) {
+        v = sums[at] + sums[kOuterCols * Cfg::SUM_PITCH + at];
+      } else {
+        const uint32_t a = smem_u32(sums + at);
+        float part[8][2];
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) part[s][h] = s < splits ? ld_cluster_f32(mapa_shared(a, s) + h * kOuterCols * Cfg::SUM_PITCH * 4) : 0.f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) v += part[s][0] + part[s][1];
+      }
+      side.out[side.rank_major ? ((long long)l * p.R + n0 + r) * side.C + c0 + c : ((long long)l * side.C + c0 + c) * p.R + n0 + r] = __float2bfloat16_rn(v);
+    }
+    if (splits > 1) {  // nobody overwrites what others still read
+      cluster_arrive();
+      cluster_wait();
+    }
+    __syncthreads();
   }
 }
 
