@@ -23,6 +23,7 @@ bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p
 int div_up(long long a, long long b) { return int((a + b - 1) / b); }
 int rank_pad(int R) { return (R + 15) / 16 * 16; }
 int chunks_of(int rows) { return div_up(rows, wb::kChunkRows); }
+bool few_rows(int rows) { return rows <= 64; }  // the kernels for few rows take them 32 at a time
 
 template <typename... P, typename... A>
 cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
@@ -81,8 +82,11 @@ int splits_for(long long units, int most) {
   while (s < 8 && 2 * s <= most && units * s < kTargetCtas * 2 / 3) s *= 2;
   return s;
 }
+// CTAs that share the groups of a chunk. Four at least where there are adapters enough: a chunk in which one sequence ends and another begins has two
+// groups, and as one CTA's work it took twice as long as the others (8192 rows of 6 sequences: 255 against 165 us); a CTA without a group
+// leaves at once.
 int group_lanes(int rows, int L, long long others) {
-  return rows <= wb::kChunkRows ? std::min(rows, L) : int(std::max(1ll, std::min<long long>(std::min(wb::kChunkRows, L), kTargetCtas / others)));
+  return few_rows(rows) ? std::min({rows, L, wb::kFewRows}) : int(std::max<long long>(std::min(4, L), std::min<long long>(std::min(wb::kChunkRows, L), kTargetCtas / others)));
 }
 
 struct AdapterCall {
@@ -113,8 +117,8 @@ int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int 
   wb::ShrinkParams p;
   p.x = x; p.w = w; p.ids = c.ids; p.scale = scale; p.hidden = hidden; p.ldx = ldx;
   p.rows = c.rows; p.K = K; p.R = c.R; p.Rp = c.Rp; p.L = c.L; p.parts = c.parts;
-  const bool few = c.rows <= wb::kChunkRows;
-  const int chunks = chunks_of(c.rows);
+  const bool few = few_rows(c.rows);
+  const int chunks = few ? div_up(c.rows, wb::kFewRows) : chunks_of(c.rows);
   const int splits = few ? splits_for(1, std::max(1, K / 512)) : splits_for(chunks, std::max(1, K / 256));
   p.split_k = div_up(div_up(K, splits), 64) * 64;
   const int vec = !trans ? 8 : !few ? 8 : c.Rp <= 16 ? 2 : c.Rp <= 32 ? 4 : 8;  // elements of a load of w
@@ -128,7 +132,7 @@ int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int 
 template <typename IdT, typename T, int P, int QN, bool TRANS>
 int launch_expand_tile(const wb::ExpandParams& p, dim3 grid, cudaStream_t s) {
   constexpr auto kernel = wb::adapter_expand_tile_kernel<IdT, T, P, QN, TRANS>;
-  const size_t smem = size_t(wb::kChunkRows) * (P * p.Rp + 8) * 2;
+  const size_t smem = size_t(wb::kChunkRows) * wb::expand_pitch(P, p.Rp) * 2;
   if (int rc = smem > 40 * 1024 ? allow_smem<kernel>() : WB200_OK) return rc;
   WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, smem, s, p));
   return WB200_OK;
@@ -148,8 +152,8 @@ int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const _
   wb::ExpandParams p;
   p.w = w; p.ids = c.ids; p.hidden = hidden; p.y = y; p.out = out; p.ldy = ldy; p.ldo = ldo;
   p.rows = c.rows; p.C = C; p.R = c.R; p.Rp = c.Rp; p.L = c.L;
-  const bool few = c.rows <= wb::kChunkRows;
-  const int chunks = chunks_of(c.rows);
+  const bool few = few_rows(c.rows);
+  const int chunks = few ? div_up(c.rows, wb::kFewRows) : chunks_of(c.rows);
   p.cols_per_cta = few ? 2 * wb::kAdapterThreads : 2048;
   if (!few)
     while (p.cols_per_cta > 256 && (long long)chunks * div_up(C, p.cols_per_cta) < kTargetCtas * 3 / 2) p.cols_per_cta /= 2;

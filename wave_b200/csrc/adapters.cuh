@@ -128,6 +128,32 @@ __device__ __forceinline__ int group_rows(RowGroups& g, const IdT* ids, int row0
   return groups;
 }
 
+// The same for a chunk of up to 32 rows, by every warp for itself: the rows of the n-th adapter (in the order of its first row) as a mask, 0 behind the
+// last one.
+constexpr int kFewRows = 32;
+struct FewRows {
+  unsigned rows, none;  // of the group; without an adapter
+  int adapter;
+};
+template <typename IdT>
+__device__ __forceinline__ FewRows few_rows(const IdT* ids, int row0, int rows, int L, int n) {
+  const int lane = threadIdx.x & 31;
+  const int mine = adapter_of(ids, row0 + lane, rows, L);
+  const unsigned same = __match_any_sync(0xffffffffu, mine);
+  const unsigned none = __ballot_sync(0xffffffffu, mine < 0 && row0 + lane < rows);
+  const bool first = mine >= 0 && lane == __ffs(same) - 1;
+  const unsigned leaders = __ballot_sync(0xffffffffu, first);
+  const bool picked = first && __popc(leaders & ((1u << lane) - 1u)) == n;
+  const int at = __ffs(__ballot_sync(0xffffffffu, picked)) - 1;
+  if (at < 0) return {0u, none, -1};
+  return {__shfl_sync(0xffffffffu, same, at), none, __shfl_sync(0xffffffffu, mine, at)};
+}
+// Place of the n-th bit that is set, -1 behind the last.
+__device__ __forceinline__ int nth_bit(unsigned mask, int n) {
+  for (int i = 0; i < n; ++i) mask &= mask - 1u;
+  return __ffs(mask) - 1;
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {  // zeros where not real
   const uint32_t bytes = real ? 16u : 0u;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -189,9 +215,9 @@ struct ShrinkParams {
 };
 
 // A split's sums of up to 64 rows and COLS ranks are in `sums` ([64][COLS + 1]) of every CTA of the cluster: this CTA adds up its share of the
-// rows over the splits, in their order, and writes the scaled bf16 parts.
-template <int COLS>
-__device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums, const RowGroups& groups, int row0, int first, int count, int n0, float scale) {
+// rows over the splits, in their order, and writes the scaled bf16 parts. row_of: row of x by its place.
+template <int COLS, typename RowOf>
+__device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums, RowOf row_of, int count, int n0, float scale) {
   __syncthreads();
   const int splits = gridDim.x, split = blockIdx.x;
   if (splits > 1) {
@@ -215,7 +241,7 @@ __device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums
     }
     __nv_bfloat16 part[3];
     split_bf16<3>(v * scale, part);
-    __nv_bfloat16* dst = p.hidden + (long long)(row0 + groups.order[first + row]) * p.parts * p.Rp + n0 + col;
+    __nv_bfloat16* dst = p.hidden + (long long)row_of(row) * p.parts * p.Rp + n0 + col;
 #pragma unroll
     for (int i = 0; i < 3; ++i)
       if (i < p.parts) dst[i * p.Rp] = part[i];
@@ -234,26 +260,25 @@ template <typename IdT, int RT, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads)
 adapter_shrink_few_kernel(const ShrinkParams p) {
   constexpr int KU = 2, COLS = RT * 8;
-  __shared__ RowGroups groups;
   __shared__ float red[kAdapterWarps][16][COLS + 2];
   __shared__ float sums[16 * (COLS + 1)];
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int row0 = blockIdx.y * kChunkRows;
-  const int ngroups = group_rows(groups, static_cast<const IdT*>(p.ids), row0, p.rows, p.L);
+  const int row0 = blockIdx.y * kFewRows;
   const int k0 = blockIdx.x * p.split_k, k1 = min(p.K, k0 + p.split_k);
-  for (int gi = blockIdx.z; gi < ngroups; gi += gridDim.z) {
-    const int end = groups.start[gi + 1];
-    const int l = groups.adapter[gi];
-    const __nv_bfloat16* w = p.w + (long long)l * p.R * p.K;
-    const float scale = p.scale ? p.scale[l] : 1.f;
-    for (int first = groups.start[gi]; first < end; first += 16) {
+  for (int gi = blockIdx.z;; gi += gridDim.z) {
+    const FewRows group = few_rows(static_cast<const IdT*>(p.ids), row0, p.rows, p.L, gi);
+    if (group.rows == 0u) break;
+    const __nv_bfloat16* w = p.w + (long long)group.adapter * p.R * p.K;
+    const float scale = p.scale ? p.scale[group.adapter] : 1.f;
+    const int end = __popc(group.rows);
+    for (int first = 0; first < end; first += 16) {
       const __nv_bfloat16* src[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int at = first + h * 8 + g;
-        src[h] = at < end ? p.x + (long long)(row0 + groups.order[at]) * p.ldx : nullptr;
+        const int at = nth_bit(group.rows, first + h * 8 + g);
+        src[h] = at >= 0 ? p.x + (long long)(row0 + at) * p.ldx : nullptr;
       }
       for (int n0 = 0; n0 < p.Rp; n0 += COLS) {
         float acc[RT][4] = {};
@@ -319,7 +344,7 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
           for (int i = 0; i < kAdapterWarps; ++i) v += red[i][row][col];
           sums[row * (COLS + 1) + col] = v;
         }
-        finish_hidden<COLS>(p, sums, groups, row0, first, min(16, end - first), n0, scale);
+        finish_hidden<COLS>(p, sums, [&](int row) { return row0 + nth_bit(group.rows, first + row); }, min(16, end - first), n0, scale);
       }
     }
   }
@@ -356,55 +381,100 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
     const int l = groups.adapter[gi];
     const __nv_bfloat16* w = p.w + (long long)l * p.R * p.K;
     const float scale = p.scale ? p.scale[l] : 1.f;
-    // rows tid / 8 and tid / 8 + 32 of x, 16-byte piece tid % 8
+    // A thread brings the same pieces of every stage: of rows tid / 8 and tid / 8 + 32 of x, and WN of w.
+    constexpr int WN = (RT * 64 + kAdapterThreads - 1) / kAdapterThreads;
     const int xr = tid >> 3, xc = tid & 7;
-    const __nv_bfloat16* src[2];
+    const __nv_bfloat16* row_of_x[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) src[h] = xr + 32 * h < count ? p.x + (long long)(row0 + groups.order[first + xr + 32 * h]) * p.ldx : nullptr;
+    for (int h = 0; h < 2; ++h) row_of_x[h] = xr + 32 * h < count ? p.x + (long long)(row0 + groups.order[first + xr + 32 * h]) * p.ldx + k0 + xc * 8 : nullptr;
     for (int n0 = 0; n0 < p.Rp; n0 += COLS) {
-      auto load = [&](int step) {
-        const uint32_t at = base + (step % STAGES) * Cfg::STAGE_BYTES;
-        const int kb = k0 + step * 64;
+      const __nv_bfloat16 *xsrc[2], *wsrc[WN];
+      int w_valid[WN], w_k[WN];  // ranks of a piece (TRANS); its k in a stage
+      uint32_t xdst[2], wdst[WN];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          copy8(at + piece<8>(xr + 32 * h, xc), src[h] + kb + xc * 8, p.x, p.x_vec != 0, src[h] ? min(8, k1 - kb - xc * 8) : 0);
+      for (int h = 0; h < 2; ++h) {
+        xsrc[h] = row_of_x[h];
+        xdst[h] = piece<8>(xr + 32 * h, xc);
+      }
+#pragma unroll
+      for (int i = 0; i < WN; ++i) {
+        const int e = tid + i * kAdapterThreads;
         if constexpr (!TRANS) {  // [rank][64 k]
-#pragma unroll
-          for (int e = tid; e < COLS * 8; e += kAdapterThreads) {
-            const int r = e >> 3, c = e & 7;
-            copy8(at + Cfg::X_BYTES + piece<8>(r, c), w + (long long)(n0 + r) * p.K + kb + c * 8, p.w, p.w_vec != 0, n0 + r < p.R ? min(8, k1 - kb - c * 8) : 0);
-          }
+          const int r = e >> 3, c = e & 7;
+          w_k[i] = c * 8;
+          w_valid[i] = e < COLS * 8 && n0 + r < p.R ? 8 : 0;
+          wsrc[i] = w + (long long)(n0 + r) * p.K + k0 + c * 8;
+          wdst[i] = Cfg::X_BYTES + piece<8>(r, c);
         } else {  // [k][ranks]
+          const int k = e / RT, c = e % RT;
+          w_k[i] = k;
+          w_valid[i] = e < 64 * RT ? min(8, p.R - n0 - c * 8) : 0;
+          wsrc[i] = w + (long long)(k0 + k) * p.R + n0 + c * 8;
+          wdst[i] = Cfg::X_BYTES + piece<RT>(k, c);
+        }
+      }
+      int left = k1 - k0;        // k that are not loaded yet
+      uint32_t to = base;        // stage of the next load
+      const long long w_step = TRANS ? 64ll * p.R : 64ll;
+      const bool fast = p.x_vec && p.w_vec;
+      auto load = [&]() {
+        if (fast && left >= 64) {  // whole pieces: nothing to look at but whether the row or rank is there
 #pragma unroll
-          for (int e = tid; e < 64 * RT; e += kAdapterThreads) {
-            const int k = e / RT, c = e % RT;
-            copy8(at + Cfg::X_BYTES + piece<RT>(k, c), w + (long long)(kb + k) * p.R + n0 + c * 8, p.w, p.w_vec != 0, kb + k < k1 ? min(8, p.R - n0 - c * 8) : 0);
+          for (int h = 0; h < 2; ++h) {
+            cp_async16(to + xdst[h], xsrc[h] ? xsrc[h] : p.x, xsrc[h] != nullptr);
+            if (xsrc[h]) xsrc[h] += 64;
+          }
+#pragma unroll
+          for (int i = 0; i < WN; ++i) {
+            if (RT * 64 < kAdapterThreads && tid >= RT * 64) break;
+            cp_async16(to + wdst[i], w_valid[i] > 0 ? wsrc[i] : p.w, w_valid[i] > 0);
+            wsrc[i] += w_step;
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            copy8(to + xdst[h], xsrc[h], p.x, p.x_vec != 0, xsrc[h] ? min(8, left - xc * 8) : 0);
+            if (xsrc[h]) xsrc[h] += 64;
+          }
+#pragma unroll
+          for (int i = 0; i < WN; ++i) {
+            if (RT * 64 < kAdapterThreads && tid >= RT * 64) break;
+            copy8(to + wdst[i], wsrc[i], p.w, p.w_vec != 0, TRANS ? (w_k[i] < left ? w_valid[i] : 0) : min(w_valid[i], left - w_k[i]));
+            wsrc[i] += w_step;
           }
         }
         cp_async_commit();
+        left -= 64;
+        to = to == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : to + Cfg::STAGE_BYTES;
       };
+      const int half = lane >> 4, in = lane & 15;
+      uint32_t xoff[2], woff[RT / 2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) xoff[m] = piece<8>(32 * wm + 16 * m + in, 2 * wq + half);
+#pragma unroll
+      for (int i = 0; i < RT; i += 2)
+        woff[i / 2] = Cfg::X_BYTES + (TRANS ? piece<RT>(16 * wq + in, i + half) : piece<8>(i * 8 + half * 8 + (in & 7), 2 * wq + (in >> 3)));
+      uint32_t from = base;
       float acc[2][RT][4] = {};
 #pragma unroll
       for (int s = 0; s < STAGES - 1; ++s) {
-        if (s < steps) load(s);
+        if (s < steps) load();
         else cp_async_commit();
       }
       for (int step = 0; step < steps; ++step) {
         cp_async_wait<STAGES - 2>();
         __syncthreads();
-        if (step + STAGES - 1 < steps) load(step + STAGES - 1);
+        if (step + STAGES - 1 < steps) load();
         else cp_async_commit();
         if (32 * wm < count) {
-          const uint32_t at = base + (step % STAGES) * Cfg::STAGE_BYTES;
-          const int half = lane >> 4, in = lane & 15;
           uint32_t xa[2][4];
 #pragma unroll
-          for (int m = 0; m < 2; ++m) ldsm4(at + piece<8>(32 * wm + 16 * m + in, 2 * wq + half), xa[m]);
+          for (int m = 0; m < 2; ++m) ldsm4(from + xoff[m], xa[m]);
 #pragma unroll
           for (int i = 0; i < RT; i += 2) {
             uint32_t wf[4];
-            if constexpr (!TRANS) ldsm4(at + Cfg::X_BYTES + piece<8>(i * 8 + half * 8 + (in & 7), 2 * wq + (in >> 3)), wf);
-            else ldsm4_trans(at + Cfg::X_BYTES + piece<RT>(16 * wq + in, i + half), wf);
+            if constexpr (!TRANS) ldsm4(from + woff[i / 2], wf);
+            else ldsm4_trans(from + woff[i / 2], wf);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
               mma_bf16(acc[m][i], xa[m][0], xa[m][1], xa[m][2], xa[m][3], wf[0], wf[1]);
@@ -412,6 +482,7 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
             }
           }
         }
+        from = from == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : from + Cfg::STAGE_BYTES;
       }
       cp_async_wait<0>();
       __syncthreads();
@@ -431,7 +502,7 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
         for (int q = 1; q < 4; ++q) v += sums[q * kChunkRows * (COLS + 1) + at];
         sums[at] = v;
       }
-      finish_hidden<COLS>(p, sums, groups, row0, first, count, n0, scale);
+      finish_hidden<COLS>(p, sums, [&](int row) { return row0 + groups.order[first + row]; }, count, n0, scale);
     }
   }
 }
@@ -491,21 +562,16 @@ __device__ __forceinline__ void write8(T* p, bool whole, int valid, const float 
 }
 
 
-// Rows without an adapter: y as it is (zeros where there is no y).
+// A row without an adapter: y as it is (zeros where there is no y).
 template <typename T>
-__device__ __forceinline__ void expand_rest(const ExpandParams& p, const RowGroups& groups, int row0, int c_begin, int c_end) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__device__ __forceinline__ void expand_rest(const ExpandParams& p, long long row, int c, int c_end, int step) {
   const T* y = static_cast<const T*>(p.y);
   T* out = static_cast<T*>(p.out);
-  if (p.out == p.y) return;
-  for (int row = warp; row < min(kChunkRows, p.rows - row0); row += kAdapterWarps) {
-    if (groups.id[row] >= 0) continue;
-    for (int c = c_begin + lane * 8; c < c_end; c += 256) {
-      const int valid = p.C - c;
-      float v[8] = {};
-      if (y) read8<T>(y + (row0 + row) * p.ldy + c, p.io_vec && valid >= 8, valid, v);
-      write8<T>(out + (row0 + row) * p.ldo + c, p.io_vec && valid >= 8, valid, v);
-    }
+  for (; c < c_end; c += step) {
+    const int valid = c_end - c;
+    float v[8] = {};
+    if (y) read8<T>(y + row * p.ldy + c, p.io_vec && valid >= 8, valid, v);
+    write8<T>(out + row * p.ldo + c, p.io_vec && valid >= 8, valid, v);
   }
 }
 
@@ -517,30 +583,51 @@ template <typename IdT, typename T, int P, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads)
 adapter_expand_few_kernel(const ExpandParams p) {
   constexpr int ROWS = 8;
-  __shared__ RowGroups groups;
   extern __shared__ __align__(16) float hs[];  // [ROWS][Rp]
   pdl_launch_dependents();
-  const int row0 = blockIdx.y * kChunkRows;
-  const int ngroups = group_rows(groups, static_cast<const IdT*>(p.ids), row0, p.rows, p.L);
+  const int row0 = blockIdx.y * kFewRows;
   const int c_begin = blockIdx.x * p.cols_per_cta, c_end = min(p.C, c_begin + p.cols_per_cta);
   const T* y = static_cast<const T*>(p.y);
   T* out = static_cast<T*>(p.out);
   const int c = c_begin + 2 * threadIdx.x;  // cols_per_cta is twice the number of threads
   const bool both = c + 1 < c_end;
   bool waited = false;
-  for (int gi = blockIdx.z; gi < ngroups; gi += gridDim.z) {
-    const __nv_bfloat16* w = p.w + (long long)groups.adapter[gi] * p.R * p.C;
-    const int end = groups.start[gi + 1];
-    for (int first = groups.start[gi]; first < end; first += ROWS) {
-      const int count = min(ROWS, end - first);
+  unsigned none = 0u;
+  for (int gi = blockIdx.z;; gi += gridDim.z) {
+    const FewRows group = few_rows(static_cast<const IdT*>(p.ids), row0, p.rows, p.L, gi);
+    none = group.none;
+    if (group.rows == 0u) break;
+    const __nv_bfloat16* w = p.w + (long long)group.adapter * p.R * p.C;
+    unsigned rest = group.rows;
+    while (rest != 0u) {
+      int row[ROWS];
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        row[i] = row0 + __ffs(rest) - 1;
+        count += rest != 0u;
+        rest &= rest - 1u;
+      }
       float acc[ROWS][2];
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         acc[i][0] = acc[i][1] = 0.f;
         if (y && i < count && c < c_end) {
-          const T* at = y + (long long)(row0 + groups.order[first + i]) * p.ldy + c;
-          acc[i][0] = as_f32<T>(at[0]);
-          if (both) acc[i][1] = as_f32<T>(at[1]);
+          const T* at = y + row[i] * p.ldy + c;
+          if (p.io_vec && both) {
+            if constexpr (sizeof(T) == 2) {
+              const uint32_t v = *reinterpret_cast<const uint32_t*>(at);
+              acc[i][0] = __uint_as_float(v << 16);
+              acc[i][1] = __uint_as_float(v & 0xffff0000u);
+            } else {
+              const float2 v = *reinterpret_cast<const float2*>(at);
+              acc[i][0] = v.x;
+              acc[i][1] = v.y;
+            }
+          } else {
+            acc[i][0] = as_f32<T>(at[0]);
+            if (both) acc[i][1] = as_f32<T>(at[1]);
+          }
         }
       }
       for (int r0 = 0; r0 < p.Rp; r0 += 16) {
@@ -575,8 +662,11 @@ adapter_expand_few_kernel(const ExpandParams p) {
           waited = true;
           __syncthreads();
           for (int e = threadIdx.x; e < count * p.Rp; e += kAdapterThreads) {
-            const int row = e / p.Rp, r = e - row * p.Rp;
-            const __nv_bfloat16* h = p.hidden + (long long)(row0 + groups.order[first + row]) * P * p.Rp + r;
+            const int in = e / p.Rp, r = e - in * p.Rp;
+            int from = row[0];
+#pragma unroll
+            for (int i = 1; i < ROWS; ++i) from = in == i ? row[i] : from;
+            const __nv_bfloat16* h = p.hidden + (long long)from * P * p.Rp + r;
             float v = 0.f;
 #pragma unroll
             for (int i = P - 1; i >= 0; --i) v += __bfloat162float(h[i * p.Rp]);
@@ -605,7 +695,7 @@ adapter_expand_few_kernel(const ExpandParams p) {
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         if (i >= count || c >= c_end) break;
-        T* at = out + (long long)(row0 + groups.order[first + i]) * p.ldo + c;
+        T* at = out + row[i] * p.ldo + c;
         if (p.io_vec && both) {
           if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(at) = pack_bf16x2(acc[i][0], acc[i][1]);
           else *reinterpret_cast<float2*>(at) = make_float2(acc[i][0], acc[i][1]);
@@ -617,8 +707,13 @@ adapter_expand_few_kernel(const ExpandParams p) {
     }
   }
   if (!waited) pdl_wait();  // (out may still be in use)
-  if (blockIdx.z == 0) expand_rest<T>(p, groups, row0, c_begin, c_end);
+  if (blockIdx.z == 0 && p.out != p.y)
+    for (; none != 0u; none &= none - 1u) expand_rest<T>(p, row0 + __ffs(none) - 1, c_begin + threadIdx.x * 8, c_end, kAdapterThreads * 8);
 }
+
+// Elements between the hidden vectors of rows in shared memory: 16 or 48 bytes past a multiple of 64, so that the 8-byte loads of 16 lanes (four rows)
+// fall into different banks.
+__host__ __device__ constexpr int expand_pitch(int parts, int Rp) { return parts * Rp + ((parts * Rp / 2) % 16 == 8 ? 0 : 16); }
 
 // Many rows: a warp takes 32 columns of all the rows of a group; a lane has 8 neighbouring columns of two rows of an MMA tile. The rows of y
 // are loaded ahead of everything else, all of a lane's at once, those of the next 32 columns while these are worked on.
@@ -627,10 +722,11 @@ template <typename IdT, typename T, int P, int QN, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads, sizeof(T) == 2 ? 2 : 1)
 adapter_expand_tile_kernel(const ExpandParams p) {
   constexpr int RAW = sizeof(T) == 2 ? 1 : 2;  // 16-byte pieces of 8 values
+  constexpr bool AHEAD = QN <= 2;               // w of the next columns is loaded ahead too: all ranks are in registers at a time (steps == QN)
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ RowGroups groups;
-  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem);  // [64][P][Rp] + 8 per row
-  const int pitch = P * p.Rp + 8;
+  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem);  // [64][P][Rp], rows `pitch` apart
+  const int pitch = expand_pitch(P, p.Rp);
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row0 = blockIdx.y * kChunkRows;
@@ -644,16 +740,19 @@ adapter_expand_tile_kernel(const ExpandParams p) {
     const int first = groups.start[gi], count = groups.start[gi + 1] - first;
     const __nv_bfloat16* w = p.w + (long long)groups.adapter[gi] * p.R * p.C;
     const int mtiles = (count + 15) >> 4;
-    int row[4][2];
+    int row[4][2];  // rows of y and out in front of the chunk's first; -1: none
 #pragma unroll
     for (int m = 0; m < 4; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = m * 16 + h * 8 + g;
-        row[m][h] = at < count ? row0 + groups.order[first + at] : -1;
+        row[m][h] = at < count ? groups.order[first + at] : -1;
       }
+    const T* y0 = y + row0 * p.ldy;
+    T* out0 = out + row0 * p.ldo;
     uint4 old[4][2][RAW];
     auto load_y = [&](int col) {  // 8 values of every row, where they are whole
+      const bool there = y && p.io_vec && col + 8 <= c_end;
 #pragma unroll
       for (int m = 0; m < 4; ++m)
 #pragma unroll
@@ -661,13 +760,36 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
           for (int i = 0; i < RAW; ++i) {
             old[m][h][i] = make_uint4(0u, 0u, 0u, 0u);
-            if (y && p.io_vec && row[m][h] >= 0 && col + 8 <= c_end) old[m][h][i] = *(reinterpret_cast<const uint4*>(y + row[m][h] * p.ldy + col) + i);
+            if (there && row[m][h] >= 0) old[m][h][i] = *(reinterpret_cast<const uint4*>(y0 + row[m][h] * p.ldy + col) + i);
           }
     };
     const int c_first = c_begin + warp * kExpandCols;
     load_y(c_first + 8 * t);
     uint32_t wf[4][QN][2];
     auto load_w = [&](int c0, int q0) {
+      if (p.w_vec && c0 + kExpandCols <= p.C && (q0 + QN) * 16 <= p.R) {  // all there
+        const __nv_bfloat16* at = TRANS ? w + (long long)(q0 * 16 + 4 * t) * p.C + c0 + 4 * g : w + (long long)(c0 + 8 * (g >> 1) + (g & 1)) * p.R + q0 * 16 + 4 * t;
+#pragma unroll
+        for (int q = 0; q < QN; ++q) {
+          if constexpr (!TRANS) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint2 v = *reinterpret_cast<const uint2*>(at + i * (2 * p.R) + q * 16);
+              wf[i][q][0] = v.x;
+              wf[i][q][1] = v.y;
+            }
+          } else {
+            uint2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint2*>(at + (long long)(q * 16 + i) * p.C);
+            wf[0][q][0] = low_halves(v[0].x, v[1].x); wf[0][q][1] = low_halves(v[2].x, v[3].x);
+            wf[1][q][0] = high_halves(v[0].x, v[1].x); wf[1][q][1] = high_halves(v[2].x, v[3].x);
+            wf[2][q][0] = low_halves(v[0].y, v[1].y); wf[2][q][1] = low_halves(v[2].y, v[3].y);
+            wf[3][q][0] = high_halves(v[0].y, v[1].y); wf[3][q][1] = high_halves(v[2].y, v[3].y);
+          }
+        }
+        return;
+      }
 #pragma unroll
       for (int q = 0; q < QN; ++q) {
         const int r = (q0 + q) * 16 + 4 * t;
@@ -694,6 +816,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
         }
       }
     };
+    if (AHEAD) load_w(c_first, 0);
     if (!waited) pdl_wait();  // for the hidden vectors; y and w are complete before the kernel that makes those starts
     waited = true;
     __syncthreads();
@@ -710,7 +833,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
       const int col = c0 + 8 * t;
       const int valid = c_end - col;
       const bool whole = p.io_vec && valid >= 8;
-      load_w(c0, 0);
+      if (!AHEAD) load_w(c0, 0);
       uint4 now[4][2][RAW];
 #pragma unroll
       for (int m = 0; m < 4; ++m)
@@ -718,7 +841,18 @@ adapter_expand_tile_kernel(const ExpandParams p) {
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < RAW; ++i) now[m][h][i] = old[m][h][i];
-      if (c0 + kAdapterWarps * kExpandCols < c_end) load_y(col + kAdapterWarps * kExpandCols);
+      uint32_t wn[4][QN][2];
+      if constexpr (AHEAD) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int q = 0; q < QN; ++q) { wn[i][q][0] = wf[i][q][0]; wn[i][q][1] = wf[i][q][1]; }
+      }
+      if (c0 + kAdapterWarps * kExpandCols < c_end) {
+        load_y(col + kAdapterWarps * kExpandCols);
+        if (AHEAD) load_w(c0 + kAdapterWarps * kExpandCols, 0);
+      }
+      auto& wu = AHEAD ? wn : wf;
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
         if (m >= mtiles) break;
@@ -734,7 +868,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
               const uint2 lo = *reinterpret_cast<const uint2*>(at + i * p.Rp);
               const uint2 hi = *reinterpret_cast<const uint2*>(at + 8 * pitch + i * p.Rp);
 #pragma unroll
-              for (int n = 0; n < 4; ++n) mma_bf16(acc[n], lo.x, hi.x, lo.y, hi.y, wf[n][q][0], wf[n][q][1]);
+              for (int n = 0; n < 4; ++n) mma_bf16(acc[n], lo.x, hi.x, lo.y, hi.y, wu[n][q][0], wu[n][q][1]);
             }
           }
         }
@@ -746,19 +880,21 @@ adapter_expand_tile_kernel(const ExpandParams p) {
             read8<T>(reinterpret_cast<const T*>(now[m][h]), true, 8, v);
           } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = y && i < valid ? as_f32<T>(y[row[m][h] * p.ldy + col + i]) : 0.f;
+            for (int i = 0; i < 8; ++i) v[i] = y && i < valid ? as_f32<T>(y0[row[m][h] * p.ldy + col + i]) : 0.f;
           }
 #pragma unroll
           for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) v[TRANS ? 4 * j + n : 2 * n + j] += acc[n][2 * h + j];
-          write8<T>(out + row[m][h] * p.ldo + col, whole, valid, v);
+          write8<T>(out0 + row[m][h] * p.ldo + col, whole, valid, v);
         }
       }
     }
   }
   if (!waited) pdl_wait();
-  if (blockIdx.z == 0) expand_rest<T>(p, groups, row0, c_begin, c_end);
+  if (blockIdx.z == 0 && p.out != p.y)
+    for (int r = warp; r < min(kChunkRows, p.rows - row0); r += kAdapterWarps)
+      if (groups.id[r] < 0) expand_rest<T>(p, row0 + r, c_begin + lane * 8, c_end, 256);
 }
 
 struct OuterSide {
@@ -817,9 +953,20 @@ adapter_outer_kernel(const OuterParams p) {
       const int seg_end = min(row_end, seg + kOuterSegment);
       const int run = (seg_end - seg + kAdapterThreads - 1) / kAdapterThreads * 32;
       const int w0 = seg + warp * run, w1 = min(seg_end, w0 + run);
+      constexpr int RUN = kOuterSegment / kAdapterThreads;  // 32-id steps of a full run
+      unsigned hits[RUN];
       int mine = 0;
       __syncthreads();
-      for (int i = w0; i < w1; i += 32) mine += __popc(__ballot_sync(0xffffffffu, i + lane < w1 && adapter_of(ids, i + lane, p.rows, p.L) == l));
+#pragma unroll
+      for (int i = 0; i < RUN; ++i) {  // all of a lane's loads in flight together
+        const int at = w0 + 32 * i + lane;
+        hits[i] = at < w1 && adapter_of(ids, at, p.rows, p.L) == l;
+      }
+#pragma unroll
+      for (int i = 0; i < RUN; ++i) {
+        hits[i] = __ballot_sync(0xffffffffu, hits[i]);
+        mine += __popc(hits[i]);
+      }
       if (lane == 0) found[warp] = mine;
       __syncthreads();
       int at = 0, total = 0;
@@ -828,44 +975,51 @@ adapter_outer_kernel(const OuterParams p) {
         at += i < warp ? found[i] : 0;
         total += found[i];
       }
-      for (int i = w0; i < w1; i += 32) {
-        const bool hit = i + lane < w1 && adapter_of(ids, i + lane, p.rows, p.L) == l;
-        const unsigned hits = __ballot_sync(0xffffffffu, hit);
-        if (hit) list[at + __popc(hits & ((1u << lane) - 1u))] = i + lane;
-        at += __popc(hits);
+#pragma unroll
+      for (int i = 0; i < RUN; ++i) {
+        if (hits[i] >> lane & 1u) list[at + __popc(hits[i] & ((1u << lane) - 1u))] = w0 + 32 * i + lane;
+        at += __popc(hits[i]);
       }
       __syncthreads();
       const int steps = (total + kChunkRows - 1) / kChunkRows;
-      auto load = [&](int step) {
-        const uint32_t to = base + (step % STAGES) * Cfg::STAGE_BYTES;
+      // A thread brings the same pieces of every stage: column piece tid % 16 of rows tid / 16 + 16 i of z, and HN pieces of the hidden vectors
+      constexpr int ZN = kChunkRows * (kOuterCols / 8) / kAdapterThreads, HN = (kChunkRows * P * RT + kAdapterThreads - 1) / kAdapterThreads;
+      const int zr = tid >> 4, zc = tid & 15;
+      const int z_valid = min(8, side.C - c0 - zc * 8);
+      const __nv_bfloat16* z_at = side.z + c0 + zc * 8;
+      int next = 0;         // place in the list of the first row of the next load
+      uint32_t to = base;   // its stage
+      auto load = [&]() {
 #pragma unroll
-        for (int e = tid; e < kChunkRows * (kOuterCols / 8); e += kAdapterThreads) {
-          const int r = e >> 4, c = e & 15;
-          const int in = step * kChunkRows + r;
-          const int row = in < total ? list[in] : 0;
-          copy8(to + piece<16>(r, c), side.z + row * side.ldz + c0 + c * 8, side.z, side.vec != 0, in < total ? min(8, side.C - c0 - c * 8) : 0);
+        for (int i = 0; i < ZN; ++i) {
+          const int in = next + zr + 16 * i;
+          const bool real = in < total;
+          copy8(to + piece<16>(zr + 16 * i, zc), real ? z_at + list[in] * side.ldz : z_at, side.z, side.vec != 0, real ? z_valid : 0);
         }
 #pragma unroll
-        for (int e = tid; e < kChunkRows * P * RT; e += kAdapterThreads) {
+        for (int i = 0; i < HN; ++i) {
+          const int e = tid + i * kAdapterThreads;
+          if (kChunkRows * P * RT < kAdapterThreads && e >= kChunkRows * P * RT) break;
           const int r = e / (P * RT), c = e % (P * RT);  // part c / RT, ranks 8 (c % RT) ..
-          const int in = step * kChunkRows + r;
-          const int row = in < total ? list[in] : 0;
           const int rank = n0 + (c % RT) * 8;
-          copy8(to + Cfg::Z_BYTES + piece<P * RT>(r, c), side.hidden + ((long long)row * P + c / RT) * p.Rp + rank, side.hidden, true, in < total && rank < p.Rp ? 8 : 0);
+          const bool real = next + r < total && rank < p.Rp;
+          cp_async16(to + Cfg::Z_BYTES + piece<P * RT>(r, c), real ? side.hidden + ((long long)list[next + r] * P + c / RT) * p.Rp + rank : side.hidden, real);
         }
         cp_async_commit();
+        next += kChunkRows;
+        to = to == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : to + Cfg::STAGE_BYTES;
       };
 #pragma unroll
       for (int s = 0; s < STAGES - 1; ++s) {
-        if (s < steps) load(s);
+        if (s < steps) load();
         else cp_async_commit();
       }
+      uint32_t from = base;
       for (int step = 0; step < steps; ++step) {
         cp_async_wait<STAGES - 2>();
         __syncthreads();
-        if (step + STAGES - 1 < steps) load(step + STAGES - 1);
+        if (step + STAGES - 1 < steps) load();
         else cp_async_commit();
-        const uint32_t from = base + (step % STAGES) * Cfg::STAGE_BYTES;
         const int half = lane >> 4, in = lane & 15;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -887,6 +1041,7 @@ adapter_outer_kernel(const OuterParams p) {
               }
             }
         }
+        from = from == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : from + Cfg::STAGE_BYTES;
       }
       cp_async_wait<0>();
     }
