@@ -129,11 +129,11 @@ int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int 
   return trans ? launch_shrink_ranks<int, true>(p, few, grid, c.stream) : launch_shrink_ranks<int, false>(p, few, grid, c.stream);
 }
 
-template <typename IdT, typename T, int P, int QN, bool TRANS>
+template <typename IdT, typename T, int P, int QN, bool TRANS, bool VEC>
 int launch_expand_tile(const wb::ExpandParams& p, dim3 grid, cudaStream_t s) {
-  constexpr auto kernel = wb::adapter_expand_tile_kernel<IdT, T, P, QN, TRANS>;
+  constexpr auto kernel = wb::adapter_expand_tile_kernel<IdT, T, P, QN, TRANS, VEC>;
   const size_t smem = size_t(wb::kChunkRows) * wb::expand_pitch(P, p.Rp) * 2;
-  if (int rc = smem > 40 * 1024 ? allow_smem<kernel>() : WB200_OK) return rc;
+  if (int rc = smem > 24 * 1024 ? allow_smem<kernel>() : WB200_OK) return rc;
   WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, smem, s, p));
   return WB200_OK;
 }
@@ -144,7 +144,9 @@ int launch_expand(const wb::ExpandParams& p, bool few, dim3 grid, cudaStream_t s
     return WB200_OK;
   }
   const int steps = p.Rp / 16;
-  return steps == 1 ? launch_expand_tile<IdT, T, P, 1, TRANS>(p, grid, s) : steps == 2 ? launch_expand_tile<IdT, T, P, 2, TRANS>(p, grid, s) : launch_expand_tile<IdT, T, P, 4, TRANS>(p, grid, s);
+  if (p.io_vec)
+    return steps == 1 ? launch_expand_tile<IdT, T, P, 1, TRANS, true>(p, grid, s) : steps == 2 ? launch_expand_tile<IdT, T, P, 2, TRANS, true>(p, grid, s) : launch_expand_tile<IdT, T, P, 4, TRANS, true>(p, grid, s);
+  return steps == 1 ? launch_expand_tile<IdT, T, P, 1, TRANS, false>(p, grid, s) : steps == 2 ? launch_expand_tile<IdT, T, P, 2, TRANS, false>(p, grid, s) : launch_expand_tile<IdT, T, P, 4, TRANS, false>(p, grid, s);
 }
 
 // out = y + ranks onto C columns.
@@ -154,9 +156,9 @@ int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const _
   p.rows = c.rows; p.C = C; p.R = c.R; p.Rp = c.Rp; p.L = c.L;
   const bool few = few_rows(c.rows);
   const int chunks = few ? div_up(c.rows, wb::kFewRows) : chunks_of(c.rows);
-  p.cols_per_cta = few ? 2 * wb::kAdapterThreads : 2048;
-  if (!few)
-    while (p.cols_per_cta > 256 && (long long)chunks * div_up(C, p.cols_per_cta) < kTargetCtas * 3 / 2) p.cols_per_cta /= 2;
+  // one wave of CTAs where that leaves each several rounds of its 256 columns: what a CTA does before its first column (grouping, hidden vectors)
+  // takes as long as a few rounds
+  p.cols_per_cta = few ? 2 * wb::kAdapterThreads : div_up(div_up(C, std::max(1, kTargetCtas / chunks)), 256) * 256;
   const size_t esz = f32 ? 4 : 2;
   p.io_vec = aligned_to(out, 16) && ldo * esz % 16 == 0 && (!y || (aligned_to(y, 16) && ldy * esz % 16 == 0));
   const int vec = few ? (trans ? 2 : 8) : 4;  // elements of a load of w

@@ -715,16 +715,19 @@ adapter_expand_few_kernel(const ExpandParams p) {
 // fall into different banks.
 __host__ __device__ constexpr int expand_pitch(int parts, int Rp) { return parts * Rp + ((parts * Rp / 2) % 16 == 8 ? 0 : 16); }
 
-// Many rows: a warp takes 32 columns of all the rows of a group; a lane has 8 neighbouring columns of two rows of an MMA tile. The rows of y
-// are loaded ahead of everything else, all of a lane's at once, those of the next 32 columns while these are worked on.
+// Many rows: a warp takes 32 columns of all the rows of a group; a lane has 8 neighbouring columns of two rows of an MMA tile. The values of y are
+// loaded ahead of everything else, a batch of rows (MB tiles of 16) at once, the next batch while this one is worked on; w of the next columns
+// with it. Rows that do not start on 16 bytes go through shared memory instead, so that 32 lanes share a row's 32 columns.
 // QN: steps of 16 ranks of w in registers at a time.
-template <typename IdT, typename T, int P, int QN, bool TRANS>
-__global__ void __launch_bounds__(kAdapterThreads, sizeof(T) == 2 ? 2 : 1)
+template <typename IdT, typename T, int P, int QN, bool TRANS, bool VEC>
+__global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_expand_tile_kernel(const ExpandParams p) {
-  constexpr int RAW = sizeof(T) == 2 ? 1 : 2;  // 16-byte pieces of 8 values
-  constexpr bool AHEAD = QN <= 2;               // w of the next columns is loaded ahead too: all ranks are in registers at a time (steps == QN)
+  constexpr int RAW = sizeof(T) == 2 ? 1 : 2;    // 16-byte pieces of 8 values
+  constexpr int MB = sizeof(T) == 2 ? 4 : 2;     // tiles of 16 rows in a batch
+  constexpr bool AHEAD = QN <= 2;                // all ranks of w are in registers at a time (steps == QN)
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ RowGroups groups;
+  __shared__ float staged[VEC ? 1 : kAdapterWarps][VEC ? 1 : 16][VEC ? 1 : kExpandCols + 1];
   __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem);  // [64][P][Rp], rows `pitch` apart
   const int pitch = expand_pitch(P, p.Rp);
   pdl_launch_dependents();
@@ -732,39 +735,39 @@ adapter_expand_tile_kernel(const ExpandParams p) {
   const int row0 = blockIdx.y * kChunkRows;
   const int ngroups = group_rows(groups, static_cast<const IdT*>(p.ids), row0, p.rows, p.L);
   const int c_begin = blockIdx.x * p.cols_per_cta, c_end = min(p.C, c_begin + p.cols_per_cta);
-  const T* y = static_cast<const T*>(p.y);
-  T* out = static_cast<T*>(p.out);
+  constexpr int STEP = kAdapterWarps * kExpandCols;
+  const T* y = static_cast<const T*>(p.y) + row0 * p.ldy;
+  T* out = static_cast<T*>(p.out) + row0 * p.ldo;
   const int steps = p.Rp / 16;
   bool waited = false;
   for (int gi = blockIdx.z; gi < ngroups; gi += gridDim.z) {
     const int first = groups.start[gi], count = groups.start[gi + 1] - first;
     const __nv_bfloat16* w = p.w + (long long)groups.adapter[gi] * p.R * p.C;
     const int mtiles = (count + 15) >> 4;
-    int row[4][2];  // rows of y and out in front of the chunk's first; -1: none
+    auto row_at = [&](int place) { return place < count ? groups.order[first + place] : -1; };
+    int row[4][2];  // in the chunk; -1: none
 #pragma unroll
     for (int m = 0; m < 4; ++m)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int at = m * 16 + h * 8 + g;
-        row[m][h] = at < count ? groups.order[first + at] : -1;
-      }
-    const T* y0 = y + row0 * p.ldy;
-    T* out0 = out + row0 * p.ldo;
-    uint4 old[4][2][RAW];
-    auto load_y = [&](int col) {  // 8 values of every row, where they are whole
-      const bool there = y && p.io_vec && col + 8 <= c_end;
+      for (int h = 0; h < 2; ++h) row[m][h] = row_at(m * 16 + h * 8 + g);
+    uint4 next[MB][2][RAW];
+    auto load_y = [&](int col, int batch) {  // 8 values of every row of the batch, where they are whole
+      const bool there = VEC && p.y && col + 8 <= c_end;
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+      for (int m = 0; m < MB; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+          int r = row[m][h];
+#pragma unroll
+          for (int b = 1; b < 4 / MB; ++b)
+            if (b == batch) r = row[b * MB + m][h];
 #pragma unroll
           for (int i = 0; i < RAW; ++i) {
-            old[m][h][i] = make_uint4(0u, 0u, 0u, 0u);
-            if (there && row[m][h] >= 0) old[m][h][i] = *(reinterpret_cast<const uint4*>(y0 + row[m][h] * p.ldy + col) + i);
+            next[m][h][i] = make_uint4(0u, 0u, 0u, 0u);
+            if (there && r >= 0) next[m][h][i] = *(reinterpret_cast<const uint4*>(y + r * p.ldy + col) + i);
           }
+        }
     };
-    const int c_first = c_begin + warp * kExpandCols;
-    load_y(c_first + 8 * t);
     uint32_t wf[4][QN][2];
     auto load_w = [&](int c0, int q0) {
       if (p.w_vec && c0 + kExpandCols <= p.C && (q0 + QN) * 16 <= p.R) {  // all there
@@ -816,6 +819,8 @@ adapter_expand_tile_kernel(const ExpandParams p) {
         }
       }
     };
+    const int c_first = c_begin + warp * kExpandCols;
+    load_y(c_first + 8 * t, 0);
     if (AHEAD) load_w(c_first, 0);
     if (!waited) pdl_wait();  // for the hidden vectors; y and w are complete before the kernel that makes those starts
     waited = true;
@@ -829,64 +834,92 @@ adapter_expand_tile_kernel(const ExpandParams p) {
     cp_async_commit();
     cp_async_wait<0>();
     __syncthreads();
-    for (int c0 = c_first; c0 < c_end; c0 += kAdapterWarps * kExpandCols) {
+    for (int c0 = c_first; c0 < c_end; c0 += STEP) {
       const int col = c0 + 8 * t;
       const int valid = c_end - col;
-      const bool whole = p.io_vec && valid >= 8;
+      const bool whole = VEC && valid >= 8;
       if (!AHEAD) load_w(c0, 0);
-      uint4 now[4][2][RAW];
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < RAW; ++i) now[m][h][i] = old[m][h][i];
       uint32_t wn[4][QN][2];
       if constexpr (AHEAD) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int q = 0; q < QN; ++q) { wn[i][q][0] = wf[i][q][0]; wn[i][q][1] = wf[i][q][1]; }
-      }
-      if (c0 + kAdapterWarps * kExpandCols < c_end) {
-        load_y(col + kAdapterWarps * kExpandCols);
-        if (AHEAD) load_w(c0 + kAdapterWarps * kExpandCols, 0);
+        if (c0 + STEP < c_end) load_w(c0 + STEP, 0);
       }
       auto& wu = AHEAD ? wn : wf;
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        if (m >= mtiles) break;
-        float acc[4][4] = {};
-        for (int q0 = 0; q0 < steps; q0 += QN) {
-          if (steps > QN && (q0 > 0 || m > 0)) load_w(c0, q0);
+      for (int batch = 0; batch < 4 / MB; ++batch) {
+        if (batch * MB >= mtiles) break;
+        uint4 now[MB][2][RAW];
 #pragma unroll
-          for (int q = 0; q < QN; ++q) {
-            if (q0 + q >= steps) break;
-            const __nv_bfloat16* at = hs + (m * 16 + g) * pitch + (q0 + q) * 16 + 4 * t;
+        for (int m = 0; m < MB; ++m)
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-              const uint2 lo = *reinterpret_cast<const uint2*>(at + i * p.Rp);
-              const uint2 hi = *reinterpret_cast<const uint2*>(at + 8 * pitch + i * p.Rp);
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int n = 0; n < 4; ++n) mma_bf16(acc[n], lo.x, hi.x, lo.y, hi.y, wu[n][q][0], wu[n][q][1]);
-            }
-          }
+            for (int i = 0; i < RAW; ++i) now[m][h][i] = next[m][h][i];
+        if (VEC) {
+          if ((batch + 1) * MB < mtiles) load_y(col, batch + 1);
+          else if (c0 + STEP < c_end) load_y(col + STEP, 0);
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (row[m][h] < 0 || valid <= 0) continue;
-          float v[8];
-          if (whole) {
-            read8<T>(reinterpret_cast<const T*>(now[m][h]), true, 8, v);
-          } else {
+        for (int mm = 0; mm < MB; ++mm) {
+          const int m = batch * MB + mm;
+          if (m >= mtiles) break;
+          float acc[4][4] = {};
+          for (int q0 = 0; q0 < steps; q0 += QN) {
+            if (steps > QN && (q0 > 0 || m > 0)) load_w(c0, q0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = y && i < valid ? as_f32<T>(y0[row[m][h] * p.ldy + col + i]) : 0.f;
+            for (int q = 0; q < QN; ++q) {
+              if (q0 + q >= steps) break;
+              const __nv_bfloat16* at = hs + (m * 16 + g) * pitch + (q0 + q) * 16 + 4 * t;
+#pragma unroll
+              for (int i = 0; i < P; ++i) {
+                const uint2 lo = *reinterpret_cast<const uint2*>(at + i * p.Rp);
+                const uint2 hi = *reinterpret_cast<const uint2*>(at + 8 * pitch + i * p.Rp);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) mma_bf16(acc[n], lo.x, hi.x, lo.y, hi.y, wu[n][q][0], wu[n][q][1]);
+              }
+            }
           }
+          if constexpr (VEC) {
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
+            for (int h = 0; h < 2; ++h) {
+              if (row[m][h] < 0 || valid <= 0) continue;
+              float v[8];
+              if (whole) {
+                read8<T>(reinterpret_cast<const T*>(now[mm][h]), true, 8, v);
+              } else {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) v[TRANS ? 4 * j + n : 2 * n + j] += acc[n][2 * h + j];
-          write8<T>(out0 + row[m][h] * p.ldo + col, whole, valid, v);
+                for (int i = 0; i < 8; ++i) v[i] = p.y && i < valid ? as_f32<T>(y[row[m][h] * p.ldy + col + i]) : 0.f;
+              }
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) v[TRANS ? 4 * j + n : 2 * n + j] += acc[n][2 * h + j];
+              write8<T>(out + row[m][h] * p.ldo + col, whole, valid, v);
+            }
+          } else {
+            float (*mine)[kExpandCols + 1] = staged[warp];
+            __syncwarp();
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mine[g + (e >> 1) * 8][8 * t + (TRANS ? 4 * (e & 1) + n : 2 * n + (e & 1))] = acc[n][e];
+            __syncwarp();
+            const bool there = c0 + lane < c_end;
+            float v[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int at = row_at(m * 16 + r);
+              v[r] = there && p.y && at >= 0 ? as_f32<T>(y[at * p.ldy + c0 + lane]) : 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int at = row_at(m * 16 + r);
+              if (there && at >= 0) out[at * p.ldo + c0 + lane] = as_out<T>(v[r] + mine[r][lane]);
+            }
+          }
         }
       }
     }
@@ -989,7 +1022,23 @@ adapter_outer_kernel(const OuterParams p) {
       const __nv_bfloat16* z_at = side.z + c0 + zc * 8;
       int next = 0;         // place in the list of the first row of the next load
       uint32_t to = base;   // its stage
+      const bool fast = side.vec && c0 + kOuterCols <= side.C && n0 + COLS <= p.Rp;
+      const int hr = tid / (P * RT), hc = tid % (P * RT);
+      const __nv_bfloat16* h_at = side.hidden + (hc / RT) * p.Rp + n0 + (hc % RT) * 8;
+      constexpr int H_ROWS = kAdapterThreads / (P * RT);  // between the pieces of a thread
       auto load = [&]() {
+        if (fast && next + kChunkRows <= total) {  // whole pieces of 64 rows
+#pragma unroll
+          for (int i = 0; i < ZN; ++i) cp_async16(to + piece<16>(zr + 16 * i, zc), z_at + list[next + zr + 16 * i] * side.ldz, true);
+#pragma unroll
+          for (int i = 0; i < HN; ++i)
+            if (hr + i * H_ROWS < kChunkRows)
+              cp_async16(to + Cfg::Z_BYTES + piece<P * RT>(hr + i * H_ROWS, hc), h_at + (long long)list[next + hr + i * H_ROWS] * (P * p.Rp), true);
+          cp_async_commit();
+          next += kChunkRows;
+          to = to == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : to + Cfg::STAGE_BYTES;
+          return;
+        }
 #pragma unroll
         for (int i = 0; i < ZN; ++i) {
           const int in = next + zr + 16 * i;
