@@ -90,26 +90,25 @@ int group_lanes(int rows, int L, long long others) {
 }
 
 struct AdapterCall {
-  const void* ids;
-  bool wide_ids;
+  wb::Ids ids;
   int rows, R, Rp, L, parts;
   cudaStream_t stream;
 };
 
-template <typename IdT, int RT, bool TRANS>
+template <int RT, bool TRANS>
 int launch_shrink(const wb::ShrinkParams& p, bool few, dim3 grid, cudaStream_t s) {
   if (few) {
-    WB_HOST_CUDA(launch_clusters(wb::adapter_shrink_few_kernel<IdT, RT, TRANS>, grid, wb::kAdapterThreads, 0, s, p));
+    WB_HOST_CUDA(launch_clusters(wb::adapter_shrink_few_kernel<RT, TRANS>, grid, wb::kAdapterThreads, 0, s, p));
     return WB200_OK;
   }
-  constexpr auto kernel = wb::adapter_shrink_tile_kernel<IdT, RT, TRANS>;
+  constexpr auto kernel = wb::adapter_shrink_tile_kernel<RT, TRANS>;
   if (int rc = allow_smem<kernel>()) return rc;
   WB_HOST_CUDA(launch_clusters(kernel, grid, wb::kAdapterThreads, wb::ShrinkTile<RT>::SMEM_BYTES, s, p));
   return WB200_OK;
 }
-template <typename IdT, bool TRANS>
+template <bool TRANS>
 int launch_shrink_ranks(const wb::ShrinkParams& p, bool few, dim3 grid, cudaStream_t s) {
-  return p.Rp <= 16 ? launch_shrink<IdT, 2, TRANS>(p, few, grid, s) : p.Rp <= 32 ? launch_shrink<IdT, 4, TRANS>(p, few, grid, s) : launch_shrink<IdT, 8, TRANS>(p, few, grid, s);
+  return p.Rp <= 16 ? launch_shrink<2, TRANS>(p, few, grid, s) : p.Rp <= 32 ? launch_shrink<4, TRANS>(p, few, grid, s) : launch_shrink<8, TRANS>(p, few, grid, s);
 }
 
 // hidden [rows][parts][Rp] = rows of x onto the ranks, scaled. trans: w is [L][K][R].
@@ -125,28 +124,27 @@ int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int 
   p.x_vec = aligned_to(x, 16) && ldx % 8 == 0 && K % 8 == 0;
   p.w_vec = aligned_to(w, 2 * vec) && (trans ? c.R : K) % vec == 0;
   const dim3 grid(splits, chunks, group_lanes(c.rows, c.L, (long long)chunks * splits));
-  if (c.wide_ids) return trans ? launch_shrink_ranks<long long, true>(p, few, grid, c.stream) : launch_shrink_ranks<long long, false>(p, few, grid, c.stream);
-  return trans ? launch_shrink_ranks<int, true>(p, few, grid, c.stream) : launch_shrink_ranks<int, false>(p, few, grid, c.stream);
+  return trans ? launch_shrink_ranks<true>(p, few, grid, c.stream) : launch_shrink_ranks<false>(p, few, grid, c.stream);
 }
 
-template <typename IdT, typename T, int P, int QN, bool TRANS, bool VEC>
+template <typename T, int P, int QN, bool TRANS, bool FAST>
 int launch_expand_tile(const wb::ExpandParams& p, dim3 grid, cudaStream_t s) {
-  constexpr auto kernel = wb::adapter_expand_tile_kernel<IdT, T, P, QN, TRANS, VEC>;
+  constexpr auto kernel = wb::adapter_expand_tile_kernel<T, P, QN, TRANS, FAST>;
   const size_t smem = size_t(wb::kChunkRows) * wb::expand_pitch(P, p.Rp) * 2;
   if (int rc = smem > 24 * 1024 ? allow_smem<kernel>() : WB200_OK) return rc;
   WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, smem, s, p));
   return WB200_OK;
 }
-template <typename IdT, typename T, int P, bool TRANS>
+template <typename T, int P, bool TRANS>
 int launch_expand(const wb::ExpandParams& p, bool few, dim3 grid, cudaStream_t s) {
   if (few) {
-    WB_HOST_CUDA(launch(wb::adapter_expand_few_kernel<IdT, T, P, TRANS>, grid, wb::kAdapterThreads, size_t(8) * p.Rp * 4, s, p));
+    WB_HOST_CUDA(launch(wb::adapter_expand_few_kernel<T, P, TRANS>, grid, wb::kAdapterThreads, size_t(8) * p.Rp * 4, s, p));
     return WB200_OK;
   }
   const int steps = p.Rp / 16;
-  if (p.io_vec)
-    return steps == 1 ? launch_expand_tile<IdT, T, P, 1, TRANS, true>(p, grid, s) : steps == 2 ? launch_expand_tile<IdT, T, P, 2, TRANS, true>(p, grid, s) : launch_expand_tile<IdT, T, P, 4, TRANS, true>(p, grid, s);
-  return steps == 1 ? launch_expand_tile<IdT, T, P, 1, TRANS, false>(p, grid, s) : steps == 2 ? launch_expand_tile<IdT, T, P, 2, TRANS, false>(p, grid, s) : launch_expand_tile<IdT, T, P, 4, TRANS, false>(p, grid, s);
+  if (p.io_vec && p.w_vec && p.C % wb::kExpandCols == 0 && p.R == p.Rp)
+    return steps == 1 ? launch_expand_tile<T, P, 1, TRANS, true>(p, grid, s) : steps == 2 ? launch_expand_tile<T, P, 2, TRANS, true>(p, grid, s) : launch_expand_tile<T, P, 4, TRANS, true>(p, grid, s);
+  return steps == 1 ? launch_expand_tile<T, P, 1, TRANS, false>(p, grid, s) : steps == 2 ? launch_expand_tile<T, P, 2, TRANS, false>(p, grid, s) : launch_expand_tile<T, P, 4, TRANS, false>(p, grid, s);
 }
 
 // out = y + ranks onto C columns.
@@ -166,16 +164,13 @@ int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const _
   const int slices = div_up(C, p.cols_per_cta);
   const dim3 grid(slices, chunks, group_lanes(c.rows, c.L, (long long)chunks * slices));
   using bf16 = __nv_bfloat16;
-  if (c.wide_ids)
-    return trans ? launch_expand<long long, bf16, 2, true>(p, few, grid, c.stream)
-           : f32 ? launch_expand<long long, float, 3, false>(p, few, grid, c.stream) : launch_expand<long long, bf16, 2, false>(p, few, grid, c.stream);
-  return trans ? launch_expand<int, bf16, 2, true>(p, few, grid, c.stream)
-         : f32 ? launch_expand<int, float, 3, false>(p, few, grid, c.stream) : launch_expand<int, bf16, 2, false>(p, few, grid, c.stream);
+  return trans ? launch_expand<bf16, 2, true>(p, few, grid, c.stream)
+         : f32 ? launch_expand<float, 3, false>(p, few, grid, c.stream) : launch_expand<bf16, 2, false>(p, few, grid, c.stream);
 }
 
-template <typename IdT, int RT>
+template <int RT>
 int launch_outer(const wb::OuterParams& p, dim3 grid, cudaStream_t s) {
-  constexpr auto kernel = wb::adapter_outer_kernel<IdT, RT>;
+  constexpr auto kernel = wb::adapter_outer_kernel<RT>;
   if (int rc = allow_smem<kernel>()) return rc;
   WB_HOST_CUDA(launch_clusters(kernel, grid, wb::kAdapterThreads, wb::OuterTile<RT>::SMEM_BYTES, s, p));
   return WB200_OK;
@@ -195,8 +190,7 @@ int run_outer(const AdapterCall& c, wb::OuterSide first, wb::OuterSide second) {
   const int blocks = p.side[0].blocks + p.side[1].blocks;
   const long long both = (long long)div_up(first.C, wb::kOuterCols) + div_up(second.C, wb::kOuterCols);
   const dim3 grid(splits_for(both * c.L, chunks_of(c.rows)), blocks, c.L);
-  if (c.wide_ids) return c.Rp <= 16 ? launch_outer<long long, 2>(p, grid, c.stream) : c.Rp <= 32 ? launch_outer<long long, 4>(p, grid, c.stream) : launch_outer<long long, 8>(p, grid, c.stream);
-  return c.Rp <= 16 ? launch_outer<int, 2>(p, grid, c.stream) : c.Rp <= 32 ? launch_outer<int, 4>(p, grid, c.stream) : launch_outer<int, 8>(p, grid, c.stream);
+  return c.Rp <= 16 ? launch_outer<2>(p, grid, c.stream) : c.Rp <= 32 ? launch_outer<4>(p, grid, c.stream) : launch_outer<8>(p, grid, c.stream);
 }
 
 int check_adapters(const char* what, int rows, int K, int N, int R, int L) {
@@ -356,13 +350,14 @@ int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, c
   if (!x || !a || !b || !ids || !y || !out || !hidden) return fail(WB200_ERR_INVALID_ARG, "adapters: null pointer");
   if (dtype != WB200_F32 && dtype != WB200_BF16) return fail(WB200_ERR_INVALID_ARG, "adapters: unknown output dtype %d", dtype);
   if (rows > 1 && (ldx < K || ldy < N || ldo < N)) return fail(WB200_ERR_INVALID_ARG, "adapters: a row pitch is smaller than a row");
+  if (ldy >= 1 << 24 || ldo >= 1 << 24) return fail(WB200_ERR_UNSUPPORTED, "adapters: a row pitch of 2^24 elements or more");
   if (!aligned_to(x, 2) || !aligned_to(a, 2) || !aligned_to(b, 2) || !aligned_to(y, dtype == WB200_F32 ? 4 : 2) || !aligned_to(out, dtype == WB200_F32 ? 4 : 2) ||
       !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(hidden, 16))
     return fail(WB200_ERR_ALIGNMENT, "adapters: a tensor is not aligned to its element size, or hidden not to 16 bytes");
   const size_t need = wb200_adapters_hidden_bytes(rows, rank, dtype);
   if (hidden_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters: hidden of %zu bytes needed (got %zu)", need, hidden_bytes);
   if (int rc = wbhost::device(nullptr, nullptr)) return rc;
-  const AdapterCall c{ids, ids_are_int64 != 0, rows, rank, rank_pad(rank), num_adapters, dtype == WB200_F32 ? 3 : 2, static_cast<cudaStream_t>(stream)};
+  const AdapterCall c{{ids, ids_are_int64 != 0}, rows, rank, rank_pad(rank), num_adapters, dtype == WB200_F32 ? 3 : 2, static_cast<cudaStream_t>(stream)};
   auto* h = static_cast<__nv_bfloat16*>(hidden);
   if (int rc = run_shrink(c, static_cast<const __nv_bfloat16*>(x), ldx, K, static_cast<const __nv_bfloat16*>(a), false, scale, h)) return rc;
   return run_expand(c, static_cast<const __nv_bfloat16*>(b), false, h, y, ldy, out, ldo, dtype == WB200_F32, N);
@@ -378,6 +373,7 @@ int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, 
   if (!ids || !g || ((dx || da) && (!b || !workspace)) || (dx && !a) || (da && !x) || (db && !hidden))
     return fail(WB200_ERR_INVALID_ARG, "adapters backward: null pointer");
   if (rows > 1 && (ldg < N || (da && ldx < K) || (dx && ldd < K))) return fail(WB200_ERR_INVALID_ARG, "adapters backward: a row pitch is smaller than a row");
+  if (ldd >= 1 << 24) return fail(WB200_ERR_UNSUPPORTED, "adapters backward: a row pitch of 2^24 elements or more");
   if (!aligned_to(x, 2) || !aligned_to(a, 2) || !aligned_to(b, 2) || !aligned_to(g, 2) || !aligned_to(dx, 2) || !aligned_to(da, 2) || !aligned_to(db, 2) ||
       !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(hidden, 16) || !aligned_to(workspace, 16))
     return fail(WB200_ERR_ALIGNMENT, "adapters backward: a tensor is not aligned to its element size, or hidden or the workspace not to 16 bytes");
@@ -385,7 +381,7 @@ int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, 
   if ((dx || da) && workspace_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters backward: workspace of %zu bytes needed (got %zu)", need, workspace_bytes);
   if (db && hidden_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters backward: hidden of %zu bytes needed (got %zu)", need, hidden_bytes);
   if (int rc = wbhost::device(nullptr, nullptr)) return rc;
-  const AdapterCall c{ids, ids_are_int64 != 0, rows, rank, rank_pad(rank), num_adapters, 2, static_cast<cudaStream_t>(stream)};
+  const AdapterCall c{{ids, ids_are_int64 != 0}, rows, rank, rank_pad(rank), num_adapters, 2, static_cast<cudaStream_t>(stream)};
   const auto* gp = static_cast<const __nv_bfloat16*>(g);
   auto* u = static_cast<__nv_bfloat16*>(workspace);
   if (dx || da)

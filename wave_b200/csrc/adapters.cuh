@@ -70,15 +70,18 @@ struct RowGroups {
   int adapter[kChunkRows];
 };
 
-template <typename IdT>
-__device__ __forceinline__ int adapter_of(const IdT* ids, int row, int rows, int L) {  // -1: none
-  const long long id = row < rows ? (long long)ids[row] : -1;
+struct Ids {
+  const void* at;  // int32, or int64 with `wide`
+  int wide;
+};
+__device__ __forceinline__ int adapter_of(const Ids& ids, int row, int rows, int L) {  // -1: none
+  if (row >= rows) return -1;
+  const long long id = ids.wide ? static_cast<const long long*>(ids.at)[row] : (long long)static_cast<const int*>(ids.at)[row];
   return id >= 0 && id < L ? int(id) : -1;
 }
 
 // Called by all threads of the CTA, 64 at least. Returns the number of groups.
-template <typename IdT>
-__device__ __forceinline__ int group_rows(RowGroups& g, const IdT* ids, int row0, int rows, int L) {
+__device__ __forceinline__ int group_rows(RowGroups& g, const Ids& ids, int row0, int rows, int L) {
   const int t = threadIdx.x;
   const int first_id = adapter_of(ids, row0, rows, L);
   const int mine = t < kChunkRows ? adapter_of(ids, row0 + t, rows, L) : first_id;
@@ -135,8 +138,7 @@ struct FewRows {
   unsigned rows, none;  // of the group; without an adapter
   int adapter;
 };
-template <typename IdT>
-__device__ __forceinline__ FewRows few_rows(const IdT* ids, int row0, int rows, int L, int n) {
+__device__ __forceinline__ FewRows few_rows(const Ids& ids, int row0, int rows, int L, int n) {
   const int lane = threadIdx.x & 31;
   const int mine = adapter_of(ids, row0 + lane, rows, L);
   const unsigned same = __match_any_sync(0xffffffffu, mine);
@@ -206,7 +208,7 @@ __device__ __forceinline__ void split_bf16(float v, __nv_bfloat16 (&part)[P]) {
 struct ShrinkParams {
   const __nv_bfloat16* x;  // [rows, K], pitch ldx
   const __nv_bfloat16* w;  // A_l [L][R][K], or (TRANS) B_l [L][K][R]
-  const void* ids;
+  Ids ids;
   const float* scale;      // [L], or null
   __nv_bfloat16* hidden;   // [rows][parts][Rp]
   long long ldx;
@@ -256,7 +258,7 @@ __device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums
 // hidden[t][r] = scale_l sum_k x[t, k] w_l[r, k]. Grid (splits of K = one cluster, chunks, group lanes).
 //
 // Few rows: operands straight from global memory to registers. The 8 warps of a CTA take blocks of 64 k in turn.
-template <typename IdT, int RT, bool TRANS>
+template <int RT, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads)
 adapter_shrink_few_kernel(const ShrinkParams p) {
   constexpr int KU = 2, COLS = RT * 8;
@@ -268,7 +270,7 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
   const int row0 = blockIdx.y * kFewRows;
   const int k0 = blockIdx.x * p.split_k, k1 = min(p.K, k0 + p.split_k);
   for (int gi = blockIdx.z;; gi += gridDim.z) {
-    const FewRows group = few_rows(static_cast<const IdT*>(p.ids), row0, p.rows, p.L, gi);
+    const FewRows group = few_rows(p.ids, row0, p.rows, p.L, gi);
     if (group.rows == 0u) break;
     const __nv_bfloat16* w = p.w + (long long)group.adapter * p.R * p.K;
     const float scale = p.scale ? p.scale[group.adapter] : 1.f;
@@ -360,7 +362,7 @@ struct ShrinkTile {
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES;  // the sums reuse it
   static_assert(4 * kChunkRows * (COLS + 1) * 4 <= SMEM_BYTES, "sums of the four k quarters");
 };
-template <typename IdT, int RT, bool TRANS>
+template <int RT, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_shrink_tile_kernel(const ShrinkParams p) {
   using Cfg = ShrinkTile<RT>;
@@ -373,7 +375,7 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int wm = warp & 1, wq = warp >> 1;
   const int row0 = blockIdx.y * kChunkRows;
-  const int ngroups = group_rows(groups, static_cast<const IdT*>(p.ids), row0, p.rows, p.L);
+  const int ngroups = group_rows(groups, p.ids, row0, p.rows, p.L);
   const int k0 = blockIdx.x * p.split_k, k1 = min(p.K, k0 + p.split_k);
   const int steps = max(0, (k1 - k0 + 63) / 64);
   for (int gi = blockIdx.z; gi < ngroups; gi += gridDim.z) {
@@ -509,7 +511,7 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
 
 struct ExpandParams {
   const __nv_bfloat16* w;       // B_l [L][C][R], or (TRANS) A_l [L][R][C]
-  const void* ids;
+  Ids ids;
   const __nv_bfloat16* hidden;  // [rows][parts][Rp]
   const void* y;                // null: zeros
   void* out;
@@ -579,7 +581,7 @@ __device__ __forceinline__ void expand_rest(const ExpandParams& p, long long row
 //
 // Few rows: a thread has two columns, with 16 of their ranks in registers at a time, and walks the rows of a group. f32 FMAs: the
 // products are few, the loads of w_l (whole sectors, all of a thread's in flight) are what counts.
-template <typename IdT, typename T, int P, bool TRANS>
+template <typename T, int P, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads)
 adapter_expand_few_kernel(const ExpandParams p) {
   constexpr int ROWS = 8;
@@ -594,7 +596,7 @@ adapter_expand_few_kernel(const ExpandParams p) {
   bool waited = false;
   unsigned none = 0u;
   for (int gi = blockIdx.z;; gi += gridDim.z) {
-    const FewRows group = few_rows(static_cast<const IdT*>(p.ids), row0, p.rows, p.L, gi);
+    const FewRows group = few_rows(p.ids, row0, p.rows, p.L, gi);
     none = group.none;
     if (group.rows == 0u) break;
     const __nv_bfloat16* w = p.w + (long long)group.adapter * p.R * p.C;
@@ -715,30 +717,33 @@ adapter_expand_few_kernel(const ExpandParams p) {
 // fall into different banks.
 __host__ __device__ constexpr int expand_pitch(int parts, int Rp) { return parts * Rp + ((parts * Rp / 2) % 16 == 8 ? 0 : 16); }
 
-// Many rows: a warp takes 32 columns of all the rows of a group; a lane has 8 neighbouring columns of two rows of an MMA tile. The values of y are
-// loaded ahead of everything else, a batch of rows (MB tiles of 16) at once, the next batch while this one is worked on; w of the next columns
-// with it. Rows that do not start on 16 bytes go through shared memory instead, so that 32 lanes share a row's 32 columns.
+// Many rows: a warp takes 32 columns of all the rows of a group; a lane has 8 neighbouring columns of two rows of an MMA tile.
+// FAST: rows that start on 16 bytes, whole blocks of 32 columns and of 16 ranks. The values of y are loaded ahead of everything else, a batch of rows
+// (MB tiles of 16) at once, the next batch while this one is worked on, w of the next columns with it; they are the accumulators' first values.
+// Otherwise the accumulators go through shared memory, so that 32 lanes share a row's 32 columns.
 // QN: steps of 16 ranks of w in registers at a time.
-template <typename IdT, typename T, int P, int QN, bool TRANS, bool VEC>
+template <typename T, int P, int QN, bool TRANS, bool FAST>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_expand_tile_kernel(const ExpandParams p) {
   constexpr int RAW = sizeof(T) == 2 ? 1 : 2;    // 16-byte pieces of 8 values
-  constexpr int MB = sizeof(T) == 2 ? 4 : 2;     // tiles of 16 rows in a batch
-  constexpr bool AHEAD = QN <= 2;                // all ranks of w are in registers at a time (steps == QN)
+  constexpr int MB = 2;                          // tiles of 16 rows in a batch
+  constexpr bool AHEAD = FAST && QN <= 2;        // all ranks of w are in registers at a time (steps == QN)
+  constexpr int STEP = kAdapterWarps * kExpandCols;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ RowGroups groups;
-  __shared__ float staged[VEC ? 1 : kAdapterWarps][VEC ? 1 : 16][VEC ? 1 : kExpandCols + 1];
+  __shared__ float staged[FAST ? 1 : kAdapterWarps][FAST ? 1 : 16][FAST ? 1 : kExpandCols + 1];
   __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem);  // [64][P][Rp], rows `pitch` apart
   const int pitch = expand_pitch(P, p.Rp);
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row0 = blockIdx.y * kChunkRows;
-  const int ngroups = group_rows(groups, static_cast<const IdT*>(p.ids), row0, p.rows, p.L);
+  const int ngroups = group_rows(groups, p.ids, row0, p.rows, p.L);
   const int c_begin = blockIdx.x * p.cols_per_cta, c_end = min(p.C, c_begin + p.cols_per_cta);
-  constexpr int STEP = kAdapterWarps * kExpandCols;
-  const T* y = static_cast<const T*>(p.y) + row0 * p.ldy;
-  T* out = static_cast<T*>(p.out) + row0 * p.ldo;
   const int steps = p.Rp / 16;
+  // rows of the chunk, by 32-bit offsets (a pitch is below 2^24 elements)
+  const char* y = static_cast<const char*>(p.y) + row0 * p.ldy * int(sizeof(T));
+  char* out = static_cast<char*>(p.out) + row0 * p.ldo * int(sizeof(T));
+  const uint32_t y_pitch = uint32_t(p.ldy) * sizeof(T), out_pitch = uint32_t(p.ldo) * sizeof(T);
   bool waited = false;
   for (int gi = blockIdx.z; gi < ngroups; gi += gridDim.z) {
     const int first = groups.start[gi], count = groups.start[gi + 1] - first;
@@ -751,8 +756,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) row[m][h] = row_at(m * 16 + h * 8 + g);
     uint4 next[MB][2][RAW];
-    auto load_y = [&](int col, int batch) {  // 8 values of every row of the batch, where they are whole
-      const bool there = VEC && p.y && col + 8 <= c_end;
+    auto load_y = [&](int c0, int batch) {  // 8 values of every row of the batch
 #pragma unroll
       for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -764,16 +768,17 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
           for (int i = 0; i < RAW; ++i) {
             next[m][h][i] = make_uint4(0u, 0u, 0u, 0u);
-            if (there && r >= 0) next[m][h][i] = *(reinterpret_cast<const uint4*>(y + r * p.ldy + col) + i);
+            if (p.y && r >= 0) next[m][h][i] = *reinterpret_cast<const uint4*>(y + (uint32_t(r) * y_pitch + uint32_t(c0 + 8 * t) * uint32_t(sizeof(T)) + 16u * i));
           }
         }
     };
     uint32_t wf[4][QN][2];
     auto load_w = [&](int c0, int q0) {
-      if (p.w_vec && c0 + kExpandCols <= p.C && (q0 + QN) * 16 <= p.R) {  // all there
+      if constexpr (FAST) {
         const __nv_bfloat16* at = TRANS ? w + (long long)(q0 * 16 + 4 * t) * p.C + c0 + 4 * g : w + (long long)(c0 + 8 * (g >> 1) + (g & 1)) * p.R + q0 * 16 + 4 * t;
 #pragma unroll
         for (int q = 0; q < QN; ++q) {
+          if (QN > 1 && (q0 + q) * 16 >= p.Rp) break;
           if constexpr (!TRANS) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -791,37 +796,41 @@ adapter_expand_tile_kernel(const ExpandParams p) {
             wf[3][q][0] = high_halves(v[0].y, v[1].y); wf[3][q][1] = high_halves(v[2].y, v[3].y);
           }
         }
-        return;
-      }
+      } else {
 #pragma unroll
-      for (int q = 0; q < QN; ++q) {
-        const int r = (q0 + q) * 16 + 4 * t;
-        if constexpr (!TRANS) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int c = c0 + 8 * (g >> 1) + 2 * i + (g & 1);
-            if (c < p.C && r < p.R) load_bf16<4>(w + (long long)c * p.R + r, p.w_vec != 0 && r + 4 <= p.R, p.R - r, wf[i][q]);
-            else wf[i][q][0] = wf[i][q][1] = 0u;
-          }
-        } else {
+        for (int q = 0; q < QN; ++q) {
+          const int r = (q0 + q) * 16 + 4 * t;
           uint32_t raw[4][2];
-          const int c = c0 + 4 * g;
+          if constexpr (!TRANS) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (c < p.C && r + i < p.R) load_bf16<4>(w + (long long)(r + i) * p.C + c, p.w_vec != 0 && c + 4 <= p.C, p.C - c, raw[i]);
-            else raw[i][0] = raw[i][1] = 0u;
+            for (int i = 0; i < 4; ++i) {
+              const int c = c0 + 8 * (g >> 1) + 2 * i + (g & 1);
+              if (c < p.C && r < p.R) load_bf16<4>(w + (long long)c * p.R + r, p.w_vec != 0 && r + 4 <= p.R, p.R - r, raw[i]);
+              else raw[i][0] = raw[i][1] = 0u;
+              wf[i][q][0] = raw[i][0];
+              wf[i][q][1] = raw[i][1];
+            }
+          } else {
+            const int c = c0 + 4 * g;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (c < p.C && r + i < p.R) load_bf16<4>(w + (long long)(r + i) * p.C + c, p.w_vec != 0 && c + 4 <= p.C, p.C - c, raw[i]);
+              else raw[i][0] = raw[i][1] = 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                wf[i][q][h] = i & 1 ? high_halves(raw[2 * h][i / 2], raw[2 * h + 1][i / 2]) : low_halves(raw[2 * h][i / 2], raw[2 * h + 1][i / 2]);
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              wf[i][q][h] = i & 1 ? high_halves(raw[2 * h][i / 2], raw[2 * h + 1][i / 2]) : low_halves(raw[2 * h][i / 2], raw[2 * h + 1][i / 2]);
         }
       }
     };
     const int c_first = c_begin + warp * kExpandCols;
-    load_y(c_first + 8 * t, 0);
-    if (AHEAD) load_w(c_first, 0);
+    if (FAST && c_first < c_end) {
+      load_y(c_first, 0);
+      if (AHEAD) load_w(c_first, 0);
+    }
     if (!waited) pdl_wait();  // for the hidden vectors; y and w are complete before the kernel that makes those starts
     waited = true;
     __syncthreads();
@@ -834,10 +843,8 @@ adapter_expand_tile_kernel(const ExpandParams p) {
     cp_async_commit();
     cp_async_wait<0>();
     __syncthreads();
+#pragma unroll 1
     for (int c0 = c_first; c0 < c_end; c0 += STEP) {
-      const int col = c0 + 8 * t;
-      const int valid = c_end - col;
-      const bool whole = VEC && valid >= 8;
       if (!AHEAD) load_w(c0, 0);
       uint32_t wn[4][QN][2];
       if constexpr (AHEAD) {
@@ -851,22 +858,26 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
       for (int batch = 0; batch < 4 / MB; ++batch) {
         if (batch * MB >= mtiles) break;
-        uint4 now[MB][2][RAW];
+        float acc[MB][4][4];
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h) {
+            float v[8] = {};
+            if constexpr (FAST) read8<T>(reinterpret_cast<const T*>(next[m][h]), true, 8, v);
 #pragma unroll
-            for (int i = 0; i < RAW; ++i) now[m][h][i] = next[m][h][i];
-        if (VEC) {
-          if ((batch + 1) * MB < mtiles) load_y(col, batch + 1);
-          else if (c0 + STEP < c_end) load_y(col + STEP, 0);
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) acc[m][n][2 * h + j] = v[TRANS ? 4 * j + n : 2 * n + j];
+          }
+        if constexpr (FAST) {
+          if ((batch + 1) * MB < mtiles) load_y(c0, batch + 1);
+          else if (c0 + STEP < c_end) load_y(c0 + STEP, 0);
         }
 #pragma unroll
         for (int mm = 0; mm < MB; ++mm) {
           const int m = batch * MB + mm;
           if (m >= mtiles) break;
-          float acc[4][4] = {};
           for (int q0 = 0; q0 < steps; q0 += QN) {
             if (steps > QN && (q0 > 0 || m > 0)) load_w(c0, q0);
 #pragma unroll
@@ -878,26 +889,20 @@ adapter_expand_tile_kernel(const ExpandParams p) {
                 const uint2 lo = *reinterpret_cast<const uint2*>(at + i * p.Rp);
                 const uint2 hi = *reinterpret_cast<const uint2*>(at + 8 * pitch + i * p.Rp);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) mma_bf16(acc[n], lo.x, hi.x, lo.y, hi.y, wu[n][q][0], wu[n][q][1]);
+                for (int n = 0; n < 4; ++n) mma_bf16(acc[mm][n], lo.x, hi.x, lo.y, hi.y, wu[n][q][0], wu[n][q][1]);
               }
             }
           }
-          if constexpr (VEC) {
+          if constexpr (FAST) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (row[m][h] < 0 || valid <= 0) continue;
+              if (row[m][h] < 0) continue;
               float v[8];
-              if (whole) {
-                read8<T>(reinterpret_cast<const T*>(now[mm][h]), true, 8, v);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = p.y && i < valid ? as_f32<T>(y[row[m][h] * p.ldy + col + i]) : 0.f;
-              }
 #pragma unroll
               for (int n = 0; n < 4; ++n)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) v[TRANS ? 4 * j + n : 2 * n + j] += acc[n][2 * h + j];
-              write8<T>(out + row[m][h] * p.ldo + col, whole, valid, v);
+                for (int j = 0; j < 2; ++j) v[TRANS ? 4 * j + n : 2 * n + j] = acc[mm][n][2 * h + j];
+              write8<T>(reinterpret_cast<T*>(out + (uint32_t(row[m][h]) * out_pitch + uint32_t(c0 + 8 * t) * uint32_t(sizeof(T)))), true, 8, v);
             }
           } else {
             float (*mine)[kExpandCols + 1] = staged[warp];
@@ -905,19 +910,19 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
             for (int n = 0; n < 4; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) mine[g + (e >> 1) * 8][8 * t + (TRANS ? 4 * (e & 1) + n : 2 * n + (e & 1))] = acc[n][e];
+              for (int e = 0; e < 4; ++e) mine[g + (e >> 1) * 8][8 * t + (TRANS ? 4 * (e & 1) + n : 2 * n + (e & 1))] = acc[mm][n][e];
             __syncwarp();
             const bool there = c0 + lane < c_end;
             float v[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int at = row_at(m * 16 + r);
-              v[r] = there && p.y && at >= 0 ? as_f32<T>(y[at * p.ldy + c0 + lane]) : 0.f;
+              v[r] = there && p.y && at >= 0 ? as_f32<T>(*reinterpret_cast<const T*>(y + (uint32_t(at) * y_pitch + uint32_t(c0 + lane) * uint32_t(sizeof(T))))) : 0.f;
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int at = row_at(m * 16 + r);
-              if (there && at >= 0) out[at * p.ldo + c0 + lane] = as_out<T>(v[r] + mine[r][lane]);
+              if (there && at >= 0) *reinterpret_cast<T*>(out + (uint32_t(at) * out_pitch + uint32_t(c0 + lane) * uint32_t(sizeof(T)))) = as_out<T>(v[r] + mine[r][lane]);
             }
           }
         }
@@ -939,7 +944,7 @@ struct OuterSide {
 };
 struct OuterParams {
   OuterSide side[2];  // blocks of columns of the first, then of the second
-  const void* ids;
+  Ids ids;
   int rows, R, Rp, L;
 };
 
@@ -960,7 +965,7 @@ struct OuterTile {
   static_assert(2 * kOuterCols * SUM_PITCH * 4 <= RING_BYTES, "sums of the two halves of the rows");
 };
 
-template <typename IdT, int RT>
+template <int RT>
 __global__ void __launch_bounds__(kAdapterThreads)
 adapter_outer_kernel(const OuterParams p) {
   using Cfg = OuterTile<RT>;
@@ -973,10 +978,11 @@ adapter_outer_kernel(const OuterParams p) {
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int second = int(blockIdx.y) >= p.side[0].blocks;
-  const OuterSide& side = p.side[second];
+  OuterSide side = p.side[0];  // (member by member: an index into the parameters would put them on the stack)
+  if (second) side = p.side[1];
   const int c0 = (int(blockIdx.y) - (second ? p.side[0].blocks : 0)) * kOuterCols;
   const int l = blockIdx.z, splits = gridDim.x, split = blockIdx.x;
-  const IdT* ids = static_cast<const IdT*>(p.ids);
+  const Ids& ids = p.ids;
   const int row_begin = int((long long)p.rows * split / splits), row_end = int((long long)p.rows * (split + 1) / splits);
   const int wc = warp & 3, wk = warp >> 2;  // 32 columns, 32 of a stage's 64 rows
   for (int n0 = 0; n0 < p.Rp; n0 += COLS) {
