@@ -325,6 +325,8 @@ def fast(lib=None):
     if _fast is None:
         names = ("wb200_mxfp4_gemm_repack_a", "wb200_mxfp8_gemm_repack_a", "wb200_mxfp4_gemm_quantize_a", "wb200_mxfp4_gemm_workspace_bytes",
                  "wb200_decode_tile_rows_for")
+        beside = ("wb200_adapters_forward", "wb200_adapters_backward", "wb200_mxfp4_input_grad", "wb200_router_workspace_bytes", "wb200_router",
+                  "wb200_router_grad", "wb200_moe_combine", "wb200_moe_combine_grad", "wb200_last_error")
         if not isinstance(lib, ctypes.CDLL) or not all(isinstance(getattr(lib, name), lib._FuncPtr) for name in names):
             return None
         try:
@@ -338,8 +340,17 @@ def fast(lib=None):
             return None
         _fast_entries.update({name: getattr(lib, name) for name in names})
         module.bind(*(ctypes.cast(_fast_entries[name], ctypes.c_void_p).value for name in names))
+        module.bind_adapt(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in beside))
         _fast, _fast_lib = module, lib
     return _fast if _fast and lib is _fast_lib else None
+
+
+def native_calls():
+    """The host module for one call of an operator, or None: where it cannot be used, or a caller has put something in the place of the library
+    or of `load`, to watch or to redirect calls."""
+    if _fast and _lib is _fast_lib and load is _loader:
+        return _fast
+    return fast() if load is _loader and _fast is None else None
 
 
 def check(rc: int) -> None:

@@ -121,6 +121,11 @@ def apply_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.T
     its y comes back. The sum is made in f32 and rounded once to y's type. out: where to write (may be y), not together with gradients.
     Differentiable in y, x, a and b for a bf16 y and pools of at most 65535 adapters; sums over rows are made in a fixed order.
     """
+    native = _lib.native_calls()
+    if native is not None:
+        result = native.adapters(y, x, a, b, ids, scale, out)
+        if result is not None:
+            return result if out is None else out
     sizes = _check(y, x, a, b, ids, scale, out)
     rows = sizes[0]
     if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad):

@@ -64,7 +64,7 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False, check
 def _run(cmd: list[str]) -> str:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
     return res.stderr
 
 
@@ -85,7 +85,8 @@ def _compile(nvcc: str, source: Path, objects: Path, variant: list[str], force: 
 
 
 FAST_OUT = PKG / "_fast.so"
-FAST_SOURCE = CSRC / "fast_call.cpp"
+FAST_SOURCES = [CSRC / "fast_call.cpp", CSRC / "fast_adapt.cpp"]
+FAST_HEADER = CSRC / "fast.h"
 
 
 def fast_target() -> str:
@@ -96,11 +97,11 @@ def fast_target() -> str:
 
 def fast_stale() -> bool:
     """`_fast.so` is missing, older than its source, or was compiled against another torch or Python."""
-    return not FAST_OUT.exists() or FAST_SOURCE.stat().st_mtime > FAST_OUT.stat().st_mtime or fast_target().encode() not in FAST_OUT.read_bytes()
+    return not FAST_OUT.exists() or any(p.stat().st_mtime > FAST_OUT.stat().st_mtime for p in [*FAST_SOURCES, FAST_HEADER]) or fast_target().encode() not in FAST_OUT.read_bytes()
 
 
 def build_fast(force: bool = False) -> Path:
-    """Compile `wave_b200._fast` (csrc/fast_call.cpp, against the installed torch) if it is not there as it should be (`fast_stale`)."""
+    """Compile `wave_b200._fast` (csrc/fast_call.cpp and fast_adapt.cpp, against the installed torch) if it is not there as it should be (`fast_stale`)."""
     if not force and not fast_stale():
         return FAST_OUT
     import sysconfig
@@ -110,13 +111,19 @@ def build_fast(force: bool = False) -> Path:
     nvcc = Path(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc").resolve()
     includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", nvcc.parent.parent / "include",
                 Path(sysconfig.get_paths()["include"])]
-    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           f'-DWB200_FAST_TARGET="{fast_target()}"',
-           *(f"-I{i}" for i in includes), str(FAST_SOURCE), "-o", str(FAST_OUT), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
-           "-ltorch_cuda", "-ltorch_python"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"g++ failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             f'-DWB200_FAST_TARGET="{fast_target()}"', *(f"-I{i}" for i in includes)]
+    gxx, objects = shutil.which("g++") or "c++", PKG / "build" / "_fast"
+    objects.mkdir(parents=True, exist_ok=True)
+
+    def compile_one(source: Path) -> str:
+        unit = objects / f"{source.stem}.o"
+        _run([gxx, *flags, "-c", str(source), "-o", str(unit)])
+        return str(unit)
+
+    with ThreadPoolExecutor(len(FAST_SOURCES)) as pool:
+        units = list(pool.map(compile_one, FAST_SOURCES))
+    _run([gxx, "-shared", *units, "-o", str(FAST_OUT), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"])
     return FAST_OUT
 
 

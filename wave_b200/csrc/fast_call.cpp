@@ -33,6 +33,8 @@
 #include <unordered_map>
 #include <vector>
 
+#include "fast.h"
+
 namespace {
 
 // A model that walks all its layers through one kernel object uses one or two packings per layer, and one plan per distinct row count. Those of weights
@@ -548,7 +550,10 @@ PyMethodDef workspaces_methods[] = {{"put", FASTCALL(workspaces_put), nullptr}, 
                                     {nullptr, nullptr, 0, nullptr}};
 PyMethodDef fence_methods[] = {{"stream", fence_stream, METH_NOARGS, nullptr}, {"done", fence_done, METH_NOARGS, nullptr},
                                {"wait", fence_wait, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
-PyMethodDef module_methods[] = {{"bind", bind, METH_VARARGS, nullptr}, {"linear", FASTCALL(linear), nullptr}, {nullptr, nullptr, 0, nullptr}};
+PyMethodDef module_methods[] = {{"bind", bind, METH_VARARGS, nullptr}, {"linear", FASTCALL(linear), nullptr},
+                                {"bind_adapt", wbfast::bind_adapt, METH_VARARGS, nullptr}, {"adapters", FASTCALL(wbfast::adapters), nullptr},
+                                {"router", FASTCALL(wbfast::router), nullptr}, {"combine_rows", FASTCALL(wbfast::combine_rows), nullptr},
+                                {"input_grad", FASTCALL(wbfast::input_grad), nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, module_methods, nullptr, nullptr, nullptr, nullptr};
 
 bool is_workspaces(PyObject* o) {
@@ -569,6 +574,11 @@ bool add_type(PyObject* module, const char* name, const char* qualified, PyMetho
 }
 
 }  // namespace
+
+namespace wbfast {
+bool plain(PyObject* o) { return ::plain(o); }
+PyObject* fail(const std::exception& e) { return ::fail(e); }
+}  // namespace wbfast
 
 PyMODINIT_FUNC PyInit__fast() {
   PyObject* m = PyModule_Create(&module_def);

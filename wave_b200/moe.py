@@ -160,6 +160,11 @@ def combine_rows(y: torch.Tensor, row_of: torch.Tensor, weight: torch.Tensor) ->
     """out[t] = sum_j weight[t, j] * y[row_of[t, j]] in f32, slot order, rounded once to y's type: `combine` with a new output, differentiable
     in the weights (the rows of y are those of frozen experts: a y that requires a gradient is refused). y [R, N] f32 or bf16, row_of [tokens, k]
     int32, negative for a dropped pair, weight [tokens, k] f32. Rows at or past R are not checked for."""
+    native = _lib.native_calls()
+    if native is not None:
+        out = native.combine_rows(y, row_of, weight)
+        if out is not None:
+            return out
     if not y.is_cuda or y.dtype not in ops._DTYPE_CODE or y.dim() != 2:
         raise ValueError(f"y must be a 2-D float32 or bfloat16 CUDA tensor, got {y.dtype} {tuple(y.shape)}")
     if row_of.dtype != torch.int32 or weight.dtype != torch.float32 or row_of.dim() != 2 or weight.shape != row_of.shape or row_of.shape[1] == 0:
@@ -279,6 +284,11 @@ def router(logits: torch.Tensor, top_k: int, mask: torch.Tensor | None = None, r
     the chosen ones alone with renormalize. balance_loss = E sum_e f_e P_e, f_e = counts[e] / (top_k n), P_e = the mean of softmax(logits)[:, e]
     over the n rows that count; 0 where none does. Its gradient takes f as a constant. mask: bool [rows], False for padding: ids -1, weight
     0, in no sum, gradient 0."""
+    native = _lib.native_calls()
+    if native is not None:
+        result = native.router(logits, top_k, mask, renormalize)
+        if result is not None:
+            return Routing(*result)
     if not 1 <= top_k <= min(logits.shape[-1], ROUTER_MAX_TOP_K):
         raise ValueError(f"top_k = {top_k} of {logits.shape[-1]} experts (at most {ROUTER_MAX_TOP_K})")
     logits, mask = _check_router(logits, mask)

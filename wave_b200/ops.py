@@ -339,6 +339,11 @@ def mxfp4_input_grad(g: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, ou
     """Gradient of a linear layer with MXFP4 weights by its input: g [M, N] @ dequant(b, b_scale) [N, K], f32 accumulation, rounded once to
     bf16. g bf16, b uint8 [N, K/2] and b_scale uint8 [N, K/32] row-major as the layer's forward takes them. Rows of g that do not start on
     16 bytes (odd N) are copied first. out: bf16 [M, K] whose rows start on 16 bytes."""
+    native = _lib.native_calls() if out is None else None
+    if native is not None:
+        dx = native.input_grad(g, b, b_scale)
+        if dx is not None:
+            return dx
     lib = _lib.load()
     if not g.is_cuda or g.dtype != torch.bfloat16 or g.dim() != 2:
         raise ValueError(f"g must be a 2-D bfloat16 CUDA tensor, got {g.dtype} {tuple(g.shape)} on {g.device}")
