@@ -358,3 +358,18 @@ def test_block_with_adapters_router_and_experts():
         assert torch.equal(h2.detach(), h) and torch.equal(y2.detach(), y) and torch.equal(r2.balance_loss.detach(), r.balance_loss)
         grads = torch.autograd.grad(y2.float().square().mean() + r2.balance_loss, (gate, pool.a, pool.b))
         assert all(t.isfinite().all() for t in grads) and (T == 1 or all(t.any() for t in grads))
+
+
+@pytest.mark.parametrize("tokens,k,N", [(300, 1, 1024), (70, 2, 4096), (5, 3, 1032), (40, 8, 2048), (9, 9, 2048), (20, 5, 6000)])
+def test_combine_of_wide_rows_is_that_of_narrow_ones(tokens, k, N):
+    """The same bits from the kernel that takes a token's whole rows and from the one that takes them in blocks of 512 columns."""
+    g = torch.Generator().manual_seed(tokens)
+    y, weight = torch.randn(tokens * k, N, generator=g).to(BF16).to(DEV), torch.randn(tokens, k, generator=g).to(DEV)
+    row_of = torch.randperm(tokens * k, generator=g).to(torch.int32)
+    row_of[::7] = -1
+    row_of = row_of.to(DEV)
+    wide, parts = torch.empty(tokens, N, dtype=BF16, device=DEV), torch.empty(tokens, N, dtype=BF16, device=DEV)
+    moe.combine(y, row_of, weight.reshape(-1), k, wide)
+    for c in range(0, N, 512):
+        moe.combine(y[:, c:c + 512], row_of, weight.reshape(-1), k, parts[:, c:c + 512])
+    assert torch.equal(wide, parts)

@@ -309,19 +309,37 @@ int check_router(const char* what, int rows, int E, int top_k, int dtype, const 
   return WB200_OK;
 }
 
+// Lanes may load their experts (1, 2, 4 or 8 neighbours) as one piece.
+int router_vec(const void* rows, long long ld, int E, int dtype) {
+  const int per_lane = E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : 8;
+  return aligned_to(rows, 16) && ld * (dtype == WB200_F32 ? 4 : 2) % 16 == 0 && E % per_lane == 0;
+}
+
 #define WB_BY_EXPERTS(KERNEL, T, E)                                                                          \
   ((E) <= 32 ? KERNEL<T, 1> : (E) <= 64 ? KERNEL<T, 2> : (E) <= 128 ? KERNEL<T, 4> : KERNEL<T, 8>)
 
+template <typename T, bool VEC, int SLOTS>
+cudaError_t launch_combine_slots(const void* g, long long ldg, const void* y, long long ldy, const int* row_of, int tokens, int top_k, int cols,
+                                float* g_weight, cudaStream_t s) {
+  return launch(wb::combine_grad_kernel<T, VEC, SLOTS>, dim3(tokens), 128, 0, s, static_cast<const T*>(g), ldg, static_cast<const T*>(y), ldy, row_of,
+                top_k, cols, g_weight);
+}
 template <typename T, bool VEC>
 cudaError_t launch_combine_grad(const void* g, long long ldg, const void* y, long long ldy, const int* row_of, int tokens, int top_k, int cols,
                                 float* g_weight, cudaStream_t s) {
-  return launch(wb::combine_grad_kernel<T, VEC>, dim3(tokens), 128, 0, s, static_cast<const T*>(g), ldg, static_cast<const T*>(y), ldy, row_of,
-                top_k, cols, g_weight);
+  return top_k <= 2 ? launch_combine_slots<T, VEC, 2>(g, ldg, y, ldy, row_of, tokens, top_k, cols, g_weight, s)
+                    : launch_combine_slots<T, VEC, 4>(g, ldg, y, ldy, row_of, tokens, top_k, cols, g_weight, s);
 }
 
 }  // namespace
 
 namespace wbhost {
+cudaError_t combine_tokens(const void* y, long long ldy, const int* row_of, const float* weight, int tokens, int top_k, int cols, void* out, long long ldo,
+                           cudaStream_t stream) {
+  auto kernel = top_k <= 2 ? wb::combine_token_kernel<2> : top_k <= 4 ? wb::combine_token_kernel<4> : wb::combine_token_kernel<8>;
+  return launch(kernel, dim3(tokens), 128, 0, stream, static_cast<const __nv_bfloat16*>(y), ldy, row_of, weight, top_k, cols, static_cast<__nv_bfloat16*>(out), ldo);
+}
+
 cudaError_t adapt_check_record(unsigned long long (&record)[3], bool reset) {
 #ifdef WB200_CHECKS
   cudaError_t e = cudaMemcpyFromSymbol(record, wb::g_check_record, sizeof(record));
@@ -444,13 +462,14 @@ int wb200_router(int rows, int num_experts, int top_k, const void* logits, int d
   p.logits = logits; p.mask = static_cast<const uint8_t*>(mask); p.given = given_ids; p.ld = ld;
   p.rows = rows; p.E = num_experts; p.top_k = top_k; p.renormalize = renormalize; p.given_i64 = given_are_int64;
   p.weight = weight; p.ids = ids; p.counts = counts; p.unit = unit; p.loss = loss;
+  p.vec = router_vec(logits, ld, num_experts, dtype);
   const int ctas = router_ctas(rows);
   p.part_p = static_cast<float*>(workspace);
   p.part_n = reinterpret_cast<int*>(p.part_p + size_t(ctas) * num_experts);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   void (*kernel)(wb::RouterParams) = dtype == WB200_F32 ? WB_BY_EXPERTS(wb::router_kernel, float, num_experts) : WB_BY_EXPERTS(wb::router_kernel, __nv_bfloat16, num_experts);
   WB_HOST_CUDA(launch(kernel, dim3(ctas), wb::kRouterWarps * 32, 0, s, p));
-  if (ctas > 1) WB_HOST_CUDA(launch(wb::router_finish_kernel, dim3(1), 1024, 0, s, p, ctas));
+  if (ctas > 1) WB_HOST_CUDA(launch_clusters(wb::router_finish_kernel, dim3(div_up(num_experts, 32)), 1024, 0, s, p, ctas));
   return WB200_OK;
 }
 
@@ -467,6 +486,7 @@ int wb200_router_grad(int rows, int num_experts, int top_k, const void* logits, 
   p.logits = logits; p.mask = static_cast<const uint8_t*>(mask); p.ids = ids; p.g_weight = g_weight; p.g_loss = g_loss; p.counts = counts;
   p.unit = unit; p.g_logits = g_logits; p.ld = ld; p.ldg = ldg;
   p.rows = rows; p.E = num_experts; p.top_k = top_k; p.renormalize = renormalize;
+  p.vec = router_vec(logits, ld, num_experts, dtype) && router_vec(g_logits, ldg, num_experts, dtype);
   void (*kernel)(wb::RouterGradParams) =
       dtype == WB200_F32 ? WB_BY_EXPERTS(wb::router_grad_kernel, float, num_experts) : WB_BY_EXPERTS(wb::router_grad_kernel, __nv_bfloat16, num_experts);
   WB_HOST_CUDA(launch(kernel, dim3(std::min(1184, div_up(rows, wb::kRouterWarps))), wb::kRouterWarps * 32, 0, static_cast<cudaStream_t>(stream), p));

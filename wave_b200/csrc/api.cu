@@ -1634,6 +1634,10 @@ int wb200_moe_combine(const void* y, long long ldy, int dtype, const int* row_of
   int rc = get_device(&dev);
   if (rc) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == WB200_BF16 && top_k <= 8 && cols % 8 == 0 && cols >= 1024 && rows_aligned(y, ldy, dtype) && rows_aligned(out, ldo, dtype)) {
+    WB_CUDA(wbhost::combine_tokens(y, ldy, row_of, weight, tokens, top_k, cols, out, ldo, s));
+    return WB200_OK;
+  }
   return dtype == WB200_F32 ? launch_combine<float>(y, ldy, row_of, weight, tokens, top_k, cols, out, ldo, false, s)
                             : launch_combine<__nv_bfloat16>(y, ldy, row_of, weight, tokens, top_k, cols, out, ldo, false, s);
 }
