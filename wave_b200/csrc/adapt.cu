@@ -135,9 +135,23 @@ int launch_expand_tile(const wb::ExpandParams& p, dim3 grid, cudaStream_t s) {
   WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, smem, s, p));
   return WB200_OK;
 }
+// Lanes that share a column of B in the kernel for few rows of whole ranks, 0 where that is not taken.
+int whole_pieces(const wb::ExpandParams& p) {
+  return p.w_vec && p.R == p.Rp && (p.R == 16 || p.R == 32 || p.R == 64) ? p.R / 8 : p.w_vec && p.R == 8 ? 1 : 0;
+}
+
 template <typename T, int P, bool TRANS>
 int launch_expand(const wb::ExpandParams& p, bool few, dim3 grid, cudaStream_t s) {
   if (few) {
+    if constexpr (!TRANS)
+      if (const int pieces = whole_pieces(p)) {
+        auto kernel = pieces == 1   ? wb::adapter_expand_few_whole_kernel<T, P, 1>
+                      : pieces == 2 ? wb::adapter_expand_few_whole_kernel<T, P, 2>
+                      : pieces == 4 ? wb::adapter_expand_few_whole_kernel<T, P, 4>
+                                    : wb::adapter_expand_few_whole_kernel<T, P, 8>;
+        WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, 0, s, p));
+        return WB200_OK;
+      }
     WB_HOST_CUDA(launch(wb::adapter_expand_few_kernel<T, P, TRANS>, grid, wb::kAdapterThreads, size_t(8) * p.Rp * 4, s, p));
     return WB200_OK;
   }
@@ -161,6 +175,8 @@ int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const _
   p.io_vec = aligned_to(out, 16) && ldo * esz % 16 == 0 && (!y || (aligned_to(y, 16) && ldy * esz % 16 == 0));
   const int vec = few ? (trans ? 2 : 8) : 4;  // elements of a load of w
   p.w_vec = aligned_to(w, 2 * vec) && (trans ? C : c.R) % (trans && few ? 4 : vec) == 0;
+  if (few && !trans)
+    if (const int pieces = whole_pieces(p)) p.cols_per_cta = wb::few_whole_steps(pieces) * wb::kAdapterThreads / pieces;
   const int slices = div_up(C, p.cols_per_cta);
   const dim3 grid(slices, chunks, group_lanes(c.rows, c.L, (long long)chunks * slices));
   using bf16 = __nv_bfloat16;

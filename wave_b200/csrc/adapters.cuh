@@ -263,7 +263,8 @@ __global__ void __launch_bounds__(kAdapterThreads)
 adapter_shrink_few_kernel(const ShrinkParams p) {
   constexpr int KU = 2, COLS = RT * 8;
   __shared__ float red[kAdapterWarps][16][COLS + 2];
-  __shared__ float sums[16 * (COLS + 1)];
+  __shared__ float sums[16][COLS];  // 16 / splits rows of this CTA from every split (a power of two)
+  bool again = false;
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -338,15 +339,42 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
             const int col = TRANS ? RT * (2 * t + (c & 1)) + i : i * 8 + 2 * t + (c & 1);
             red[warp][g + (c >> 1) * 8][col] = acc[i][c];
           }
+        // every split sends its sums of a row to the CTA that finishes it, which adds them up in their order
+        const int count = min(16, end - first), splits = gridDim.x, split = blockIdx.x, share = 16 / splits;
         __syncthreads();
-        for (int e = threadIdx.x; e < 16 * COLS; e += kAdapterThreads) {
+        if (again && splits > 1) {  // what came before has been read
+          cluster_arrive();
+          cluster_wait();
+        }
+        again = true;
+        for (int e = threadIdx.x; e < count * COLS; e += kAdapterThreads) {
           const int row = e / COLS, col = e % COLS;
           float v = 0.f;
 #pragma unroll
           for (int i = 0; i < kAdapterWarps; ++i) v += red[i][row][col];
-          sums[row * (COLS + 1) + col] = v;
+          const int owner = row % splits;
+          float* to = &sums[split * share + row / splits][col];
+          if (owner == split) *to = v;
+          else asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(to), owner)), "f"(v) : "memory");
         }
-        finish_hidden<COLS>(p, sums, [&](int row) { return row0 + nth_bit(group.rows, first + row); }, min(16, end - first), n0, scale);
+        __syncthreads();
+        if (splits > 1) {
+          cluster_arrive();
+          cluster_wait();
+        }
+        for (int e = threadIdx.x; e < count * COLS; e += kAdapterThreads) {
+          const int mine = e / COLS, col = e % COLS, row = mine * splits + split;
+          if (row >= count) break;
+          if (n0 + col >= p.Rp) continue;
+          float v = 0.f;
+          for (int i = 0; i < splits; ++i) v += sums[i * share + mine][col];
+          __nv_bfloat16 part[3];
+          split_bf16<3>(v * scale, part);
+          __nv_bfloat16* dst = p.hidden + (long long)(row0 + nth_bit(group.rows, first + row)) * p.parts * p.Rp + n0 + col;
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+            if (i < p.parts) dst[i * p.Rp] = part[i];
+        }
       }
     }
   }
@@ -704,6 +732,80 @@ adapter_expand_few_kernel(const ExpandParams p) {
         } else {
           at[0] = as_out<T>(acc[i][0]);
           if (both) at[1] = as_out<T>(acc[i][1]);
+        }
+      }
+    }
+  }
+  if (!waited) pdl_wait();  // (out may still be in use)
+  if (blockIdx.z == 0 && p.out != p.y)
+    for (; none != 0u; none &= none - 1u) expand_rest<T>(p, row0 + __ffs(none) - 1, c_begin + threadIdx.x * 8, c_end, kAdapterThreads * 8);
+}
+
+// The same for ranks of 8 PIECES whose rows of B start on 16 bytes: PIECES lanes share a column, each with 8 of its ranks, so that a warp's load is 512
+// consecutive bytes, STEPS of them in flight; the lanes' sums meet by shuffles, and the u-th lane of a column keeps every so-manieth column.
+__host__ __device__ constexpr int few_whole_steps(int pieces) { return pieces > 4 ? pieces : 4; }
+template <typename T, int P, int PIECES>
+__global__ void __launch_bounds__(kAdapterThreads, 3)
+adapter_expand_few_whole_kernel(const ExpandParams p) {
+  constexpr int STEPS = few_whole_steps(PIECES), ROWS = 2, KEPT = STEPS / PIECES, COLS = kAdapterThreads / PIECES;  // COLS: of a step
+  pdl_launch_dependents();
+  const int row0 = blockIdx.y * kFewRows;
+  const int c_begin = blockIdx.x * p.cols_per_cta, c_end = min(p.C, c_begin + p.cols_per_cta);  // cols_per_cta = STEPS * COLS
+  const T* y = static_cast<const T*>(p.y);
+  T* out = static_cast<T*>(p.out);
+  const int pc = threadIdx.x % PIECES, c = c_begin + threadIdx.x / PIECES;
+  bool waited = false;
+  unsigned none = 0u;
+  for (int gi = blockIdx.z;; gi += gridDim.z) {
+    const FewRows group = few_rows(p.ids, row0, p.rows, p.L, gi);
+    none = group.none;
+    if (group.rows == 0u) break;
+    const __nv_bfloat16* w = p.w + (long long)group.adapter * p.R * p.C + pc * 8;
+    uint4 wr[STEPS];
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) wr[u] = c + u * COLS < c_end ? *reinterpret_cast<const uint4*>(w + (long long)(c + u * COLS) * p.R) : make_uint4(0u, 0u, 0u, 0u);
+    unsigned rest = group.rows;
+    while (rest != 0u) {
+      int row[ROWS], count = 0;
+      float old[ROWS][KEPT];
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        row[i] = row0 + __ffs(rest) - 1;
+        count += rest != 0u;
+        rest &= rest - 1u;
+#pragma unroll
+        for (int k = 0; k < KEPT; ++k) {
+          const int col = c + (k * PIECES + pc) * COLS;
+          old[i][k] = y && i < count && col < c_end ? as_f32<T>(y[row[i] * p.ldy + col]) : 0.f;
+        }
+      }
+      if (!waited) pdl_wait();  // the hidden vectors are the only thing here that the kernel before this one writes
+      waited = true;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        if (i >= count) break;
+        float h[8] = {};
+#pragma unroll
+        for (int q = P - 1; q >= 0; --q) {
+          float v[8];
+          read8<__nv_bfloat16>(p.hidden + (row[i] * (long long)P + q) * p.Rp + pc * 8, true, 8, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) h[j] += v[j];
+        }
+#pragma unroll
+        for (int u = 0; u < STEPS; ++u) {
+          float v[8], sum = 0.f;
+          read8<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(&wr[u]), true, 8, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum = fmaf(h[j], v[j], sum);
+#pragma unroll
+          for (int o = 1; o < PIECES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (u % PIECES == pc) old[i][u / PIECES] += sum;
+        }
+#pragma unroll
+        for (int k = 0; k < KEPT; ++k) {
+          const int col = c + (k * PIECES + pc) * COLS;
+          if (col < c_end) out[row[i] * p.ldo + col] = as_out<T>(old[i][k]);
         }
       }
     }
