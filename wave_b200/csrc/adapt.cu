@@ -127,9 +127,9 @@ int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int 
   return trans ? launch_shrink_ranks<true>(p, few, grid, c.stream) : launch_shrink_ranks<false>(p, few, grid, c.stream);
 }
 
-template <typename T, int P, int QN, bool TRANS, bool FAST>
+template <typename T, int P, int QN, bool TRANS, bool FAST, bool EXACT>
 int launch_expand_tile(const wb::ExpandParams& p, dim3 grid, cudaStream_t s) {
-  constexpr auto kernel = wb::adapter_expand_tile_kernel<T, P, QN, TRANS, FAST>;
+  constexpr auto kernel = wb::adapter_expand_tile_kernel<T, P, QN, TRANS, FAST, EXACT>;
   const size_t smem = size_t(wb::kChunkRows) * wb::expand_pitch(P, p.Rp) * 2;
   if (int rc = smem > 24 * 1024 ? allow_smem<kernel>() : WB200_OK) return rc;
   WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, smem, s, p));
@@ -157,8 +157,11 @@ int launch_expand(const wb::ExpandParams& p, bool few, dim3 grid, cudaStream_t s
   }
   const int steps = p.Rp / 16;
   if (p.io_vec && p.w_vec && p.C % wb::kExpandCols == 0 && p.R == p.Rp)
-    return steps == 1 ? launch_expand_tile<T, P, 1, TRANS, true>(p, grid, s) : steps == 2 ? launch_expand_tile<T, P, 2, TRANS, true>(p, grid, s) : launch_expand_tile<T, P, 4, TRANS, true>(p, grid, s);
-  return steps == 1 ? launch_expand_tile<T, P, 1, TRANS, false>(p, grid, s) : steps == 2 ? launch_expand_tile<T, P, 2, TRANS, false>(p, grid, s) : launch_expand_tile<T, P, 4, TRANS, false>(p, grid, s);
+    return steps == 1   ? launch_expand_tile<T, P, 1, TRANS, true, true>(p, grid, s)
+           : steps == 2 ? launch_expand_tile<T, P, 2, TRANS, true, true>(p, grid, s)
+           : steps == 4 ? launch_expand_tile<T, P, 4, TRANS, true, true>(p, grid, s)
+                        : launch_expand_tile<T, P, 4, TRANS, true, false>(p, grid, s);
+  return steps == 1 ? launch_expand_tile<T, P, 1, TRANS, false, true>(p, grid, s) : launch_expand_tile<T, P, 2, TRANS, false, false>(p, grid, s);
 }
 
 // out = y + ranks onto C columns.

@@ -385,10 +385,12 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
 template <int RT>
 struct ShrinkTile {
   static constexpr int X_BYTES = kChunkRows * 128, W_BYTES = RT * 1024, STAGE_BYTES = X_BYTES + W_BYTES;
-  static constexpr int STAGES = RT == 2 ? 8 : RT == 4 ? 7 : 6;
+  static constexpr int STAGES = RT == 8 ? 6 : 8;
+  static constexpr int PER_SYNC = 2;  // stages that are worked on between two barriers
+  static constexpr int GROUPS = STAGES / PER_SYNC;
   static constexpr int COLS = RT * 8;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES;  // the sums reuse it
-  static_assert(4 * kChunkRows * (COLS + 1) * 4 <= SMEM_BYTES, "sums of the four k quarters");
+  static_assert(STAGES % PER_SYNC == 0 && 4 * kChunkRows * (COLS + 1) * 4 <= SMEM_BYTES, "whole groups; sums of the four k quarters");
 };
 template <int RT, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
@@ -473,7 +475,6 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
             wsrc[i] += w_step;
           }
         }
-        cp_async_commit();
         left -= 64;
         to = to == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : to + Cfg::STAGE_BYTES;
       };
@@ -486,33 +487,38 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
         woff[i / 2] = Cfg::X_BYTES + (TRANS ? piece<RT>(16 * wq + in, i + half) : piece<8>(i * 8 + half * 8 + (in & 7), 2 * wq + (in >> 3)));
       uint32_t from = base;
       float acc[2][RT][4] = {};
+      auto load_group = [&]() {
 #pragma unroll
-      for (int s = 0; s < STAGES - 1; ++s) {
-        if (s < steps) load();
-        else cp_async_commit();
-      }
-      for (int step = 0; step < steps; ++step) {
-        cp_async_wait<STAGES - 2>();
+        for (int i = 0; i < Cfg::PER_SYNC; ++i)
+          if (left > 0) load();
+        cp_async_commit();
+      };
+#pragma unroll
+      for (int i = 0; i < Cfg::GROUPS - 1; ++i) load_group();
+      for (int step = 0; step < steps; step += Cfg::PER_SYNC) {
+        cp_async_wait<Cfg::GROUPS - 2>();
         __syncthreads();
-        if (step + STAGES - 1 < steps) load();
-        else cp_async_commit();
-        if (32 * wm < count) {
-          uint32_t xa[2][4];
+        load_group();
 #pragma unroll
-          for (int m = 0; m < 2; ++m) ldsm4(from + xoff[m], xa[m]);
+        for (int sub = 0; sub < Cfg::PER_SYNC; ++sub) {
+          if (32 * wm < count && step + sub < steps) {
+            uint32_t xa[2][4];
 #pragma unroll
-          for (int i = 0; i < RT; i += 2) {
-            uint32_t wf[4];
-            if constexpr (!TRANS) ldsm4(from + woff[i / 2], wf);
-            else ldsm4_trans(from + woff[i / 2], wf);
+            for (int m = 0; m < 2; ++m) ldsm4(from + xoff[m], xa[m]);
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              mma_bf16(acc[m][i], xa[m][0], xa[m][1], xa[m][2], xa[m][3], wf[0], wf[1]);
-              mma_bf16(acc[m][i + 1], xa[m][0], xa[m][1], xa[m][2], xa[m][3], wf[2], wf[3]);
+            for (int i = 0; i < RT; i += 2) {
+              uint32_t wf[4];
+              if constexpr (!TRANS) ldsm4(from + woff[i / 2], wf);
+              else ldsm4_trans(from + woff[i / 2], wf);
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                mma_bf16(acc[m][i], xa[m][0], xa[m][1], xa[m][2], xa[m][3], wf[0], wf[1]);
+                mma_bf16(acc[m][i + 1], xa[m][0], xa[m][1], xa[m][2], xa[m][3], wf[2], wf[3]);
+              }
             }
           }
+          from = from == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : from + Cfg::STAGE_BYTES;
         }
-        from = from == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : from + Cfg::STAGE_BYTES;
       }
       cp_async_wait<0>();
       __syncthreads();
@@ -824,24 +830,25 @@ __host__ __device__ constexpr int expand_pitch(int parts, int Rp) { return parts
 // (MB tiles of 16) at once, the next batch while this one is worked on, w of the next columns with it; they are the accumulators' first values.
 // Otherwise the accumulators go through shared memory, so that 32 lanes share a row's 32 columns.
 // QN: steps of 16 ranks of w in registers at a time.
-template <typename T, int P, int QN, bool TRANS, bool FAST>
+template <typename T, int P, int QN, bool TRANS, bool FAST, bool EXACT>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_expand_tile_kernel(const ExpandParams p) {
+  const int Rp = EXACT ? 16 * QN : p.Rp;         // EXACT: known when compiled, and with it every address in shared memory
   constexpr int RAW = sizeof(T) == 2 ? 1 : 2;    // 16-byte pieces of 8 values
   constexpr int MB = 2;                          // tiles of 16 rows in a batch
-  constexpr bool AHEAD = FAST && QN <= 2;        // all ranks of w are in registers at a time (steps == QN)
+  constexpr bool AHEAD = FAST && EXACT && QN <= 2;  // all ranks of w are in registers at a time
   constexpr int STEP = kAdapterWarps * kExpandCols;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ RowGroups groups;
   __shared__ float staged[FAST ? 1 : kAdapterWarps][FAST ? 1 : 16][FAST ? 1 : kExpandCols + 1];
   __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem);  // [64][P][Rp], rows `pitch` apart
-  const int pitch = expand_pitch(P, p.Rp);
+  const int pitch = expand_pitch(P, Rp);
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row0 = blockIdx.y * kChunkRows;
   const int ngroups = group_rows(groups, p.ids, row0, p.rows, p.L);
   const int c_begin = blockIdx.x * p.cols_per_cta, c_end = min(p.C, c_begin + p.cols_per_cta);
-  const int steps = p.Rp / 16;
+  const int steps = Rp / 16;
   // rows of the chunk, by 32-bit offsets (a pitch is below 2^24 elements)
   const char* y = static_cast<const char*>(p.y) + row0 * p.ldy * int(sizeof(T));
   char* out = static_cast<char*>(p.out) + row0 * p.ldo * int(sizeof(T));
@@ -880,7 +887,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
         const __nv_bfloat16* at = TRANS ? w + (long long)(q0 * 16 + 4 * t) * p.C + c0 + 4 * g : w + (long long)(c0 + 8 * (g >> 1) + (g & 1)) * p.R + q0 * 16 + 4 * t;
 #pragma unroll
         for (int q = 0; q < QN; ++q) {
-          if (QN > 1 && (q0 + q) * 16 >= p.Rp) break;
+          if (QN > 1 && (q0 + q) * 16 >= Rp) break;
           if constexpr (!TRANS) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -936,11 +943,11 @@ adapter_expand_tile_kernel(const ExpandParams p) {
     if (!waited) pdl_wait();  // for the hidden vectors; y and w are complete before the kernel that makes those starts
     waited = true;
     __syncthreads();
-    const int pieces = P * p.Rp / 8;
+    const int pieces = P * Rp / 8;
     for (int e = threadIdx.x; e < mtiles * 16 * pieces; e += kAdapterThreads) {
       const int r = e / pieces, c = e - r * pieces;
       const int in = r < count ? row0 + groups.order[first + r] : row0;
-      cp_async16(smem_u32(hs + r * pitch + c * 8), p.hidden + (long long)in * P * p.Rp + c * 8, r < count);
+      cp_async16(smem_u32(hs + r * pitch + c * 8), p.hidden + (long long)in * P * Rp + c * 8, r < count);
     }
     cp_async_commit();
     cp_async_wait<0>();
@@ -988,8 +995,8 @@ adapter_expand_tile_kernel(const ExpandParams p) {
               const __nv_bfloat16* at = hs + (m * 16 + g) * pitch + (q0 + q) * 16 + 4 * t;
 #pragma unroll
               for (int i = 0; i < P; ++i) {
-                const uint2 lo = *reinterpret_cast<const uint2*>(at + i * p.Rp);
-                const uint2 hi = *reinterpret_cast<const uint2*>(at + 8 * pitch + i * p.Rp);
+                const uint2 lo = *reinterpret_cast<const uint2*>(at + i * Rp);
+                const uint2 hi = *reinterpret_cast<const uint2*>(at + 8 * pitch + i * Rp);
 #pragma unroll
                 for (int n = 0; n < 4; ++n) mma_bf16(acc[mm][n], lo.x, hi.x, lo.y, hi.y, wu[n][q][0], wu[n][q][1]);
               }
