@@ -130,7 +130,7 @@ int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int 
 template <typename T, int P, int QN, bool TRANS, bool FAST, bool EXACT>
 int launch_expand_tile(const wb::ExpandParams& p, dim3 grid, cudaStream_t s) {
   constexpr auto kernel = wb::adapter_expand_tile_kernel<T, P, QN, TRANS, FAST, EXACT>;
-  const size_t smem = size_t(wb::kChunkRows) * wb::expand_pitch(P, p.Rp) * 2;
+  const size_t smem = size_t(wb::kChunkRows) * wb::expand_pitch(P, p.Rp, FAST && EXACT && QN % 2 == 0) * 2;
   if (int rc = smem > 24 * 1024 ? allow_smem<kernel>() : WB200_OK) return rc;
   WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, smem, s, p));
   return WB200_OK;
@@ -176,7 +176,7 @@ int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const _
   p.cols_per_cta = few ? 2 * wb::kAdapterThreads : div_up(div_up(C, std::max(1, kTargetCtas / chunks)), 256) * 256;
   const size_t esz = f32 ? 4 : 2;
   p.io_vec = aligned_to(out, 16) && ldo * esz % 16 == 0 && (!y || (aligned_to(y, 16) && ldy * esz % 16 == 0));
-  const int vec = few ? (trans ? 2 : 8) : 4;  // elements of a load of w
+  const int vec = few ? (trans ? 2 : 8) : !trans && c.R % 8 == 0 ? 8 : 4;  // elements of a load of w
   p.w_vec = aligned_to(w, 2 * vec) && (trans ? C : c.R) % (trans && few ? 4 : vec) == 0;
   if (few && !trans)
     if (const int pieces = whole_pieces(p)) p.cols_per_cta = wb::few_whole_steps(pieces) * wb::kAdapterThreads / pieces;

@@ -821,9 +821,12 @@ adapter_expand_few_whole_kernel(const ExpandParams p) {
     for (; none != 0u; none &= none - 1u) expand_rest<T>(p, row0 + __ffs(none) - 1, c_begin + threadIdx.x * 8, c_end, kAdapterThreads * 8);
 }
 
-// Elements between the hidden vectors of rows in shared memory: 16 or 48 bytes past a multiple of 64, so that the 8-byte loads of 16 lanes (four rows)
-// fall into different banks.
-__host__ __device__ constexpr int expand_pitch(int parts, int Rp) { return parts * Rp + ((parts * Rp / 2) % 16 == 8 ? 0 : 16); }
+// Elements between the hidden vectors of rows in shared memory: a distance at which the loads that move together fall into different banks, those of
+// four rows of 8-byte pieces, or (PAIRED) of two rows of 16-byte pieces.
+__host__ __device__ constexpr int expand_pitch(int parts, int Rp, bool paired) {
+  const int words = parts * Rp / 2;
+  return paired ? 2 * (words + (words % 32 == 16 ? 0 : 16)) : 2 * (words + (words % 16 == 8 ? 0 : 8));
+}
 
 // Many rows: a warp takes 32 columns of all the rows of a group; a lane has 8 neighbouring columns of two rows of an MMA tile.
 // FAST: rows that start on 16 bytes, whole blocks of 32 columns and of 16 ranks. The values of y are loaded ahead of everything else, a batch of rows
@@ -842,7 +845,9 @@ adapter_expand_tile_kernel(const ExpandParams p) {
   __shared__ RowGroups groups;
   __shared__ float staged[FAST ? 1 : kAdapterWarps][FAST ? 1 : 16][FAST ? 1 : kExpandCols + 1];
   __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem);  // [64][P][Rp], rows `pitch` apart
-  const int pitch = expand_pitch(P, Rp);
+  // A lane's ranks in two steps of 16: eight neighbours (PAIRED: one 16-byte piece serves both steps), or four of each
+  constexpr bool PAIRED = FAST && EXACT && QN % 2 == 0;
+  const int pitch = expand_pitch(P, Rp, PAIRED);
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row0 = blockIdx.y * kChunkRows;
@@ -884,11 +889,22 @@ adapter_expand_tile_kernel(const ExpandParams p) {
     uint32_t wf[4][QN][2];
     auto load_w = [&](int c0, int q0) {
       if constexpr (FAST) {
-        const __nv_bfloat16* at = TRANS ? w + (long long)(q0 * 16 + 4 * t) * p.C + c0 + 4 * g : w + (long long)(c0 + 8 * (g >> 1) + (g & 1)) * p.R + q0 * 16 + 4 * t;
+        const int lane_rank = q0 * 16 + (PAIRED ? 8 : 4) * t;
+        const __nv_bfloat16* at = TRANS ? w + (long long)lane_rank * p.C + c0 + 4 * g : w + (long long)(c0 + 8 * (g >> 1) + (g & 1)) * p.R + lane_rank;
 #pragma unroll
         for (int q = 0; q < QN; ++q) {
-          if (QN > 1 && (q0 + q) * 16 >= Rp) break;
-          if constexpr (!TRANS) {
+          if (!EXACT && (q0 + q) * 16 >= Rp) break;
+          if constexpr (!TRANS && PAIRED) {
+            if (q % 2 == 0)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4*>(at + i * (2 * p.R) + q * 16);
+                wf[i][q][0] = v.x;
+                wf[i][q][1] = v.y;
+                wf[i][q + 1 < QN ? q + 1 : q][0] = v.z;
+                wf[i][q + 1 < QN ? q + 1 : q][1] = v.w;
+              }
+          } else if constexpr (!TRANS) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint2 v = *reinterpret_cast<const uint2*>(at + i * (2 * p.R) + q * 16);
@@ -898,7 +914,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
           } else {
             uint2 v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint2*>(at + (long long)(q * 16 + i) * p.C);
+            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint2*>(at + (long long)(PAIRED ? (q / 2) * 32 + (q % 2) * 4 + i : q * 16 + i) * p.C);
             wf[0][q][0] = low_halves(v[0].x, v[1].x); wf[0][q][1] = low_halves(v[2].x, v[3].x);
             wf[1][q][0] = high_halves(v[0].x, v[1].x); wf[1][q][1] = high_halves(v[2].x, v[3].x);
             wf[2][q][0] = low_halves(v[0].y, v[1].y); wf[2][q][1] = low_halves(v[2].y, v[3].y);
@@ -936,9 +952,19 @@ adapter_expand_tile_kernel(const ExpandParams p) {
       }
     };
     const int c_first = c_begin + warp * kExpandCols;
-    if (FAST && c_first < c_end) {
-      load_y(c_first, 0);
-      if (AHEAD) load_w(c_first, 0);
+    // not FAST: a row's 32 columns to the lanes, the rows of a tile at once, those of the next tile ahead
+    float old[FAST ? 1 : 16];
+    auto load_tile = [&](int c0, int m) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int at = row_at(m * 16 + r);
+        old[FAST ? 0 : r] = c0 + lane < c_end && p.y && at >= 0 ? as_f32<T>(*reinterpret_cast<const T*>(y + (uint32_t(at) * y_pitch + uint32_t(c0 + lane) * uint32_t(sizeof(T))))) : 0.f;
+      }
+    };
+    if (c_first < c_end) {
+      if constexpr (FAST) load_y(c_first, 0);
+      else load_tile(c_first, 0);
+      if (AHEAD || (!FAST && steps <= QN)) load_w(c_first, 0);
     }
     if (!waited) pdl_wait();  // for the hidden vectors; y and w are complete before the kernel that makes those starts
     waited = true;
@@ -954,7 +980,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
     __syncthreads();
 #pragma unroll 1
     for (int c0 = c_first; c0 < c_end; c0 += STEP) {
-      if (!AHEAD) load_w(c0, 0);
+      if (!AHEAD && (FAST || steps > QN || c0 > c_first)) load_w(c0, 0);
       uint32_t wn[4][QN][2];
       if constexpr (AHEAD) {
 #pragma unroll
@@ -989,6 +1015,22 @@ adapter_expand_tile_kernel(const ExpandParams p) {
           if (m >= mtiles) break;
           for (int q0 = 0; q0 < steps; q0 += QN) {
             if (steps > QN && (q0 > 0 || m > 0)) load_w(c0, q0);
+            if constexpr (PAIRED) {
+#pragma unroll
+              for (int q = 0; q < QN; q += 2) {
+                const __nv_bfloat16* at = hs + (m * 16 + g) * pitch + q * 16 + 8 * t;
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                  const uint4 lo = *reinterpret_cast<const uint4*>(at + i * Rp);
+                  const uint4 hi = *reinterpret_cast<const uint4*>(at + 8 * pitch + i * Rp);
+#pragma unroll
+                  for (int n = 0; n < 4; ++n) mma_bf16(acc[mm][n], lo.x, hi.x, lo.y, hi.y, wu[n][q][0], wu[n][q][1]);
+#pragma unroll
+                  for (int n = 0; n < 4; ++n) mma_bf16(acc[mm][n], lo.z, hi.z, lo.w, hi.w, wu[n][q + 1][0], wu[n][q + 1][1]);
+                }
+              }
+              break;
+            }
 #pragma unroll
             for (int q = 0; q < QN; ++q) {
               if (q0 + q >= steps) break;
@@ -1021,18 +1063,17 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) mine[g + (e >> 1) * 8][8 * t + (TRANS ? 4 * (e & 1) + n : 2 * n + (e & 1))] = acc[mm][n][e];
             __syncwarp();
-            const bool there = c0 + lane < c_end;
             float v[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int at = row_at(m * 16 + r);
-              v[r] = there && p.y && at >= 0 ? as_f32<T>(*reinterpret_cast<const T*>(y + (uint32_t(at) * y_pitch + uint32_t(c0 + lane) * uint32_t(sizeof(T))))) : 0.f;
-            }
+            for (int r = 0; r < 16; ++r) v[r] = old[FAST ? 0 : r] + mine[r][lane];
+            if (m + 1 < mtiles) load_tile(c0, m + 1);
+            else if (c0 + STEP < c_end) load_tile(c0 + STEP, 0);
+            if (c0 + lane < c_end)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int at = row_at(m * 16 + r);
-              if (there && at >= 0) *reinterpret_cast<T*>(out + (uint32_t(at) * out_pitch + uint32_t(c0 + lane) * uint32_t(sizeof(T)))) = as_out<T>(v[r] + mine[r][lane]);
-            }
+              for (int r = 0; r < 16; ++r) {
+                const int at = row_at(m * 16 + r);
+                if (at >= 0) *reinterpret_cast<T*>(out + (uint32_t(at) * out_pitch + uint32_t(c0 + lane) * uint32_t(sizeof(T)))) = as_out<T>(v[r]);
+              }
           }
         }
       }
