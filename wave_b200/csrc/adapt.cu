@@ -23,7 +23,10 @@ bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p
 int div_up(long long a, long long b) { return int((a + b - 1) / b); }
 int rank_pad(int R) { return (R + 15) / 16 * 16; }
 int chunks_of(int rows) { return div_up(rows, wb::kChunkRows); }
-bool few_rows(int rows) { return rows <= 64; }  // the kernels for few rows take them 32 at a time
+// The kernels for few rows (taken 32 at a time) are those for groups of a few rows: a group's rows share the loads of its adapter but not its arithmetic.
+// us, few / many, K = N = 4096: rank 16, 1 row 5.0 / 6.6, 8 rows of one adapter 8.0 / 6.6, 32 rows of one 20.8 / 7.4, of eight 8.1 / 8.8, of 64
+// 8.8 / 12.2; rank 64, 4 rows of one adapter 9.1 / 9.2, 64 rows of 16 14.0 / 14.9.
+bool few_rows(int rows, int L) { return rows <= 64 && rows < 8ll * L; }
 
 template <typename... P, typename... A>
 cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
@@ -86,7 +89,7 @@ int splits_for(long long units, int most) {
 // groups, and as one CTA's work it took twice as long as the others (8192 rows of 6 sequences: 255 against 165 us); a CTA without a group
 // leaves at once.
 int group_lanes(int rows, int L, long long others) {
-  return few_rows(rows) ? std::min({rows, L, wb::kFewRows}) : int(std::max<long long>(std::min(4, L), std::min<long long>(std::min(wb::kChunkRows, L), kTargetCtas / others)));
+  return few_rows(rows, L) ? std::min({rows, L, wb::kFewRows}) : int(std::max<long long>(std::min(4, L), std::min<long long>(std::min(wb::kChunkRows, L), kTargetCtas / others)));
 }
 
 struct AdapterCall {
@@ -116,7 +119,7 @@ int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int 
   wb::ShrinkParams p;
   p.x = x; p.w = w; p.ids = c.ids; p.scale = scale; p.hidden = hidden; p.ldx = ldx;
   p.rows = c.rows; p.K = K; p.R = c.R; p.Rp = c.Rp; p.L = c.L; p.parts = c.parts;
-  const bool few = few_rows(c.rows);
+  const bool few = few_rows(c.rows, c.L);
   const int chunks = few ? div_up(c.rows, wb::kFewRows) : chunks_of(c.rows);
   const int splits = few ? splits_for(1, std::max(1, K / 512)) : splits_for(chunks, std::max(1, K / 256));
   p.split_k = div_up(div_up(K, splits), 64) * 64;
@@ -169,7 +172,7 @@ int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const _
   wb::ExpandParams p;
   p.w = w; p.ids = c.ids; p.hidden = hidden; p.y = y; p.out = out; p.ldy = ldy; p.ldo = ldo;
   p.rows = c.rows; p.C = C; p.R = c.R; p.Rp = c.Rp; p.L = c.L;
-  const bool few = few_rows(c.rows);
+  const bool few = few_rows(c.rows, c.L);
   const int chunks = few ? div_up(c.rows, wb::kFewRows) : chunks_of(c.rows);
   // one wave of CTAs where that leaves each several rounds of its 256 columns: what a CTA does before its first column (grouping, hidden vectors)
   // takes as long as a few rounds

@@ -1109,14 +1109,21 @@ struct OuterTile {
   static constexpr int P = 2, COLS = RT * 8;
   static constexpr int Z_BYTES = kChunkRows * kOuterCols * 2, H_BYTES = kChunkRows * P * COLS * 2, STAGE_BYTES = Z_BYTES + H_BYTES;
   static constexpr int STAGES = RT == 8 ? 3 : 4;
-  static constexpr int SUM_PITCH = COLS + 1;
+  static constexpr int SUM_PITCH = COLS + 4;  // 16-byte pieces of 8 neighbouring columns in different banks
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int SMEM_BYTES = RING_BYTES + kOuterSegment * 4;
   static_assert(2 * kOuterCols * SUM_PITCH * 4 <= RING_BYTES, "sums of the two halves of the rows");
 };
 
+__device__ __forceinline__ void zero_fill(__nv_bfloat16* p, int n, int thread, int threads) {
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && n % 8 == 0)
+    for (int i = thread; i < n / 8; i += threads) reinterpret_cast<uint4*>(p)[i] = make_uint4(0u, 0u, 0u, 0u);
+  else
+    for (int i = thread; i < n; i += threads) p[i] = __float2bfloat16_rn(0.f);
+}
+
 template <int RT>
-__global__ void __launch_bounds__(kAdapterThreads)
+__global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_outer_kernel(const OuterParams p) {
   using Cfg = OuterTile<RT>;
   constexpr int STAGES = Cfg::STAGES, P = Cfg::P, COLS = Cfg::COLS;
@@ -1135,6 +1142,7 @@ adapter_outer_kernel(const OuterParams p) {
   const Ids& ids = p.ids;
   const int row_begin = int((long long)p.rows * split / splits), row_end = int((long long)p.rows * (split + 1) / splits);
   const int wc = warp & 3, wk = warp >> 2;  // 32 columns, 32 of a stage's 64 rows
+  bool any = false;
   for (int n0 = 0; n0 < p.Rp; n0 += COLS) {
     float acc[2][RT][4] = {};
     for (int seg = row_begin; seg < row_end; seg += kOuterSegment) {
@@ -1171,6 +1179,7 @@ adapter_outer_kernel(const OuterParams p) {
       }
       __syncthreads();
       const int steps = (total + kChunkRows - 1) / kChunkRows;
+      any |= total > 0;
       // A thread brings the same pieces of every stage: column piece tid % 16 of rows tid / 16 + 16 i of z, and HN pieces of the hidden vectors
       constexpr int ZN = kChunkRows * (kOuterCols / 8) / kAdapterThreads, HN = (kChunkRows * P * RT + kAdapterThreads - 1) / kAdapterThreads;
       const int zr = tid >> 4, zc = tid & 15;
@@ -1250,6 +1259,15 @@ adapter_outer_kernel(const OuterParams p) {
       }
       cp_async_wait<0>();
     }
+    if (splits == 1 && !any) {  // an adapter without rows
+      const int cols = min(kOuterCols, side.C - c0);
+      if (side.rank_major) {
+        for (int r = warp; r < p.R; r += kAdapterWarps) zero_fill(side.out + ((long long)l * p.R + r) * side.C + c0, cols, lane, 32);
+      } else {
+        zero_fill(side.out + ((long long)l * side.C + c0) * p.R, cols * p.R, tid, kAdapterThreads);
+      }
+      return;
+    }
     __syncthreads();
     float* sums = reinterpret_cast<float*>(smem);  // [2 halves of the rows][128 columns][SUM_PITCH]
 #pragma unroll
@@ -1260,29 +1278,58 @@ adapter_outer_kernel(const OuterParams p) {
         for (int e = 0; e < 4; ++e)
           sums[(wk * kOuterCols + 32 * wc + 16 * m + g + (e >> 1) * 8) * Cfg::SUM_PITCH + i * 8 + 2 * t + (e & 1)] = acc[m][i][e];
     __syncthreads();
+    constexpr int QUADS = COLS / 4;  // four ranks of a column at a time
+    float4* quads = reinterpret_cast<float4*>(sums);
+    constexpr int QP = Cfg::SUM_PITCH / 4;
+    for (int e = tid; e < kOuterCols * QUADS; e += kAdapterThreads) {  // the two halves of the rows
+      float4& v = quads[e / QUADS * QP + e % QUADS];
+      const float4 w = quads[(kOuterCols + e / QUADS) * QP + e % QUADS];
+      v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
+    }
+    __syncthreads();
     if (splits > 1) {
       cluster_arrive();
       cluster_wait();
     }
     const int s0 = kOuterCols * split / splits, own = kOuterCols * (split + 1) / splits - s0;  // columns that this CTA finishes
-    for (int e = tid; e < own * COLS; e += kAdapterThreads) {
-      const int c = s0 + (side.rank_major ? e % own : e / COLS), r = side.rank_major ? e / own : e % COLS;
-      if (c0 + c >= side.C || n0 + r >= p.R) continue;
-      const int at = c * Cfg::SUM_PITCH + r;
-      float v = 0.f;
+    for (int e = tid; e < own * QUADS; e += kAdapterThreads) {
+      const int c = s0 + (side.rank_major ? e % own : e / QUADS), q = side.rank_major ? e / own : e % QUADS;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (splits == 1) {
-        v = sums[at] + sums[kOuterCols * Cfg::SUM_PITCH + at];
+        v = quads[c * QP + q];
       } else {
-        const uint32_t a = smem_u32(sums + at);
-        float part[8][2];
+        const uint32_t at = smem_u32(quads + c * QP + q);
+        float4 part[8];
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
+        for (int s = 0; s < 8; ++s) {
+          part[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (s < splits)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(part[s].x), "=f"(part[s].y), "=f"(part[s].z), "=f"(part[s].w)
+                         : "r"(mapa_shared(at, s))
+                         : "memory");
+        }
 #pragma unroll
-          for (int h = 0; h < 2; ++h) part[s][h] = s < splits ? ld_cluster_f32(mapa_shared(a, s) + h * kOuterCols * Cfg::SUM_PITCH * 4) : 0.f;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) v += part[s][0] + part[s][1];
+        for (int s = 0; s < 8; ++s) v = make_float4(v.x + part[s].x, v.y + part[s].y, v.z + part[s].z, v.w + part[s].w);
       }
-      side.out[side.rank_major ? ((long long)l * p.R + n0 + r) * side.C + c0 + c : ((long long)l * side.C + c0 + c) * p.R + n0 + r] = __float2bfloat16_rn(v);
+      const int r = n0 + 4 * q, col = c0 + c;
+      if (col >= side.C || r >= p.R) continue;
+      const float f[4] = {v.x, v.y, v.z, v.w};
+      if (side.rank_major) {
+        __nv_bfloat16* to = side.out + ((long long)l * p.R + r) * side.C + col;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (r + i < p.R) to[(long long)i * side.C] = __float2bfloat16_rn(f[i]);
+      } else {
+        __nv_bfloat16* to = side.out + ((long long)l * side.C + col) * p.R + r;
+        if (p.R % 4 == 0 && (reinterpret_cast<uintptr_t>(side.out) & 7) == 0) {
+          *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (r + i < p.R) to[i] = __float2bfloat16_rn(f[i]);
+        }
+      }
     }
     if (splits > 1) {  // nobody overwrites what others still read
       cluster_arrive();
