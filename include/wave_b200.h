@@ -459,8 +459,9 @@ int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, c
                            int dtype, void* hidden, size_t hidden_bytes, void* stream);
 /* Its gradients for g = the gradient of a bf16 out [rows, N]: dx [rows, K] (the adapters' part, or with accumulate_dx != 0 added to what dx
  * holds), da and db laid out as a and b (zeros for an adapter without rows), all bf16; each may be null. hidden: as the forward call left it
- * (read for db). Sums over rows are made in a fixed order. At most 65535 adapters. workspace (for dx and da): as many bytes as hidden, 16-byte
- * aligned. */
+ * (read for db). Sums over rows are made in a fixed order, which does not depend on which gradients are asked for. At most 65535 adapters.
+ * workspace: wb200_adapters_backward_workspace_bytes(rows, N, rank) bytes, 16-byte aligned. */
+size_t wb200_adapters_backward_workspace_bytes(int rows, int N, int rank);
 int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,
                             const void* ids, int ids_are_int64, const float* scale, const void* g, long long ldg, const void* hidden,
                             size_t hidden_bytes, void* dx, long long ldd, int accumulate_dx, void* da, void* db, void* workspace,

@@ -81,9 +81,9 @@ def test_forward_rows_and_ranks(rows, rank, pool):
     check_forward(make(rows, 256, 200, rank, pool, seed=rows * rank))
 
 
-@pytest.mark.parametrize("K,N", [(8, 1), (32, 7), (264, 33), (1024, 4001), (4096, 64), (2048, 1030)])
+@pytest.mark.parametrize("K,N", [(8, 1), (32, 7), (264, 33), (1024, 4001), (4096, 64), (2048, 1030), (96, 1096)])
 @pytest.mark.parametrize("y_dtype", [BF16, F32])
-@pytest.mark.parametrize("rank", [12, 100, 256])
+@pytest.mark.parametrize("rank", [7, 12, 64, 100, 256])
 def test_forward_widths_and_types(K, N, y_dtype, rank):
     check_forward(make(90, K, N, rank, 4, y_dtype, ids="runs", seed=K + N))
     check_forward(make(5, K, N, rank, 4, y_dtype, ids="mixed", seed=K + N + 1))
@@ -145,7 +145,8 @@ def test_values_that_are_not_finite_stay_in_their_rows():
 
 @pytest.mark.parametrize("rows,K,N,rank,pool,ids", [(1, 64, 64, 4, 1, "last"), (16, 256, 200, 8, 3, "mixed"), (130, 520, 333, 16, 4, "runs"), (300, 256, 1000, 32, 5, "mixed"),
                                                     (700, 1024, 512, 64, 2, "runs"), (260, 128, 264, 100, 3, "mixed"), (129, 2048, 96, 12, 30, "mixed"),
-                                                    (64, 96, 65, 16, 7, "none"), (2000, 256, 256, 16, 1, "last")])
+                                                    (64, 96, 65, 16, 7, "none"), (2000, 256, 256, 16, 1, "last"),
+                                                    (500, 128, 1027, 20, 3, "mixed"), (40, 64, 1030, 8, 20, "mixed"), (5000, 64, 40, 4, 2, "mixed")])
 def test_gradients(rows, K, N, rank, pool, ids):
     y, x, a, b, at, s = make(rows, K, N, rank, pool, ids=ids, seed=rows)
     g = (torch.randn(rows, N, generator=torch.Generator().manual_seed(1)) * 0.01).to(BF16).to(DEV)

@@ -96,6 +96,7 @@ EXPORTED_SYMBOLS = (
     "wb200_moe_combine",
     "wb200_adapters_hidden_bytes",
     "wb200_adapters_forward",
+    "wb200_adapters_backward_workspace_bytes",
     "wb200_adapters_backward",
     "wb200_mxfp4_input_grad",
     "wb200_router_workspace_bytes",
@@ -242,6 +243,8 @@ def load() -> ctypes.CDLL:
     lib.wb200_adapters_forward.restype = c_int
     lib.wb200_adapters_forward.argtypes = [c_int] * 5 + [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_ll, c_void_p,
                                                          c_ll, c_int, c_void_p, c_size_t, c_void_p]
+    lib.wb200_adapters_backward_workspace_bytes.restype = c_size_t
+    lib.wb200_adapters_backward_workspace_bytes.argtypes = [c_int] * 3
     lib.wb200_adapters_backward.restype = c_int
     lib.wb200_adapters_backward.argtypes = [c_int] * 5 + [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_ll, c_void_p,
                                                           c_size_t, c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
@@ -326,7 +329,7 @@ def fast(lib=None):
         names = ("wb200_mxfp4_gemm_repack_a", "wb200_mxfp8_gemm_repack_a", "wb200_mxfp4_gemm_quantize_a", "wb200_mxfp4_gemm_workspace_bytes",
                  "wb200_decode_tile_rows_for")
         beside = ("wb200_adapters_forward", "wb200_adapters_backward", "wb200_mxfp4_input_grad", "wb200_router_workspace_bytes", "wb200_router",
-                  "wb200_router_grad", "wb200_moe_combine", "wb200_moe_combine_grad", "wb200_last_error")
+                  "wb200_router_grad", "wb200_moe_combine", "wb200_moe_combine_grad", "wb200_last_error", "wb200_adapters_backward_workspace_bytes")
         if not isinstance(lib, ctypes.CDLL) or not all(isinstance(getattr(lib, name), lib._FuncPtr) for name in names):
             return None
         try:

@@ -103,12 +103,13 @@ class _Adapters(torch.autograd.Function):
         if need_x or need_a or need_b:
             lib = _lib.load()
             rows_g = _rows(g)
-            ws = torch.empty_like(hidden)
+            nbytes = int(lib.wb200_adapters_backward_workspace_bytes(rows, N, rank))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
             ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
             _launch(x.device, lambda stream: lib.wb200_adapters_backward(
                 rows, K, N, rank, pool, x.data_ptr(), _pitch(x), a.data_ptr(), b.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64),
                 ptr(scale), rows_g.data_ptr(), _pitch(rows_g), hidden.data_ptr(), 2 * hidden.numel(), ptr(dx), K, 0, ptr(da), ptr(db),
-                ws.data_ptr(), 2 * ws.numel(), stream))
+                ws.data_ptr(), nbytes, stream))
         return (g if need_y else None), dx, da, db, None, None, None
 
 

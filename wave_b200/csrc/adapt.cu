@@ -124,7 +124,7 @@ int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int 
   const int splits = few ? splits_for(1, std::max(1, K / 512)) : splits_for(chunks, std::max(1, K / 256));
   p.split_k = div_up(div_up(K, splits), 64) * 64;
   const int vec = !trans ? 8 : !few ? 8 : c.Rp <= 16 ? 2 : c.Rp <= 32 ? 4 : 8;  // elements of a load of w
-  p.x_vec = aligned_to(x, 16) && ldx % 8 == 0 && K % 8 == 0;
+  p.x_vec = aligned_to(x, 16) && ldx % 8 == 0 && ldx >= (K + 7) / 8 * 8;  // (a piece that K ends in is there, zeros behind)
   p.w_vec = aligned_to(w, 2 * vec) && (trans ? c.R : K) % vec == 0;
   const dim3 grid(splits, chunks, group_lanes(c.rows, c.L, (long long)chunks * splits));
   return trans ? launch_shrink_ranks<true>(p, few, grid, c.stream) : launch_shrink_ranks<false>(p, few, grid, c.stream);
@@ -159,7 +159,7 @@ int launch_expand(const wb::ExpandParams& p, bool few, dim3 grid, cudaStream_t s
     return WB200_OK;
   }
   const int steps = p.Rp / 16;
-  if (p.io_vec && p.w_vec && p.C % wb::kExpandCols == 0 && p.R == p.Rp)
+  if (p.io_vec && p.w_vec && p.C % 8 == 0 && (TRANS || steps % 2 == 1 || p.R % 8 == 0))
     return steps == 1   ? launch_expand_tile<T, P, 1, TRANS, true, true>(p, grid, s)
            : steps == 2 ? launch_expand_tile<T, P, 2, TRANS, true, true>(p, grid, s)
            : steps == 4 ? launch_expand_tile<T, P, 4, TRANS, true, true>(p, grid, s)
@@ -179,6 +179,7 @@ int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const _
   p.cols_per_cta = few ? 2 * wb::kAdapterThreads : div_up(div_up(C, std::max(1, kTargetCtas / chunks)), 256) * 256;
   const size_t esz = f32 ? 4 : 2;
   p.io_vec = aligned_to(out, 16) && ldo * esz % 16 == 0 && (!y || (aligned_to(y, 16) && ldy * esz % 16 == 0));
+  p.io_pairs = !f32 && C % 2 == 0 && aligned_to(out, 4) && ldo % 2 == 0 && (!y || (aligned_to(y, 4) && ldy % 2 == 0));
   const int vec = few ? (trans ? 2 : 8) : !trans && c.R % 8 == 0 ? 8 : 4;  // elements of a load of w
   p.w_vec = aligned_to(w, 2 * vec) && (trans ? C : c.R) % (trans && few ? 4 : vec) == 0;
   if (few && !trans)
@@ -205,7 +206,7 @@ int run_outer(const AdapterCall& c, wb::OuterSide first, wb::OuterSide second) {
   p.side[1] = second;
   for (wb::OuterSide& side : p.side) {
     side.blocks = side.out ? div_up(side.C, wb::kOuterCols) : 0;
-    side.vec = aligned_to(side.z, 16) && side.ldz % 8 == 0 && side.C % 8 == 0;
+    side.vec = aligned_to(side.z, 16) && side.ldz % 8 == 0 && side.ldz >= (side.C + 7) / 8 * 8;
   }
   p.ids = c.ids;
   p.rows = c.rows; p.R = c.R; p.Rp = c.Rp; p.L = c.L;
@@ -403,6 +404,12 @@ int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, c
   return run_expand(c, static_cast<const __nv_bfloat16*>(b), false, h, y, ldy, out, ldo, dtype == WB200_F32, N);
 }
 
+size_t wb200_adapters_backward_workspace_bytes(int rows, int N, int rank) {
+  if (rows <= 0 || N <= 0 || rank <= 0) return 0;
+  const size_t hidden = (wb200_adapters_hidden_bytes(rows, rank, WB200_BF16) + 255) / 256 * 256;
+  return hidden + (N % 8 ? size_t(rows) * ((N + 7) / 8 * 8) * 2 : 0);  // and a copy of g whose rows start on 16 bytes
+}
+
 int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,
                             const void* ids, int ids_are_int64, const float* scale, const void* g, long long ldg, const void* hidden,
                             size_t hidden_bytes, void* dx, long long ldd, int accumulate_dx, void* da, void* db, void* workspace,
@@ -410,19 +417,27 @@ int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, 
   if (int rc = check_adapters("adapters backward", rows, K, N, rank, num_adapters)) return rc;
   if (num_adapters > 65535) return fail(WB200_ERR_UNSUPPORTED, "adapters backward: at most 65535 adapters (got %d)", num_adapters);
   if (!dx && !da && !db) return fail(WB200_ERR_INVALID_ARG, "adapters backward: no gradient is asked for");
-  if (!ids || !g || ((dx || da) && (!b || !workspace)) || (dx && !a) || (da && !x) || (db && !hidden))
+  if (!ids || !g || !workspace || ((dx || da) && !b) || (dx && !a) || (da && !x) || (db && !hidden))
     return fail(WB200_ERR_INVALID_ARG, "adapters backward: null pointer");
   if (rows > 1 && (ldg < N || (da && ldx < K) || (dx && ldd < K))) return fail(WB200_ERR_INVALID_ARG, "adapters backward: a row pitch is smaller than a row");
   if (ldd >= 1 << 24) return fail(WB200_ERR_UNSUPPORTED, "adapters backward: a row pitch of 2^24 elements or more");
   if (!aligned_to(x, 2) || !aligned_to(a, 2) || !aligned_to(b, 2) || !aligned_to(g, 2) || !aligned_to(dx, 2) || !aligned_to(da, 2) || !aligned_to(db, 2) ||
       !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(hidden, 16) || !aligned_to(workspace, 16))
     return fail(WB200_ERR_ALIGNMENT, "adapters backward: a tensor is not aligned to its element size, or hidden or the workspace not to 16 bytes");
+  const size_t ws_need = wb200_adapters_backward_workspace_bytes(rows, N, rank);
+  if (workspace_bytes < ws_need) return fail(WB200_ERR_WORKSPACE, "adapters backward: workspace of %zu bytes needed (got %zu)", ws_need, workspace_bytes);
   const size_t need = wb200_adapters_hidden_bytes(rows, rank, WB200_BF16);
-  if ((dx || da) && workspace_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters backward: workspace of %zu bytes needed (got %zu)", need, workspace_bytes);
   if (db && hidden_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters backward: hidden of %zu bytes needed (got %zu)", need, hidden_bytes);
   if (int rc = wbhost::device(nullptr, nullptr)) return rc;
   const AdapterCall c{{ids, ids_are_int64 != 0}, rows, rank, rank_pad(rank), num_adapters, 2, static_cast<cudaStream_t>(stream)};
   const auto* gp = static_cast<const __nv_bfloat16*>(g);
+  if (N % 8) {
+    auto* copy = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(workspace) + (need + 255) / 256 * 256);
+    const int pitch = (N + 7) / 8 * 8;
+    WB_HOST_CUDA(launch(wb::adapter_align_kernel, dim3(std::min(148 * 8, div_up((long long)rows * pitch / 8, 256))), 256, 0, c.stream, gp, ldg, rows, N, copy, pitch));
+    gp = copy;
+    ldg = pitch;
+  }
   auto* u = static_cast<__nv_bfloat16*>(workspace);
   if (dx || da)
     if (int rc = run_shrink(c, gp, ldg, N, static_cast<const __nv_bfloat16*>(b), true, scale, u)) return rc;

@@ -551,7 +551,7 @@ struct ExpandParams {
   void* out;
   long long ldy, ldo;
   int rows, C, R, Rp, L, cols_per_cta;
-  int io_vec, w_vec;
+  int io_vec, w_vec, io_pairs;  // rows of y and out start on 16 bytes; vector loads of w; bf16 rows start on 4 bytes and C is even
 };
 
 template <typename T>
@@ -829,7 +829,7 @@ __host__ __device__ constexpr int expand_pitch(int parts, int Rp, bool paired) {
 }
 
 // Many rows: a warp takes 32 columns of all the rows of a group; a lane has 8 neighbouring columns of two rows of an MMA tile.
-// FAST: rows that start on 16 bytes, whole blocks of 32 columns and of 16 ranks. The values of y are loaded ahead of everything else, a batch of rows
+// FAST: rows that start on 16 bytes, columns in eights, ranks in fours (eights where two steps are loaded as one piece). The values of y are loaded ahead of everything else, a batch of rows
 // (MB tiles of 16) at once, the next batch while this one is worked on, w of the next columns with it; they are the accumulators' first values.
 // Otherwise the accumulators go through shared memory, so that 32 lanes share a row's 32 columns.
 // QN: steps of 16 ranks of w in registers at a time.
@@ -843,6 +843,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
   constexpr int STEP = kAdapterWarps * kExpandCols;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ RowGroups groups;
+  __shared__ uint32_t y_off[FAST ? 1 : kChunkRows], out_off[FAST ? 1 : kChunkRows];  // of a group's rows, in bytes; all ones: none
   __shared__ float staged[FAST ? 1 : kAdapterWarps][FAST ? 1 : 16][FAST ? 1 : kExpandCols + 1];
   __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem);  // [64][P][Rp], rows `pitch` apart
   // A lane's ranks in two steps of 16: eight neighbours (PAIRED: one 16-byte piece serves both steps), or four of each
@@ -864,6 +865,15 @@ adapter_expand_tile_kernel(const ExpandParams p) {
     const __nv_bfloat16* w = p.w + (long long)groups.adapter[gi] * p.R * p.C;
     const int mtiles = (count + 15) >> 4;
     auto row_at = [&](int place) { return place < count ? groups.order[first + place] : -1; };
+    if constexpr (!FAST) {
+      __syncthreads();
+      if (threadIdx.x < kChunkRows) {
+        const int r = row_at(threadIdx.x);
+        y_off[threadIdx.x] = r >= 0 && p.y ? uint32_t(r) * y_pitch : 0xffffffffu;
+        out_off[threadIdx.x] = r >= 0 ? uint32_t(r) * out_pitch : 0xffffffffu;
+      }
+      __syncthreads();
+    }
     int row[4][2];  // in the chunk; -1: none
 #pragma unroll
     for (int m = 0; m < 4; ++m)
@@ -871,6 +881,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
       for (int h = 0; h < 2; ++h) row[m][h] = row_at(m * 16 + h * 8 + g);
     uint4 next[MB][2][RAW];
     auto load_y = [&](int c0, int batch) {  // 8 values of every row of the batch
+      const bool there = p.y && c0 + 8 * t < p.C;  // (C is a multiple of 8)
 #pragma unroll
       for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -882,7 +893,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
           for (int i = 0; i < RAW; ++i) {
             next[m][h][i] = make_uint4(0u, 0u, 0u, 0u);
-            if (p.y && r >= 0) next[m][h][i] = *reinterpret_cast<const uint4*>(y + (uint32_t(r) * y_pitch + uint32_t(c0 + 8 * t) * uint32_t(sizeof(T)) + 16u * i));
+            if (there && r >= 0) next[m][h][i] = *reinterpret_cast<const uint4*>(y + (uint32_t(r) * y_pitch + uint32_t(c0 + 8 * t) * uint32_t(sizeof(T)) + 16u * i));
           }
         }
     };
@@ -894,11 +905,14 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
         for (int q = 0; q < QN; ++q) {
           if (!EXACT && (q0 + q) * 16 >= Rp) break;
+          // ranks and columns behind the last are zeros (a lane's piece is there or not: R is a multiple of its ranks, C of 8)
+          const bool rank_there = lane_rank + (PAIRED ? q / 2 * 32 : q * 16) < p.R;
           if constexpr (!TRANS && PAIRED) {
             if (q % 2 == 0)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const uint4 v = *reinterpret_cast<const uint4*>(at + i * (2 * p.R) + q * 16);
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (rank_there && c0 + 8 * (g >> 1) < p.C) v = *reinterpret_cast<const uint4*>(at + i * (2 * p.R) + q * 16);
                 wf[i][q][0] = v.x;
                 wf[i][q][1] = v.y;
                 wf[i][q + 1 < QN ? q + 1 : q][0] = v.z;
@@ -907,14 +921,19 @@ adapter_expand_tile_kernel(const ExpandParams p) {
           } else if constexpr (!TRANS) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint2 v = *reinterpret_cast<const uint2*>(at + i * (2 * p.R) + q * 16);
+              uint2 v = make_uint2(0u, 0u);
+              if (rank_there && c0 + 8 * (g >> 1) < p.C) v = *reinterpret_cast<const uint2*>(at + i * (2 * p.R) + q * 16);
               wf[i][q][0] = v.x;
               wf[i][q][1] = v.y;
             }
           } else {
             uint2 v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint2*>(at + (long long)(PAIRED ? (q / 2) * 32 + (q % 2) * 4 + i : q * 16 + i) * p.C);
+            for (int i = 0; i < 4; ++i) {
+              const int r = PAIRED ? (q / 2) * 32 + (q % 2) * 4 + i : q * 16 + i;
+              v[i] = make_uint2(0u, 0u);
+              if (lane_rank + r < p.R && c0 + 4 * g < p.C) v[i] = *reinterpret_cast<const uint2*>(at + (long long)r * p.C);
+            }
             wf[0][q][0] = low_halves(v[0].x, v[1].x); wf[0][q][1] = low_halves(v[2].x, v[3].x);
             wf[1][q][0] = high_halves(v[0].x, v[1].x); wf[1][q][1] = high_halves(v[2].x, v[3].x);
             wf[2][q][0] = low_halves(v[0].y, v[1].y); wf[2][q][1] = low_halves(v[2].y, v[3].y);
@@ -954,11 +973,26 @@ adapter_expand_tile_kernel(const ExpandParams p) {
     const int c_first = c_begin + warp * kExpandCols;
     // not FAST: a row's 32 columns to the lanes, the rows of a tile at once, those of the next tile ahead
     float old[FAST ? 1 : 16];
+    // (bf16 rows that start on 4 bytes: two columns to a lane, two rows to a load)
+    const bool pairs = sizeof(T) == 2 && p.io_pairs;
+    const int lane_row = pairs ? lane >> 4 : 0, lane_col = pairs ? (lane & 15) * 2 : lane;
     auto load_tile = [&](int c0, int m) {
+      const bool there = c0 + lane_col < c_end;
+      const uint32_t at = uint32_t(c0 + lane_col) * uint32_t(sizeof(T));
+      if (pairs) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const uint32_t off = y_off[FAST ? 0 : m * 16 + 2 * r + lane_row];
+          const uint32_t v = there && off != 0xffffffffu ? *reinterpret_cast<const uint32_t*>(y + (off + at)) : 0u;
+          old[FAST ? 0 : 2 * r] = __uint_as_float(v << 16);
+          old[FAST ? 0 : 2 * r + 1] = __uint_as_float(v & 0xffff0000u);
+        }
+        return;
+      }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int at = row_at(m * 16 + r);
-        old[FAST ? 0 : r] = c0 + lane < c_end && p.y && at >= 0 ? as_f32<T>(*reinterpret_cast<const T*>(y + (uint32_t(at) * y_pitch + uint32_t(c0 + lane) * uint32_t(sizeof(T))))) : 0.f;
+        const uint32_t off = y_off[FAST ? 0 : m * 16 + r];
+        old[FAST ? 0 : r] = there && off != 0xffffffffu ? as_f32<T>(*reinterpret_cast<const T*>(y + (off + at))) : 0.f;
       }
     };
     if (c_first < c_end) {
@@ -1047,7 +1081,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
           if constexpr (FAST) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (row[m][h] < 0) continue;
+              if (row[m][h] < 0 || c0 + 8 * t >= p.C) continue;
               float v[8];
 #pragma unroll
               for (int n = 0; n < 4; ++n)
@@ -1065,15 +1099,25 @@ adapter_expand_tile_kernel(const ExpandParams p) {
             __syncwarp();
             float v[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) v[r] = old[FAST ? 0 : r] + mine[r][lane];
+            for (int r = 0; r < 16; ++r) v[r] = old[FAST ? 0 : r] + (pairs ? mine[(r & ~1) + lane_row][lane_col + (r & 1)] : mine[r][lane]);
             if (m + 1 < mtiles) load_tile(c0, m + 1);
             else if (c0 + STEP < c_end) load_tile(c0 + STEP, 0);
-            if (c0 + lane < c_end)
+            if (c0 + lane_col < c_end) {
+              const uint32_t at = uint32_t(c0 + lane_col) * uint32_t(sizeof(T));
+              if (pairs) {
 #pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const int at = row_at(m * 16 + r);
-                if (at >= 0) *reinterpret_cast<T*>(out + (uint32_t(at) * out_pitch + uint32_t(c0 + lane) * uint32_t(sizeof(T)))) = as_out<T>(v[r]);
+                for (int r = 0; r < 8; ++r) {
+                  const uint32_t off = out_off[FAST ? 0 : m * 16 + 2 * r + lane_row];
+                  if (off != 0xffffffffu) *reinterpret_cast<uint32_t*>(out + (off + at)) = pack_bf16x2(v[2 * r], v[2 * r + 1]);
+                }
+              } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                  const uint32_t off = out_off[FAST ? 0 : m * 16 + r];
+                  if (off != 0xffffffffu) *reinterpret_cast<T*>(out + (off + at)) = as_out<T>(v[r]);
+                }
               }
+            }
           }
         }
       }
@@ -1083,6 +1127,20 @@ adapter_expand_tile_kernel(const ExpandParams p) {
   if (blockIdx.z == 0 && p.out != p.y)
     for (int r = warp; r < min(kChunkRows, p.rows - row0); r += kAdapterWarps)
       if (groups.id[r] < 0) expand_rest<T>(p, row0 + r, c_begin + lane * 8, c_end, 256);
+}
+
+// Rows of any alignment into rows of `pitch` (a multiple of 8) elements, zeros behind the last: what follows copies whole pieces.
+__global__ void __launch_bounds__(256) adapter_align_kernel(const __nv_bfloat16* src, long long ld, int rows, int cols, __nv_bfloat16* dst, int pitch) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int pieces = pitch / 8;
+  const long long total = (long long)rows * pieces;
+  for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (long long)gridDim.x * blockDim.x) {
+    const int row = int(e / pieces), c = int(e - (long long)row * pieces) * 8;
+    uint32_t r[4];
+    load_bf16<8>(src + row * ld + c, false, cols - c, r);
+    *reinterpret_cast<uint4*>(dst + e * 8) = make_uint4(r[0], r[1], r[2], r[3]);
+  }
 }
 
 struct OuterSide {

@@ -42,6 +42,7 @@ struct Abi {
   int (*combine)(const void*, long long, int, const int*, const float*, int, int, int, void*, long long, void*);
   int (*combine_grad)(const void*, long long, const void*, long long, int, const int*, int, int, int, float*, void*);
   const char* (*last_error)();
+  size_t (*adapters_backward_workspace_bytes)(int, int, int);
 } entry;
 
 void check(int rc) { TORCH_CHECK(rc == 0, "wave_b200: ", entry.last_error(), " (status ", rc, ")"); }
@@ -112,11 +113,12 @@ struct AdaptersNode : torch::autograd::Function<AdaptersNode> {
     if (ctx->needs_input_grad(2)) da = fresh(a.sizes(), at::kBFloat16, x);
     if (ctx->needs_input_grad(3)) db = fresh(b.sizes(), at::kBFloat16, x);
     if (dx.defined() || da.defined() || db.defined()) {
-      const Tensor ws = fresh(hidden.sizes(), at::kBFloat16, x);
+      const size_t bytes = entry.adapters_backward_workspace_bytes(int(x.size(0)), int(b.size(1)), int(a.size(1)));
+      const Tensor ws = fresh({int64_t(bytes)}, at::kByte, x);
       check(entry.adapters_backward(int(x.size(0)), int(x.size(1)), int(b.size(1)), int(a.size(1)), int(a.size(0)), x.data_ptr(), pitch(x), a.data_ptr(),
                                   b.data_ptr(), ids.data_ptr(), ids.scalar_type() == at::kLong, static_cast<const float*>(ptr(scale)), g.data_ptr(), pitch(g),
                                   hidden.data_ptr(), size_t(hidden.numel()) * 2, ptr(dx), x.size(1), 0, ptr(da), ptr(db), ws.data_ptr(),
-                                  size_t(ws.numel()) * 2, stream_of(x)));
+                                  bytes, stream_of(x)));
       variable_list mine = once({dx, da, db});
       for (int i = 0; i < 3; ++i) result[1 + i] = mine[i];
     }
@@ -342,10 +344,11 @@ PyObject* input_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
-// bind_adapt(adapters_forward, adapters_backward, input_grad, router_workspace_bytes, router, router_grad, combine, combine_grad, last_error)
+// bind_adapt(adapters_forward, adapters_backward, input_grad, router_workspace_bytes, router, router_grad, combine, combine_grad, last_error,
+//            adapters_backward_workspace_bytes)
 PyObject* bind_adapt(PyObject*, PyObject* args) {
-  unsigned long long p[9];
-  if (!PyArg_ParseTuple(args, "KKKKKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7], &p[8])) return nullptr;
+  unsigned long long p[10];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7], &p[8], &p[9])) return nullptr;
   entry.adapters_forward = reinterpret_cast<decltype(entry.adapters_forward)>(p[0]);
   entry.adapters_backward = reinterpret_cast<decltype(entry.adapters_backward)>(p[1]);
   entry.input_grad = reinterpret_cast<decltype(entry.input_grad)>(p[2]);
@@ -355,6 +358,7 @@ PyObject* bind_adapt(PyObject*, PyObject* args) {
   entry.combine = reinterpret_cast<decltype(entry.combine)>(p[6]);
   entry.combine_grad = reinterpret_cast<decltype(entry.combine_grad)>(p[7]);
   entry.last_error = reinterpret_cast<decltype(entry.last_error)>(p[8]);
+  entry.adapters_backward_workspace_bytes = reinterpret_cast<decltype(entry.adapters_backward_workspace_bytes)>(p[9]);
   Py_RETURN_NONE;
 }
 
