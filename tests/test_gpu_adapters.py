@@ -343,6 +343,24 @@ def test_layer_trains_adapters_through_frozen_layers():
         assert float((got.double() - ref).norm()) <= 4 * 2.0 ** -8 * float(ref.norm())
 
 
+@pytest.mark.parametrize("rows,N", [(5, 192), (200, 96), (90, 77)])
+def test_layer_gradient_is_the_layers_part_with_the_adapters_on_it(rows, N):
+    g = torch.Generator().manual_seed(rows)
+    layer = wb.MXFP4Linear.from_float((torch.randn(N, 256, generator=g) / 16).to(DEV), input_grad=True)
+    y, x, a, b, ids, s = make(rows, 256, N, 16, 4, seed=rows)
+    pool = wb.LowRankAdapters(a, b, s)
+    up = torch.randn(rows, N, generator=g).to(BF16).to(DEV)
+    x.requires_grad_()
+    out = layer(x, pool, ids)
+    dx, = torch.autograd.grad(out, x, up)
+    assert torch.equal(out.detach(), wb.apply_adapters(layer._base(x.detach()), x.detach(), a, b, ids, s))
+    part = wb.mxfp4_input_grad(up, layer.weight_codes, layer.weight_scales)
+    _, (want, size), _, _ = definition(y, x, a, b, ids, s, up)
+    assert_near(dx, part.double() + want, size, N + 16, 2)
+    assert torch.equal(dx[ids < 0], part[ids < 0])
+    assert torch.equal(out.detach()[ids < 0], layer._base(x.detach())[ids < 0])
+
+
 def test_every_combination_of_wanted_gradients():
     y, x, a, b, ids, s = make(70, 128, 64, 16, 3)
     g = torch.randn(70, 64, generator=torch.Generator().manual_seed(4)).to(BF16).to(DEV)

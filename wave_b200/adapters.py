@@ -95,22 +95,54 @@ class _Adapters(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         x, a, b, ids, scale, hidden = ctx.saved_tensors
-        rows, K, N, rank, pool = ctx.sizes
-        need_y, need_x, need_a, need_b = ctx.needs_input_grad[:4]
-        dx = torch.empty(rows, K, dtype=torch.bfloat16, device=x.device) if need_x else None
-        da = torch.empty_like(a) if need_a else None
-        db = torch.empty_like(b) if need_b else None
-        if need_x or need_a or need_b:
-            lib = _lib.load()
-            rows_g = _rows(g)
-            nbytes = int(lib.wb200_adapters_backward_workspace_bytes(rows, N, rank))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-            _launch(x.device, lambda stream: lib.wb200_adapters_backward(
-                rows, K, N, rank, pool, x.data_ptr(), _pitch(x), a.data_ptr(), b.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64),
-                ptr(scale), rows_g.data_ptr(), _pitch(rows_g), hidden.data_ptr(), 2 * hidden.numel(), ptr(dx), K, 0, ptr(da), ptr(db),
-                ws.data_ptr(), nbytes, stream))
-        return (g if need_y else None), dx, da, db, None, None, None
+        need = ctx.needs_input_grad
+        dx = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) if need[1] else None
+        da, db = _backward(ctx.sizes, x, a, b, ids, scale, _rows(g), hidden, dx, False, need[2], need[3])
+        return (g if need[0] else None), dx, da, db, None, None, None
+
+
+def _backward(sizes, x, a, b, ids, scale, g, hidden, dx, accumulate: bool, need_a: bool, need_b: bool):
+    """Writes dx (or with `accumulate` adds to it), if it is given, and returns the gradients of a and b that are asked for."""
+    rows, K, N, rank, pool = sizes
+    da = torch.empty_like(a) if need_a else None
+    db = torch.empty_like(b) if need_b else None
+    if dx is None and not need_a and not need_b:
+        return da, db
+    lib = _lib.load()
+    nbytes = int(lib.wb200_adapters_backward_workspace_bytes(rows, N, rank))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    _launch(x.device, lambda stream: lib.wb200_adapters_backward(
+        rows, K, N, rank, pool, x.data_ptr(), _pitch(x), a.data_ptr(), b.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), ptr(scale),
+        g.data_ptr(), _pitch(g), hidden.data_ptr(), 2 * hidden.numel(), ptr(dx), K, int(accumulate), ptr(da), ptr(db), ws.data_ptr(), nbytes, stream))
+    return da, db
+
+
+class AdaptedLinear(torch.autograd.Function):
+    """A frozen layer with adapters as one node: x [rows, K], the adapters' part written onto the layer's output, and onto the layer's part of the
+    gradient of x."""
+
+    @staticmethod
+    def forward(ctx, x, a, b, ids, scale, layer):
+        y = layer._base(x)
+        sizes = _check(y, x, a, b, ids, scale, None)
+        if y.dtype != torch.bfloat16 or sizes[4] > MAX_TRAINED:
+            raise ValueError(f"gradients need a bfloat16 output and at most {MAX_TRAINED} adapters, got {y.dtype} and {sizes[4]}")
+        x, a, b, ids = _rows(x), a.contiguous(), b.contiguous(), ids.contiguous()
+        scale = scale.contiguous() if scale is not None else None
+        hidden = _forward(sizes, y, x, a, b, ids, scale, y)
+        ctx.save_for_backward(x, a, b, ids, scale, hidden, layer.weight_codes, layer.weight_scales)
+        ctx.sizes = sizes
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, a, b, ids, scale, hidden, codes, scales = ctx.saved_tensors
+        g = _rows(g)
+        dx = ops.mxfp4_input_grad(g, codes, scales) if ctx.needs_input_grad[0] else None
+        da, db = _backward(ctx.sizes, x, a, b, ids, scale, g, hidden, dx, True, *ctx.needs_input_grad[1:3])
+        return dx, da, db, None, None, None
 
 
 def apply_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, scale: torch.Tensor | None = None,

@@ -160,6 +160,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool r
   const uint32_t bytes = real ? 16u : 0u;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async_bytes(uint32_t dst, const void* src, uint32_t bytes) {  // zeros behind `bytes`
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -420,12 +423,14 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) row_of_x[h] = xr + 32 * h < count ? p.x + (long long)(row0 + groups.order[first + xr + 32 * h]) * p.ldx + k0 + xc * 8 : nullptr;
     for (int n0 = 0; n0 < p.Rp; n0 += COLS) {
+      // a piece that is not there (a row behind the group's last, a rank behind R) is zeros: its address stays where it is, with a size of 0
       const __nv_bfloat16 *xsrc[2], *wsrc[WN];
-      int w_valid[WN], w_k[WN];  // ranks of a piece (TRANS); its k in a stage
+      int x_there[2], w_there[WN], w_k[WN];  // elements of a piece that are there; its first k in a stage
       uint32_t xdst[2], wdst[WN];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        xsrc[h] = row_of_x[h];
+        x_there[h] = row_of_x[h] ? 8 : 0;
+        xsrc[h] = row_of_x[h] ? row_of_x[h] : p.x;
         xdst[h] = piece<8>(xr + 32 * h, xc);
       }
 #pragma unroll
@@ -434,65 +439,65 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
         if constexpr (!TRANS) {  // [rank][64 k]
           const int r = e >> 3, c = e & 7;
           w_k[i] = c * 8;
-          w_valid[i] = e < COLS * 8 && n0 + r < p.R ? 8 : 0;
-          wsrc[i] = w + (long long)(n0 + r) * p.K + k0 + c * 8;
+          w_there[i] = e < COLS * 8 && n0 + r < p.R ? 8 : 0;
+          wsrc[i] = w_there[i] ? w + (long long)(n0 + r) * p.K + k0 + c * 8 : p.w;
           wdst[i] = Cfg::X_BYTES + piece<8>(r, c);
         } else {  // [k][ranks]
           const int k = e / RT, c = e % RT;
           w_k[i] = k;
-          w_valid[i] = e < 64 * RT ? min(8, p.R - n0 - c * 8) : 0;
-          wsrc[i] = w + (long long)(k0 + k) * p.R + n0 + c * 8;
+          w_there[i] = e < 64 * RT ? max(0, min(8, p.R - n0 - c * 8)) : 0;
+          wsrc[i] = w_there[i] ? w + (long long)(k0 + k) * p.R + n0 + c * 8 : p.w;
           wdst[i] = Cfg::X_BYTES + piece<RT>(k, c);
         }
       }
-      int left = k1 - k0;        // k that are not loaded yet
-      uint32_t to = base;        // stage of the next load
+      const bool w_mine = RT * 64 >= kAdapterThreads || tid < RT * 64;
       const long long w_step = TRANS ? 64ll * p.R : 64ll;
       const bool fast = p.x_vec && p.w_vec;
-      auto load = [&]() {
-        if (fast && left >= 64) {  // whole pieces: nothing to look at but whether the row or rank is there
+      int left = k1 - k0;        // k that are not loaded yet
+      uint32_t to = base;        // first stage of the next load
+      constexpr uint32_t LAST = (STAGES - Cfg::PER_SYNC) * Cfg::STAGE_BYTES;
+      auto load_group = [&]() {
+        if (fast && left >= 64 * Cfg::PER_SYNC) {  // whole pieces
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            cp_async16(to + xdst[h], xsrc[h] ? xsrc[h] : p.x, xsrc[h] != nullptr);
-            if (xsrc[h]) xsrc[h] += 64;
-          }
+          for (int sub = 0; sub < Cfg::PER_SYNC; ++sub) {
 #pragma unroll
-          for (int i = 0; i < WN; ++i) {
-            if (RT * 64 < kAdapterThreads && tid >= RT * 64) break;
-            cp_async16(to + wdst[i], w_valid[i] > 0 ? wsrc[i] : p.w, w_valid[i] > 0);
-            wsrc[i] += w_step;
+            for (int h = 0; h < 2; ++h) cp_async_bytes(to + sub * Cfg::STAGE_BYTES + xdst[h], xsrc[h] + (x_there[h] ? sub * 64 : 0), 2 * x_there[h]);
+#pragma unroll
+            for (int i = 0; i < WN; ++i)
+              if (w_mine) cp_async_bytes(to + sub * Cfg::STAGE_BYTES + wdst[i], wsrc[i] + (w_there[i] ? sub * w_step : 0), w_there[i] ? 16 : 0);
           }
         } else {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            copy8(to + xdst[h], xsrc[h], p.x, p.x_vec != 0, xsrc[h] ? min(8, left - xc * 8) : 0);
-            if (xsrc[h]) xsrc[h] += 64;
-          }
+          for (int sub = 0; sub < Cfg::PER_SYNC; ++sub) {
+            const int rest = left - 64 * sub;
+            if (rest <= 0) break;
 #pragma unroll
-          for (int i = 0; i < WN; ++i) {
-            if (RT * 64 < kAdapterThreads && tid >= RT * 64) break;
-            copy8(to + wdst[i], wsrc[i], p.w, p.w_vec != 0, TRANS ? (w_k[i] < left ? w_valid[i] : 0) : min(w_valid[i], left - w_k[i]));
-            wsrc[i] += w_step;
+            for (int h = 0; h < 2; ++h)
+              copy8(to + sub * Cfg::STAGE_BYTES + xdst[h], xsrc[h] + sub * 64, p.x, p.x_vec != 0, x_there[h] ? min(8, rest - xc * 8) : 0);
+#pragma unroll
+            for (int i = 0; i < WN; ++i)
+              if (w_mine)
+                copy8(to + sub * Cfg::STAGE_BYTES + wdst[i], wsrc[i] + sub * w_step, p.w, p.w_vec != 0, TRANS ? (w_k[i] < rest ? w_there[i] : 0) : min(w_there[i], rest - w_k[i]));
           }
         }
-        left -= 64;
-        to = to == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : to + Cfg::STAGE_BYTES;
+        cp_async_commit();
+        left -= 64 * Cfg::PER_SYNC;
+        to = to == base + LAST ? base : to + Cfg::PER_SYNC * Cfg::STAGE_BYTES;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (x_there[h]) xsrc[h] += 64 * Cfg::PER_SYNC;
+#pragma unroll
+        for (int i = 0; i < WN; ++i)
+          if (w_there[i]) wsrc[i] += Cfg::PER_SYNC * w_step;
       };
       const int half = lane >> 4, in = lane & 15;
-      uint32_t xoff[2], woff[RT / 2];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) xoff[m] = piece<8>(32 * wm + 16 * m + in, 2 * wq + half);
+      const uint32_t xoff = piece<8>(32 * wm + in, 2 * wq + half);  // 16 rows on: 2048 bytes, the same swizzle
+      uint32_t woff[RT / 2];
 #pragma unroll
       for (int i = 0; i < RT; i += 2)
-        woff[i / 2] = Cfg::X_BYTES + (TRANS ? piece<RT>(16 * wq + in, i + half) : piece<8>(i * 8 + half * 8 + (in & 7), 2 * wq + (in >> 3)));
+        woff[i / 2] = Cfg::X_BYTES + (TRANS ? piece<RT>(16 * wq + in, i + half) : piece<8>(half * 8 + (in & 7), 2 * wq + (in >> 3)) + i * 1024);
       uint32_t from = base;
       float acc[2][RT][4] = {};
-      auto load_group = [&]() {
-#pragma unroll
-        for (int i = 0; i < Cfg::PER_SYNC; ++i)
-          if (left > 0) load();
-        cp_async_commit();
-      };
 #pragma unroll
       for (int i = 0; i < Cfg::GROUPS - 1; ++i) load_group();
       for (int step = 0; step < steps; step += Cfg::PER_SYNC) {
@@ -504,12 +509,12 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
           if (32 * wm < count && step + sub < steps) {
             uint32_t xa[2][4];
 #pragma unroll
-            for (int m = 0; m < 2; ++m) ldsm4(from + xoff[m], xa[m]);
+            for (int m = 0; m < 2; ++m) ldsm4(from + xoff + sub * Cfg::STAGE_BYTES + m * 2048, xa[m]);
 #pragma unroll
             for (int i = 0; i < RT; i += 2) {
               uint32_t wf[4];
-              if constexpr (!TRANS) ldsm4(from + woff[i / 2], wf);
-              else ldsm4_trans(from + woff[i / 2], wf);
+              if constexpr (!TRANS) ldsm4(from + woff[0] + sub * Cfg::STAGE_BYTES + i * 1024, wf);
+              else ldsm4_trans(from + woff[i / 2] + sub * Cfg::STAGE_BYTES, wf);
 #pragma unroll
               for (int m = 0; m < 2; ++m) {
                 mma_bf16(acc[m][i], xa[m][0], xa[m][1], xa[m][2], xa[m][3], wf[0], wf[1]);
@@ -517,8 +522,8 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
               }
             }
           }
-          from = from == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : from + Cfg::STAGE_BYTES;
         }
+        from = from == base + LAST ? base : from + Cfg::PER_SYNC * Cfg::STAGE_BYTES;
       }
       cp_async_wait<0>();
       __syncthreads();
@@ -880,8 +885,9 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) row[m][h] = row_at(m * 16 + h * 8 + g);
     uint4 next[MB][2][RAW];
-    auto load_y = [&](int c0, int batch) {  // 8 values of every row of the batch
-      const bool there = p.y && c0 + 8 * t < p.C;  // (C is a multiple of 8)
+    // 8 values of every row of the batch. A row or column that is not there reads the first one's: what comes of it is not stored.
+    auto load_y = [&](int c0, int batch) {
+      const uint32_t at = uint32_t(c0 + 8 * t < p.C ? c0 + 8 * t : 0) * uint32_t(sizeof(T));  // (C is a multiple of 8)
 #pragma unroll
       for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -891,28 +897,26 @@ adapter_expand_tile_kernel(const ExpandParams p) {
           for (int b = 1; b < 4 / MB; ++b)
             if (b == batch) r = row[b * MB + m][h];
 #pragma unroll
-          for (int i = 0; i < RAW; ++i) {
-            next[m][h][i] = make_uint4(0u, 0u, 0u, 0u);
-            if (there && r >= 0) next[m][h][i] = *reinterpret_cast<const uint4*>(y + (uint32_t(r) * y_pitch + uint32_t(c0 + 8 * t) * uint32_t(sizeof(T)) + 16u * i));
-          }
+          for (int i = 0; i < RAW; ++i) next[m][h][i] = p.y ? *reinterpret_cast<const uint4*>(y + (uint32_t(max(r, 0)) * y_pitch + at + 16u * i)) : make_uint4(0u, 0u, 0u, 0u);
         }
     };
     uint32_t wf[4][QN][2];
     auto load_w = [&](int c0, int q0) {
       if constexpr (FAST) {
         const int lane_rank = q0 * 16 + (PAIRED ? 8 : 4) * t;
-        const __nv_bfloat16* at = TRANS ? w + (long long)lane_rank * p.C + c0 + 4 * g : w + (long long)(c0 + 8 * (g >> 1) + (g & 1)) * p.R + lane_rank;
+        const int cw = TRANS ? (c0 + 4 * g < p.C ? c0 + 4 * g : 0) : (c0 + 8 * (g >> 1) < p.C ? c0 + 8 * (g >> 1) : 0) + (g & 1);  // (columns as in load_y)
+        const __nv_bfloat16* at = TRANS ? w + (long long)lane_rank * p.C + cw : w + (long long)cw * p.R + lane_rank;
 #pragma unroll
         for (int q = 0; q < QN; ++q) {
           if (!EXACT && (q0 + q) * 16 >= Rp) break;
-          // ranks and columns behind the last are zeros (a lane's piece is there or not: R is a multiple of its ranks, C of 8)
-          const bool rank_there = lane_rank + (PAIRED ? q / 2 * 32 : q * 16) < p.R;
+          // ranks behind the last are zeros (a lane's piece is there or not: R is a multiple of its ranks)
+          const bool rank_there = p.R == Rp || lane_rank + (PAIRED ? q / 2 * 32 : q * 16) < p.R;
           if constexpr (!TRANS && PAIRED) {
             if (q % 2 == 0)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (rank_there && c0 + 8 * (g >> 1) < p.C) v = *reinterpret_cast<const uint4*>(at + i * (2 * p.R) + q * 16);
+                if (rank_there) v = *reinterpret_cast<const uint4*>(at + i * (2 * p.R) + q * 16);
                 wf[i][q][0] = v.x;
                 wf[i][q][1] = v.y;
                 wf[i][q + 1 < QN ? q + 1 : q][0] = v.z;
@@ -922,7 +926,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint2 v = make_uint2(0u, 0u);
-              if (rank_there && c0 + 8 * (g >> 1) < p.C) v = *reinterpret_cast<const uint2*>(at + i * (2 * p.R) + q * 16);
+              if (rank_there) v = *reinterpret_cast<const uint2*>(at + i * (2 * p.R) + q * 16);
               wf[i][q][0] = v.x;
               wf[i][q][1] = v.y;
             }
@@ -932,7 +936,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
             for (int i = 0; i < 4; ++i) {
               const int r = PAIRED ? (q / 2) * 32 + (q % 2) * 4 + i : q * 16 + i;
               v[i] = make_uint2(0u, 0u);
-              if (lane_rank + r < p.R && c0 + 4 * g < p.C) v[i] = *reinterpret_cast<const uint2*>(at + (long long)r * p.C);
+              if (p.R == Rp || lane_rank + r < p.R) v[i] = *reinterpret_cast<const uint2*>(at + (long long)r * p.C);
             }
             wf[0][q][0] = low_halves(v[0].x, v[1].x); wf[0][q][1] = low_halves(v[2].x, v[3].x);
             wf[1][q][0] = high_halves(v[0].x, v[1].x); wf[1][q][1] = high_halves(v[2].x, v[3].x);

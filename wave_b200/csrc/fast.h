@@ -7,7 +7,7 @@
 
 namespace wbfast {
 
-bool plain(PyObject* o);                  // an ordinary CUDA tensor (fast_call.cpp)
+bool plain_or_parameter(PyObject* o);     // an ordinary CUDA tensor, or one as a module's parameter (fast_call.cpp)
 PyObject* fail(const std::exception& e);  // raises it, returns null
 
 PyObject* bind_adapt(PyObject*, PyObject* args);

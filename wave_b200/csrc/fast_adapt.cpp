@@ -58,7 +58,7 @@ void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.devi
 bool fits(int64_t n) { return n > 0 && n <= 0x7fffffff; }
 // A tensor on the current device that needs nothing from the Python code; false leaves the call to it.
 bool here(PyObject* o, Tensor* t) {
-  if (!wbfast::plain(o)) return false;
+  if (!wbfast::plain_or_parameter(o)) return false;
   *t = THPVariable_Unpack(o);
   return t->device().index() == c10::cuda::current_device();
 }

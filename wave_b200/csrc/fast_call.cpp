@@ -74,15 +74,14 @@ void set_mark(PyObject* m) { PyList_SetItem(PyTuple_GET_ITEM(m, 0), 0, Py_NewRef
 
 // An ordinary CUDA tensor: no subclass, no wrapper of a functional transform. Tensors made in inference mode count (a layer's output there is the
 // next one's input): they only lack the autograd keys.
-bool plain(PyObject* o) {
-  if (Py_TYPE(o) != reinterpret_cast<PyTypeObject*>(THPVariableClass)) return false;
-  const at::Tensor& t = THPVariable_Unpack(o);
+bool ordinary(const at::Tensor& t) {
   static const c10::DispatchKeySet inference = c10::DispatchKeySet(c10::DispatchKey::CUDA) |
                                                c10::getAutocastRelatedKeySetFromBackend(c10::BackendComponent::CUDABit);
-  static const c10::DispatchKeySet ordinary = inference | c10::DispatchKeySet(c10::DispatchKey::ADInplaceOrView) |
+  static const c10::DispatchKeySet with_autograd = inference | c10::DispatchKeySet(c10::DispatchKey::ADInplaceOrView) |
                                               c10::getAutogradRelatedKeySetFromBackend(c10::BackendComponent::CUDABit);
-  return (t.key_set() == ordinary || t.key_set() == inference) && t.layout() == at::kStrided;
+  return (t.key_set() == with_autograd || t.key_set() == inference) && t.layout() == at::kStrided;
 }
+bool plain(PyObject* o) { return Py_TYPE(o) == reinterpret_cast<PyTypeObject*>(THPVariableClass) && ordinary(THPVariable_Unpack(o)); }
 
 struct Signature {
   int64_t size[2], stride[2];
@@ -576,7 +575,16 @@ bool add_type(PyObject* module, const char* name, const char* qualified, PyMetho
 }  // namespace
 
 namespace wbfast {
-bool plain(PyObject* o) { return ::plain(o); }
+bool plain_or_parameter(PyObject* o) {
+  static PyObject* parameter = [] {  // of torch.nn; null: not to be had, parameters are then left to the Python code
+    PyObject* module = PyImport_ImportModule("torch.nn.parameter");
+    PyObject* type = module ? PyObject_GetAttrString(module, "Parameter") : nullptr;
+    Py_XDECREF(module);
+    if (!type) PyErr_Clear();
+    return type;
+  }();
+  return ::plain(o) || (parameter && Py_TYPE(o) == reinterpret_cast<PyTypeObject*>(parameter) && ::ordinary(THPVariable_Unpack(o)));
+}
 PyObject* fail(const std::exception& e) { return ::fail(e); }
 }  // namespace wbfast
 

@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib, ops
+from .adapters import AdaptedLinear
 from .lang import as_output_dtype
 
 
@@ -118,22 +119,24 @@ class MXFP4Linear(torch.nn.Module):
         return self._forward_trained(x, adapters, ids)
 
     def _forward_trained(self, x: torch.Tensor, adapters, ids) -> torch.Tensor:
-        if torch.is_grad_enabled() and x.requires_grad:
+        through = torch.is_grad_enabled() and x.requires_grad
+        if through:
             if not self.input_grad:
                 raise ValueError("the gradient of x needs the layer's part: make the layer with input_grad=True, or pass x.detach()")
             if x.dtype != torch.bfloat16:
                 raise ValueError(f"the gradient of x needs a bfloat16 x, got {x.dtype}")
-            y = _FrozenLinear.apply(x, self)
-        else:
-            y = self._base(x)
         if adapters is None:
-            return y
+            return _FrozenLinear.apply(x, self) if through else self._base(x)
         if ids is None or ids.shape != x.shape[:-1]:
             raise ValueError(f"ids must hold the adapter of every row of x, {tuple(x.shape[:-1])}")
-        trained = torch.is_grad_enabled() and (y.requires_grad or adapters.a.requires_grad or adapters.b.requires_grad)
-        y2 = y.reshape(-1, self.out_features)
-        z = adapters(y2, x.reshape(-1, self.in_features), ids.reshape(-1), out=None if trained else y2)
-        return z.reshape(y.shape)
+        x2, ids = x.reshape(-1, self.in_features), ids.reshape(-1)
+        if through and x2.shape[0]:
+            y = AdaptedLinear.apply(x2, adapters.a, adapters.b, ids, adapters.scale, self)
+        else:
+            y = self._base(x2)
+            trained = torch.is_grad_enabled() and (adapters.a.requires_grad or adapters.b.requires_grad)
+            y = adapters(y, x2, ids, out=None if trained else y)
+        return y.reshape(*x.shape[:-1], self.out_features)
 
     def _base(self, x: torch.Tensor) -> torch.Tensor:
         # a call whose tensors need no preparation; anything else comes back unhandled
