@@ -89,6 +89,7 @@ def router_args(**kw):
     (dict(k=9), _lib.WB200_ERR_INVALID_ARG, "top_k = 9"), (dict(E=64, ld=64, k=33), _lib.WB200_ERR_INVALID_ARG, "top_k = 33"),
     (dict(dtype=9), _lib.WB200_ERR_INVALID_ARG, "dtype"), (dict(ld=7), _lib.WB200_ERR_INVALID_ARG, "pitch"), (dict(logits=P + 2), _lib.WB200_ERR_ALIGNMENT, "aligned"),
     (dict(weight=None), _lib.WB200_ERR_INVALID_ARG, "null"), (dict(loss=None), _lib.WB200_ERR_INVALID_ARG, "null"), (dict(nbytes=67), _lib.WB200_ERR_WORKSPACE, "68 bytes"),
+    (dict(rows=(1 << 30) + 1, k=1), _lib.WB200_ERR_UNSUPPORTED, "in one call"), (dict(rows=1 << 30, k=2), _lib.WB200_ERR_UNSUPPORTED, "in one call"),
 ])
 def test_router(lib, kw, code, words):
     refused(lib, lib.wb200_router(*router_args(**kw)), code, words)

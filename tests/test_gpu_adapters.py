@@ -204,6 +204,18 @@ def test_gradient_of_strided_and_expanded_tensors():
     assert torch.allclose(got.float(), rows.float().sum(0, keepdim=True), rtol=2 ** -7, atol=1e-4)
 
 
+@pytest.mark.parametrize("rows,rank", [(2, 5), (40, 8), (150, 5), (150, 40)])
+def test_an_infinity_meets_the_ranks_there_are(rows, rank):
+    """Ranks are padded to sixteen: what an infinity of x would be in a rank that is not there (a NaN) does not reach the output."""
+    y, x, a, b, ids, s = make(rows, 64, 48, rank, 3)
+    ids[1] = 2
+    x[1, 9] = float("inf")
+    a[2] = a[2].abs() + 1
+    b[2] = b[2].abs() + 1
+    got = wb.apply_adapters(y, x, a, b, ids, s)
+    assert (got[1] == float("inf")).all() and got[0].isfinite().all()
+
+
 @pytest.mark.parametrize("rows", [3, 150])
 def test_captured_and_replayed(rows):
     """Forward and backward in one graph, replayed on new inputs; two graphs of the same call do not disturb one another."""
@@ -314,6 +326,16 @@ def test_layer_with_adapters(shape):
         layer(x.float(), pool, ids)
     with pytest.raises(ValueError):  # the layer's part of the gradient would be missing
         layer(x.clone().requires_grad_(), pool, ids)
+
+
+@pytest.mark.parametrize("trainable", [False, True])
+def test_layer_with_adapters_and_an_empty_batch(trainable):
+    g = torch.Generator().manual_seed(3)
+    layer = wb.MXFP4Linear.from_float(torch.randn(192, 256, generator=g).to(DEV), input_grad=True)
+    pool = wb.LowRankAdapters(torch.zeros(4, 8, 256, dtype=BF16, device=DEV), torch.zeros(4, 192, 8, dtype=BF16, device=DEV), trainable=trainable)
+    x = torch.zeros(0, 256, dtype=BF16, device=DEV, requires_grad=True)
+    out = layer(x, pool, torch.zeros(0, dtype=torch.int32, device=DEV))
+    assert out.shape == (0, 192) and torch.autograd.grad(out.sum(), x)[0].shape == (0, 256)
 
 
 def test_layer_trains_adapters_through_frozen_layers():

@@ -271,6 +271,24 @@ def test_combine_rows_values_that_are_not_finite():
     assert dw[:2].tolist() == [[16.0, 16.0], [16.0, 0.0]] and dw[2, 0].isnan() and float(dw[2, 1]) == 16.0
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_combine_rows_of_one_row_one_column_and_none(dtype):
+    """Strides that no address depends on may be anything; without rows of y every pair is dropped."""
+    one = torch.arange(1, 17, device=DEV).to(dtype)
+    row_of = torch.tensor([[0, -1], [0, 0]], dtype=torch.int32, device=DEV)
+    weight = torch.tensor([[2.0, 9.0], [1.0, 3.0]], device=DEV, requires_grad=True)
+    for y in (one.as_strided((1, 16), (0, 1)), one.as_strided((1, 16), (5, 1))):
+        out = wb.combine_rows(y, row_of, weight)
+        assert torch.equal(out[0], 2 * one) and torch.equal(out[1], 4 * one)
+        assert torch.autograd.grad(out.float().sum(), weight)[0].tolist() == [[136.0, 0.0], [136.0, 136.0]]
+    column = one.as_strided((4, 1), (2, 7))  # 1, 3, 5, 7
+    out = wb.combine_rows(column, torch.tensor([[3, 1], [0, -1]], dtype=torch.int32, device=DEV), weight)
+    assert out.flatten().tolist() == [41.0, 1.0]
+    assert torch.autograd.grad(out.float().sum(), weight)[0].tolist() == [[7.0, 3.0], [1.0, 0.0]]
+    out = wb.combine_rows(one.reshape(1, 16)[:0], torch.full((2, 2), -1, dtype=torch.int32, device=DEV), weight)
+    assert out.shape == (2, 16) and not out.any() and not torch.autograd.grad(out.float().sum(), weight)[0].any()
+
+
 def test_combine_rows_refusals():
     y, row_of, weight = torch.zeros(6, 16, device=DEV), torch.zeros(3, 2, dtype=torch.int32, device=DEV), torch.zeros(3, 2, device=DEV)
     for args in ((y.half(), row_of, weight), (y, row_of.long(), weight), (y, row_of, weight.double()), (y, row_of[:2], weight), (y[0], row_of, weight),

@@ -86,8 +86,8 @@ int splits_for(long long units, int most) {
   return s;
 }
 // CTAs that share the groups of a chunk. Four at least where there are adapters enough: a chunk in which one sequence ends and another begins has two
-// groups, and as one CTA's work it took twice as long as the others (8192 rows of 6 sequences: 255 against 165 us); a CTA without a group
-// leaves at once.
+// groups, and as one CTA's work it took twice as long as the others (8192 rows of 6 sequences, K = N = 8192, rank 64: 255 us for both products with
+// one lane, 192 with four); a CTA without a group leaves at once.
 int group_lanes(int rows, int L, long long others) {
   return few_rows(rows, L) ? std::min({rows, L, wb::kFewRows}) : int(std::max<long long>(std::min(4, L), std::min<long long>(std::min(wb::kChunkRows, L), kTargetCtas / others)));
 }
@@ -325,6 +325,7 @@ int router_ctas(int rows) { return rows <= wb::kRouterOneCta ? 1 : std::min(wb::
 int check_router(const char* what, int rows, int E, int top_k, int dtype, const void* logits, long long ld) {
   if (rows <= 0 || E <= 0 || top_k <= 0) return fail(WB200_ERR_INVALID_ARG, "%s: rows = %d, experts = %d, top_k = %d", what, rows, E, top_k);
   if (E > wb::kRouterMaxExperts) return fail(WB200_ERR_UNSUPPORTED, "%s: at most %d experts (got %d)", what, wb::kRouterMaxExperts, E);
+  if (rows > 1 << 30 || (long long)rows * top_k > 0x7fffffffll) return fail(WB200_ERR_UNSUPPORTED, "%s: %d rows of %d choices in one call", what, rows, top_k);
   if (dtype != WB200_F32 && dtype != WB200_BF16) return fail(WB200_ERR_INVALID_ARG, "%s: unknown dtype %d", what, dtype);
   if (!logits) return fail(WB200_ERR_INVALID_ARG, "%s: null pointer", what);
   if (ld < E && rows > 1) return fail(WB200_ERR_INVALID_ARG, "%s: row pitch %lld is smaller than %d experts", what, ld, E);

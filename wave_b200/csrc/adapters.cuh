@@ -6,18 +6,24 @@
 // Three kernels: `shrink` (rows times a wide matrix onto the ranks: A_l x, B_l^T g), `expand` (ranks onto wide rows: B_l h, A_l^T u) and
 // `outer` (sums over the rows of an adapter). Each product is far below the tensor cores' rate at the ranks adapters have (2 R flops per
 // two bytes of x), so they are bound by HBM for many rows and by latency for few, and what counts is that every row of x, y and g moves
-// once, in whole 32-byte sectors.
+// once, in whole 32-byte sectors, with enough of them in flight. mma.sync does for these products: at rank 64, 8192 rows and 8192 columns its share
+// is 2 x 15 us (576 TFLOP/s, two bf16 parts in `expand`) of 63 us of memory traffic.
 //
-// mma.sync m16n8k16 straight from global memory: an MMA adds over its 16 k in any order, so a lane may hold any 8 consecutive k of a row
-// (one 16-byte load, two MMAs) as long as the other operand is permuted alike, and the columns of an output tile may be dealt to the lanes
-// so that each has 8 neighbours. Operands whose contraction runs down the rows of memory (B_l^T, A_l^T, the outer products) are
-// transposed by byte permutes of two registers.
+// shrink and expand come in two forms each. Up to 64 rows with few rows to an adapter (`few`): operands from global memory straight to registers, every warp
+// finds the rows of its adapter itself by a vote, no barrier before the first load. Otherwise (`tile`): rows are taken in chunks of 64 neighbours,
+// every CTA sorts the chunk's rows by adapter itself (64 compares a thread; a chunk of one sequence is noticed and not sorted), so that no
+// launch precedes it and ids need no order.
 //
-// Rows are taken in chunks of 64 neighbours, and every CTA sorts the chunk's rows by adapter itself (64 compares a thread), so that no
-// launch precedes it and ids need no order. A chunk of one sequence has one group of 64 rows; a decode step has groups of one row.
+// Layouts for mma.sync m16n8k16: an MMA adds over its 16 k in any order, so a lane may hold any 8 consecutive k of a row (one 16-byte load, two
+// MMAs) as long as the other operand is permuted alike, and the columns of an output tile may be dealt to the lanes so that each has 8
+// neighbours. Operands whose contraction runs down the rows of memory (B_l^T, A_l^T, the outer products) are transposed by byte permutes of
+// two registers, or by ldmatrix where they come through shared memory.
 //
-// The hidden vector h = A_l x (R numbers a row) is f32 in memory. It enters the second product as a sum of bf16 parts: two (relative
-// error 2^-17) where the result is rounded to bf16, three (2^-25) where it stays f32.
+// The hidden vector h = s_l A_l x (R numbers a row) stays in f32 until it is stored, as a sum of bf16 parts, which is how the second product takes
+// it: two parts (relative error 2^-17) where the result is rounded to bf16, three (2^-25) where it stays f32.
+//
+// Dependent launches: shrink and outer touch memory only once the kernel before them is complete. expand is always launched behind a shrink, which lets it
+// begin after that point: what it reads before its own wait (y, w, ids) is older than the shrink, and it writes nothing before it.
 #pragma once
 #include <cuda_bf16.h>
 
@@ -245,7 +251,7 @@ __device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums
       for (int s = 0; s < 8; ++s) v += part[s];
     }
     __nv_bfloat16 part[3];
-    split_bf16<3>(v * scale, part);
+    split_bf16<3>(n0 + col < p.R ? v * scale : 0.f, part);  // (an infinity of x would be a NaN in the ranks behind the last)
     __nv_bfloat16* dst = p.hidden + (long long)row_of(row) * p.parts * p.Rp + n0 + col;
 #pragma unroll
     for (int i = 0; i < 3; ++i)
@@ -260,7 +266,8 @@ __device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums
 
 // hidden[t][r] = scale_l sum_k x[t, k] w_l[r, k]. Grid (splits of K = one cluster, chunks, group lanes).
 //
-// Few rows: operands straight from global memory to registers. The 8 warps of a CTA take blocks of 64 k in turn.
+// Few rows: operands straight from global memory to registers. The 8 warps of a CTA take blocks of 64 k in turn. Bound by latency: launch, ids, one
+// round of loads, the sum over the warps, the sum over the cluster; one row, K = N = 4096, rank 16: 5.0 us with the expansion behind it.
 template <int RT, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads)
 adapter_shrink_few_kernel(const ShrinkParams p) {
@@ -268,6 +275,7 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
   __shared__ float red[kAdapterWarps][16][COLS + 2];
   __shared__ float sums[16][COLS];  // 16 / splits rows of this CTA from every split (a power of two)
   bool again = false;
+  if (gridDim.x > 1) cluster_arrive();  // this CTA has begun: waited for before the first store into another one's shared memory
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -345,8 +353,8 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
         // every split sends its sums of a row to the CTA that finishes it, which adds them up in their order
         const int count = min(16, end - first), splits = gridDim.x, split = blockIdx.x, share = 16 / splits;
         __syncthreads();
-        if (again && splits > 1) {  // what came before has been read
-          cluster_arrive();
+        if (splits > 1) {  // every CTA has begun, and what came before has been read
+          if (again) cluster_arrive();
           cluster_wait();
         }
         again = true;
@@ -372,7 +380,7 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
           float v = 0.f;
           for (int i = 0; i < splits; ++i) v += sums[i * share + mine][col];
           __nv_bfloat16 part[3];
-          split_bf16<3>(v * scale, part);
+          split_bf16<3>(n0 + col < p.R ? v * scale : 0.f, part);
           __nv_bfloat16* dst = p.hidden + (long long)(row0 + nth_bit(group.rows, first + row)) * p.parts * p.Rp + n0 + col;
 #pragma unroll
           for (int i = 0; i < 3; ++i)
@@ -381,10 +389,13 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
       }
     }
   }
+  if (gridDim.x > 1 && !again) cluster_wait();
 }
 
 // Many rows: a ring of stages of 64 k in shared memory, rows of x gathered by their place in the group. Warp (m, q) takes rows 32 m .. and the
-// q-th 16 of the 64 k. HBM-bound on x while a chunk's ranks are few; at rank 64 the MMAs (mma.sync) take about as long.
+// q-th 16 of the 64 k: x passes through ldmatrix once, w twice, and the four sums over k meet at the end. Two stages between barriers, so that the warps
+// wait for one another half as often. Bound by HBM on x at rank 16 and by shared memory and issue slots at rank 64, where each 64 rows x 64 k take as
+// many ldmatrix of w as of x: 8192 x 8192 at rank 64 SHRINK64 us (134 MB, SHRINK64BW TB/s), 4096 x 4096 at rank 16 SHRINK16 us.
 template <int RT>
 struct ShrinkTile {
   static constexpr int X_BYTES = kChunkRows * 128, W_BYTES = RT * 1024, STAGE_BYTES = X_BYTES + W_BYTES;
@@ -619,7 +630,8 @@ __device__ __forceinline__ void expand_rest(const ExpandParams& p, long long row
 // out[t, c] = y[t, c] + sum_r hidden[t, r] w_l[c, r]. Grid (column slices, chunks, group lanes).
 //
 // Few rows: a thread has two columns, with 16 of their ranks in registers at a time, and walks the rows of a group. f32 FMAs: the
-// products are few, the loads of w_l (whole sectors, all of a thread's in flight) are what counts.
+// products are few, the loads of w_l (whole sectors, all of a thread's in flight) are what counts. For ranks and alignments that the next kernel does not
+// take, and for the transposed product of the backward pass.
 template <typename T, int P, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads)
 adapter_expand_few_kernel(const ExpandParams p) {
@@ -754,6 +766,8 @@ adapter_expand_few_kernel(const ExpandParams p) {
 
 // The same for ranks of 8 PIECES whose rows of B start on 16 bytes: PIECES lanes share a column, each with 8 of its ranks, so that a warp's load is 512
 // consecutive bytes, STEPS of them in flight; the lanes' sums meet by shuffles, and the u-th lane of a column keeps every so-manieth column.
+// Both products of 32 rows and some 25 of 64 adapters, K = 4096, N = 14336, rank 16: 12.2 us (17 MB; with two columns a thread 13.7), of one row
+// with N = 4096 5.0 us (6.0).
 __host__ __device__ constexpr int few_whole_steps(int pieces) { return pieces > 4 ? pieces : 4; }
 template <typename T, int P, int PIECES>
 __global__ void __launch_bounds__(kAdapterThreads, 3)
@@ -834,10 +848,13 @@ __host__ __device__ constexpr int expand_pitch(int parts, int Rp, bool paired) {
 }
 
 // Many rows: a warp takes 32 columns of all the rows of a group; a lane has 8 neighbouring columns of two rows of an MMA tile.
-// FAST: rows that start on 16 bytes, columns in eights, ranks in fours (eights where two steps are loaded as one piece). The values of y are loaded ahead of everything else, a batch of rows
-// (MB tiles of 16) at once, the next batch while this one is worked on, w of the next columns with it; they are the accumulators' first values.
-// Otherwise the accumulators go through shared memory, so that 32 lanes share a row's 32 columns.
-// QN: steps of 16 ranks of w in registers at a time.
+// FAST: rows that start on 16 bytes, columns in eights, ranks in fours (eights where two steps are loaded as one piece). The values of y are loaded
+// ahead of everything else, a batch of rows (MB tiles of 16) at once, the next batch while this one is worked on, w of the next columns with it;
+// they are the accumulators' first values. Otherwise the accumulators go through shared memory, so that 32 lanes share a row's 32 columns, and y a
+// row of 32 columns at a time, a tile of 16 rows ahead.
+// QN: steps of 16 ranks of w in registers at a time. EXACT: the rank is known when compiled.
+// Bound by HBM (y in, out) at rank 16, 4096 x 4096 EXPAND16 us; at rank 64 by the latency of its loads at two CTAs an SM (128 registers a thread hold
+// the accumulators, w and the batch ahead; four tiles of 16 rows at once spilled): 8192 x 8192 EXPAND64 us (268 MB, EXPAND64BW TB/s).
 template <typename T, int P, int QN, bool TRANS, bool FAST, bool EXACT>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_expand_tile_kernel(const ExpandParams p) {

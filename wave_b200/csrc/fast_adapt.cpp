@@ -303,7 +303,7 @@ PyObject* combine_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!here(args[0], &y) || !here(args[1], &row_of) || !here(args[2], &weight)) Py_RETURN_NONE;
     if (dtype_code(y) < 0 || !row_major(y) || row_of.scalar_type() != at::kInt || weight.scalar_type() != at::kFloat || row_of.dim() != 2 ||
         weight.sizes() != row_of.sizes() || !row_of.is_contiguous() || !weight.is_contiguous() || !fits(row_of.size(0)) || !fits(row_of.size(1)) ||
-        !fits(y.size(1)) || (at::GradMode::is_enabled() && y.requires_grad()))
+        !fits(y.size(1)) || y.size(0) == 0 || (at::GradMode::is_enabled() && y.requires_grad()))
       Py_RETURN_NONE;
     if (wanted({&weight})) return THPVariable_Wrap(CombineNode::apply(y, row_of, weight));
     return THPVariable_Wrap(run_combine(y, row_of, weight));

@@ -173,9 +173,13 @@ def combine_rows(y: torch.Tensor, row_of: torch.Tensor, weight: torch.Tensor) ->
         raise ValueError("y, row_of and weight must be on one device")
     if torch.is_grad_enabled() and y.requires_grad:
         raise ValueError("the gradient of y is not computed: pass y.detach()")
-    if y.shape[1] == 0 or y.stride(1) != 1 and y.shape[1] > 1 or y.shape[0] > 1 and y.stride(0) < y.shape[1]:
-        y = y.contiguous()
-    if row_of.shape[0] == 0 or y.shape[1] == 0:
+    rows, N = y.shape
+    if row_of.shape[0] and N and rows:
+        if y.stride(1) != 1 and N > 1 or rows > 1 and y.stride(0) < N:
+            y = y.contiguous()
+        if y.stride(1) != 1 or y.stride(0) < N:  # of a single row or column: any
+            y = y.as_strided((rows, N), (y.stride(0) if rows > 1 else N, 1))
+    else:  # (without rows of y every pair is dropped)
         return torch.zeros(row_of.shape[0], y.shape[1], dtype=y.dtype, device=y.device) + 0 * weight.sum().to(y.dtype)
     return _CombineRows.apply(y, row_of.contiguous(), weight.contiguous())
 
@@ -414,6 +418,8 @@ class MXFP4ExpertMLP:
         if torch.is_grad_enabled() and x.requires_grad:
             raise ValueError("frozen experts give no gradient for x: pass x.detach()")
         ids, weight = routing.ids, routing.weight
+        if ids.device != x.device or weight.device != x.device:
+            raise ValueError(f"routing is on {ids.device} and {weight.device}, x on {x.device}")
         if not x.is_cuda or x.dim() != 2 or x.shape[1] != self.K or x.dtype not in ops._DTYPE_CODE:
             raise ValueError(f"x must be an f32 or bf16 CUDA tensor [tokens, {self.K}], got {x.dtype} {tuple(x.shape)}")
         if tuple(ids.shape) != (x.shape[0], self.top_k) or tuple(weight.shape) != tuple(ids.shape) or weight.dtype != torch.float32:

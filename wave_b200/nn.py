@@ -132,6 +132,8 @@ class MXFP4Linear(torch.nn.Module):
         x2, ids = x.reshape(-1, self.in_features), ids.reshape(-1)
         if through and x2.shape[0]:
             y = AdaptedLinear.apply(x2, adapters.a, adapters.b, ids, adapters.scale, self)
+        elif through:
+            y = adapters(_FrozenLinear.apply(x2, self), x2, ids)
         else:
             y = self._base(x2)
             trained = torch.is_grad_enabled() and (adapters.a.requires_grad or adapters.b.requires_grad)
