@@ -329,13 +329,15 @@ def test_layer_with_adapters(shape):
 
 
 @pytest.mark.parametrize("trainable", [False, True])
-def test_layer_with_adapters_and_an_empty_batch(trainable):
+@pytest.mark.parametrize("through", [False, True])
+def test_layer_refuses_an_empty_batch_with_adapters_as_without(trainable, through):
     g = torch.Generator().manual_seed(3)
     layer = wb.MXFP4Linear.from_float(torch.randn(192, 256, generator=g).to(DEV), input_grad=True)
     pool = wb.LowRankAdapters(torch.zeros(4, 8, 256, dtype=BF16, device=DEV), torch.zeros(4, 192, 8, dtype=BF16, device=DEV), trainable=trainable)
-    x = torch.zeros(0, 256, dtype=BF16, device=DEV, requires_grad=True)
-    out = layer(x, pool, torch.zeros(0, dtype=torch.int32, device=DEV))
-    assert out.shape == (0, 192) and torch.autograd.grad(out.sum(), x)[0].shape == (0, 256)
+    x = torch.zeros(0, 256, dtype=BF16, device=DEV, requires_grad=through)
+    for args in ((x,), (x, pool, torch.zeros(0, dtype=torch.int32, device=DEV))):
+        with pytest.raises(ValueError):
+            layer(*args)
 
 
 def test_layer_trains_adapters_through_frozen_layers():

@@ -133,7 +133,7 @@ int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int 
 template <typename T, int P, int QN, bool TRANS, bool FAST, bool EXACT>
 int launch_expand_tile(const wb::ExpandParams& p, dim3 grid, cudaStream_t s) {
   constexpr auto kernel = wb::adapter_expand_tile_kernel<T, P, QN, TRANS, FAST, EXACT>;
-  const size_t smem = size_t(wb::kChunkRows) * wb::expand_pitch(P, p.Rp, FAST && EXACT && QN % 2 == 0) * 2;
+  const size_t smem = size_t(wb::kChunkRows) * wb::expand_pitch(P, p.Rp, FAST && EXACT && QN % 2 == 0) * 2 + (FAST ? wb::expand_ring_bytes(sizeof(T), EXACT) : 0);
   if (int rc = smem > 24 * 1024 ? allow_smem<kernel>() : WB200_OK) return rc;
   WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, smem, s, p));
   return WB200_OK;

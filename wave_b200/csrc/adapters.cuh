@@ -847,6 +847,10 @@ __host__ __device__ constexpr int expand_pitch(int parts, int Rp, bool paired) {
   return paired ? 2 * (words + (words % 32 == 16 ? 0 : 16)) : 2 * (words + (words % 16 == 8 ? 0 : 8));
 }
 
+// Batches of y that are on their way to shared memory at a time: 64 KB of a CTA, 32 KB next to the hidden vectors of ranks that may be large.
+__host__ __device__ constexpr int expand_depth(int esz, bool exact) { return (exact ? 8 : 4) / esz; }
+__host__ __device__ constexpr int expand_ring_bytes(int esz, bool exact) { return expand_depth(esz, exact) * 2 * esz * kAdapterThreads * 16; }
+
 // Many rows: a warp takes 32 columns of all the rows of a group; a lane has 8 neighbouring columns of two rows of an MMA tile.
 // FAST: rows that start on 16 bytes, columns in eights, ranks in fours (eights where two steps are loaded as one piece). The values of y are loaded
 // ahead of everything else, a batch of rows (MB tiles of 16) at once, the next batch while this one is worked on, w of the next columns with it;
@@ -863,11 +867,13 @@ adapter_expand_tile_kernel(const ExpandParams p) {
   constexpr int MB = 2;                          // tiles of 16 rows in a batch
   constexpr bool AHEAD = FAST && EXACT && QN <= 2;  // all ranks of w are in registers at a time
   constexpr int STEP = kAdapterWarps * kExpandCols;
+  constexpr int DEPTH = expand_depth(sizeof(T), EXACT), SLOT = MB * 2 * RAW * kAdapterThreads * 16;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ RowGroups groups;
   __shared__ uint32_t y_off[FAST ? 1 : kChunkRows], out_off[FAST ? 1 : kChunkRows];  // of a group's rows, in bytes; all ones: none
   __shared__ float staged[FAST ? 1 : kAdapterWarps][FAST ? 1 : 16][FAST ? 1 : kExpandCols + 1];
-  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem);  // [64][P][Rp], rows `pitch` apart
+  // FAST: a ring of batches of y, in which every thread has 16-byte slots of its own (no barrier): [DEPTH][MB][2][RAW][threads]
+  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem + (FAST ? DEPTH * SLOT : 0));  // [64][P][Rp], rows `pitch` apart
   // A lane's ranks in two steps of 16: eight neighbours (PAIRED: one 16-byte piece serves both steps), or four of each
   constexpr bool PAIRED = FAST && EXACT && QN % 2 == 0;
   const int pitch = expand_pitch(P, Rp, PAIRED);
@@ -901,22 +907,34 @@ adapter_expand_tile_kernel(const ExpandParams p) {
     for (int m = 0; m < 4; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) row[m][h] = row_at(m * 16 + h * 8 + g);
-    uint4 next[MB][2][RAW];
-    // 8 values of every row of the batch. A row or column that is not there reads the first one's: what comes of it is not stored.
-    auto load_y = [&](int c0, int batch) {
-      const uint32_t at = uint32_t(c0 + 8 * t < p.C ? c0 + 8 * t : 0) * uint32_t(sizeof(T));  // (C is a multiple of 8)
+    // The next batch of y into the ring: 8 values of every row of it, zeros for a row or column that is not there.
+    const uint32_t ring = smem_u32(smem) + threadIdx.x * 16u;
+    const int batches = (mtiles + MB - 1) / MB;
+    int ahead_c = c_begin + warp * kExpandCols + 8 * t, ahead_batch = 0;
+    uint32_t ahead_slot = 0;
+    auto load_y = [&]() {
+      if (ahead_c - 8 * t < c_end) {
+        const bool col_there = p.y && ahead_c < p.C;  // (C is a multiple of 8)
 #pragma unroll
-      for (int m = 0; m < MB; ++m)
+        for (int m = 0; m < MB; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          int r = row[m][h];
+          for (int h = 0; h < 2; ++h) {
+            int r = row[m][h];
 #pragma unroll
-          for (int b = 1; b < 4 / MB; ++b)
-            if (b == batch) r = row[b * MB + m][h];
+            for (int b = 1; b < 4 / MB; ++b)
+              if (b == ahead_batch) r = row[b * MB + m][h];
+            const bool there = col_there && r >= 0;
+            const char* from = there ? y + (uint32_t(r) * y_pitch + uint32_t(ahead_c) * uint32_t(sizeof(T))) : reinterpret_cast<const char*>(p.hidden);
 #pragma unroll
-          for (int i = 0; i < RAW; ++i) next[m][h][i] = p.y ? *reinterpret_cast<const uint4*>(y + (uint32_t(max(r, 0)) * y_pitch + at + 16u * i)) : make_uint4(0u, 0u, 0u, 0u);
-        }
+            for (int i = 0; i < RAW; ++i)
+              cp_async_bytes(ring + ahead_slot * SLOT + ((m * 2 + h) * RAW + i) * (kAdapterThreads * 16), from + (there ? 16 * i : 0), there ? 16u : 0u);
+          }
+        if (++ahead_batch == batches) { ahead_batch = 0; ahead_c += STEP; }
+        ahead_slot = ahead_slot + 1 == DEPTH ? 0 : ahead_slot + 1;
+      }
+      cp_async_commit();
     };
+    uint32_t slot = 0;
     uint32_t wf[4][QN][2];
     auto load_w = [&](int c0, int q0) {
       if constexpr (FAST) {
@@ -1016,9 +1034,11 @@ adapter_expand_tile_kernel(const ExpandParams p) {
         old[FAST ? 0 : r] = there && off != 0xffffffffu ? as_f32<T>(*reinterpret_cast<const T*>(y + (off + at))) : 0.f;
       }
     };
+    if constexpr (FAST)
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) load_y();
     if (c_first < c_end) {
-      if constexpr (FAST) load_y(c_first, 0);
-      else load_tile(c_first, 0);
+      if constexpr (!FAST) load_tile(c_first, 0);
       if (AHEAD || (!FAST && steps <= QN)) load_w(c_first, 0);
     }
     if (!waited) pdl_wait();  // for the hidden vectors; y and w are complete before the kernel that makes those starts
@@ -1049,20 +1069,26 @@ adapter_expand_tile_kernel(const ExpandParams p) {
       for (int batch = 0; batch < 4 / MB; ++batch) {
         if (batch * MB >= mtiles) break;
         float acc[MB][4][4];
+        if constexpr (FAST) cp_async_wait<DEPTH - 1>();
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float v[8] = {};
-            if constexpr (FAST) read8<T>(reinterpret_cast<const T*>(next[m][h]), true, 8, v);
+            if constexpr (FAST) {
+              uint4 raw[RAW];
+#pragma unroll
+              for (int i = 0; i < RAW; ++i) raw[i] = *reinterpret_cast<const uint4*>(smem + slot * SLOT + ((m * 2 + h) * RAW + i) * (kAdapterThreads * 16) + threadIdx.x * 16);
+              read8<T>(reinterpret_cast<const T*>(raw), true, 8, v);
+            }
 #pragma unroll
             for (int n = 0; n < 4; ++n)
 #pragma unroll
               for (int j = 0; j < 2; ++j) acc[m][n][2 * h + j] = v[TRANS ? 4 * j + n : 2 * n + j];
           }
         if constexpr (FAST) {
-          if ((batch + 1) * MB < mtiles) load_y(c0, batch + 1);
-          else if (c0 + STEP < c_end) load_y(c0 + STEP, 0);
+          load_y();
+          slot = slot + 1 == DEPTH ? 0 : slot + 1;
         }
 #pragma unroll
         for (int mm = 0; mm < MB; ++mm) {

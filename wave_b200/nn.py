@@ -130,10 +130,8 @@ class MXFP4Linear(torch.nn.Module):
         if ids is None or ids.shape != x.shape[:-1]:
             raise ValueError(f"ids must hold the adapter of every row of x, {tuple(x.shape[:-1])}")
         x2, ids = x.reshape(-1, self.in_features), ids.reshape(-1)
-        if through and x2.shape[0]:
+        if through:
             y = AdaptedLinear.apply(x2, adapters.a, adapters.b, ids, adapters.scale, self)
-        elif through:
-            y = adapters(_FrozenLinear.apply(x2, self), x2, ids)
         else:
             y = self._base(x2)
             trained = torch.is_grad_enabled() and (adapters.a.requires_grad or adapters.b.requires_grad)
