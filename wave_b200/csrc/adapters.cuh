@@ -275,7 +275,10 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
   __shared__ float red[kAdapterWarps][16][COLS + 2];
   __shared__ float sums[16][COLS];  // 16 / splits rows of this CTA from every split (a power of two)
   bool again = false;
-  if (gridDim.x > 1) cluster_arrive();  // this CTA has begun: waited for before the first store into another one's shared memory
+  if (gridDim.x > 1) {  // every CTA has begun before the first store into its shared memory; here, where the kernel before this one still runs
+    cluster_arrive();
+    cluster_wait();
+  }
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -353,8 +356,8 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
         // every split sends its sums of a row to the CTA that finishes it, which adds them up in their order
         const int count = min(16, end - first), splits = gridDim.x, split = blockIdx.x, share = 16 / splits;
         __syncthreads();
-        if (splits > 1) {  // every CTA has begun, and what came before has been read
-          if (again) cluster_arrive();
+        if (again && splits > 1) {  // what came before has been read
+          cluster_arrive();
           cluster_wait();
         }
         again = true;
@@ -389,7 +392,6 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
       }
     }
   }
-  if (gridDim.x > 1 && !again) cluster_wait();
 }
 
 // Many rows: a ring of stages of 64 k in shared memory, rows of x gathered by their place in the group. Warp (m, q) takes rows 32 m .. and the
@@ -907,14 +909,15 @@ adapter_expand_tile_kernel(const ExpandParams p) {
     for (int m = 0; m < 4; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) row[m][h] = row_at(m * 16 + h * 8 + g);
+    const bool has_y = !TRANS || p.y;  // (only a gradient may have nothing to be added to)
     // The next batch of y into the ring: 8 values of every row of it, zeros for a row or column that is not there.
     const uint32_t ring = smem_u32(smem) + threadIdx.x * 16u;
     const int batches = (mtiles + MB - 1) / MB;
     int ahead_c = c_begin + warp * kExpandCols + 8 * t, ahead_batch = 0;
     uint32_t ahead_slot = 0;
     auto load_y = [&]() {
-      if (ahead_c - 8 * t < c_end) {
-        const bool col_there = p.y && ahead_c < p.C;  // (C is a multiple of 8)
+      if (has_y && ahead_c - 8 * t < c_end) {
+        const bool col_there = ahead_c < p.C;  // (C is a multiple of 8)
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -1075,7 +1078,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float v[8] = {};
-            if constexpr (FAST) {
+            if (FAST && has_y) {
               uint4 raw[RAW];
 #pragma unroll
               for (int i = 0; i < RAW; ++i) raw[i] = *reinterpret_cast<const uint4*>(smem + slot * SLOT + ((m * 2 + h) * RAW + i) * (kAdapterThreads * 16) + threadIdx.x * 16);
