@@ -397,7 +397,8 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
 // Many rows: a ring of stages of 64 k in shared memory, rows of x gathered by their place in the group. Warp (m, q) takes rows 32 m .. and the
 // q-th 16 of the 64 k: x passes through ldmatrix once, w twice, and the four sums over k meet at the end. Two stages between barriers, so that the warps
 // wait for one another half as often. Bound by HBM on x at rank 16 and by shared memory and issue slots at rank 64, where each 64 rows x 64 k take as
-// many ldmatrix of w as of x: 8192 x 8192 at rank 64 SHRINK64 us (134 MB, SHRINK64BW TB/s), 4096 x 4096 at rank 16 SHRINK16 us.
+// many ldmatrix of w as of x: 8192 x 8192 at rank 64 50 us (134 MB of x, 2.7 TB/s; MMA pipe 39 %), 4096 x 4096 at rank 16
+// 11 us.
 template <int RT>
 struct ShrinkTile {
   static constexpr int X_BYTES = kChunkRows * 128, W_BYTES = RT * 1024, STAGE_BYTES = X_BYTES + W_BYTES;
@@ -859,8 +860,9 @@ __host__ __device__ constexpr int expand_ring_bytes(int esz, bool exact) { retur
 // they are the accumulators' first values. Otherwise the accumulators go through shared memory, so that 32 lanes share a row's 32 columns, and y a
 // row of 32 columns at a time, a tile of 16 rows ahead.
 // QN: steps of 16 ranks of w in registers at a time. EXACT: the rank is known when compiled.
-// Bound by HBM (y in, out) at rank 16, 4096 x 4096 EXPAND16 us; at rank 64 by the latency of its loads at two CTAs an SM (128 registers a thread hold
-// the accumulators, w and the batch ahead; four tiles of 16 rows at once spilled): 8192 x 8192 EXPAND64 us (268 MB, EXPAND64BW TB/s).
+// Bound by its start-up and HBM at rank 16 (4096 x 4096 14 us); at rank 64 by shared memory (59 %) and the MMA pipe (51 %) between them, at two CTAs of
+// 128 registers a thread: 8192 x 8192 63 us (268 MB of y and out, 4.3 TB/s). With the batch ahead in registers instead of the ring 76 us; w of the
+// next columns through the ring too: no faster.
 template <typename T, int P, int QN, bool TRANS, bool FAST, bool EXACT>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_expand_tile_kernel(const ExpandParams p) {
@@ -1209,7 +1211,8 @@ struct OuterParams {
 // out_l[c, r] = sum over the rows t of adapter l of z[t, c] hidden[t, r]: B's gradient from g and A x, A's from x and B^T g.
 // Grid (row splits = one cluster, blocks of 128 columns of both sides, adapters). A CTA picks the rows of its adapter out of its range of ids,
 // in order, and adds up their outer products with MMAs whose k runs over the rows, from a ring of 64 rows a stage. The splits are
-// added up through distributed shared memory, in their order.
+// added up through distributed shared memory, in their order. Both sums of a backward pass are one launch: 4096 rows, 4096 + 4096 columns, rank 16
+// 19 us (67 MB, 3.5 TB/s); bound by the start-up (ids, list, first loads) and the barriers of the ring.
 constexpr int kOuterCols = 128;
 constexpr int kOuterSegment = 4096;  // ids looked through at a time
 template <int RT>
