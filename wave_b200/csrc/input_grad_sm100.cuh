@@ -147,29 +147,40 @@ template <int CG, int S>
 __device__ __forceinline__ void sum_slices(const InputGradParams& p, uint32_t smem_base, int mt, int kt, int rank, int slice) {
   using Cfg = InputGradCfg<CG>;
   const int first = Cfg::BM * slice / S, rows = Cfg::BM * (slice + 1) / S - first;
-  for (int e = threadIdx.x; e < rows * (Cfg::TILE_K / 8); e += Cfg::THREADS) {
-    const int in = first + e / (Cfg::TILE_K / 8), c = e % (Cfg::TILE_K / 8) * 8;
-    const int row = (mt * CG + rank) * Cfg::BM + in, col = kt * Cfg::TILE_K + c;
-    if (row >= p.M || col >= p.K) continue;
-    float v[S][8];
+  constexpr int ITEMS = S == 2 ? 3 : S == 3 ? 2 : 1;  // pieces of a thread in flight: what registers there are hold
+  for (int e0 = threadIdx.x; e0 < rows * (Cfg::TILE_K / 8); e0 += ITEMS * Cfg::THREADS) {
+    float v[ITEMS][S][8];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const uint32_t at = mapa_shared(smem_base + uint32_t(in) * Cfg::SUM_PITCH + c * 4, uint32_t(s * CG + rank));
+    for (int i = 0; i < ITEMS; ++i) {
+      const int e = e0 + i * Cfg::THREADS;
+      if (ITEMS > 1 && e >= rows * (Cfg::TILE_K / 8)) break;
+      const int in = first + e / (Cfg::TILE_K / 8), c = e % (Cfg::TILE_K / 8) * 8;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v[s][4 * h]), "=f"(v[s][4 * h + 1]), "=f"(v[s][4 * h + 2]), "=f"(v[s][4 * h + 3])
-                     : "r"(at + 16 * h));
+      for (int s = 0; s < S; ++s) {
+        const uint32_t at = mapa_shared(smem_base + uint32_t(in) * Cfg::SUM_PITCH + c * 4, uint32_t(s * CG + rank));
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[i][s][4 * h]), "=f"(v[i][s][4 * h + 1]), "=f"(v[i][s][4 * h + 2]), "=f"(v[i][s][4 * h + 3])
+                       : "r"(at + 16 * h));
+      }
     }
-    float sum[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      sum[j] = v[0][j];
+    for (int i = 0; i < ITEMS; ++i) {
+      const int e = e0 + i * Cfg::THREADS;
+      if (ITEMS > 1 && e >= rows * (Cfg::TILE_K / 8)) break;
+      const int row = (mt * CG + rank) * Cfg::BM + first + e / (Cfg::TILE_K / 8), col = kt * Cfg::TILE_K + e % (Cfg::TILE_K / 8) * 8;
+      if (row >= p.M || col >= p.K) continue;
+      float sum[8];
 #pragma unroll
-      for (int s = 1; s < S; ++s) sum[j] += v[s][j];
+      for (int j = 0; j < 8; ++j) {
+        sum[j] = v[i][0][j];
+#pragma unroll
+        for (int s = 1; s < S; ++s) sum[j] += v[i][s][j];
+      }
+      *reinterpret_cast<uint4*>(p.dx + (long long)row * p.ldd + col) = make_uint4(pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]),
+                                                                                  pack_bf16x2(sum[4], sum[5]), pack_bf16x2(sum[6], sum[7]));
     }
-    *reinterpret_cast<uint4*>(p.dx + (long long)row * p.ldd + col) = make_uint4(pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]),
-                                                                                pack_bf16x2(sum[4], sum[5]), pack_bf16x2(sum[6], sum[7]));
   }
 }
 
@@ -319,6 +330,7 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
   } else if (warp < 6) {
     const int quad = warp & 3;
     int it = 0;
+    if (p.slices == 1)
     for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++it) {
       int mt, kt;
       tile_at(tile, mt, kt);
@@ -332,14 +344,6 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
         uint32_t r[32];
         tmem_ld_32x32(tmem_base + (uint32_t(quad * 32) << 16) + as * Cfg::TILE_K + c, r);
         tmem_ld_wait();
-        if (p.slices > 1) {  // into this CTA's shared memory, whose stages are all read
-          const uint32_t at = smem_base + uint32_t(quad * 32 + lane) * Cfg::SUM_PITCH + c * 4;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + 16 * j), "r"(r[4 * j]), "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3])
-                         : "memory");
-          continue;
-        }
         const int col = kt * Cfg::TILE_K + c;
         if (row < p.M && col < p.K) {  // K is a multiple of 32
           uint4* q = reinterpret_cast<uint4*>(dst + col);
@@ -461,6 +465,25 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
   }
 
   if (p.slices > 1) {
+    // the one accumulator into this CTA's shared memory, whose stages are all read once it is complete: 32 columns at a time, the expanding
+    // warps help
+    if (warp >= 2 && warp < 6 + Cfg::EXPAND_WARPS) {
+      mbar_wait(acc_full(0), 0u, ctx, WB_DEV_TIMEOUT_EPILOGUE);
+      tc_fence_after_sync();
+      const int quad = warp & 3;
+#pragma unroll 1
+      for (int c = (warp - 2) / 4 * 32; c < Cfg::TILE_K; c += (4 + Cfg::EXPAND_WARPS) / 4 * 32) {
+        uint32_t r[32];
+        tmem_ld_32x32(tmem_base + (uint32_t(quad * 32) << 16) + c, r);
+        tmem_ld_wait();
+        const uint32_t at = smem_base + uint32_t(quad * 32 + lane) * Cfg::SUM_PITCH + c * 4;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + 16 * j), "r"(r[4 * j]), "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3])
+                       : "memory");
+      }
+      tc_fence_before_sync();
+    }
     __syncthreads();
     cluster_arrive();
     cluster_wait();
