@@ -204,6 +204,54 @@ def test_gradient_of_strided_and_expanded_tensors():
     assert torch.allclose(got.float(), rows.float().sum(0, keepdim=True), rtol=2 ** -7, atol=1e-4)
 
 
+# ---- the kernels on the tensor cores: many rows, ranks above 32 ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,K,N,rank,pool,ids", [
+    (2048, 512, 136, 8, 3, "runs"), (2500, 1024, 72, 16, 70, "mixed"), (2049, 64, 264, 24, 4, "mixed"), (300, 4096, 200, 64, 2, "runs"), (257, 192, 96, 100, 5, "mixed"),
+    (70, 2048, 64, 256, 1, "last"), (4100, 1088, 64, 36, 2, "none"), (129, 64, 8, 40, 130, "mixed")])
+@pytest.mark.parametrize("y_dtype", [BF16, F32])
+def test_many_rows_onto_the_ranks(rows, K, N, rank, pool, ids, y_dtype):
+    check_forward(make(rows, K, N, rank, pool, y_dtype, ids, seed=rows))
+
+
+@pytest.mark.parametrize("rows,K,N,rank,pool,ids", [
+    (8192, 64, 4096, 64, 1, "last"), (8200, 128, 4104, 64, 7, "runs"), (65540, 64, 520, 40, 3, "mixed"), (4097, 64, 8264, 48, 130, "mixed"), (9000, 64, 3800, 56, 2, "none"),
+    (131100, 64, 264, 64, 4, "runs")])
+def test_many_rows_onto_the_columns(rows, K, N, rank, pool, ids):
+    args = make(rows, K, N, rank, pool, ids=ids, seed=rows)
+    got = check_forward(args)
+    y = args[0].clone()  # in place, and beside other columns
+    assert torch.equal(wb.apply_adapters(y, *args[1:], out=y), got)
+    wide = torch.full((rows, N + 16), 7.0, dtype=BF16, device=DEV)
+    wb.apply_adapters(*args, out=wide[:, 8:N + 8])
+    assert torch.equal(wide[:, 8:N + 8], got) and bool((wide[:, :8] == 7).all()) and bool((wide[:, N + 8:] == 7).all())
+
+
+@pytest.mark.parametrize("rows,K,N,rank,pool,ids", [(8200, 4160, 64, 64, 3, "runs"), (8500, 4000, 128, 48, 5, "mixed"), (2100, 256, 192, 16, 2, "runs"), (300, 64, 1024, 40, 3, "mixed")])
+def test_gradients_of_many_rows(rows, K, N, rank, pool, ids):
+    y, x, a, b, at, s = make(rows, K, N, rank, pool, ids=ids, seed=rows)
+    g = torch.randn(rows, N, generator=torch.Generator().manual_seed(1)).to(BF16).to(DEV)
+    x, a, b = (t.requires_grad_() for t in (x, a, b))
+    grads = torch.autograd.grad(wb.apply_adapters(y, x, a, b, at, s), (x, a, b), g)
+    _, (dx, sx), (da, sa), (db, sb) = definition(y, x, a, b, at, s, g)
+    for got, want, size, terms in zip(grads, (dx, da, db), (sx, sa, sb), (N + rank, rows + N, rows + K)):
+        assert_near(got, want, size, terms, 2)
+
+
+def test_an_adapter_that_is_not_finite_stays_with_its_rows():
+    y, x, a, b, ids, s = make(8200, 64, 4096, 64, 5, ids="runs")
+    want = wb.apply_adapters(y, x, a, b, ids, s)
+    a, b = a.clone(), b.clone()
+    a[1], b[3] = float("inf"), float("nan")
+    x2 = x.clone()
+    x2[5] = float("nan")
+    got = wb.apply_adapters(y, x2, a, b, ids, s)
+    clean = (ids != 1) & (ids != 3)
+    clean[5] = False
+    assert torch.equal(got[clean], want[clean]) and got[ids == 3].isnan().all() and got[5].isnan().all()
+
+
 @pytest.mark.parametrize("rows,rank", [(2, 5), (40, 8), (150, 5), (150, 40)])
 def test_an_infinity_meets_the_ranks_there_are(rows, rank):
     """Ranks are padded to sixteen: what an infinity of x would be in a rank that is not there (a NaN) does not reach the output."""

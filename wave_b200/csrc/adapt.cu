@@ -96,6 +96,8 @@ struct AdapterCall {
   wb::Ids ids;
   int rows, R, Rp, L, parts;
   cudaStream_t stream;
+  int* status;
+  int sms;
 };
 
 template <int RT, bool TRANS>
@@ -114,17 +116,47 @@ int launch_shrink_ranks(const wb::ShrinkParams& p, bool few, dim3 grid, cudaStre
   return p.Rp <= 16 ? launch_shrink<2, TRANS>(p, few, grid, s) : p.Rp <= 32 ? launch_shrink<4, TRANS>(p, few, grid, s) : launch_shrink<8, TRANS>(p, few, grid, s);
 }
 
+template <int N, bool TRANS>
+int launch_shrink_wide(const AdapterCall& c, wb::ShrinkParams p, int chunks) {
+  using Cfg = wb::ShrinkWide<N, TRANS>;
+  const int splits = splits_for(chunks, std::max(1, p.K / 256));
+  p.split_k = div_up(div_up(p.K, splits), 64) * 64;
+  CUtensorMap x, w;
+  if (int rc = wbhost::tensor_map(&x, p.x, p.K, p.rows, (unsigned long long)p.ldx * 2, 64, Cfg::ROWS, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return rc;
+  const unsigned long long inner = TRANS ? p.R : p.K, outer = (unsigned long long)p.L * (TRANS ? p.K : p.R);
+  if (int rc = wbhost::tensor_map(&w, p.w, inner, outer, inner * 2, 64, TRANS ? 64 : N, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  constexpr auto kernel = wb::adapter_shrink_wide_kernel<N, TRANS>;
+  if (int rc = allow_smem<kernel>()) return rc;
+  const int lanes = int(std::max<long long>(1, std::min<long long>(div_up(std::min(Cfg::ROWS, c.L), 2), kTargetCtas / ((long long)chunks * splits))));
+  WB_HOST_CUDA(launch_clusters(kernel, dim3(splits, chunks, lanes), wb::kAdapterThreads, Cfg::SMEM_BYTES, c.stream, x, w, p, c.status));
+  return WB200_OK;
+}
+// The tensor cores take 2048 rows or more, and any number of more than 32 ranks. us of both products, ring of copies / tensor cores, K = N = 4096, three sequences:
+// rank 16, 1024 rows 15.7 / 18.3, 2048 rows 25.8 / 22.0, 8192 rows 44.5 / 44.3; rank 64, 256 rows 18.3 / 16.6, 2048 rows 36.4 / 27.9; 4096 rows of mixed
+// adapters at rank 16 102 / 77. Rows of few ranks are short pieces for the copy engine (trans): 4096 rows of rank 16 with gradients 68 / 71 with both.
+bool wide_shrink(const AdapterCall& c, const wb::ShrinkParams& p, bool trans) {
+  return p.x_vec && aligned_to(p.w, 16) && p.K % 64 == 0 && (!trans || p.R % 8 == 0) && (long long)p.L * std::max(p.K, p.R) < 0x7fffffff &&
+         (c.Rp > 32 || (c.rows >= 2048 && !trans));
+}
+
 // hidden [rows][parts][Rp] = rows of x onto the ranks, scaled. trans: w is [L][K][R].
 int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int K, const __nv_bfloat16* w, bool trans, const float* scale, __nv_bfloat16* hidden) {
   wb::ShrinkParams p;
   p.x = x; p.w = w; p.ids = c.ids; p.scale = scale; p.hidden = hidden; p.ldx = ldx;
   p.rows = c.rows; p.K = K; p.R = c.R; p.Rp = c.Rp; p.L = c.L; p.parts = c.parts;
   const bool few = few_rows(c.rows, c.L);
+  p.x_vec = aligned_to(x, 16) && ldx % 8 == 0 && ldx >= (K + 7) / 8 * 8;  // (a piece that K ends in is there, zeros behind)
+  if (!few && wide_shrink(c, p, trans)) {
+    const int wide = div_up(c.rows, 128);
+    return trans        ? launch_shrink_wide<64, true>(c, p, wide)
+           : c.Rp <= 16 ? launch_shrink_wide<16, false>(c, p, wide)
+           : c.Rp <= 32 ? launch_shrink_wide<32, false>(c, p, wide)
+                        : launch_shrink_wide<64, false>(c, p, wide);
+  }
   const int chunks = few ? div_up(c.rows, wb::kFewRows) : chunks_of(c.rows);
   const int splits = few ? splits_for(1, std::max(1, K / 512)) : splits_for(chunks, std::max(1, K / 256));
   p.split_k = div_up(div_up(K, splits), 64) * 64;
   const int vec = !trans ? 8 : !few ? 8 : c.Rp <= 16 ? 2 : c.Rp <= 32 ? 4 : 8;  // elements of a load of w
-  p.x_vec = aligned_to(x, 16) && ldx % 8 == 0 && ldx >= (K + 7) / 8 * 8;  // (a piece that K ends in is there, zeros behind)
   p.w_vec = aligned_to(w, 2 * vec) && (trans ? c.R : K) % vec == 0;
   const dim3 grid(splits, chunks, group_lanes(c.rows, c.L, (long long)chunks * splits));
   return trans ? launch_shrink_ranks<true>(p, few, grid, c.stream) : launch_shrink_ranks<false>(p, few, grid, c.stream);
@@ -167,6 +199,36 @@ int launch_expand(const wb::ExpandParams& p, bool few, dim3 grid, cudaStream_t s
   return steps == 1 ? launch_expand_tile<T, P, 1, TRANS, false, true>(p, grid, s) : launch_expand_tile<T, P, 2, TRANS, false, false>(p, grid, s);
 }
 
+template <bool TRANS>
+int launch_expand_wide(const AdapterCall& c, const wb::ExpandParams& e) {
+  using Cfg = wb::ExpandWide<TRANS>;
+  wb::ExpandWideParams p;
+  p.ids = e.ids; p.rows = e.rows; p.C = e.C; p.R = e.R; p.Rp = e.Rp; p.L = e.L;
+  p.chunks = div_up(e.rows, Cfg::ROWS); p.tiles = div_up(e.C, Cfg::COLS);
+  p.has_y = e.y != nullptr; p.in_place = e.out == e.y; p.status = c.status;
+  constexpr auto bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  constexpr auto swizzle = CU_TENSOR_MAP_SWIZZLE_128B;
+  constexpr auto promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
+  CUtensorMap h, w, y, out;
+  if (int rc = wbhost::tensor_map(&h, e.hidden, 2 * e.Rp, e.rows, 4ull * e.Rp, 64, Cfg::ROWS, bf16, swizzle)) return rc;
+  const unsigned long long inner = TRANS ? e.C : e.R, outer = (unsigned long long)e.L * (TRANS ? e.R : e.C);
+  if (int rc = wbhost::tensor_map(&w, e.w, inner, outer, inner * 2, 64, TRANS ? e.Rp : Cfg::COLS, bf16, swizzle)) return rc;
+  if (int rc = wbhost::tensor_map(&out, e.out, e.C, e.rows, (unsigned long long)e.ldo * 2, 64, Cfg::ROWS, bf16, swizzle)) return rc;
+  y = out;
+  if (e.y)
+    if (int rc = wbhost::tensor_map(&y, e.y, e.C, e.rows, (unsigned long long)e.ldy * 2, 64, Cfg::ROWS, bf16, swizzle, promotion)) return rc;
+  constexpr auto kernel = wb::adapter_expand_wide_kernel<TRANS>;
+  if (int rc = allow_smem<kernel>()) return rc;
+  const dim3 grid(unsigned(std::min<long long>(c.sms, (long long)p.chunks * p.tiles)));
+  WB_HOST_CUDA(launch(kernel, grid, Cfg::THREADS, Cfg::SMEM_BYTES, c.stream, h, w, y, out, p));
+  return WB200_OK;
+}
+// The tensor cores take more than 32 ranks where y and out are larger than L2. us of both products with the shrinking one on the tensor cores, rank 64:
+// 4096 x 4096 36.5 / 42.4, 8192 x 4096 61.7 / 56.5, 16384 x 8192 193 / 158; rank 32, 16384 x 8192 156 / 153, 8192 x 4096 49.3 / 53.3.
+bool wide_expand(const AdapterCall& c, const wb::ExpandParams& p, bool trans, bool f32) {
+  return !f32 && p.io_vec && aligned_to(p.w, 16) && p.C % 8 == 0 && p.Rp <= 64 && p.R % (trans ? 16 : 8) == 0 && (long long)p.L * std::max(p.C, p.R) < 0x7fffff00 && p.Rp > 32 && (long long)c.rows * p.C >= 1 << 25;
+}
+
 // out = y + ranks onto C columns.
 int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const __nv_bfloat16* hidden, const void* y, long long ldy, void* out, long long ldo, bool f32, int C) {
   wb::ExpandParams p;
@@ -180,6 +242,7 @@ int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const _
   const size_t esz = f32 ? 4 : 2;
   p.io_vec = aligned_to(out, 16) && ldo * esz % 16 == 0 && (!y || (aligned_to(y, 16) && ldy * esz % 16 == 0));
   p.io_pairs = !f32 && C % 2 == 0 && aligned_to(out, 4) && ldo % 2 == 0 && (!y || (aligned_to(y, 4) && ldy % 2 == 0));
+  if (!few && wide_expand(c, p, trans, f32)) return trans ? launch_expand_wide<true>(c, p) : launch_expand_wide<false>(c, p);
   const int vec = few ? (trans ? 2 : 8) : !trans && c.R % 8 == 0 ? 8 : 4;  // elements of a load of w
   p.w_vec = aligned_to(w, 2 * vec) && (trans ? C : c.R) % (trans && few ? 4 : vec) == 0;
   if (few && !trans)
@@ -398,8 +461,9 @@ int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, c
     return fail(WB200_ERR_ALIGNMENT, "adapters: a tensor is not aligned to its element size, or hidden not to 16 bytes");
   const size_t need = wb200_adapters_hidden_bytes(rows, rank, dtype);
   if (hidden_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters: hidden of %zu bytes needed (got %zu)", need, hidden_bytes);
-  if (int rc = wbhost::device(nullptr, nullptr)) return rc;
-  const AdapterCall c{{ids, ids_are_int64 != 0}, rows, rank, rank_pad(rank), num_adapters, dtype == WB200_F32 ? 3 : 2, static_cast<cudaStream_t>(stream)};
+  int *status = nullptr, sms = 0;
+  if (int rc = wbhost::device(&sms, &status)) return rc;
+  const AdapterCall c{{ids, ids_are_int64 != 0}, rows, rank, rank_pad(rank), num_adapters, dtype == WB200_F32 ? 3 : 2, static_cast<cudaStream_t>(stream), status, sms};
   auto* h = static_cast<__nv_bfloat16*>(hidden);
   if (int rc = run_shrink(c, static_cast<const __nv_bfloat16*>(x), ldx, K, static_cast<const __nv_bfloat16*>(a), false, scale, h)) return rc;
   return run_expand(c, static_cast<const __nv_bfloat16*>(b), false, h, y, ldy, out, ldo, dtype == WB200_F32, N);
@@ -429,8 +493,9 @@ int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, 
   if (workspace_bytes < ws_need) return fail(WB200_ERR_WORKSPACE, "adapters backward: workspace of %zu bytes needed (got %zu)", ws_need, workspace_bytes);
   const size_t need = wb200_adapters_hidden_bytes(rows, rank, WB200_BF16);
   if (db && hidden_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters backward: hidden of %zu bytes needed (got %zu)", need, hidden_bytes);
-  if (int rc = wbhost::device(nullptr, nullptr)) return rc;
-  const AdapterCall c{{ids, ids_are_int64 != 0}, rows, rank, rank_pad(rank), num_adapters, 2, static_cast<cudaStream_t>(stream)};
+  int *status = nullptr, sms = 0;
+  if (int rc = wbhost::device(&sms, &status)) return rc;
+  const AdapterCall c{{ids, ids_are_int64 != 0}, rows, rank, rank_pad(rank), num_adapters, 2, static_cast<cudaStream_t>(stream), status, sms};
   const auto* gp = static_cast<const __nv_bfloat16*>(g);
   if (N % 8) {
     auto* copy = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(workspace) + (need + 255) / 256 * 256);

@@ -27,6 +27,8 @@
 #pragma once
 #include <cuda_bf16.h>
 
+#include "checks.cuh"
+#include "input_grad_sm100.cuh"
 #include "ptx.cuh"
 
 namespace wb {
@@ -68,13 +70,15 @@ __device__ __forceinline__ void load_bf16(const __nv_bfloat16* p, bool whole, in
 }
 
 // Rows of a chunk by adapter.
-struct RowGroups {
-  alignas(16) int id[kChunkRows];
-  alignas(16) int leader[kChunkRows];  // the adapter at its first row, elsewhere a number above all
-  int order[kChunkRows];               // rows of the chunk, those of one adapter together, in their order
-  int start[kChunkRows + 1];           // first place of a group
-  int adapter[kChunkRows];
+template <int ROWS>
+struct RowGroupsOf {
+  alignas(16) int id[ROWS];
+  alignas(16) int leader[ROWS];  // the adapter at its first row, elsewhere a number above all
+  int order[ROWS];               // rows of the chunk, those of one adapter together, in their order
+  int start[ROWS + 1];           // first place of a group
+  int adapter[ROWS];
 };
+using RowGroups = RowGroupsOf<kChunkRows>;
 
 struct Ids {
   const void* at;  // int32, or int64 with `wide`
@@ -86,15 +90,16 @@ __device__ __forceinline__ int adapter_of(const Ids& ids, int row, int rows, int
   return id >= 0 && id < L ? int(id) : -1;
 }
 
-// Called by all threads of the CTA, 64 at least. Returns the number of groups.
-__device__ __forceinline__ int group_rows(RowGroups& g, const Ids& ids, int row0, int rows, int L) {
+// Called by all threads of the CTA, ROWS at least. Returns the number of groups.
+template <int ROWS>
+__device__ __forceinline__ int group_rows(RowGroupsOf<ROWS>& g, const Ids& ids, int row0, int rows, int L) {
   const int t = threadIdx.x;
   const int first_id = adapter_of(ids, row0, rows, L);
-  const int mine = t < kChunkRows ? adapter_of(ids, row0 + t, rows, L) : first_id;
-  if (t < kChunkRows) g.id[t] = mine;
-  if (__syncthreads_and(mine == first_id || (t < kChunkRows && row0 + t >= rows))) {  // one sequence: the usual chunk of a prefill
-    const int count = first_id < 0 ? 0 : min(kChunkRows, rows - row0);
-    if (t < kChunkRows) g.order[t] = t;
+  const int mine = t < ROWS ? adapter_of(ids, row0 + t, rows, L) : first_id;
+  if (t < ROWS) g.id[t] = mine;
+  if (__syncthreads_and(mine == first_id || (t < ROWS && row0 + t >= rows))) {  // one sequence: the usual chunk of a prefill
+    const int count = first_id < 0 ? 0 : min(ROWS, rows - row0);
+    if (t < ROWS) g.order[t] = t;
     if (t == 0) {
       g.start[0] = 0;
       g.start[1] = count;
@@ -104,10 +109,10 @@ __device__ __forceinline__ int group_rows(RowGroups& g, const Ids& ids, int row0
     return count > 0 ? 1 : 0;
   }
   int before = 0;
-  bool first = t < kChunkRows && mine >= 0;
+  bool first = t < ROWS && mine >= 0;
   if (first) {
 #pragma unroll
-    for (int j = 0; j < kChunkRows; j += 4) {
+    for (int j = 0; j < ROWS; j += 4) {
       const int4 o = *reinterpret_cast<const int4*>(g.id + j);
       const int v[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
@@ -119,13 +124,13 @@ __device__ __forceinline__ int group_rows(RowGroups& g, const Ids& ids, int row0
     }
     g.order[before] = t;
   }
-  if (t < kChunkRows) g.leader[t] = first ? mine : 0x7fffffff;
-  const int placed = __syncthreads_count(t < kChunkRows && mine >= 0);
+  if (t < ROWS) g.leader[t] = first ? mine : 0x7fffffff;
+  const int placed = __syncthreads_count(t < ROWS && mine >= 0);
   const int groups = __syncthreads_count(first);
   if (first) {
     int at = 0;
 #pragma unroll
-    for (int j = 0; j < kChunkRows; j += 4) {
+    for (int j = 0; j < ROWS; j += 4) {
       const int4 o = *reinterpret_cast<const int4*>(g.leader + j);
       at += (o.x < mine) + (o.y < mine) + (o.z < mine) + (o.w < mine);
     }
@@ -225,10 +230,10 @@ struct ShrinkParams {
   int x_vec, w_vec;        // 16-byte loads of x; vector loads of w
 };
 
-// A split's sums of up to 64 rows and COLS ranks are in `sums` ([64][COLS + 1]) of every CTA of the cluster: this CTA adds up its share of the
-// rows over the splits, in their order, and writes the scaled bf16 parts. row_of: row of x by its place.
-template <int COLS, typename RowOf>
-__device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums, RowOf row_of, int count, int n0, float scale) {
+// A split's sums of `count` rows and COLS ranks are in `sums` ([..][COLS + 1]) of every CTA of the cluster: this CTA adds up its share of the
+// rows over the splits, in their order, and writes the scaled bf16 parts. By its place, a row's: number in `sums`, row of x, scale.
+template <int COLS, typename SumRow, typename RowOf, typename ScaleOf>
+__device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums, SumRow sum_row, RowOf row_of, ScaleOf scale_of, int count, int n0) {
   __syncthreads();
   const int splits = gridDim.x, split = blockIdx.x;
   if (splits > 1) {
@@ -241,9 +246,9 @@ __device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums
     if (n0 + col >= p.Rp) continue;
     float v = 0.f;
     if (splits == 1) {
-      v = sums[row * (COLS + 1) + col];
+      v = sums[sum_row(row) * (COLS + 1) + col];
     } else {
-      const uint32_t at = smem_u32(sums + row * (COLS + 1) + col);
+      const uint32_t at = smem_u32(sums + sum_row(row) * (COLS + 1) + col);
       float part[8];
 #pragma unroll
       for (int s = 0; s < 8; ++s) part[s] = s < splits ? ld_cluster_f32(mapa_shared(at, s)) : 0.f;
@@ -251,7 +256,7 @@ __device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums
       for (int s = 0; s < 8; ++s) v += part[s];
     }
     __nv_bfloat16 part[3];
-    split_bf16<3>(n0 + col < p.R ? v * scale : 0.f, part);  // (an infinity of x would be a NaN in the ranks behind the last)
+    split_bf16<3>(n0 + col < p.R ? v * scale_of(row) : 0.f, part);  // (an infinity of x would be a NaN in the ranks behind the last)
     __nv_bfloat16* dst = p.hidden + (long long)row_of(row) * p.parts * p.Rp + n0 + col;
 #pragma unroll
     for (int i = 0; i < 3; ++i)
@@ -557,8 +562,137 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
         for (int q = 1; q < 4; ++q) v += sums[q * kChunkRows * (COLS + 1) + at];
         sums[at] = v;
       }
-      finish_hidden<COLS>(p, sums, [&](int row) { return row0 + groups.order[first + row]; }, count, n0, scale);
+      finish_hidden<COLS>(p, sums, [](int row) { return row; }, [&](int row) { return row0 + groups.order[first + row]; }, [&](int) { return scale; }, count, n0);
     }
+  }
+}
+
+// The same for many aligned rows and K a multiple of 64, on the tensor cores: the 128 rows of a chunk x N ranks of two adapters at a time, an accumulator
+// of N columns for each; a row takes the sums of its own. Rows come as one tile, w as one a adapter: A_l's rows K-major, B_l's (TRANS) as they
+// lie, with the ranks in an MN-major operand. Ranks behind the last are the next adapter's or zeros and are not kept. No load passes through
+// registers, w is read once for 128 rows, and a chunk in which one sequence ends and another begins takes a third longer than others.
+template <int N, bool TRANS>
+struct ShrinkWide {
+  static constexpr int ROWS = 128, X_BYTES = ROWS * 128, W_BYTES = TRANS ? 64 * 128 : N * 128, STAGE_BYTES = X_BYTES + 2 * W_BYTES;
+  static constexpr int STAGES = STAGE_BYTES > 24 * 1024 ? 3 : 4;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;  // the sums reuse it
+  static constexpr int TMEM_COLS = N < 32 ? 64 : 2 * N;           // (32 columns are read at a time)
+  static_assert(ROWS * (N + 1) * 4 <= STAGES * STAGE_BYTES && ROWS <= kAdapterThreads, "sums; a thread per row where rows are grouped");
+};
+template <int N, bool TRANS>
+__global__ void __launch_bounds__(kAdapterThreads, 2)
+adapter_shrink_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const ShrinkParams p, int* status) {
+  using Cfg = ShrinkWide<N, TRANS>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ RowGroupsOf<Cfg::ROWS> groups;
+  __shared__ __align__(8) uint64_t bars[2 * Cfg::STAGES + 1];
+  __shared__ uint32_t tmem_slot, abort_word;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  float* sums = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)));  // [128][N + 1]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto full = [&](uint32_t st) { return smem_u32(bars + st); };
+  auto empty = [&](uint32_t st) { return smem_u32(bars + Cfg::STAGES + st); };
+  const uint32_t acc_full = smem_u32(bars + 2 * Cfg::STAGES);
+  WaitCtx ctx{&abort_word, status};
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2 * Cfg::STAGES + 1; ++i) mbar_init(smem_u32(bars + i), 1);
+    abort_word = 0u;
+    fence_mbar_init();
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_w);
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(smem_u32(&tmem_slot), Cfg::TMEM_COLS);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int row0 = blockIdx.y * Cfg::ROWS;
+  const int ngroups = group_rows(groups, p.ids, row0, p.rows, p.L);
+  const int k0 = blockIdx.x * p.split_k, steps = max(0, min(p.K, k0 + p.split_k) - k0) / 64;  // K and split_k are multiples of 64
+  uint32_t stage = 0, phase = 0, acc_phase = 0;
+  for (int gi = 2 * blockIdx.z; gi < ngroups; gi += 2 * gridDim.z) {
+    const int ng = min(2, ngroups - gi);
+    const int first = groups.start[gi], middle = groups.start[gi + 1], count = groups.start[gi + ng] - first;
+    const int l[2] = {groups.adapter[gi], groups.adapter[gi + ng - 1]};
+    const float scale[2] = {p.scale ? p.scale[l[0]] : 1.f, p.scale ? p.scale[l[1]] : 1.f};
+    for (int n0 = 0; n0 < p.Rp; n0 += N) {
+      if (warp == 0) {
+        for (int s = 0; s < steps; ++s) {
+          if (!mbar_wait(empty(stage), phase ^ 1u, ctx, WB_DEV_TIMEOUT_PRODUCER)) continue;  // given up: nothing more is issued
+          const uint32_t to = base + stage * Cfg::STAGE_BYTES;
+          const int k = k0 + s * 64;
+          if (elect_one()) {
+            mbar_expect_tx(full(stage), uint32_t(Cfg::X_BYTES + ng * Cfg::W_BYTES));
+            tma_load_2d<1>(to, &map_x, k, row0, full(stage));
+            for (int i = 0; i < ng; ++i) {
+              if constexpr (TRANS) tma_load_2d<1>(to + Cfg::X_BYTES + i * Cfg::W_BYTES, &map_w, n0, l[i] * p.K + k, full(stage));
+              else tma_load_2d<1>(to + Cfg::X_BYTES + i * Cfg::W_BYTES, &map_w, k, l[i] * p.R + n0, full(stage));
+            }
+          }
+          __syncwarp();
+          if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1u; }
+        }
+      } else if (warp == 1) {
+        constexpr uint32_t idesc = make_idesc_bf16_bt(Cfg::ROWS, N) & ~(TRANS ? 0u : 1u << 16);  // B K-major, or MN-major
+        for (int s = 0; s < steps; ++s) {
+          mbar_wait(full(stage), phase, ctx, WB_DEV_TIMEOUT_MMA_FULL);
+          tc_fence_after_sync();
+          const uint32_t at = base + stage * Cfg::STAGE_BYTES;
+          if (elect_one()) {
+            const uint64_t a = make_desc_k_sw128(at);
+            for (int i = 0; i < ng; ++i) {
+              const uint32_t w_at = at + Cfg::X_BYTES + i * Cfg::W_BYTES;
+              const uint64_t b = TRANS ? make_desc_mn_sw128(w_at, 64 * 128) : make_desc_k_sw128(w_at);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_f16<1>(tmem + i * N, a + uint64_t(k * 2), b + uint64_t(k * (TRANS ? 2048 >> 4 : 2)), idesc, (s > 0 || k > 0) ? 1u : 0u);
+            }
+            tc_commit<1>(empty(stage));
+            if (s == steps - 1) tc_commit<1>(acc_full);
+          }
+          __syncwarp();
+          if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (steps > 0) {
+        mbar_wait(acc_full, acc_phase, ctx, WB_DEV_TIMEOUT_EPILOGUE);
+        acc_phase ^= 1u;
+        tc_fence_after_sync();
+      }
+      // warps w and w + 4 read rows 32 (w % 4) .., 32 columns each; every stage has been read by now
+      const int row = (warp & 3) * 32 + lane, c = (warp >> 2) * 32;
+      if (c < N) {
+        for (int i = 0; i < ng; ++i) {
+          uint32_t v[32];
+          if (steps > 0) {
+            tmem_ld_32x32(tmem + (uint32_t((warp & 3) * 32) << 16) + i * N + c, v);
+            tmem_ld_wait();
+          }
+          if (groups.id[row] == l[i])
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j < N) sums[row * (N + 1) + c + j] = steps > 0 ? __uint_as_float(v[j]) : 0.f;
+        }
+      }
+      tc_fence_before_sync();
+      finish_hidden<N>(
+          p, sums, [&](int place) { return groups.order[first + place]; }, [&](int place) { return row0 + groups.order[first + place]; },
+          [&](int place) { return first + place < middle ? scale[0] : scale[1]; }, count, n0);
+      fence_proxy_async_smem();  // the copy engine writes next where the sums have been read
+      __syncthreads();
+      tc_fence_after_sync();
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc<1>(tmem, Cfg::TMEM_COLS);
   }
 }
 
@@ -1179,6 +1313,255 @@ adapter_expand_tile_kernel(const ExpandParams p) {
   if (blockIdx.z == 0 && p.out != p.y)
     for (int r = warp; r < min(kChunkRows, p.rows - row0); r += kAdapterWarps)
       if (groups.id[r] < 0) expand_rest<T>(p, row0 + r, c_begin + lane * 8, c_end, 256);
+}
+
+// The same for many aligned bf16 rows and ranks up to 64, on the tensor cores: 128 rows of a chunk x 128 columns, both parts of the hidden vectors against the
+// same tile of w (A operand: the chunk's hidden vectors, brought once; B: B_l's rows K-major, or (TRANS) A_l's as they lie, MN-major). Two adapters at
+// a time have accumulators, a row takes the sums of its own; y comes by the copy engine, is added to in shared memory and leaves from there.
+// One CTA per SM works through its share of all (chunk, 128 columns) in order.
+//   warp 0: y and w by TMA; warp 1: tcgen05.mma; warps 2 .. 9: sums, thread = row, 64 columns; warp 10: out by TMA
+template <bool TRANS>
+struct ExpandWide {
+  static constexpr int ROWS = 128, COLS = 128, A_BYTES = 2 * ROWS * 128, B_BYTES = COLS * 128, Y_BYTES = ROWS * COLS * 2;
+  static constexpr int B_STAGES = 4, Y_STAGES = 3, EPILOGUE_WARPS = 8, THREADS = (3 + EPILOGUE_WARPS) * 32;
+  static constexpr int B_BASE = A_BYTES, Y_BASE = B_BASE + B_STAGES * B_BYTES;
+  static constexpr int SMEM_BYTES = Y_BASE + Y_STAGES * Y_BYTES + 1024;
+  static constexpr int TMEM_COLS = 512;  // two buffers of two adapters
+};
+struct ExpandWideParams {
+  Ids ids;
+  int rows, C, R, Rp, L, chunks, tiles;
+  int has_y, in_place;
+  int* status;
+};
+// A CTA's share of the tiles. A tile of a chunk in which one sequence ends and another begins takes a quarter longer (8192 x 8192 at rank 64: one sequence
+// 51 us, seven 63 where the tiles are shared out by number), which up to kWideChunks chunks is weighed, by a chunk's first and last row.
+constexpr int kWideChunks = 512;
+struct WideShares {
+  int weight[kWideChunks];
+  int at[2];  // first tile, and the one behind the last
+};
+__device__ __forceinline__ void wide_share(WideShares& s, const ExpandWideParams& p) {
+  const int cta = blockIdx.x, ctas = gridDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long tiles = (long long)p.chunks * p.tiles;
+  if (p.chunks > kWideChunks) {
+    if (threadIdx.x < 2) s.at[threadIdx.x] = int(tiles * (cta + int(threadIdx.x)) / ctas);
+    __syncthreads();
+    return;
+  }
+  for (int c = threadIdx.x; c < p.chunks; c += blockDim.x)
+    s.weight[c] = adapter_of(p.ids, c * 128, p.rows, p.L) == adapter_of(p.ids, min(c * 128 + 127, p.rows - 1), p.rows, p.L) ? 4 : 5;
+  __syncthreads();
+  if (warp == 0) {
+    const int per = (p.chunks + 31) / 32, first = lane * per;
+    int sum = 0;
+    for (int c = first; c < min(first + per, p.chunks); ++c) sum += s.weight[c];
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += v;
+    }
+    const int total = __shfl_sync(0xffffffffu, before, 31);
+    before -= sum;
+    for (int i = 0; i < 2; ++i) {
+      long long rest = (long long)total * p.tiles * (cta + i) / ctas - (long long)before * p.tiles;  // in weighted tiles, from the lane's first chunk on
+      if (rest >= 0 && rest < (long long)sum * p.tiles) {
+        int c = first;
+        while (rest >= (long long)s.weight[c] * p.tiles) rest -= (long long)s.weight[c++] * p.tiles;
+        s.at[i] = c * p.tiles + int(rest) / s.weight[c];
+      }
+    }
+    if (lane == 0 && cta + 1 == ctas) s.at[1] = int(tiles);
+  }
+  __syncthreads();
+}
+template <bool TRANS>
+__global__ void __launch_bounds__(ExpandWide<TRANS>::THREADS, 1)
+adapter_expand_wide_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y,
+                           const __grid_constant__ CUtensorMap map_out, const ExpandWideParams p) {
+  using Cfg = ExpandWide<TRANS>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ RowGroupsOf<Cfg::ROWS> groups;
+  __shared__ WideShares shares;
+  constexpr int BARS = 5 + 2 * Cfg::B_STAGES + 3 * Cfg::Y_STAGES;
+  __shared__ __align__(8) uint64_t bars[BARS];
+  __shared__ uint32_t tmem_slot, abort_word;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t a_full = smem_u32(bars);
+  auto acc_full = [&](uint32_t i) { return smem_u32(bars + 1 + i); };
+  auto acc_empty = [&](uint32_t i) { return smem_u32(bars + 3 + i); };
+  auto b_full = [&](uint32_t i) { return smem_u32(bars + 5 + i); };
+  auto b_empty = [&](uint32_t i) { return smem_u32(bars + 5 + Cfg::B_STAGES + i); };
+  auto y_full = [&](uint32_t i) { return smem_u32(bars + 5 + 2 * Cfg::B_STAGES + i); };
+  auto y_empty = [&](uint32_t i) { return smem_u32(bars + 5 + 2 * Cfg::B_STAGES + Cfg::Y_STAGES + i); };
+  auto out_full = [&](uint32_t i) { return smem_u32(bars + 5 + 2 * Cfg::B_STAGES + 2 * Cfg::Y_STAGES + i); };
+  WaitCtx ctx{&abort_word, p.status};
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < BARS; ++i) mbar_init(smem_u32(bars + i), i == 3 || i == 4 || i >= BARS - Cfg::Y_STAGES ? Cfg::EPILOGUE_WARPS : 1);
+    abort_word = 0u;
+    fence_mbar_init();
+    prefetch_tensormap(&map_h);
+    prefetch_tensormap(&map_w);
+    prefetch_tensormap(&map_y);
+    prefetch_tensormap(&map_out);
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(smem_u32(&tmem_slot), Cfg::TMEM_COLS);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+  wide_share(shares, p);
+  const int u_end = shares.at[1];
+  const int ksteps = p.Rp / 16;
+  uint32_t a_phase = 0, bs = 0, b_phase = 0, ys = 0, y_phase = 0, acc = 0, acc_phase = 0;  // (each warp's own)
+  for (int u = shares.at[0]; u < u_end;) {
+    const int chunk = u / p.tiles, t0 = u - chunk * p.tiles, t1 = min(p.tiles, t0 + u_end - u);
+    u += t1 - t0;
+    const int row0 = chunk * Cfg::ROWS;
+    __syncthreads();  // the groups of the chunk before have been read
+    const int ngroups = group_rows(groups, p.ids, row0, p.rows, p.L);
+    if (ngroups == 0 && p.in_place) continue;
+    if (warp == 0) {
+      if (ngroups > 0 && elect_one()) {
+        mbar_expect_tx(a_full, Cfg::A_BYTES);
+        tma_load_2d<1>(base, &map_h, 0, row0, a_full);
+        tma_load_2d<1>(base + Cfg::A_BYTES / 2, &map_h, p.Rp, row0, a_full);
+      }
+      __syncwarp();
+      for (int t = t0; t < t1; ++t) {
+        const int c0 = t * Cfg::COLS;
+        const int halves = c0 + 64 < p.C ? 2 : 1;
+        if (p.has_y) {
+          if (!mbar_wait(y_empty(ys), y_phase ^ 1u, ctx, WB_DEV_TIMEOUT_PRODUCER)) continue;  // given up: nothing more is issued
+          if (elect_one()) {
+            mbar_expect_tx(y_full(ys), uint32_t(halves * (Cfg::Y_BYTES / 2)));
+            for (int h = 0; h < halves; ++h) tma_load_2d<1>(base + Cfg::Y_BASE + ys * Cfg::Y_BYTES + h * (Cfg::Y_BYTES / 2), &map_y, c0 + 64 * h, row0, y_full(ys));
+          }
+          __syncwarp();
+          if (++ys == Cfg::Y_STAGES) { ys = 0; y_phase ^= 1u; }
+        }
+        for (int gi = 0; gi < ngroups; ++gi) {
+          if (!mbar_wait(b_empty(bs), b_phase ^ 1u, ctx, WB_DEV_TIMEOUT_PRODUCER)) continue;
+          if (elect_one()) {
+            const uint32_t to = base + Cfg::B_BASE + bs * Cfg::B_BYTES;
+            const int l = groups.adapter[gi];
+            if constexpr (TRANS) {
+              mbar_expect_tx(b_full(bs), uint32_t(halves * p.Rp * 128));
+              for (int h = 0; h < halves; ++h) tma_load_2d<1>(to + h * (Cfg::B_BYTES / 2), &map_w, c0 + 64 * h, l * p.R, b_full(bs));
+            } else {
+              mbar_expect_tx(b_full(bs), Cfg::B_BYTES);
+              tma_load_2d<1>(to, &map_w, 0, l * p.C + c0, b_full(bs));
+            }
+          }
+          __syncwarp();
+          if (++bs == Cfg::B_STAGES) { bs = 0; b_phase ^= 1u; }
+        }
+      }
+    } else if (warp == 1) {
+      constexpr uint32_t idesc = make_idesc_bf16_bt(Cfg::ROWS, Cfg::COLS) & ~(TRANS ? 0u : 1u << 16);  // B K-major, or MN-major
+      if (ngroups > 0) {
+        mbar_wait(a_full, a_phase, ctx, WB_DEV_TIMEOUT_MMA_FULL);
+        a_phase ^= 1u;
+      }
+      for (int t = t0; t < t1; ++t)
+        for (int gi = 0; gi < ngroups; gi += 2) {
+          mbar_wait(acc_empty(acc), acc_phase ^ 1u, ctx, WB_DEV_TIMEOUT_MMA_ACC);
+          tc_fence_after_sync();
+          const int ng = min(2, ngroups - gi);
+          for (int i = 0; i < ng; ++i) {
+            mbar_wait(b_full(bs), b_phase, ctx, WB_DEV_TIMEOUT_MMA_FULL);
+            tc_fence_after_sync();
+            if (elect_one()) {
+              const uint32_t at = base + Cfg::B_BASE + bs * Cfg::B_BYTES;
+              const uint64_t b = TRANS ? make_desc_mn_sw128(at, Cfg::B_BYTES / 2) : make_desc_k_sw128(at);
+              for (int part = 0; part < 2; ++part) {
+                const uint64_t a = make_desc_k_sw128(base + part * (Cfg::A_BYTES / 2));
+                for (int k = 0; k < ksteps; ++k)
+                  mma_f16<1>(tmem + (acc * 2 + i) * Cfg::COLS, a + uint64_t(k * 2), b + uint64_t(k * (TRANS ? 2048 >> 4 : 2)), idesc, (part > 0 || k > 0) ? 1u : 0u);
+              }
+              tc_commit<1>(b_empty(bs));
+              if (i == ng - 1) tc_commit<1>(acc_full(acc));
+            }
+            __syncwarp();
+            if (++bs == Cfg::B_STAGES) { bs = 0; b_phase ^= 1u; }
+          }
+          acc ^= 1u;
+          if (acc == 0u) acc_phase ^= 1u;
+        }
+    } else if (warp < 2 + Cfg::EPILOGUE_WARPS) {
+      const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane, id = groups.id[row];
+      for (int t = t0; t < t1; ++t) {
+        const int c0 = t * Cfg::COLS;
+        mbar_wait(p.has_y ? y_full(ys) : y_empty(ys), p.has_y ? y_phase : y_phase ^ 1u, ctx, WB_DEV_TIMEOUT_EPILOGUE);
+        const uint32_t mine = base + Cfg::Y_BASE + ys * Cfg::Y_BYTES + half * (Cfg::Y_BYTES / 2) + row * 128;
+        auto at = [&](int piece_of_row) { return mine + uint32_t((piece_of_row ^ (row & 7)) << 4); };
+        if (!p.has_y && id < 0)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at(i)), "r"(0u) : "memory");
+        for (int gi = 0; gi < ngroups; gi += 2) {
+          mbar_wait(acc_full(acc), acc_phase, ctx, WB_DEV_TIMEOUT_EPILOGUE);
+          tc_fence_after_sync();
+          const int ng = min(2, ngroups - gi);
+          for (int i = 0; i < ng; ++i) {
+            const bool hit = id == groups.adapter[gi + i];
+            if (!__any_sync(0xffffffffu, hit)) continue;
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+              uint32_t v[32];
+              tmem_ld_32x32(tmem + (uint32_t(quad * 32) << 16) + (acc * 2 + i) * Cfg::COLS + half * 64 + c, v);
+              tmem_ld_wait();
+              if (hit)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  uint32_t o[4] = {0u, 0u, 0u, 0u};
+                  if (p.has_y) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(at(c / 8 + q)));
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    o[j] = pack_bf16x2(__uint_as_float(o[j] << 16) + __uint_as_float(v[8 * q + 2 * j]), __uint_as_float(o[j] & 0xffff0000u) + __uint_as_float(v[8 * q + 2 * j + 1]));
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at(c / 8 + q)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                }
+            }
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty(acc));
+          acc ^= 1u;
+          if (acc == 0u) acc_phase ^= 1u;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(out_full(ys));
+        if (++ys == Cfg::Y_STAGES) { ys = 0; y_phase ^= 1u; }
+      }
+    } else {
+      for (int t = t0; t < t1; ++t) {
+        if (!mbar_wait(out_full(ys), y_phase, ctx, WB_DEV_TIMEOUT_EPILOGUE)) continue;  // given up
+        if (lane == 0) {
+          for (int h = 0; h < 2; ++h)
+            if (t * Cfg::COLS + 64 * h < p.C) tma_store_2d(&map_out, base + Cfg::Y_BASE + ys * Cfg::Y_BYTES + h * (Cfg::Y_BYTES / 2), t * Cfg::COLS + 64 * h, row0);
+          bulk_commit_group();
+          bulk_wait_group_read<0>();
+          mbar_arrive(y_empty(ys));
+        }
+        __syncwarp();
+        if (++ys == Cfg::Y_STAGES) { ys = 0; y_phase ^= 1u; }
+      }
+    }
+  }
+  if (threadIdx.x == (2 + Cfg::EPILOGUE_WARPS) * 32) bulk_wait_group<0>();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc<1>(tmem, Cfg::TMEM_COLS);
+  }
 }
 
 // Rows of any alignment into rows of `pitch` (a multiple of 8) elements, zeros behind the last: what follows copies whole pieces.

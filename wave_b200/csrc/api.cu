@@ -1294,8 +1294,8 @@ int device(int* sm_count, int** status) {
   return WB200_OK;
 }
 int tensor_map(CUtensorMap* map, const void* base, unsigned long long d0, unsigned long long d1, unsigned long long stride, unsigned box0,
-               unsigned box1, CUtensorMapDataType dtype, CUtensorMapSwizzle swizzle) {
-  const MapKey k{base, d0, d1, stride, box0, box1, int(dtype), int(swizzle), int(CU_TENSOR_MAP_L2_PROMOTION_NONE)};
+               unsigned box1, CUtensorMapDataType dtype, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+  const MapKey k{base, d0, d1, stride, box0, box1, int(dtype), int(swizzle), int(promotion)};
   const CUresult r = encode_2d(map, k);
   if (r != CUDA_SUCCESS) return ::fail(WB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (%llu x %llu)", int(r), d0, d1);
   return WB200_OK;

@@ -16,7 +16,8 @@ WB_HIDDEN int fail(int code, const char* fmt, ...);             // keeps the mes
 WB_HIDDEN int device(int* sm_count, int** status);              // of the current device; status may be null
 // A 2-D tensor map: d0 x d1 elements (d0 contiguous), rows `stride` bytes apart, boxes of box0 x box1.
 WB_HIDDEN int tensor_map(CUtensorMap* map, const void* base, unsigned long long d0, unsigned long long d1, unsigned long long stride,
-                         unsigned box0, unsigned box1, CUtensorMapDataType dtype, CUtensorMapSwizzle swizzle);
+                         unsigned box0, unsigned box1, CUtensorMapDataType dtype, CUtensorMapSwizzle swizzle,
+                         CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_NONE);
 // moe_combine for bf16 rows that start on 16 bytes, at most 8 pairs a token (adapt.cu).
 WB_HIDDEN cudaError_t combine_tokens(const void* y, long long ldy, const int* row_of, const float* weight, int tokens, int top_k, int cols, void* out,
                                      long long ldo, cudaStream_t stream);
