@@ -402,8 +402,8 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
 // Many rows: a ring of stages of 64 k in shared memory, rows of x gathered by their place in the group. Warp (m, q) takes rows 32 m .. and the
 // q-th 16 of the 64 k: x passes through ldmatrix once, w twice, and the four sums over k meet at the end. Two stages between barriers, so that the warps
 // wait for one another half as often. Bound by HBM on x at rank 16 and by shared memory and issue slots at rank 64, where each 64 rows x 64 k take as
-// many ldmatrix of w as of x: 8192 x 8192 at rank 64 50 us (134 MB of x, 2.7 TB/s; MMA pipe 39 %), 4096 x 4096 at rank 16
-// 11 us.
+// many ldmatrix of w as of x: 8192 x 8192 at rank 64 50 us (134 MB of x, 2.7 TB/s; MMA pipe 39 %), where the tensor cores take 35;
+// 4096 x 4096 at rank 16 11 us.
 template <int RT>
 struct ShrinkTile {
   static constexpr int X_BYTES = kChunkRows * 128, W_BYTES = RT * 1024, STAGE_BYTES = X_BYTES + W_BYTES;
@@ -571,6 +571,8 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
 // of N columns for each; a row takes the sums of its own. Rows come as one tile, w as one a adapter: A_l's rows K-major, B_l's (TRANS) as they
 // lie, with the ranks in an MN-major operand. Ranks behind the last are the next adapter's or zeros and are not kept. No load passes through
 // registers, w is read once for 128 rows, and a chunk in which one sequence ends and another begins takes a third longer than others.
+// 8192 x 8192 at rank 64 35 us for seven sequences, 31 for one (134 MB, 4.3 TB/s). Bound by HBM, which 128 bytes of a row at a time do not bring to its full
+// rate; 256 bytes fetched into L2 at a time gained 2 us. Rows gathered by the copy engine, four to a request, took 55.
 template <int N, bool TRANS>
 struct ShrinkWide {
   static constexpr int ROWS = 128, X_BYTES = ROWS * 128, W_BYTES = TRANS ? 64 * 128 : N * 128, STAGE_BYTES = X_BYTES + 2 * W_BYTES;
@@ -1318,7 +1320,8 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 // The same for many aligned bf16 rows and ranks up to 64, on the tensor cores: 128 rows of a chunk x 128 columns, both parts of the hidden vectors against the
 // same tile of w (A operand: the chunk's hidden vectors, brought once; B: B_l's rows K-major, or (TRANS) A_l's as they lie, MN-major). Two adapters at
 // a time have accumulators, a row takes the sums of its own; y comes by the copy engine, is added to in shared memory and leaves from there.
-// One CTA per SM works through its share of all (chunk, 128 columns) in order.
+// One CTA per SM works through its share of all (chunk, 128 columns) in order. 8192 x 8192 at rank 64 50 us for one sequence (268 MB, 5.4 TB/s), 57 for
+// seven; the mma.sync form 63 to 70. Bound by HBM, and below 8192 x 4096 by the start-up of one large CTA per SM.
 //   warp 0: y and w by TMA; warp 1: tcgen05.mma; warps 2 .. 9: sums, thread = row, 64 columns; warp 10: out by TMA
 template <bool TRANS>
 struct ExpandWide {
