@@ -337,23 +337,37 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
       const int as = it & 1;
       mbar_wait(acc_full(as), uint32_t(it >> 1) & 1u, ctx, WB_DEV_TIMEOUT_EPILOGUE);
       tc_fence_after_sync();
-      const int row = (mt * CG + int(rank)) * Cfg::BM + quad * 32 + lane;
-      __nv_bfloat16* dst = p.dx + (long long)row * p.ldd;
+      const int row = (mt * CG + int(rank)) * Cfg::BM + quad * 32 + (lane & ~3);  // of this lane's first store
+      __nv_bfloat16* dst = p.dx + (long long)row * p.ldd + (lane & 3) * 8;
+      const long long pitch = p.ldd / 8;
 #pragma unroll 1
       for (int c = 0; c < Cfg::TILE_K; c += 32) {
         uint32_t r[32];
         tmem_ld_32x32(tmem_base + (uint32_t(quad * 32) << 16) + as * Cfg::TILE_K + c, r);
         tmem_ld_wait();
         const int col = kt * Cfg::TILE_K + c;
-        if (row < p.M && col < p.K) {  // K is a multiple of 32
-          uint4* q = reinterpret_cast<uint4*>(dst + col);
+        if (col >= p.K) break;  // K is a multiple of 32
+        // Four neighbouring lanes exchange their rows' four pieces of 8 columns, so that a store writes 64 consecutive bytes of each of 8 rows
+        // (6826 x 256 x 5216, mostly epilogue: 47.5 us with a row to a lane, 37.3)
+        uint32_t q[4][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            q[j] = make_uint4(pack_bf16x2(__uint_as_float(r[8 * j]), __uint_as_float(r[8 * j + 1])),
-                              pack_bf16x2(__uint_as_float(r[8 * j + 2]), __uint_as_float(r[8 * j + 3])),
-                              pack_bf16x2(__uint_as_float(r[8 * j + 4]), __uint_as_float(r[8 * j + 5])),
-                              pack_bf16x2(__uint_as_float(r[8 * j + 6]), __uint_as_float(r[8 * j + 7])));
-        }
+        for (int j = 0; j < 16; ++j) q[j / 4][j % 4] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j & o) continue;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, (lane & o) ? q[j][w] : q[j | o][w], o);
+              if (lane & o) q[j][w] = got;
+              else q[j | o][w] = got;
+            }
+          }
+        uint4* at = reinterpret_cast<uint4*>(dst + col);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (row + j < p.M) at[j * pitch] = make_uint4(q[j][0], q[j][1], q[j][2], q[j][3]);
       }
       tc_fence_before_sync();
       __syncwarp();
