@@ -433,6 +433,23 @@ def test_layer_gradient_is_the_layers_part_with_the_adapters_on_it(rows, N):
     assert torch.equal(out.detach()[ids < 0], layer._base(x.detach())[ids < 0])
 
 
+@pytest.mark.parametrize("ids", ["runs", "mixed"])
+def test_layer_gradient_of_many_rows(ids):
+    """The adapters' part added to the layer's in place by the kernels for many rows, whole chunks without an adapter among them."""
+    rows, K, N = 8300, 4096, 96
+    g = torch.Generator().manual_seed(4)
+    layer = wb.MXFP4Linear.from_float((torch.randn(N, K, generator=g) / 64).to(DEV), input_grad=True)
+    y, x, a, b, at, s = make(rows, K, N, 48, 4, ids=ids, seed=rows)
+    at[1000:1500] = -1
+    up = torch.randn(rows, N, generator=g).to(BF16).to(DEV)
+    x.requires_grad_()
+    dx, = torch.autograd.grad(layer(x, wb.LowRankAdapters(a, b, s), at), x, up)
+    part = wb.mxfp4_input_grad(up, layer.weight_codes, layer.weight_scales)
+    _, (want, size), _, _ = definition(y, x, a, b, at, s, up)
+    assert_near(dx, part.double() + want, size, N + 48, 2)
+    assert torch.equal(dx[at < 0], part[at < 0])
+
+
 def test_every_combination_of_wanted_gradients():
     y, x, a, b, ids, s = make(70, 128, 64, 16, 3)
     g = torch.randn(70, 64, generator=torch.Generator().manual_seed(4)).to(BF16).to(DEV)
