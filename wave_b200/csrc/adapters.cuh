@@ -577,8 +577,11 @@ template <int N, bool TRANS>
 struct ShrinkWide {
   static constexpr int ROWS = 128, X_BYTES = ROWS * 128, W_BYTES = TRANS ? 64 * 128 : N * 128, STAGE_BYTES = X_BYTES + 2 * W_BYTES;
   static constexpr int STAGES = STAGE_BYTES > 24 * 1024 ? 3 : 4;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;  // the sums reuse it
-  static constexpr int TMEM_COLS = N < 32 ? 64 : 2 * N;           // (32 columns are read at a time)
+  // Two CTAs to an SM, and beside them none of the library's other kernels that take tensor memory (they ask for 160 KB or more): a CTA holds its columns
+  // while it waits for its cluster, so that one that waited for columns of another kernel's, in another stream, might wait for good.
+  static constexpr int SMEM_BYTES = 97 * 1024;           // the sums reuse the stages
+  static constexpr int TMEM_COLS = N < 32 ? 64 : 2 * N;  // (32 columns are read at a time)
+  static_assert(STAGES * STAGE_BYTES + 1024 <= SMEM_BYTES && 2 * TMEM_COLS <= 512, "stages; columns of two CTAs");
   static_assert(ROWS * (N + 1) * 4 <= STAGES * STAGE_BYTES && ROWS <= kAdapterThreads, "sums; a thread per row where rows are grouped");
 };
 template <int N, bool TRANS>
