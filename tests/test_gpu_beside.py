@@ -79,6 +79,28 @@ def test_threads_with_streams_of_their_own():
     assert len(got) == 3 and all(torch.equal(p, q) for res in got.values() for p, q in zip(res, want))
 
 
+def test_layers_and_adapters_in_two_streams_at_once():
+    """Kernels that take tensor memory and wait within clusters, side by side: the same bits as one after the other."""
+    g = torch.Generator().manual_seed(2)
+    layer = wb.MXFP4Linear.from_float((torch.randn(4096, 4096, generator=g) / 64).to(DEV), input_grad=True)
+    xs = [torch.randn(rows, 4096, generator=g).to(BF16).to(DEV) for rows in (8, 500, 4096)]
+    a, b = (torch.randn(6, 64, 4096, generator=g) / 64).to(BF16).to(DEV), (torch.randn(6, 4096, 64, generator=g) / 8).to(BF16).to(DEV)
+    ids = [torch.randint(-1, 6, (x.shape[0],), generator=g).sort().values.to(DEV) for x in xs]
+    works = [lambda: [layer(x) for x in xs] + [wb.mxfp4_input_grad(x, layer.weight_codes, layer.weight_scales) for x in xs],
+             lambda: [wb.apply_adapters(x, x, a, b, i) for x, i in zip(xs, ids)]]
+    want = [work() for work in works]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for stream, work in zip(streams, works):
+            with torch.cuda.stream(stream):
+                got.append(work())
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for one, other in zip(got, want) for p, q in zip(one, other))
+    wb.ops.check_device_status()
+
+
 @pytest.mark.parametrize("python", [False, True])
 def test_a_derivative_of_a_derivative_is_refused(python, monkeypatch):
     if python:
