@@ -451,7 +451,7 @@ int wb200_multi_gpu_time_end(wb200_multi_gpu_t* h, float* max_ms);
  * [0, num_adapters) have no adapter and keep y. x [rows, K] bf16 (pitch ldx), a [num_adapters, rank, K] and b [num_adapters, N, rank]
  * bf16, contiguous; ids int32 or int64; scale f32 [num_adapters], or null for ones; y and out [rows, N] of `dtype`, out may be y (in
  * place), otherwise they do not overlap. K is a multiple of 8, rank at most 256, N any. hidden: wb200_adapters_hidden_bytes(rows, rank, dtype)
- * bytes, 16-byte aligned, left with scale[l] * A_l x[t] as sums of bf16 parts, which the backward call reads. Two launches, no order of the
+ * bytes, 16-byte aligned, left with scale[l] * A_l x[t] in f32, which the backward call reads. Two launches, no order of the
  * ids needed. */
 size_t wb200_adapters_hidden_bytes(int rows, int rank, int dtype);
 int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,

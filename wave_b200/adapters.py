@@ -72,11 +72,11 @@ def _forward(sizes, y, x, a, b, ids, scale, out) -> torch.Tensor:
     """Writes out, returns the hidden vectors."""
     rows, K, N, rank, pool = sizes
     lib = _lib.load()
-    hidden = torch.empty(rows, 2 if y.dtype == torch.bfloat16 else 3, (rank + 15) // 16 * 16, dtype=torch.bfloat16, device=x.device)
+    hidden = torch.empty(int(lib.wb200_adapters_hidden_bytes(rows, rank, _OUT_CODE[y.dtype])), dtype=torch.uint8, device=x.device)
     _launch(x.device, lambda stream: lib.wb200_adapters_forward(
         rows, K, N, rank, pool, x.data_ptr(), _pitch(x), a.data_ptr(), b.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64),
         scale.data_ptr() if scale is not None else None, y.data_ptr(), _pitch(y), out.data_ptr(), _pitch(out), _OUT_CODE[out.dtype],
-        hidden.data_ptr(), 2 * hidden.numel(), stream))
+        hidden.data_ptr(), hidden.numel(), stream))
     return hidden
 
 
@@ -114,7 +114,7 @@ def _backward(sizes, x, a, b, ids, scale, g, hidden, dx, accumulate: bool, need_
     ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
     _launch(x.device, lambda stream: lib.wb200_adapters_backward(
         rows, K, N, rank, pool, x.data_ptr(), _pitch(x), a.data_ptr(), b.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), ptr(scale),
-        g.data_ptr(), _pitch(g), hidden.data_ptr(), 2 * hidden.numel(), ptr(dx), K, int(accumulate), ptr(da), ptr(db), ws.data_ptr(), nbytes, stream))
+        g.data_ptr(), _pitch(g), hidden.data_ptr(), hidden.numel(), ptr(dx), K, int(accumulate), ptr(da), ptr(db), ws.data_ptr(), nbytes, stream))
     return da, db
 
 

@@ -43,14 +43,14 @@ cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cu
   return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
-// Lets a kernel have up to 200 KB of dynamic shared memory, once per device.
-template <auto Kernel>
+// Lets a kernel have up to BYTES of dynamic shared memory, once per device.
+template <auto Kernel, int BYTES = 200 * 1024>
 int allow_smem() {
   static bool done[wbhost::kMaxDevices] = {};
   int dev = 0;
   WB_HOST_CUDA(cudaGetDevice(&dev));
   if (!done[dev]) {
-    WB_HOST_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    WB_HOST_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
     done[dev] = true;
   }
   return WB200_OK;
@@ -94,7 +94,7 @@ int group_lanes(int rows, int L, long long others) {
 
 struct AdapterCall {
   wb::Ids ids;
-  int rows, R, Rp, L, parts;
+  int rows, R, Rp, L;
   cudaStream_t stream;
   int* status;
   int sms;
@@ -139,11 +139,11 @@ bool wide_shrink(const AdapterCall& c, const wb::ShrinkParams& p, bool trans) {
          (c.Rp > 32 || (c.rows >= 2048 && !trans));
 }
 
-// hidden [rows][parts][Rp] = rows of x onto the ranks, scaled. trans: w is [L][K][R].
-int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int K, const __nv_bfloat16* w, bool trans, const float* scale, __nv_bfloat16* hidden) {
+// hidden [rows][Rp] = rows of x onto the ranks, scaled. trans: w is [L][K][R].
+int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int K, const __nv_bfloat16* w, bool trans, const float* scale, float* hidden) {
   wb::ShrinkParams p;
   p.x = x; p.w = w; p.ids = c.ids; p.scale = scale; p.hidden = hidden; p.ldx = ldx;
-  p.rows = c.rows; p.K = K; p.R = c.R; p.Rp = c.Rp; p.L = c.L; p.parts = c.parts;
+  p.rows = c.rows; p.K = K; p.R = c.R; p.Rp = c.Rp; p.L = c.L;
   const bool few = few_rows(c.rows, c.L);
   p.x_vec = aligned_to(x, 16) && ldx % 8 == 0 && ldx >= (K + 7) / 8 * 8;  // (a piece that K ends in is there, zeros behind)
   if (!few && wide_shrink(c, p, trans)) {
@@ -162,10 +162,10 @@ int run_shrink(const AdapterCall& c, const __nv_bfloat16* x, long long ldx, int 
   return trans ? launch_shrink_ranks<true>(p, few, grid, c.stream) : launch_shrink_ranks<false>(p, few, grid, c.stream);
 }
 
-template <typename T, int P, int QN, bool TRANS, bool FAST, bool EXACT>
+template <typename T, int QN, bool TRANS, bool FAST, bool EXACT>
 int launch_expand_tile(const wb::ExpandParams& p, dim3 grid, cudaStream_t s) {
-  constexpr auto kernel = wb::adapter_expand_tile_kernel<T, P, QN, TRANS, FAST, EXACT>;
-  const size_t smem = size_t(wb::kChunkRows) * wb::expand_pitch(P, p.Rp, FAST && EXACT && QN % 2 == 0) * 2 + (FAST ? wb::expand_ring_bytes(sizeof(T), EXACT) : 0);
+  constexpr auto kernel = wb::adapter_expand_tile_kernel<T, QN, TRANS, FAST, EXACT>;
+  const size_t smem = size_t(wb::kChunkRows) * wb::expand_pitch(p.Rp, FAST && EXACT && QN % 2 == 0) * 2 + (FAST ? wb::expand_ring_bytes(sizeof(T), EXACT) : 0);
   if (int rc = smem > 24 * 1024 ? allow_smem<kernel>() : WB200_OK) return rc;
   WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, smem, s, p));
   return WB200_OK;
@@ -175,42 +175,41 @@ int whole_pieces(const wb::ExpandParams& p) {
   return p.w_vec && p.R == p.Rp && (p.R == 16 || p.R == 32 || p.R == 64) ? p.R / 8 : p.w_vec && p.R == 8 ? 1 : 0;
 }
 
-template <typename T, int P, bool TRANS>
+template <typename T, bool TRANS>
 int launch_expand(const wb::ExpandParams& p, bool few, dim3 grid, cudaStream_t s) {
   if (few) {
     if constexpr (!TRANS)
       if (const int pieces = whole_pieces(p)) {
-        auto kernel = pieces == 1   ? wb::adapter_expand_few_whole_kernel<T, P, 1>
-                      : pieces == 2 ? wb::adapter_expand_few_whole_kernel<T, P, 2>
-                      : pieces == 4 ? wb::adapter_expand_few_whole_kernel<T, P, 4>
-                                    : wb::adapter_expand_few_whole_kernel<T, P, 8>;
+        auto kernel = pieces == 1   ? wb::adapter_expand_few_whole_kernel<T, 1>
+                      : pieces == 2 ? wb::adapter_expand_few_whole_kernel<T, 2>
+                      : pieces == 4 ? wb::adapter_expand_few_whole_kernel<T, 4>
+                                    : wb::adapter_expand_few_whole_kernel<T, 8>;
         WB_HOST_CUDA(launch(kernel, grid, wb::kAdapterThreads, 0, s, p));
         return WB200_OK;
       }
-    WB_HOST_CUDA(launch(wb::adapter_expand_few_kernel<T, P, TRANS>, grid, wb::kAdapterThreads, size_t(8) * p.Rp * 4, s, p));
+    WB_HOST_CUDA(launch(wb::adapter_expand_few_kernel<T, TRANS>, grid, wb::kAdapterThreads, size_t(8) * p.Rp * 4, s, p));
     return WB200_OK;
   }
   const int steps = p.Rp / 16;
   if (p.io_vec && p.w_vec && p.C % 8 == 0 && (TRANS || steps % 2 == 1 || p.R % 8 == 0))
-    return steps == 1   ? launch_expand_tile<T, P, 1, TRANS, true, true>(p, grid, s)
-           : steps == 2 ? launch_expand_tile<T, P, 2, TRANS, true, true>(p, grid, s)
-           : steps == 4 ? launch_expand_tile<T, P, 4, TRANS, true, true>(p, grid, s)
-                        : launch_expand_tile<T, P, 4, TRANS, true, false>(p, grid, s);
-  return steps == 1 ? launch_expand_tile<T, P, 1, TRANS, false, true>(p, grid, s) : launch_expand_tile<T, P, 2, TRANS, false, false>(p, grid, s);
+    return steps == 1   ? launch_expand_tile<T, 1, TRANS, true, true>(p, grid, s)
+           : steps == 2 ? launch_expand_tile<T, 2, TRANS, true, true>(p, grid, s)
+           : steps == 4 ? launch_expand_tile<T, 4, TRANS, true, true>(p, grid, s)
+                        : launch_expand_tile<T, 4, TRANS, true, false>(p, grid, s);
+  return steps == 1 ? launch_expand_tile<T, 1, TRANS, false, true>(p, grid, s) : launch_expand_tile<T, 2, TRANS, false, false>(p, grid, s);
 }
 
 template <bool TRANS>
 int launch_expand_wide(const AdapterCall& c, const wb::ExpandParams& e) {
   using Cfg = wb::ExpandWide<TRANS>;
   wb::ExpandWideParams p;
-  p.ids = e.ids; p.rows = e.rows; p.C = e.C; p.R = e.R; p.Rp = e.Rp; p.L = e.L;
+  p.ids = e.ids; p.hidden = e.hidden; p.rows = e.rows; p.C = e.C; p.R = e.R; p.Rp = e.Rp; p.L = e.L;
   p.chunks = div_up(e.rows, Cfg::ROWS); p.tiles = div_up(e.C, Cfg::COLS);
   p.has_y = e.y != nullptr; p.in_place = e.out == e.y; p.status = c.status;
   constexpr auto bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   constexpr auto swizzle = CU_TENSOR_MAP_SWIZZLE_128B;
   constexpr auto promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
-  CUtensorMap h, w, y, out;
-  if (int rc = wbhost::tensor_map(&h, e.hidden, 2 * e.Rp, e.rows, 4ull * e.Rp, 64, Cfg::ROWS, bf16, swizzle)) return rc;
+  CUtensorMap w, y, out;
   const unsigned long long inner = TRANS ? e.C : e.R, outer = (unsigned long long)e.L * (TRANS ? e.R : e.C);
   if (int rc = wbhost::tensor_map(&w, e.w, inner, outer, inner * 2, 64, TRANS ? e.Rp : Cfg::COLS, bf16, swizzle)) return rc;
   if (int rc = wbhost::tensor_map(&out, e.out, e.C, e.rows, (unsigned long long)e.ldo * 2, 64, Cfg::ROWS, bf16, swizzle)) return rc;
@@ -218,9 +217,9 @@ int launch_expand_wide(const AdapterCall& c, const wb::ExpandParams& e) {
   if (e.y)
     if (int rc = wbhost::tensor_map(&y, e.y, e.C, e.rows, (unsigned long long)e.ldy * 2, 64, Cfg::ROWS, bf16, swizzle, promotion)) return rc;
   constexpr auto kernel = wb::adapter_expand_wide_kernel<TRANS>;
-  if (int rc = allow_smem<kernel>()) return rc;
+  if (int rc = allow_smem<kernel, Cfg::SMEM_BYTES>()) return rc;
   const dim3 grid(unsigned(std::min<long long>(c.sms, (long long)p.chunks * p.tiles)));
-  WB_HOST_CUDA(launch(kernel, grid, Cfg::THREADS, Cfg::SMEM_BYTES, c.stream, h, w, y, out, p));
+  WB_HOST_CUDA(launch(kernel, grid, Cfg::THREADS, Cfg::SMEM_BYTES, c.stream, w, y, out, p));
   return WB200_OK;
 }
 // The tensor cores take more than 32 ranks where y and out are larger than L2. us of both products with the shrinking one on the tensor cores, rank 64:
@@ -230,7 +229,7 @@ bool wide_expand(const AdapterCall& c, const wb::ExpandParams& p, bool trans, bo
 }
 
 // out = y + ranks onto C columns.
-int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const __nv_bfloat16* hidden, const void* y, long long ldy, void* out, long long ldo, bool f32, int C) {
+int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const float* hidden, const void* y, long long ldy, void* out, long long ldo, bool f32, int C) {
   wb::ExpandParams p;
   p.w = w; p.ids = c.ids; p.hidden = hidden; p.y = y; p.out = out; p.ldy = ldy; p.ldo = ldo;
   p.rows = c.rows; p.C = C; p.R = c.R; p.Rp = c.Rp; p.L = c.L;
@@ -250,8 +249,8 @@ int run_expand(const AdapterCall& c, const __nv_bfloat16* w, bool trans, const _
   const int slices = div_up(C, p.cols_per_cta);
   const dim3 grid(slices, chunks, group_lanes(c.rows, c.L, (long long)chunks * slices));
   using bf16 = __nv_bfloat16;
-  return trans ? launch_expand<bf16, 2, true>(p, few, grid, c.stream)
-         : f32 ? launch_expand<float, 3, false>(p, few, grid, c.stream) : launch_expand<bf16, 2, false>(p, few, grid, c.stream);
+  return trans ? launch_expand<bf16, true>(p, few, grid, c.stream)
+         : f32 ? launch_expand<float, false>(p, few, grid, c.stream) : launch_expand<bf16, false>(p, few, grid, c.stream);
 }
 
 template <int RT>
@@ -443,9 +442,10 @@ cudaError_t adapt_check_record(unsigned long long (&record)[3], bool reset) {
 
 extern "C" {
 
+// One f32 a rank and row; callers that write f32 are asked for half as much again, of which nothing is used (the size that they know).
 size_t wb200_adapters_hidden_bytes(int rows, int rank, int dtype) {
   if (rows <= 0 || rank <= 0) return 0;
-  return size_t(rows) * (dtype == WB200_F32 ? 3 : 2) * rank_pad(rank) * sizeof(__nv_bfloat16);
+  return size_t(rows) * (dtype == WB200_F32 ? 6 : 4) * rank_pad(rank);
 }
 
 int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,
@@ -463,8 +463,8 @@ int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, c
   if (hidden_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters: hidden of %zu bytes needed (got %zu)", need, hidden_bytes);
   int *status = nullptr, sms = 0;
   if (int rc = wbhost::device(&sms, &status)) return rc;
-  const AdapterCall c{{ids, ids_are_int64 != 0}, rows, rank, rank_pad(rank), num_adapters, dtype == WB200_F32 ? 3 : 2, static_cast<cudaStream_t>(stream), status, sms};
-  auto* h = static_cast<__nv_bfloat16*>(hidden);
+  const AdapterCall c{{ids, ids_are_int64 != 0}, rows, rank, rank_pad(rank), num_adapters, static_cast<cudaStream_t>(stream), status, sms};
+  auto* h = static_cast<float*>(hidden);
   if (int rc = run_shrink(c, static_cast<const __nv_bfloat16*>(x), ldx, K, static_cast<const __nv_bfloat16*>(a), false, scale, h)) return rc;
   return run_expand(c, static_cast<const __nv_bfloat16*>(b), false, h, y, ldy, out, ldo, dtype == WB200_F32, N);
 }
@@ -495,7 +495,7 @@ int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, 
   if (db && hidden_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters backward: hidden of %zu bytes needed (got %zu)", need, hidden_bytes);
   int *status = nullptr, sms = 0;
   if (int rc = wbhost::device(&sms, &status)) return rc;
-  const AdapterCall c{{ids, ids_are_int64 != 0}, rows, rank, rank_pad(rank), num_adapters, 2, static_cast<cudaStream_t>(stream), status, sms};
+  const AdapterCall c{{ids, ids_are_int64 != 0}, rows, rank, rank_pad(rank), num_adapters, static_cast<cudaStream_t>(stream), status, sms};
   const auto* gp = static_cast<const __nv_bfloat16*>(g);
   if (N % 8) {
     auto* copy = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(workspace) + (need + 255) / 256 * 256);
@@ -504,13 +504,13 @@ int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, 
     gp = copy;
     ldg = pitch;
   }
-  auto* u = static_cast<__nv_bfloat16*>(workspace);
+  auto* u = static_cast<float*>(workspace);
   if (dx || da)
     if (int rc = run_shrink(c, gp, ldg, N, static_cast<const __nv_bfloat16*>(b), true, scale, u)) return rc;
   if (dx)
     if (int rc = run_expand(c, static_cast<const __nv_bfloat16*>(a), true, u, accumulate_dx ? dx : nullptr, ldd, dx, ldd, false, K)) return rc;
   if (da || db) {
-    wb::OuterSide for_b = {gp, static_cast<const __nv_bfloat16*>(hidden), static_cast<__nv_bfloat16*>(db), ldg, N, 0, 0, 0};
+    wb::OuterSide for_b = {gp, static_cast<const float*>(hidden), static_cast<__nv_bfloat16*>(db), ldg, N, 0, 0, 0};
     wb::OuterSide for_a = {static_cast<const __nv_bfloat16*>(x), u, static_cast<__nv_bfloat16*>(da), ldx, K, 0, 0, 1};
     return run_outer(c, for_b, for_a);
   }

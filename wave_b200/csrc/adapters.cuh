@@ -19,8 +19,9 @@
 // neighbours. Operands whose contraction runs down the rows of memory (B_l^T, A_l^T, the outer products) are transposed by byte permutes of
 // two registers, or by ldmatrix where they come through shared memory.
 //
-// The hidden vector h = s_l A_l x (R numbers a row) stays in f32 until it is stored, as a sum of bf16 parts, which is how the second product takes
-// it: two parts (relative error 2^-17) where the result is rounded to bf16, three (2^-25) where it stays f32.
+// The hidden vector h = s_l A_l x (R numbers a row) is f32, in memory too. The second product takes it as three bf16 parts, 8 bits of its significand
+// each, which add up to it exactly: nothing of an f32 sum is lost on the way, whatever the result's type. Two parts (17 bits) would save a third of
+// that product's MMAs, and show in a result whose y cancels most of what the adapter adds.
 //
 // Dependent launches: shrink and outer touch memory only once the kernel before them is complete. expand is always launched behind a shrink, which lets it
 // begin after that point: what it reads before its own wait (y, w, ids) is older than the shrink, and it writes nothing before it.
@@ -208,15 +209,19 @@ __device__ __forceinline__ uint32_t piece(int row, int c) {
   return uint32_t((row * PIECES + (c ^ ((row / PER_LINE) & (PIECES >= 8 ? 7 : PIECES - 1)))) * 16);
 }
 
-// P bf16 values whose sum is v (each the rounding of what the ones before it leave).
-template <int P>
-__device__ __forceinline__ void split_bf16(float v, __nv_bfloat16 (&part)[P]) {
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    part[i] = __float2bfloat16_rn(v);
-    const float rest = v - __bfloat162float(part[i]);
-    v = fabsf(rest) < INFINITY ? rest : 0.f;  // an infinity or NaN is whole in its first part
-  }
+// Two f32 values as three pairs of bf16 that add up to them: a part is the upper half of what the ones before it leave, the next 8 bits of the
+// significand, so that no part is rounded. An infinity or NaN is whole in its first part.
+constexpr int kParts = 3;
+__device__ __forceinline__ float behind_first(float v) {
+  const float rest = v - __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+  return fabsf(v) < INFINITY ? rest : 0.f;
+}
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&part)[kParts]) {
+  part[0] = high_halves(__float_as_uint(a), __float_as_uint(b));
+  const float a1 = behind_first(a), b1 = behind_first(b);
+  part[1] = high_halves(__float_as_uint(a1), __float_as_uint(b1));
+  const float a2 = a1 - __uint_as_float(__float_as_uint(a1) & 0xffff0000u), b2 = b1 - __uint_as_float(__float_as_uint(b1) & 0xffff0000u);
+  part[2] = high_halves(__float_as_uint(a2), __float_as_uint(b2));
 }
 
 struct ShrinkParams {
@@ -224,14 +229,14 @@ struct ShrinkParams {
   const __nv_bfloat16* w;  // A_l [L][R][K], or (TRANS) B_l [L][K][R]
   Ids ids;
   const float* scale;      // [L], or null
-  __nv_bfloat16* hidden;   // [rows][parts][Rp]
+  float* hidden;           // [rows][Rp]
   long long ldx;
-  int rows, K, R, Rp, L, parts, split_k;
+  int rows, K, R, Rp, L, split_k;
   int x_vec, w_vec;        // 16-byte loads of x; vector loads of w
 };
 
 // A split's sums of `count` rows and COLS ranks are in `sums` ([..][COLS + 1]) of every CTA of the cluster: this CTA adds up its share of the
-// rows over the splits, in their order, and writes the scaled bf16 parts. By its place, a row's: number in `sums`, row of x, scale.
+// rows over the splits, in their order, and writes them, scaled. By its place, a row's: number in `sums`, row of x, scale.
 template <int COLS, typename SumRow, typename RowOf, typename ScaleOf>
 __device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums, SumRow sum_row, RowOf row_of, ScaleOf scale_of, int count, int n0) {
   __syncthreads();
@@ -255,12 +260,7 @@ __device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums
 #pragma unroll
       for (int s = 0; s < 8; ++s) v += part[s];
     }
-    __nv_bfloat16 part[3];
-    split_bf16<3>(n0 + col < p.R ? v * scale_of(row) : 0.f, part);  // (an infinity of x would be a NaN in the ranks behind the last)
-    __nv_bfloat16* dst = p.hidden + (long long)row_of(row) * p.parts * p.Rp + n0 + col;
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (i < p.parts) dst[i * p.Rp] = part[i];
+    p.hidden[(long long)row_of(row) * p.Rp + n0 + col] = n0 + col < p.R ? v * scale_of(row) : 0.f;  // (an infinity of x would be a NaN in the ranks behind the last)
   }
   if (splits > 1) {  // nobody overwrites what others still read
     cluster_arrive();
@@ -387,12 +387,7 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
           if (n0 + col >= p.Rp) continue;
           float v = 0.f;
           for (int i = 0; i < splits; ++i) v += sums[i * share + mine][col];
-          __nv_bfloat16 part[3];
-          split_bf16<3>(n0 + col < p.R ? v * scale : 0.f, part);
-          __nv_bfloat16* dst = p.hidden + (long long)(row0 + nth_bit(group.rows, first + row)) * p.parts * p.Rp + n0 + col;
-#pragma unroll
-          for (int i = 0; i < 3; ++i)
-            if (i < p.parts) dst[i * p.Rp] = part[i];
+          p.hidden[(long long)(row0 + nth_bit(group.rows, first + row)) * p.Rp + n0 + col] = n0 + col < p.R ? v * scale : 0.f;
         }
       }
     }
@@ -567,7 +562,7 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
   }
 }
 
-// The same for many aligned rows and K a multiple of 64, on the tensor cores: the 128 rows of a chunk x N ranks of two adapters at a time, an accumulator
+// The same for many aligned rows and K a multiple of 64, on the tensor cores: the 128 rows of a chunk x N ranks of two adapters at a time, accumulators
 // of N columns for each; a row takes the sums of its own. Rows come as one tile, w as one a adapter: A_l's rows K-major, B_l's (TRANS) as they
 // lie, with the ranks in an MN-major operand. Ranks behind the last are the next adapter's or zeros and are not kept. No load passes through
 // registers, w is read once for 128 rows, and a chunk in which one sequence ends and another begins takes a third longer than others.
@@ -580,8 +575,12 @@ struct ShrinkWide {
   // Two CTAs to an SM, and beside them none of the library's other kernels that take tensor memory (they ask for 160 KB or more): a CTA holds its columns
   // while it waits for its cluster, so that one that waited for columns of another kernel's, in another stream, might wait for good.
   static constexpr int SMEM_BYTES = 97 * 1024;           // the sums reuse the stages
-  static constexpr int TMEM_COLS = N < 32 ? 64 : 2 * N;  // (32 columns are read at a time)
+  // Accumulators of an adapter, taken in turn by the stages: an MMA drops the bits of its f32 sum that do not fit, always towards zero, and 2048 k in one
+  // accumulator shrink by 1.8e-6 of themselves where an f32 sum with rounding is 1e-6 off at random.
+  static constexpr int ACCS = N == 64 ? 2 : 4;
+  static constexpr int TMEM_COLS = 256;
   static_assert(STAGES * STAGE_BYTES + 1024 <= SMEM_BYTES && 2 * TMEM_COLS <= 512, "stages; columns of two CTAs");
+  static_assert((2 * ACCS - 1) * N + (N < 32 ? 32 : N) <= TMEM_COLS, "accumulators of two adapters, of which 32 columns are read at a time");
   static_assert(ROWS * (N + 1) * 4 <= STAGES * STAGE_BYTES && ROWS <= kAdapterThreads, "sums; a thread per row where rows are grouped");
 };
 template <int N, bool TRANS>
@@ -655,7 +654,8 @@ adapter_shrink_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
               const uint64_t b = TRANS ? make_desc_mn_sw128(w_at, 64 * 128) : make_desc_k_sw128(w_at);
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                mma_f16<1>(tmem + i * N, a + uint64_t(k * 2), b + uint64_t(k * (TRANS ? 2048 >> 4 : 2)), idesc, (s > 0 || k > 0) ? 1u : 0u);
+                mma_f16<1>(tmem + (i * Cfg::ACCS + s % Cfg::ACCS) * N, a + uint64_t(k * 2), b + uint64_t(k * (TRANS ? 2048 >> 4 : 2)), idesc,
+                           (s >= Cfg::ACCS || k > 0) ? 1u : 0u);
             }
             tc_commit<1>(empty(stage));
             if (s == steps - 1) tc_commit<1>(acc_full);
@@ -673,15 +673,18 @@ adapter_shrink_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
       const int row = (warp & 3) * 32 + lane, c = (warp >> 2) * 32;
       if (c < N) {
         for (int i = 0; i < ng; ++i) {
-          uint32_t v[32];
-          if (steps > 0) {
-            tmem_ld_32x32(tmem + (uint32_t((warp & 3) * 32) << 16) + i * N + c, v);
+          float sum[32] = {};
+          for (int a = 0; a < min(steps, Cfg::ACCS); ++a) {
+            uint32_t v[32];
+            tmem_ld_32x32(tmem + (uint32_t((warp & 3) * 32) << 16) + (i * Cfg::ACCS + a) * N + c, v);
             tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[j] += __uint_as_float(v[j]);
           }
           if (groups.id[row] == l[i])
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (c + j < N) sums[row * (N + 1) + c + j] = steps > 0 ? __uint_as_float(v[j]) : 0.f;
+              if (c + j < N) sums[row * (N + 1) + c + j] = sum[j];
         }
       }
       tc_fence_before_sync();
@@ -704,7 +707,7 @@ adapter_shrink_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
 struct ExpandParams {
   const __nv_bfloat16* w;       // B_l [L][C][R], or (TRANS) A_l [L][R][C]
   Ids ids;
-  const __nv_bfloat16* hidden;  // [rows][parts][Rp]
+  const float* hidden;          // [rows][Rp]
   const void* y;                // null: zeros
   void* out;
   long long ldy, ldo;
@@ -774,7 +777,7 @@ __device__ __forceinline__ void expand_rest(const ExpandParams& p, long long row
 // Few rows: a thread has two columns, with 16 of their ranks in registers at a time, and walks the rows of a group. f32 FMAs: the
 // products are few, the loads of w_l (whole sectors, all of a thread's in flight) are what counts. For ranks and alignments that the next kernel does not
 // take, and for the transposed product of the backward pass.
-template <typename T, int P, bool TRANS>
+template <typename T, bool TRANS>
 __global__ void __launch_bounds__(kAdapterThreads)
 adapter_expand_few_kernel(const ExpandParams p) {
   constexpr int ROWS = 8;
@@ -861,11 +864,7 @@ adapter_expand_few_kernel(const ExpandParams p) {
             int from = row[0];
 #pragma unroll
             for (int i = 1; i < ROWS; ++i) from = in == i ? row[i] : from;
-            const __nv_bfloat16* h = p.hidden + (long long)from * P * p.Rp + r;
-            float v = 0.f;
-#pragma unroll
-            for (int i = P - 1; i >= 0; --i) v += __bfloat162float(h[i * p.Rp]);
-            hs[e] = v;
+            hs[e] = p.hidden[(long long)from * p.Rp + r];
           }
           __syncthreads();
         }
@@ -911,7 +910,7 @@ adapter_expand_few_kernel(const ExpandParams p) {
 // Both products of 32 rows and some 25 of 64 adapters, K = 4096, N = 14336, rank 16: 12.2 us (17 MB; with two columns a thread 13.7), of one row
 // with N = 4096 5.0 us (6.0).
 __host__ __device__ constexpr int few_whole_steps(int pieces) { return pieces > 4 ? pieces : 4; }
-template <typename T, int P, int PIECES>
+template <typename T, int PIECES>
 __global__ void __launch_bounds__(kAdapterThreads, 3)
 adapter_expand_few_whole_kernel(const ExpandParams p) {
   constexpr int STEPS = few_whole_steps(PIECES), ROWS = 2, KEPT = STEPS / PIECES, COLS = kAdapterThreads / PIECES;  // COLS: of a step
@@ -951,14 +950,8 @@ adapter_expand_few_whole_kernel(const ExpandParams p) {
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         if (i >= count) break;
-        float h[8] = {};
-#pragma unroll
-        for (int q = P - 1; q >= 0; --q) {
-          float v[8];
-          read8<__nv_bfloat16>(p.hidden + (row[i] * (long long)P + q) * p.Rp + pc * 8, true, 8, v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) h[j] += v[j];
-        }
+        float h[8];
+        read8<float>(p.hidden + (long long)row[i] * p.Rp + pc * 8, true, 8, h);
 #pragma unroll
         for (int u = 0; u < STEPS; ++u) {
           float v[8], sum = 0.f;
@@ -984,8 +977,8 @@ adapter_expand_few_whole_kernel(const ExpandParams p) {
 
 // Elements between the hidden vectors of rows in shared memory: a distance at which the loads that move together fall into different banks, those of
 // four rows of 8-byte pieces, or (PAIRED) of two rows of 16-byte pieces.
-__host__ __device__ constexpr int expand_pitch(int parts, int Rp, bool paired) {
-  const int words = parts * Rp / 2;
+__host__ __device__ constexpr int expand_pitch(int Rp, bool paired) {
+  const int words = kParts * Rp / 2;
   return paired ? 2 * (words + (words % 32 == 16 ? 0 : 16)) : 2 * (words + (words % 16 == 8 ? 0 : 8));
 }
 
@@ -1002,7 +995,7 @@ __host__ __device__ constexpr int expand_ring_bytes(int esz, bool exact) { retur
 // Bound by its start-up and HBM at rank 16 (4096 x 4096 14 us); at rank 64 by shared memory (59 %) and the MMA pipe (51 %) between them, at two CTAs of
 // 128 registers a thread: 8192 x 8192 63 us (268 MB of y and out, 4.3 TB/s). With the batch ahead in registers instead of the ring 76 us; w of the
 // next columns through the ring too: no faster.
-template <typename T, int P, int QN, bool TRANS, bool FAST, bool EXACT>
+template <typename T, int QN, bool TRANS, bool FAST, bool EXACT>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_expand_tile_kernel(const ExpandParams p) {
   const int Rp = EXACT ? 16 * QN : p.Rp;         // EXACT: known when compiled, and with it every address in shared memory
@@ -1016,10 +1009,10 @@ adapter_expand_tile_kernel(const ExpandParams p) {
   __shared__ uint32_t y_off[FAST ? 1 : kChunkRows], out_off[FAST ? 1 : kChunkRows];  // of a group's rows, in bytes; all ones: none
   __shared__ float staged[FAST ? 1 : kAdapterWarps][FAST ? 1 : 16][FAST ? 1 : kExpandCols + 1];
   // FAST: a ring of batches of y, in which every thread has 16-byte slots of its own (no barrier): [DEPTH][MB][2][RAW][threads]
-  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem + (FAST ? DEPTH * SLOT : 0));  // [64][P][Rp], rows `pitch` apart
+  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(smem + (FAST ? DEPTH * SLOT : 0));  // [64][kParts][Rp], rows `pitch` apart
   // A lane's ranks in two steps of 16: eight neighbours (PAIRED: one 16-byte piece serves both steps), or four of each
   constexpr bool PAIRED = FAST && EXACT && QN % 2 == 0;
-  const int pitch = expand_pitch(P, Rp, PAIRED);
+  const int pitch = expand_pitch(Rp, PAIRED);
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row0 = blockIdx.y * kChunkRows;
@@ -1188,14 +1181,26 @@ adapter_expand_tile_kernel(const ExpandParams p) {
     if (!waited) pdl_wait();  // for the hidden vectors; y and w are complete before the kernel that makes those starts
     waited = true;
     __syncthreads();
-    const int pieces = P * Rp / 8;
-    for (int e = threadIdx.x; e < mtiles * 16 * pieces; e += kAdapterThreads) {
-      const int r = e / pieces, c = e - r * pieces;
-      const int in = r < count ? row0 + groups.order[first + r] : row0;
-      cp_async16(smem_u32(hs + r * pitch + c * 8), p.hidden + (long long)in * P * Rp + c * 8, r < count);
+    const int quads = Rp / 4;  // four ranks of a row at a time, the loads of four such pieces in flight
+    for (int e0 = threadIdx.x; e0 < mtiles * 16 * quads; e0 += 4 * kAdapterThreads) {
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = e0 + i * kAdapterThreads, r = e / quads;
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < count) v[i] = *reinterpret_cast<const float4*>(p.hidden + (long long)(row0 + groups.order[first + r]) * Rp + (e - r * quads) * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = e0 + i * kAdapterThreads, r = e / quads;
+        if (r >= mtiles * 16) break;
+        uint32_t lo[kParts], hi[kParts];
+        split_pair(v[i].x, v[i].y, lo);
+        split_pair(v[i].z, v[i].w, hi);
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) *reinterpret_cast<uint2*>(hs + r * pitch + q * Rp + (e - r * quads) * 4) = make_uint2(lo[q], hi[q]);
+      }
     }
-    cp_async_commit();
-    cp_async_wait<0>();
     __syncthreads();
 #pragma unroll 1
     for (int c0 = c_first; c0 < c_end; c0 += STEP) {
@@ -1245,7 +1250,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
               for (int q = 0; q < QN; q += 2) {
                 const __nv_bfloat16* at = hs + (m * 16 + g) * pitch + q * 16 + 8 * t;
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
+                for (int i = 0; i < kParts; ++i) {
                   const uint4 lo = *reinterpret_cast<const uint4*>(at + i * Rp);
                   const uint4 hi = *reinterpret_cast<const uint4*>(at + 8 * pitch + i * Rp);
 #pragma unroll
@@ -1261,7 +1266,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
               if (q0 + q >= steps) break;
               const __nv_bfloat16* at = hs + (m * 16 + g) * pitch + (q0 + q) * 16 + 4 * t;
 #pragma unroll
-              for (int i = 0; i < P; ++i) {
+              for (int i = 0; i < kParts; ++i) {
                 const uint2 lo = *reinterpret_cast<const uint2*>(at + i * Rp);
                 const uint2 hi = *reinterpret_cast<const uint2*>(at + 8 * pitch + i * Rp);
 #pragma unroll
@@ -1320,22 +1325,24 @@ adapter_expand_tile_kernel(const ExpandParams p) {
       if (groups.id[r] < 0) expand_rest<T>(p, row0 + r, c_begin + lane * 8, c_end, 256);
 }
 
-// The same for many aligned bf16 rows and ranks up to 64, on the tensor cores: 128 rows of a chunk x 128 columns, both parts of the hidden vectors against the
-// same tile of w (A operand: the chunk's hidden vectors, brought once; B: B_l's rows K-major, or (TRANS) A_l's as they lie, MN-major). Two adapters at
-// a time have accumulators, a row takes the sums of its own; y comes by the copy engine, is added to in shared memory and leaves from there.
+// The same for many aligned bf16 rows and ranks up to 64, on the tensor cores: 128 rows of a chunk x 128 columns, the three parts of the hidden vectors against
+// the same tile of w (A operand: the chunk's hidden vectors, split into parts once, by the warps that later read the sums; B: B_l's rows K-major, or
+// (TRANS) A_l's as they lie, MN-major). Two adapters at a time have accumulators, a row takes the sums of its own; y comes by the copy engine, is added to in shared memory and leaves from there.
 // One CTA per SM works through its share of all (chunk, 128 columns) in order. 8192 x 8192 at rank 64 50 us for one sequence (268 MB, 5.4 TB/s), 57 for
 // seven; the mma.sync form 63 to 70. Bound by HBM, and below 8192 x 4096 by the start-up of one large CTA per SM.
 //   warp 0: y and w by TMA; warp 1: tcgen05.mma; warps 2 .. 9: sums, thread = row, 64 columns; warp 10: out by TMA
 template <bool TRANS>
 struct ExpandWide {
-  static constexpr int ROWS = 128, COLS = 128, A_BYTES = 2 * ROWS * 128, B_BYTES = COLS * 128, Y_BYTES = ROWS * COLS * 2;
+  static constexpr int ROWS = 128, COLS = 128, A_BYTES = kParts * ROWS * 128, B_BYTES = COLS * 128, Y_BYTES = ROWS * COLS * 2;
   static constexpr int B_STAGES = 4, Y_STAGES = 3, EPILOGUE_WARPS = 8, THREADS = (3 + EPILOGUE_WARPS) * 32;
   static constexpr int B_BASE = A_BYTES, Y_BASE = B_BASE + B_STAGES * B_BYTES;
   static constexpr int SMEM_BYTES = Y_BASE + Y_STAGES * Y_BYTES + 1024;
   static constexpr int TMEM_COLS = 512;  // two buffers of two adapters
+  static_assert(EPILOGUE_WARPS * 32 == 2 * ROWS, "two threads split a row's hidden vector");
 };
 struct ExpandWideParams {
   Ids ids;
+  const float* hidden;  // [rows][Rp]
   int rows, C, R, Rp, L, chunks, tiles;
   int has_y, in_place;
   int* status;
@@ -1384,8 +1391,8 @@ __device__ __forceinline__ void wide_share(WideShares& s, const ExpandWideParams
 }
 template <bool TRANS>
 __global__ void __launch_bounds__(ExpandWide<TRANS>::THREADS, 1)
-adapter_expand_wide_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y,
-                           const __grid_constant__ CUtensorMap map_out, const ExpandWideParams p) {
+adapter_expand_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_out,
+                           const ExpandWideParams p) {
   using Cfg = ExpandWide<TRANS>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ RowGroupsOf<Cfg::ROWS> groups;
@@ -1405,10 +1412,9 @@ adapter_expand_wide_kernel(const __grid_constant__ CUtensorMap map_h, const __gr
   auto out_full = [&](uint32_t i) { return smem_u32(bars + 5 + 2 * Cfg::B_STAGES + 2 * Cfg::Y_STAGES + i); };
   WaitCtx ctx{&abort_word, p.status};
   if (threadIdx.x == 0) {
-    for (int i = 0; i < BARS; ++i) mbar_init(smem_u32(bars + i), i == 3 || i == 4 || i >= BARS - Cfg::Y_STAGES ? Cfg::EPILOGUE_WARPS : 1);
+    for (int i = 0; i < BARS; ++i) mbar_init(smem_u32(bars + i), i == 0 || i == 3 || i == 4 || i >= BARS - Cfg::Y_STAGES ? Cfg::EPILOGUE_WARPS : 1);
     abort_word = 0u;
     fence_mbar_init();
-    prefetch_tensormap(&map_h);
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_y);
     prefetch_tensormap(&map_out);
@@ -1435,12 +1441,6 @@ adapter_expand_wide_kernel(const __grid_constant__ CUtensorMap map_h, const __gr
     const int ngroups = group_rows(groups, p.ids, row0, p.rows, p.L);
     if (ngroups == 0 && p.in_place) continue;
     if (warp == 0) {
-      if (ngroups > 0 && elect_one()) {
-        mbar_expect_tx(a_full, Cfg::A_BYTES);
-        tma_load_2d<1>(base, &map_h, 0, row0, a_full);
-        tma_load_2d<1>(base + Cfg::A_BYTES / 2, &map_h, p.Rp, row0, a_full);
-      }
-      __syncwarp();
       for (int t = t0; t < t1; ++t) {
         const int c0 = t * Cfg::COLS;
         const int halves = c0 + 64 < p.C ? 2 : 1;
@@ -1487,8 +1487,8 @@ adapter_expand_wide_kernel(const __grid_constant__ CUtensorMap map_h, const __gr
             if (elect_one()) {
               const uint32_t at = base + Cfg::B_BASE + bs * Cfg::B_BYTES;
               const uint64_t b = TRANS ? make_desc_mn_sw128(at, Cfg::B_BYTES / 2) : make_desc_k_sw128(at);
-              for (int part = 0; part < 2; ++part) {
-                const uint64_t a = make_desc_k_sw128(base + part * (Cfg::A_BYTES / 2));
+              for (int part = 0; part < kParts; ++part) {
+                const uint64_t a = make_desc_k_sw128(base + part * (Cfg::A_BYTES / kParts));
                 for (int k = 0; k < ksteps; ++k)
                   mma_f16<1>(tmem + (acc * 2 + i) * Cfg::COLS, a + uint64_t(k * 2), b + uint64_t(k * (TRANS ? 2048 >> 4 : 2)), idesc, (part > 0 || k > 0) ? 1u : 0u);
               }
@@ -1503,6 +1503,27 @@ adapter_expand_wide_kernel(const __grid_constant__ CUtensorMap map_h, const __gr
         }
     } else if (warp < 2 + Cfg::EPILOGUE_WARPS) {
       const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane, id = groups.id[row];
+      if (ngroups > 0) {  // the chunk's hidden vectors, pieces of 8 ranks (every MMA on those of the chunk before is complete: its sums were waited for)
+        const int r = (int(threadIdx.x) - 64) >> 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = 2 * i + (threadIdx.x & 1);
+          if (c * 8 >= p.Rp) break;
+          float v[8] = {};
+          if (row0 + r < p.rows) read8<float>(p.hidden + (long long)(row0 + r) * p.Rp + c * 8, true, 8, v);
+          uint32_t part[4][kParts];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) split_pair(v[2 * j], v[2 * j + 1], part[j]);
+#pragma unroll
+          for (int q = 0; q < kParts; ++q)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + q * (Cfg::A_BYTES / kParts) + r * 128 + ((c ^ (r & 7)) << 4)), "r"(part[0][q]), "r"(part[1][q]),
+                         "r"(part[2][q]), "r"(part[3][q])
+                         : "memory");
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(a_full);
+      }
       for (int t = t0; t < t1; ++t) {
         const int c0 = t * Cfg::COLS;
         mbar_wait(p.has_y ? y_full(ys) : y_empty(ys), p.has_y ? y_phase : y_phase ^ 1u, ctx, WB_DEV_TIMEOUT_EPILOGUE);
@@ -1586,7 +1607,7 @@ __global__ void __launch_bounds__(256) adapter_align_kernel(const __nv_bfloat16*
 
 struct OuterSide {
   const __nv_bfloat16* z;       // [rows, C], pitch ldz
-  const __nv_bfloat16* hidden;  // [rows][2][Rp]
+  const float* hidden;          // [rows][Rp]
   __nv_bfloat16* out;           // [L][C][R], or rank-major [L][R][C]
   long long ldz;
   int C, blocks, vec, rank_major;
@@ -1600,19 +1621,28 @@ struct OuterParams {
 // out_l[c, r] = sum over the rows t of adapter l of z[t, c] hidden[t, r]: B's gradient from g and A x, A's from x and B^T g.
 // Grid (row splits = one cluster, blocks of 128 columns of both sides, adapters). A CTA picks the rows of its adapter out of its range of ids,
 // in order, and adds up their outer products with MMAs whose k runs over the rows, from a ring of 64 rows a stage. The splits are
-// added up through distributed shared memory, in their order. Both sums of a backward pass are one launch: 4096 rows, 4096 + 4096 columns, rank 16
-// 19 us (67 MB, 3.5 TB/s); bound by the start-up (ids, list, first loads) and the barriers of the ring.
+// added up through distributed shared memory, in their order. An MMA drops the bits of its f32 sum that do not fit, always towards zero, so that the
+// products of 16 rows are summed by it and added to the others with rounding: over thousands of rows the sums would shrink by 3e-6 of themselves, several
+// times what rounding costs. The warps stand side by side over the ranks first and over the columns where there are fewer ranks, so that a hidden number
+// is split into its bf16 parts by as few of them as possible. Both sums of a backward pass are one launch: 4096 rows, 4096 + 4096 columns, rank 16
+// 25 us (67 MB, 2.7 TB/s); bound by the start-up (ids, list, first loads), the barriers of the ring and the MMAs: a part takes 2 us of it.
 constexpr int kOuterCols = 128;
 constexpr int kOuterSegment = 4096;  // ids looked through at a time
 template <int RT>
 struct OuterTile {
-  static constexpr int P = 2, COLS = RT * 8;
-  static constexpr int Z_BYTES = kChunkRows * kOuterCols * 2, H_BYTES = kChunkRows * P * COLS * 2, STAGE_BYTES = Z_BYTES + H_BYTES;
+  static constexpr int COLS = RT * 8;                                                     // ranks at a time
+  static constexpr int WARPS_R = RT < 4 ? RT : 4, OCTETS = RT / WARPS_R;                  // warps over the ranks, eights of ranks of each
+  static constexpr int WARPS_C = 4 / WARPS_R, MT = kOuterCols / 16 / WARPS_C;             // warps over the columns, sixteens of columns of each
+  static constexpr int H_PIECES = COLS / 4;                                               // 16-byte pieces of a row of hidden numbers
+  static constexpr int Z_BYTES = kChunkRows * kOuterCols * 2, H_BYTES = kChunkRows * COLS * 4, STAGE_BYTES = Z_BYTES + H_BYTES;
   static constexpr int STAGES = RT == 8 ? 3 : 4;
   static constexpr int SUM_PITCH = COLS + 4;  // 16-byte pieces of 8 neighbouring columns in different banks
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int SMEM_BYTES = RING_BYTES + kOuterSegment * 4;
   static_assert(2 * kOuterCols * SUM_PITCH * 4 <= RING_BYTES, "sums of the two halves of the rows");
+  static_assert(kChunkRows * H_PIECES % kAdapterThreads == 0, "whole pieces of hidden numbers to a thread");
+  // Place of 16-byte piece c of a row of hidden numbers: four lanes that read rows 2 apart meet different banks.
+  __device__ static __forceinline__ uint32_t hidden_piece(int row, int c) { return uint32_t(row * H_PIECES + (c ^ ((((row >> 1) & 3) << 1) & (H_PIECES - 1)))) * 16; }
 };
 
 __device__ __forceinline__ void zero_fill(__nv_bfloat16* p, int n, int thread, int threads) {
@@ -1626,7 +1656,7 @@ template <int RT>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_outer_kernel(const OuterParams p) {
   using Cfg = OuterTile<RT>;
-  constexpr int STAGES = Cfg::STAGES, P = Cfg::P, COLS = Cfg::COLS;
+  constexpr int STAGES = Cfg::STAGES, COLS = Cfg::COLS, OCTETS = Cfg::OCTETS, MT = Cfg::MT;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int found[kAdapterWarps + 1];
   int* list = reinterpret_cast<int*>(smem + Cfg::RING_BYTES);
@@ -1641,10 +1671,10 @@ adapter_outer_kernel(const OuterParams p) {
   const int l = blockIdx.z, splits = gridDim.x, split = blockIdx.x;
   const Ids& ids = p.ids;
   const int row_begin = int((long long)p.rows * split / splits), row_end = int((long long)p.rows * (split + 1) / splits);
-  const int wc = warp & 3, wk = warp >> 2;  // 32 columns, 32 of a stage's 64 rows
+  const int wr = (warp & 3) % Cfg::WARPS_R, wc = (warp & 3) / Cfg::WARPS_R, wk = warp >> 2;  // ranks, columns, 32 of a stage's 64 rows
   bool any = false;
   for (int n0 = 0; n0 < p.Rp; n0 += COLS) {
-    float acc[2][RT][4] = {};
+    float acc[MT][OCTETS][4] = {};
     for (int seg = row_begin; seg < row_end; seg += kOuterSegment) {
       // the segment's rows of this adapter, in order: a warp looks through a run of ids, then knows how many the warps before it found
       const int seg_end = min(row_end, seg + kOuterSegment);
@@ -1681,24 +1711,23 @@ adapter_outer_kernel(const OuterParams p) {
       const int steps = (total + kChunkRows - 1) / kChunkRows;
       any |= total > 0;
       // A thread brings the same pieces of every stage: column piece tid % 16 of rows tid / 16 + 16 i of z, and HN pieces of the hidden vectors
-      constexpr int ZN = kChunkRows * (kOuterCols / 8) / kAdapterThreads, HN = (kChunkRows * P * RT + kAdapterThreads - 1) / kAdapterThreads;
+      constexpr int ZN = kChunkRows * (kOuterCols / 8) / kAdapterThreads, HN = kChunkRows * Cfg::H_PIECES / kAdapterThreads;
       const int zr = tid >> 4, zc = tid & 15;
       const int z_valid = min(8, side.C - c0 - zc * 8);
       const __nv_bfloat16* z_at = side.z + c0 + zc * 8;
       int next = 0;         // place in the list of the first row of the next load
       uint32_t to = base;   // its stage
       const bool fast = side.vec && c0 + kOuterCols <= side.C && n0 + COLS <= p.Rp;
-      const int hr = tid / (P * RT), hc = tid % (P * RT);
-      const __nv_bfloat16* h_at = side.hidden + (hc / RT) * p.Rp + n0 + (hc % RT) * 8;
-      constexpr int H_ROWS = kAdapterThreads / (P * RT);  // between the pieces of a thread
+      const int hr = tid / Cfg::H_PIECES, hc = tid % Cfg::H_PIECES;
+      const float* h_at = side.hidden + n0 + hc * 4;
+      constexpr int H_ROWS = kAdapterThreads / Cfg::H_PIECES;  // between the pieces of a thread
       auto load = [&]() {
         if (fast && next + kChunkRows <= total) {  // whole pieces of 64 rows
 #pragma unroll
           for (int i = 0; i < ZN; ++i) cp_async16(to + piece<16>(zr + 16 * i, zc), z_at + list[next + zr + 16 * i] * side.ldz, true);
 #pragma unroll
           for (int i = 0; i < HN; ++i)
-            if (hr + i * H_ROWS < kChunkRows)
-              cp_async16(to + Cfg::Z_BYTES + piece<P * RT>(hr + i * H_ROWS, hc), h_at + (long long)list[next + hr + i * H_ROWS] * (P * p.Rp), true);
+            cp_async16(to + Cfg::Z_BYTES + Cfg::hidden_piece(hr + i * H_ROWS, hc), h_at + (long long)list[next + hr + i * H_ROWS] * p.Rp, true);
           cp_async_commit();
           next += kChunkRows;
           to = to == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : to + Cfg::STAGE_BYTES;
@@ -1712,12 +1741,9 @@ adapter_outer_kernel(const OuterParams p) {
         }
 #pragma unroll
         for (int i = 0; i < HN; ++i) {
-          const int e = tid + i * kAdapterThreads;
-          if (kChunkRows * P * RT < kAdapterThreads && e >= kChunkRows * P * RT) break;
-          const int r = e / (P * RT), c = e % (P * RT);  // part c / RT, ranks 8 (c % RT) ..
-          const int rank = n0 + (c % RT) * 8;
-          const bool real = next + r < total && rank < p.Rp;
-          cp_async16(to + Cfg::Z_BYTES + piece<P * RT>(r, c), real ? side.hidden + ((long long)list[next + r] * P + c / RT) * p.Rp + rank : side.hidden, real);
+          const int r = hr + i * H_ROWS;
+          const bool real = next + r < total && n0 + hc * 4 < p.Rp;
+          cp_async16(to + Cfg::Z_BYTES + Cfg::hidden_piece(r, hc), real ? h_at + (long long)list[next + r] * p.Rp : side.hidden, real);
         }
         cp_async_commit();
         next += kChunkRows;
@@ -1738,22 +1764,30 @@ adapter_outer_kernel(const OuterParams p) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int r = 32 * wk + 16 * k;
-          if (step * kChunkRows + r >= total) break;
-          uint32_t za[2][4];  // matrices (k 0-7, c 0-7), (k 0-7, c 8-15), (k 8-15, c 0-7), (k 8-15, c 8-15)
+          // the lane's four rows of a rank (a column of the second operand): 2 t, 2 t + 1 and the same eight rows on
+          uint32_t hf[OCTETS][2][kParts];
+          const unsigned char* h_rows = smem + (from - base) + Cfg::Z_BYTES + (r + 2 * t) * (COLS * 4);
 #pragma unroll
-          for (int m = 0; m < 2; ++m) ldsm4_trans(from + piece<16>(r + (in & 7) + half * 8, 4 * wc + 2 * m + (in >> 3)), za[m]);
+          for (int o = 0; o < OCTETS; ++o) {
+            const int rank = (wr * OCTETS + o) * 8 + g;
+            const unsigned char* at = h_rows + (((rank >> 2) ^ ((2 * t) & (Cfg::H_PIECES - 1))) << 4) + (rank & 3) * 4;  // (hidden_piece of each of them)
 #pragma unroll
-          for (int q = 0; q < P; ++q)
+            for (int h = 0; h < 2; ++h)
+              split_pair(*reinterpret_cast<const float*>(at + h * (COLS * 32)), *reinterpret_cast<const float*>(at + h * (COLS * 32) + COLS * 4), hf[o][h]);
+          }
 #pragma unroll
-            for (int i = 0; i < RT; i += 2) {
-              uint32_t hf[4];
-              ldsm4_trans(from + Cfg::Z_BYTES + piece<P * RT>(r + in, q * RT + i + half), hf);
+          for (int m = 0; m < MT; ++m) {
+            uint32_t za[4];  // matrices (k 0-7, c 0-7), (k 0-7, c 8-15), (k 8-15, c 0-7), (k 8-15, c 8-15)
+            ldsm4_trans(from + piece<16>(r + (in & 7) + half * 8, 2 * (wc * MT + m) + (in >> 3)), za);
 #pragma unroll
-              for (int m = 0; m < 2; ++m) {
-                mma_bf16(acc[m][i], za[m][0], za[m][1], za[m][2], za[m][3], hf[0], hf[1]);
-                mma_bf16(acc[m][i + 1], za[m][0], za[m][1], za[m][2], za[m][3], hf[2], hf[3]);
-              }
+            for (int o = 0; o < OCTETS; ++o) {
+              float sum[4] = {};
+#pragma unroll
+              for (int q = 0; q < kParts; ++q) mma_bf16(sum, za[0], za[1], za[2], za[3], hf[o][0][q], hf[o][1][q]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[m][o][e] += sum[e];
             }
+          }
         }
         from = from == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : from + Cfg::STAGE_BYTES;
       }
@@ -1771,12 +1805,12 @@ adapter_outer_kernel(const OuterParams p) {
     __syncthreads();
     float* sums = reinterpret_cast<float*>(smem);  // [2 halves of the rows][128 columns][SUM_PITCH]
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
+      for (int o = 0; o < OCTETS; ++o)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          sums[(wk * kOuterCols + 32 * wc + 16 * m + g + (e >> 1) * 8) * Cfg::SUM_PITCH + i * 8 + 2 * t + (e & 1)] = acc[m][i][e];
+          sums[(wk * kOuterCols + 16 * (wc * MT + m) + g + (e >> 1) * 8) * Cfg::SUM_PITCH + (wr * OCTETS + o) * 8 + 2 * t + (e & 1)] = acc[m][o][e];
     __syncthreads();
     constexpr int QUADS = COLS / 4;  // four ranks of a column at a time
     float4* quads = reinterpret_cast<float4*>(sums);

@@ -84,10 +84,10 @@ variable_list once(variable_list grads) {
 // ---------------------------------------------------------------------------------------------
 Tensor run_adapters(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& ids, const Tensor& scale, const Tensor& out) {
   const int64_t rank = a.size(1), padded = (rank + 15) / 16 * 16;
-  const Tensor hidden = fresh({x.size(0), y.scalar_type() == at::kFloat ? 3 : 2, padded}, at::kBFloat16, x);
+  const Tensor hidden = fresh({x.size(0) * padded * (y.scalar_type() == at::kFloat ? 6 : 4)}, at::kByte, x);  // wb200_adapters_hidden_bytes
   check(entry.adapters_forward(int(x.size(0)), int(x.size(1)), int(y.size(1)), int(rank), int(a.size(0)), x.data_ptr(), pitch(x), a.data_ptr(), b.data_ptr(),
                              ids.data_ptr(), ids.scalar_type() == at::kLong, static_cast<const float*>(ptr(scale)), y.data_ptr(), pitch(y), out.data_ptr(),
-                             pitch(out), dtype_code(out), hidden.data_ptr(), size_t(hidden.numel()) * 2, stream_of(x)));
+                             pitch(out), dtype_code(out), hidden.data_ptr(), size_t(hidden.numel()), stream_of(x)));
   return hidden;
 }
 
@@ -117,7 +117,7 @@ struct AdaptersNode : torch::autograd::Function<AdaptersNode> {
       const Tensor ws = fresh({int64_t(bytes)}, at::kByte, x);
       check(entry.adapters_backward(int(x.size(0)), int(x.size(1)), int(b.size(1)), int(a.size(1)), int(a.size(0)), x.data_ptr(), pitch(x), a.data_ptr(),
                                   b.data_ptr(), ids.data_ptr(), ids.scalar_type() == at::kLong, static_cast<const float*>(ptr(scale)), g.data_ptr(), pitch(g),
-                                  hidden.data_ptr(), size_t(hidden.numel()) * 2, ptr(dx), x.size(1), 0, ptr(da), ptr(db), ws.data_ptr(),
+                                  hidden.data_ptr(), size_t(hidden.numel()), ptr(dx), x.size(1), 0, ptr(da), ptr(db), ws.data_ptr(),
                                   bytes, stream_of(x)));
       variable_list mine = once({dx, da, db});
       for (int i = 0; i < 3; ++i) result[1 + i] = mine[i];
