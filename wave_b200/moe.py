@@ -179,8 +179,8 @@ def combine_rows(y: torch.Tensor, row_of: torch.Tensor, weight: torch.Tensor) ->
             y = y.contiguous()
         if y.stride(1) != 1 or y.stride(0) < N:  # of a single row or column: any
             y = y.as_strided((rows, N), (y.stride(0) if rows > 1 else N, 1))
-    else:  # (without rows of y every pair is dropped)
-        return torch.zeros(row_of.shape[0], y.shape[1], dtype=y.dtype, device=y.device) + 0 * weight.sum().to(y.dtype)
+    else:  # (without rows of y every pair is dropped, whatever its weight; the sum of no weights keeps the result in their graph)
+        return torch.zeros(row_of.shape[0], y.shape[1], dtype=y.dtype, device=y.device) + weight[:0].sum().to(y.dtype)
     return _CombineRows.apply(y, row_of.contiguous(), weight.contiguous())
 
 
