@@ -23,3 +23,32 @@ def test_combine_without_rows_drops_pairs_of_any_weight(dtype, value):
         assert out.dtype == dtype and torch.equal(out, torch.zeros_like(out))
         grad, = torch.autograd.grad(out, weight, torch.ones_like(out))
         assert torch.equal(grad, torch.zeros_like(grad))
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """A dual tensor's tangent would be dropped in silence: every call refuses it, in native code and without."""
+    import torch.autograd.forward_ad as fwd
+
+    g = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g).to(DEV)  # noqa: E731
+    y, x, a, b = r(4, 32).to(BF16), r(4, 64).to(BF16), r(2, 8, 64).to(BF16), r(2, 32, 8).to(BF16)
+    ids, logits = torch.zeros(4, dtype=torch.int32, device=DEV), r(4, 8)
+    row_of, weight = torch.zeros(4, 2, dtype=torch.int32, device=DEV), r(4, 2)
+    layer = wb.MXFP4Linear.from_float(r(32, 64), input_grad=True)
+    pool = wb.LowRankAdapters(a, b)
+    codes, scales = layer.weight_codes, layer.weight_scales
+    experts = wb.MXFP4ExpertMLP(*[list(torch.zeros(s, dtype=torch.uint8, device=DEV)) for s in ((2, 256, 32), (2, 256, 2), (2, 64, 64), (2, 64, 4))], top_k=2)
+    routing = wb.Routing(weight, row_of, ids, logits.sum())
+    calls = [(y, lambda d: wb.apply_adapters(d, x, a, b, ids)), (x, lambda d: wb.apply_adapters(y, d, a, b, ids)), (a, lambda d: wb.apply_adapters(y, x, d, b, ids)),
+             (b, lambda d: wb.apply_adapters(y, x, a, d, ids)), (logits, lambda d: wb.router(d, 2)), (logits, lambda d: wb.balance_loss(d, row_of)),
+             (y, lambda d: wb.combine_rows(d, row_of, weight)), (weight, lambda d: wb.combine_rows(y, row_of, d)), (y, lambda d: wb.mxfp4_input_grad(d, codes, scales)),
+             (x, lambda d: layer(d)), (x, lambda d: layer(d, pool, ids)), (x, lambda d: experts.forward_routed(d, routing))]
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(wb._lib, "native_calls", lambda *names: None)
+        for tensor, call in calls:
+            call(tensor)
+            with fwd.dual_level():
+                with pytest.raises(ValueError, match="forward-mode"):
+                    call(fwd.make_dual(tensor, torch.ones_like(tensor)))
+                call(tensor)  # one without a tangent, at the same time

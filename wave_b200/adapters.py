@@ -22,6 +22,7 @@ def _check(y, x, a, b, ids, scale, out) -> tuple[int, int, int, int, int]:
     """(rows, K, N, rank, adapters); everything that would make the kernels read or write elsewhere is refused."""
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor; wave_b200 has no CPU path")
+    ops.refuse_tangents(y, x, a, b, scale)
     if x.dtype != torch.bfloat16 or a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
         raise ValueError(f"x, a and b must be bfloat16, got {x.dtype}, {a.dtype} and {b.dtype}")
     if x.dim() != 2 or y.dim() != 2 or a.dim() != 3 or b.dim() != 3:

@@ -60,7 +60,7 @@ bool fits(int64_t n) { return n > 0 && n <= 0x7fffffff; }
 bool here(PyObject* o, Tensor* t) {
   if (!wbfast::plain_or_parameter(o)) return false;
   *t = THPVariable_Unpack(o);
-  return t->device().index() == c10::cuda::current_device();
+  return t->device().index() == c10::cuda::current_device() && !t->_fw_grad(0).defined();  // (a forward-mode derivative is refused there)
 }
 
 // The gradients of a node whose backward is a kernel: differentiating them again is an error that is raised if it is done.

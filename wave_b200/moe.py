@@ -171,6 +171,7 @@ def combine_rows(y: torch.Tensor, row_of: torch.Tensor, weight: torch.Tensor) ->
         raise ValueError(f"row_of (int32) and weight (float32) must be [tokens, k], got {row_of.dtype} {tuple(row_of.shape)} and {weight.dtype} {tuple(weight.shape)}")
     if row_of.device != y.device or weight.device != y.device:
         raise ValueError("y, row_of and weight must be on one device")
+    ops.refuse_tangents(y, weight)
     if torch.is_grad_enabled() and y.requires_grad:
         raise ValueError("the gradient of y is not computed: pass y.detach()")
     rows, N = y.shape
@@ -197,6 +198,7 @@ class Routing:
 def _check_router(logits, mask) -> tuple[torch.Tensor, torch.Tensor | None]:
     if not logits.is_cuda or logits.dtype not in ops._DTYPE_CODE or logits.dim() != 2:
         raise ValueError(f"logits must be a 2-D float32 or bfloat16 CUDA tensor, got {logits.dtype} {tuple(logits.shape)} on {logits.device}")
+    ops.refuse_tangents(logits)
     rows, E = logits.shape
     if not 1 <= E <= ROUTER_MAX_EXPERTS:
         raise ValueError(f"{E} experts (1 .. {ROUTER_MAX_EXPERTS})")
@@ -417,6 +419,7 @@ class MXFP4ExpertMLP:
         add nothing. Never waits for the GPU."""
         if torch.is_grad_enabled() and x.requires_grad:
             raise ValueError("frozen experts give no gradient for x: pass x.detach()")
+        ops.refuse_tangents(x)
         ids, weight = routing.ids, routing.weight
         if ids.device != x.device or weight.device != x.device:
             raise ValueError(f"routing is on {ids.device} and {weight.device}, x on {x.device}")

@@ -119,6 +119,7 @@ class MXFP4Linear(torch.nn.Module):
         return self._forward_trained(x, adapters, ids)
 
     def _forward_trained(self, x: torch.Tensor, adapters, ids) -> torch.Tensor:
+        ops.refuse_tangents(x)
         through = torch.is_grad_enabled() and x.requires_grad
         if through:
             if not self.input_grad:

@@ -52,6 +52,13 @@ class PackedScales:
         return self.data.device
 
 
+def refuse_tangents(*tensors) -> None:
+    """Raise where a tensor carries a forward-mode derivative (torch.autograd.forward_ad): the kernels' outputs would come without one."""
+    for t in tensors:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("forward-mode derivatives are not computed here: differentiate backwards, or unpack the dual tensor")
+
+
 def packed_scale_bytes(rows: int, K: int) -> int:
     return int(_lib.load().wb200_packed_scale_bytes(rows, K))
 
@@ -345,6 +352,7 @@ def mxfp4_input_grad(g: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, ou
         if dx is not None:
             return dx
     lib = _lib.load()
+    refuse_tangents(g)
     if not g.is_cuda or g.dtype != torch.bfloat16 or g.dim() != 2:
         raise ValueError(f"g must be a 2-D bfloat16 CUDA tensor, got {g.dtype} {tuple(g.shape)} on {g.device}")
     _as_u8(b, "b")
