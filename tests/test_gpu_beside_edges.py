@@ -52,3 +52,42 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
                 with pytest.raises(ValueError, match="forward-mode"):
                     call(fwd.make_dual(tensor, torch.ones_like(tensor)))
                 call(tensor)  # one without a tangent, at the same time
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_given_output_counts_as_changed(native, monkeypatch):
+    """An operator that kept y for its backward pass learns that y was written over, as by an in-place operation of torch; an out that is part of a graph
+    is refused."""
+    if not native:
+        monkeypatch.setattr(wb._lib, "native_calls", lambda *names: None)
+    g = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g).to(BF16).to(DEV)  # noqa: E731
+    y, x, a, b, ids = r(6, 32), r(6, 64), r(2, 8, 64), r(2, 32, 8), torch.zeros(6, dtype=torch.int32, device=DEV)
+    w = r(6, 32).requires_grad_()
+    layer = wb.MXFP4Linear.from_float(torch.randn(32, 64, generator=g).to(DEV))
+    up = y.clone()
+    for kept, change in ((y, lambda t: wb.apply_adapters(t, x, a, b, ids, out=t)), (y, lambda t: wb.apply_adapters(y.clone(), x, a, b, ids, out=t)),
+                         (r(6, 64), lambda t: wb.mxfp4_input_grad(up, layer.weight_codes, layer.weight_scales, out=t))):
+        z = kept * (w if kept.shape == w.shape else w[:, :1])
+        with torch.no_grad():
+            change(kept)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.sum().backward()
+        assert w.grad is None
+        z = kept * (w if kept.shape == w.shape else w[:, :1])
+        z.sum().backward()
+        w.grad = None
+        leaf = kept.clone().requires_grad_()
+        with pytest.raises(ValueError):
+            change(leaf)
+        with torch.inference_mode():  # a tensor without a version
+            change(kept.clone())
+
+
+def test_a_call_that_makes_its_output_changes_none():
+    g = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g).to(BF16).to(DEV)  # noqa: E731
+    args = r(6, 32), r(6, 64), r(2, 8, 64), r(2, 32, 8), torch.zeros(6, dtype=torch.int32, device=DEV)
+    before = [t._version for t in args]
+    out = wb.apply_adapters(*args)
+    assert [t._version for t in args] == before and out._version == 0

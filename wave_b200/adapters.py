@@ -172,6 +172,10 @@ def apply_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.T
         return _Adapters.apply(y, x, a, b, ids, scale, sizes)
     if out is None:
         out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    elif torch.is_grad_enabled() and out.requires_grad:
+        raise ValueError("out is not taken together with gradients")
+    else:
+        ops.written(out)
     if rows:
         _forward(sizes, _rows(y), _rows(x), a.contiguous(), b.contiguous(), ids.contiguous(), scale.contiguous() if scale is not None else None, out)
     return out

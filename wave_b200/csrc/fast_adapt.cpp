@@ -246,8 +246,10 @@ PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
       return THPVariable_Wrap(AdaptersNode::apply(y, x, a, b, ids, given(scale)));
     }
     if (out.defined() && out.requires_grad()) Py_RETURN_NONE;
-    if (!out.defined()) out = fresh(y.sizes(), y.scalar_type(), y);
+    const bool given_out = out.defined();
+    if (!given_out) out = fresh(y.sizes(), y.scalar_type(), y);
     run_adapters(y, x, a, b, ids, scale, out);
+    if (given_out && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();  // autograd may hold what it was
     return THPVariable_Wrap(out);
   } catch (const c10::Error& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());

@@ -59,6 +59,12 @@ def refuse_tangents(*tensors) -> None:
             raise ValueError("forward-mode derivatives are not computed here: differentiate backwards, or unpack the dual tensor")
 
 
+def written(out: torch.Tensor) -> None:
+    """Tell autograd that a caller's tensor holds something else now: the backward pass of an operator that kept it raises."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def packed_scale_bytes(rows: int, K: int) -> int:
     return int(_lib.load().wb200_packed_scale_bytes(rows, K))
 
@@ -371,6 +377,10 @@ def mxfp4_input_grad(g: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, ou
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (M, K) or out.device != g.device or out.stride(1) != 1 or not rows_aligned(out) or \
             (M > 1 and out.stride(0) < K):
         raise ValueError(f"out must be bfloat16 [{M}, {K}] on {g.device} with rows that start on 16 bytes")
+    elif torch.is_grad_enabled() and out.requires_grad:
+        raise ValueError("out is not taken together with gradients")
+    else:
+        written(out)
     if M == 0:
         return out
     if g.stride(1) != 1 and N > 1 or not rows_aligned(g) or M > 1 and g.stride(0) < N:
