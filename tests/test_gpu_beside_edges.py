@@ -45,7 +45,7 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
              (x, lambda d: layer(d)), (x, lambda d: layer(d, pool, ids)), (x, lambda d: experts.forward_routed(d, routing))]
     for native in (True, False):
         if not native:
-            monkeypatch.setattr(wb._lib, "native_calls", lambda *names: None)
+            monkeypatch.setattr(wb._lib, "native_calls", lambda: None)
         for tensor, call in calls:
             call(tensor)
             with fwd.dual_level():
@@ -59,7 +59,7 @@ def test_a_given_output_counts_as_changed(native, monkeypatch):
     """An operator that kept y for its backward pass learns that y was written over, as by an in-place operation of torch; an out that is part of a graph
     is refused."""
     if not native:
-        monkeypatch.setattr(wb._lib, "native_calls", lambda *names: None)
+        monkeypatch.setattr(wb._lib, "native_calls", lambda: None)
     g = torch.Generator().manual_seed(0)
     r = lambda *s: torch.randn(*s, generator=g).to(BF16).to(DEV)  # noqa: E731
     y, x, a, b, ids = r(6, 32), r(6, 64), r(2, 8, 64), r(2, 32, 8), torch.zeros(6, dtype=torch.int32, device=DEV)
@@ -91,3 +91,32 @@ def test_a_call_that_makes_its_output_changes_none():
     before = [t._version for t in args]
     out = wb.apply_adapters(*args)
     assert [t._version for t in args] == before and out._version == 0
+
+
+def test_watched_functions_of_the_library_are_called(monkeypatch):
+    """A wrapper around one of the library's functions sees the calls and the backward passes of an operator, from the next call on."""
+    lib, seen = wb._lib.load(), []
+
+    def watch(name):
+        real = getattr(lib, name)
+        monkeypatch.setattr(lib, name, lambda *args: (seen.append(name), real(*args))[1])
+
+    g = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g).to(DEV)  # noqa: E731
+    y, x, a, b, ids = r(4, 32).to(BF16), r(4, 64).to(BF16), r(2, 8, 64).to(BF16).requires_grad_(), r(2, 32, 8).to(BF16), torch.zeros(4, dtype=torch.int32, device=DEV)
+    logits, weight = r(4, 8).requires_grad_(), r(4, 2).requires_grad_()
+    layer = wb.MXFP4Linear.from_float(r(32, 64))
+    calls = {"wb200_adapters_forward": lambda: wb.apply_adapters(y, x, a, b, ids), "wb200_router": lambda: wb.router(logits, 2).weight,
+             "wb200_moe_combine": lambda: wb.combine_rows(y, torch.zeros(4, 2, dtype=torch.int32, device=DEV), weight),
+             "wb200_mxfp4_input_grad": lambda: wb.mxfp4_input_grad(y, layer.weight_codes, layer.weight_scales)}
+    backward = {"wb200_adapters_forward": "wb200_adapters_backward", "wb200_router": "wb200_router_grad", "wb200_moe_combine": "wb200_moe_combine_grad"}
+    want = {name: call().detach() for name, call in calls.items()}
+    for name in [*calls, *backward.values()]:
+        watch(name)
+    for name, call in calls.items():
+        seen.clear()
+        out = call()
+        assert seen == [name] and torch.equal(out, want[name])
+        if name in backward:
+            out.sum().backward()
+            assert seen == [name, backward[name]]

@@ -330,7 +330,7 @@ def fast(lib=None):
                  "wb200_decode_tile_rows_for")
         beside = ("wb200_adapters_forward", "wb200_adapters_backward", "wb200_mxfp4_input_grad", "wb200_router_workspace_bytes", "wb200_router",
                   "wb200_router_grad", "wb200_moe_combine", "wb200_moe_combine_grad", "wb200_last_error", "wb200_adapters_backward_workspace_bytes")
-        if not isinstance(lib, ctypes.CDLL) or not all(isinstance(getattr(lib, name), lib._FuncPtr) for name in names):
+        if not isinstance(lib, ctypes.CDLL) or not all(isinstance(getattr(lib, name), lib._FuncPtr) for name in names + beside):
             return None
         try:
             from . import _fast as module, build
@@ -341,19 +341,27 @@ def fast(lib=None):
             warnings.warn(f"wave_b200._fast cannot be used ({e}): repeated calls take the slower Python path. Build it with "
                           "`python -m wave_b200.build`", RuntimeWarning, stacklevel=2)
             return None
-        _fast_entries.update({name: getattr(lib, name) for name in names})
+        _fast_entries.update({name: getattr(lib, name) for name in names + beside})
         module.bind(*(ctypes.cast(_fast_entries[name], ctypes.c_void_p).value for name in names))
-        module.bind_adapt(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in beside))
+        module.bind_adapt(*(ctypes.cast(_fast_entries[name], ctypes.c_void_p).value for name in beside))
         _fast, _fast_lib = module, lib
     return _fast if _fast and lib is _fast_lib else None
 
 
 def native_calls():
     """The host module for one call of an operator, or None: where it cannot be used, or a caller has put something in the place of the library
-    or of `load`, to watch or to redirect calls."""
+    or of `load`, to watch or to redirect calls. The operator asks for the functions that it is made of by `unwatched`."""
     if _fast and _lib is _fast_lib and load is _loader:
         return _fast
     return fast() if load is _loader and _fast is None else None
+
+
+def unwatched(*names: str) -> bool:
+    """Functions of the library are its own, as the host module calls them: nothing was put in their place."""
+    for name in names:
+        if getattr(_lib, name) is not _fast_entries[name]:
+            return False
+    return True
 
 
 def check(rc: int) -> None:

@@ -161,7 +161,7 @@ def combine_rows(y: torch.Tensor, row_of: torch.Tensor, weight: torch.Tensor) ->
     in the weights (the rows of y are those of frozen experts: a y that requires a gradient is refused). y [R, N] f32 or bf16, row_of [tokens, k]
     int32, negative for a dropped pair, weight [tokens, k] f32. Rows at or past R are not checked for."""
     native = _lib.native_calls()
-    if native is not None:
+    if native is not None and _lib.unwatched("wb200_moe_combine", "wb200_moe_combine_grad"):
         out = native.combine_rows(y, row_of, weight)
         if out is not None:
             return out
@@ -291,7 +291,7 @@ def router(logits: torch.Tensor, top_k: int, mask: torch.Tensor | None = None, r
     over the n rows that count; 0 where none does. Its gradient takes f as a constant. mask: bool [rows], False for padding: ids -1, weight
     0, in no sum, gradient 0."""
     native = _lib.native_calls()
-    if native is not None:
+    if native is not None and _lib.unwatched("wb200_router", "wb200_router_grad"):
         result = native.router(logits, top_k, mask, renormalize)
         if result is not None:
             return Routing(*result)

@@ -353,7 +353,7 @@ def mxfp4_input_grad(g: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, ou
     bf16. g bf16, b uint8 [N, K/2] and b_scale uint8 [N, K/32] row-major as the layer's forward takes them. Rows of g that do not start on
     16 bytes (odd N) are copied first. out: bf16 [M, K] whose rows start on 16 bytes."""
     native = _lib.native_calls() if out is None else None
-    if native is not None:
+    if native is not None and _lib.unwatched("wb200_mxfp4_input_grad"):
         dx = native.input_grad(g, b, b_scale)
         if dx is not None:
             return dx
