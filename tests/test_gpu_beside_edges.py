@@ -1,5 +1,7 @@
 """Edges of the calls beside frozen weights: what is dropped, watched, written in place or differentiated in another way."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -120,3 +122,30 @@ def test_watched_functions_of_the_library_are_called(monkeypatch):
         if name in backward:
             out.sum().backward()
             assert seen == [name, backward[name]]
+
+
+def test_the_interpreter_lock_is_given_back_around_launches():
+    """In the place of every entry that launches, the host module gets Python's own question whether this thread holds the lock: a yes is an error status."""
+    lib, module = wb._lib.load(), wb._lib.fast()
+    names = ("wb200_adapters_forward", "wb200_adapters_backward", "wb200_mxfp4_input_grad", "wb200_router_workspace_bytes", "wb200_router", "wb200_router_grad",
+             "wb200_moe_combine", "wb200_moe_combine_grad", "wb200_last_error", "wb200_adapters_backward_workspace_bytes")
+    asked = ctypes.cast(ctypes.pythonapi.PyGILState_Check, ctypes.c_void_p).value
+    own = [ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names]
+    g = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g).to(DEV)  # noqa: E731
+    y, x, a, b, ids = r(4, 32).to(BF16), r(4, 64).to(BF16), r(2, 8, 64).to(BF16), r(2, 32, 8).to(BF16), torch.zeros(4, dtype=torch.int32, device=DEV)
+    row_of = torch.zeros(4, 2, dtype=torch.int32, device=DEV)
+    layer = wb.MXFP4Linear.from_float(r(32, 64))
+    module.bind_adapt(*(p if name.endswith(("_bytes", "_error")) else asked for name, p in zip(names, own)))
+    try:
+        wb.mxfp4_input_grad(y, layer.weight_codes, layer.weight_scales)
+        for trained in (False, True):
+            leaf, logits, weight = a.clone().requires_grad_(trained), r(4, 8).requires_grad_(trained), r(4, 2).requires_grad_(trained)
+            outs = wb.apply_adapters(y, x, leaf, b, ids), wb.router(logits, 2).weight, wb.combine_rows(y, row_of, weight)
+            if trained:
+                for out in outs:
+                    out.sum().backward()
+        wb.apply_adapters(y, x, a, b, ids, out=y)
+    finally:
+        module.bind_adapt(*own)
+    assert ctypes.pythonapi.PyGILState_Check() == 1  # and it is held again

@@ -63,6 +63,15 @@ bool here(PyObject* o, Tensor* t) {
   return t->device().index() == c10::cuda::current_device() && !t->_fw_grad(0).defined();  // (a forward-mode derivative is refused there)
 }
 
+// The interpreter lock is given back while a call allocates, launches and builds its node, and taken again where the scope ends: a launch waits where the
+// queue is full, and what the stream waits for may be a host function that needs the lock.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 // The gradients of a node whose backward is a kernel: differentiating them again is an error that is raised if it is done.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -243,12 +252,20 @@ PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (out.defined() && (out.scalar_type() != y.scalar_type() || out.sizes() != y.sizes() || !row_major(out))) Py_RETURN_NONE;
     if (wanted({&y, &x, &a, &b})) {
       if (out.defined() || y.scalar_type() != at::kBFloat16 || pool > 65535) Py_RETURN_NONE;
-      return THPVariable_Wrap(AdaptersNode::apply(y, x, a, b, ids, given(scale)));
+      Tensor result;
+      {
+        const Unlocked scope;
+        result = AdaptersNode::apply(y, x, a, b, ids, given(scale));
+      }
+      return THPVariable_Wrap(result);
     }
     if (out.defined() && out.requires_grad()) Py_RETURN_NONE;
     const bool given_out = out.defined();
-    if (!given_out) out = fresh(y.sizes(), y.scalar_type(), y);
-    run_adapters(y, x, a, b, ids, scale, out);
+    {
+      const Unlocked scope;
+      if (!given_out) out = fresh(y.sizes(), y.scalar_type(), y);
+      run_adapters(y, x, a, b, ids, scale, out);
+    }
     if (given_out && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();  // autograd may hold what it was
     return THPVariable_Wrap(out);
   } catch (const c10::Error& e) {
@@ -276,11 +293,14 @@ PyObject* router(PyObject*, PyObject* const* args, Py_ssize_t n) {
       Py_RETURN_NONE;
     if (mask.defined() && (mask.scalar_type() != at::kBool || mask.dim() != 1 || mask.size(0) != logits.size(0) || !mask.is_contiguous())) Py_RETURN_NONE;
     variable_list r;
-    if (wanted({&logits})) {
-      r = RouterNode::apply(logits, given(mask), int64_t(top_k), renormalize != 0);
-    } else {
-      const Routed v = run_router(logits, mask, top_k, renormalize != 0);
-      r = {v.weight, v.ids, v.counts, v.loss};
+    {
+      const Unlocked scope;
+      if (wanted({&logits})) {
+        r = RouterNode::apply(logits, given(mask), int64_t(top_k), renormalize != 0);
+      } else {
+        const Routed v = run_router(logits, mask, top_k, renormalize != 0);
+        r = {v.weight, v.ids, v.counts, v.loss};
+      }
     }
     PyObject* result = PyTuple_New(4);
     if (!result) return nullptr;
@@ -307,8 +327,12 @@ PyObject* combine_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
         weight.sizes() != row_of.sizes() || !row_of.is_contiguous() || !weight.is_contiguous() || !fits(row_of.size(0)) || !fits(row_of.size(1)) ||
         !fits(y.size(1)) || y.size(0) == 0 || (at::GradMode::is_enabled() && y.requires_grad()))
       Py_RETURN_NONE;
-    if (wanted({&weight})) return THPVariable_Wrap(CombineNode::apply(y, row_of, weight));
-    return THPVariable_Wrap(run_combine(y, row_of, weight));
+    Tensor result;
+    {
+      const Unlocked scope;
+      result = wanted({&weight}) ? CombineNode::apply(y, row_of, weight) : run_combine(y, row_of, weight);
+    }
+    return THPVariable_Wrap(result);
   } catch (const c10::Error& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
     return nullptr;
@@ -335,8 +359,12 @@ PyObject* input_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!fits(M) || !fits(N) || !fits(K) || K % 32 || codes.size(0) != N || scales.size(0) != N || scales.size(1) != K / 32 || !aligned(g) || !aligned(codes) ||
         (M > 1 ? g.stride(0) : N) % 8 || N % 8)
       Py_RETURN_NONE;
-    const Tensor dx = fresh({M, K}, at::kBFloat16, g);
-    check(entry.input_grad(int(M), int(N), int(K), g.data_ptr(), pitch(g), codes.data_ptr(), scales.data_ptr(), pitch(scales), dx.data_ptr(), K, stream_of(g)));
+    Tensor dx;
+    {
+      const Unlocked scope;
+      dx = fresh({M, K}, at::kBFloat16, g);
+      check(entry.input_grad(int(M), int(N), int(K), g.data_ptr(), pitch(g), codes.data_ptr(), scales.data_ptr(), pitch(scales), dx.data_ptr(), K, stream_of(g)));
+    }
     return THPVariable_Wrap(dx);
   } catch (const c10::Error& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
