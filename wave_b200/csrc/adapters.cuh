@@ -1661,8 +1661,8 @@ adapter_outer_kernel(const OuterParams p) {
   __shared__ int found[kAdapterWarps + 1];
   int* list = reinterpret_cast<int*>(smem + Cfg::RING_BYTES);
   const uint32_t base = smem_u32(smem);
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();  // only now: this is the first kernel of a call that wants B's gradient alone
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int second = int(blockIdx.y) >= p.side[0].blocks;
   OuterSide side = p.side[0];  // (member by member: an index into the parameters would put them on the stack)
