@@ -572,14 +572,15 @@ template <int N, bool TRANS>
 struct ShrinkWide {
   static constexpr int ROWS = 128, X_BYTES = ROWS * 128, W_BYTES = TRANS ? 64 * 128 : N * 128, STAGE_BYTES = X_BYTES + 2 * W_BYTES;
   static constexpr int STAGES = STAGE_BYTES > 24 * 1024 ? 3 : 4;
-  // Two CTAs to an SM, and beside them none of the library's other kernels that take tensor memory (they ask for 160 KB or more): a CTA holds its columns
-  // while it waits for its cluster, so that one that waited for columns of another kernel's, in another stream, might wait for good.
+  // Two CTAs to an SM, which share its columns, and beside them none of the library's other kernels that take tensor memory: a CTA holds its columns
+  // while it waits for its cluster.
   static constexpr int SMEM_BYTES = 97 * 1024;           // the sums reuse the stages
   // Accumulators of an adapter, taken in turn by the stages: an MMA drops the bits of its f32 sum that do not fit, always towards zero, and 2048 k in one
   // accumulator shrink by 1.8e-6 of themselves where an f32 sum with rounding is 1e-6 off at random.
   static constexpr int ACCS = N == 64 ? 2 : 4;
   static constexpr int TMEM_COLS = 256;
   static_assert(STAGES * STAGE_BYTES + 1024 <= SMEM_BYTES && 2 * TMEM_COLS <= 512, "stages; columns of two CTAs");
+  static_assert(SMEM_BYTES + kSmemOfTmemKernel > kSmemOfSm && 3 * SMEM_BYTES > kSmemOfSm, "no other kernel with tensor memory beside one CTA, no third CTA");
   static_assert((2 * ACCS - 1) * N + (N < 32 ? 32 : N) <= TMEM_COLS, "accumulators of two adapters, of which 32 columns are read at a time");
   static_assert(ROWS * (N + 1) * 4 <= STAGES * STAGE_BYTES && ROWS <= kAdapterThreads, "sums; a thread per row where rows are grouped");
 };
@@ -1338,6 +1339,7 @@ struct ExpandWide {
   static constexpr int B_BASE = A_BYTES, Y_BASE = B_BASE + B_STAGES * B_BYTES;
   static constexpr int SMEM_BYTES = Y_BASE + Y_STAGES * Y_BYTES + 1024;
   static constexpr int TMEM_COLS = 512;  // two buffers of two adapters
+  static_assert(SMEM_BYTES >= kSmemOfTmemKernel, "keeps other kernels with tensor memory off the SM");
   static_assert(EPILOGUE_WARPS * 32 == 2 * ROWS, "two threads split a row's hidden vector");
 };
 struct ExpandWideParams {

@@ -59,6 +59,7 @@ struct ClusterSplitCfg {
   static constexpr int STAGES = Base::STAGES;
   static constexpr int NUM_BARRIERS = 2 * STAGES + 1;
   static constexpr int SMEM_BYTES = 1024 + STAGES * Base::STAGE_BYTES + NUM_BARRIERS * 8 + 64;
+  static_assert(SMEM_BYTES >= kSmemOfTmemKernel, "keeps other kernels with tensor memory off the SM");
   static constexpr int CHUNKS = BN / 32;
   static constexpr int OWNED = (CHUNKS + 1) / 2;  // chunks that a pair owns at most: with two slices
   static constexpr int CHUNK_BYTES = 128 * 128;  // 128 rows x 32 columns of f32

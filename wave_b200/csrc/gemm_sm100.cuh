@@ -67,6 +67,7 @@ struct GemmCfg {
   static constexpr int NUM_BARRIERS = 2 * STAGES + 4;
   static constexpr int SMEM_BYTES = 1024 /*alignment slack*/ + STAGES * STAGE_BYTES + STAGING_BYTES + NUM_BARRIERS * 8 + 64;
   static_assert(STAGES >= 3, "pipeline needs at least 3 stages");
+  static_assert(SMEM_BYTES >= kSmemOfTmemKernel, "keeps other kernels with tensor memory off the SM");
   // tensor-memory columns
   static constexpr int TMEM_COLS = 512;
   static constexpr bool OVERLAP = (BN == 256);

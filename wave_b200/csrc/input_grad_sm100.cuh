@@ -57,6 +57,7 @@ struct InputGradCfg {
   static constexpr int GROUP_WARPS = EXPAND_WARPS / GROUPS;
   static_assert(GROUPS <= B_STAGES && GROUPS <= SCALE_BATCH && EXPAND_WARPS % GROUPS == 0, "a group moves on by less than a ring");
   static constexpr int THREADS = (7 + EXPAND_WARPS) * 32;
+  static_assert(SMEM_BYTES >= kSmemOfTmemKernel, "keeps other kernels with tensor memory off the SM");
   static_assert(CODE_BASE % 1024 == 0 && CODE_BYTES % 1024 == 0 && BAR_BASE % 8 == 0 && BM * SUM_PITCH <= CODE_BASE && SMEM_BYTES <= 227 * 1024, "shared memory");
 };
 

@@ -40,6 +40,7 @@ struct MixedDecodeCfg {
   static constexpr int SF_SETS = 4;
   static_assert(SF_COL + SF_SETS * SF_SET_COLS <= TMEM_COLS, "tensor memory");
   static_assert(STAGES >= 4 && SMEM_BYTES <= SMEM_LIMIT, "shared memory");
+  static_assert(SMEM_BYTES >= kSmemOfTmemKernel, "keeps other kernels with tensor memory off the SM");
   static_assert(STAGE_BYTES >= 128 * 128, "the MMA reads 128 rows from the head of a stage");
 };
 

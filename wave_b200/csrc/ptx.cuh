@@ -241,6 +241,12 @@ __device__ __forceinline__ uint64_t l2_policy_evict_last() {
 // ---------------------------------------------------------------------------------------------
 // tensor memory
 // ---------------------------------------------------------------------------------------------
+// A CTA that asks for columns which another kernel's CTA on its SM holds waits for that one to end. Where the holder itself waits for the rest of its
+// cluster, whose CTAs may wait for columns elsewhere, the two kernels (in two streams) would wait for good. So kernels with tensor memory keep each other
+// off an SM by their shared memory: every one of them asks for at least this much, and one that asks for less states that it still leaves no
+// room for it.
+constexpr int kSmemOfSm = 228 * 1024;
+constexpr int kSmemOfTmemKernel = 160 * 1024;
 template <int CTA_GROUP>
 __device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t ncols) {
   if constexpr (CTA_GROUP == 1)

@@ -72,6 +72,7 @@ struct SkinnyCfg {
   static constexpr int SF_COL = 256;
   static constexpr int SF_SETS = 8;
   static_assert(STAGE_BYTES % 1024 == 0, "stages must keep the 1024-byte swizzle alignment");
+  static_assert(SMEM_BYTES >= kSmemOfTmemKernel, "keeps other kernels with tensor memory off the SM");
 };
 
 constexpr int kSkinnyCounterWords = 4096;  // 32-bit tile counters at the head of every workspace

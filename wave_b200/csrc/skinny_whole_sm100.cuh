@@ -42,6 +42,7 @@ struct SkinnyWholeCfg {
   static constexpr int MISC_BYTES = 64 + kWholeItemQueue * 4;
   static constexpr int SMEM_BYTES = 1024 + STAGES_ * STAGE_BYTES + STAGING_BYTES + NUM_BARRIERS * 8 + MISC_BYTES;
   static_assert(SMEM_BYTES <= 232448, "over the dynamic shared memory a CTA may ask for");
+  static_assert(SMEM_BYTES >= kSmemOfTmemKernel, "keeps other kernels with tensor memory off the SM");
 };
 
 struct SkinnyWholeParams {
