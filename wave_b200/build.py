@@ -69,18 +69,22 @@ def _run(cmd: list[str]) -> str:
 
 
 def _compile(nvcc: str, source: Path, objects: Path, variant: list[str], force: bool, verbose: bool) -> Path:
-    """One source to an object, unless that is newer than all it was compiled from (nvcc writes them down beside it)."""
-    unit, made_from = objects / f"{source.stem}.o", objects / f"{source.stem}.d"
-    if not force and not verbose and unit.exists() and made_from.exists():
+    """One source to an object, unless there is one of the same command that is newer than all it was compiled from (nvcc writes that down beside it)."""
+    unit, made_from, made_by = (objects / f"{source.stem}{end}" for end in (".o", ".d", ".cmd"))
+    cmd = [nvcc, *NVCC_FLAGS, *variant, "-MD", "-MF", str(made_from), "-c", "-o", str(unit), str(source)]
+    line = " ".join(cmd)
+    if not force and not verbose and unit.exists() and made_from.exists() and made_by.exists() and made_by.read_text() == line:
         deps = [Path(d) for d in made_from.read_text().replace("\\\n", " ").split(":", 1)[1].split()]
         if all(d.exists() and d.stat().st_mtime <= unit.stat().st_mtime for d in deps):
             return unit
-    cmd = [nvcc, *NVCC_FLAGS, *variant, *(["-Xptxas", "-v"] if verbose else []), "-MD", "-MF", str(made_from), "-c", "-o", str(unit), str(source)]
+    made_by.unlink(missing_ok=True)  # (nothing is claimed of an object that is being written)
     if verbose:
+        cmd[1:1] = ["-Xptxas", "-v"]
         print(" ".join(cmd))
     said = _run(cmd)
     if verbose:
         print(said)
+    made_by.write_text(line)
     return unit
 
 
