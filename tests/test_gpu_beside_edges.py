@@ -1,6 +1,7 @@
 """Edges of the calls beside frozen weights: what is dropped, watched, written in place or differentiated in another way."""
 
 import ctypes
+import sys
 
 import pytest
 import torch
@@ -149,3 +150,17 @@ def test_the_interpreter_lock_is_given_back_around_launches():
     finally:
         module.bind_adapt(*own)
     assert ctypes.pythonapi.PyGILState_Check() == 1  # and it is held again
+
+
+def test_a_layer_without_adapters_is_called_as_directly_as_before():
+    """Of the package's Python functions only forward itself and the question for the host module run in front of the native call."""
+    layer = wb.MXFP4Linear.from_float(torch.randn(64, 128, device=DEV))
+    x = torch.randn(4, 128, device=DEV).to(BF16)
+    want = layer(x)
+    seen = []
+    sys.setprofile(lambda frame, event, arg: seen.append(frame.f_code.co_name) if event == "call" and "wave_b200" in frame.f_code.co_filename else None)
+    try:
+        got = layer(x)
+    finally:
+        sys.setprofile(None)
+    assert seen == ["forward", "_native"] and torch.equal(got, want)

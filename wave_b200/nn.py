@@ -29,6 +29,9 @@ def _native():
     return _lib._fast
 
 
+_ALONE = object()  # in the place of ids: the layer's own output
+
+
 class _FrozenLinear(torch.autograd.Function):
     """A layer's output with the gradient of its input; the rounding of the activations to MXFP4 counts as the identity."""
 
@@ -114,9 +117,18 @@ class MXFP4Linear(torch.nn.Module):
     def forward(self, x: torch.Tensor, adapters=None, ids: torch.Tensor | None = None) -> torch.Tensor:
         """x [..., K] -> [..., N]. adapters: a `LowRankAdapters` pool, ids [...]: the adapter of every row (outside the pool: none); what they
         add is rounded onto the layer's rounded output. They take a bf16 x."""
-        if adapters is None and not self.input_grad:
-            return self._base(x)
-        return self._forward_trained(x, adapters, ids)
+        if adapters is not None or (self.input_grad and ids is not _ALONE):
+            return self._forward_trained(x, adapters, ids)
+        # a call whose tensors need no preparation (here, not a function away: it is microseconds long); anything else comes back unhandled
+        native, scales = _native(), self._native_scales
+        if native is None or scales is None:
+            return self._forward_checked(x)
+        y = native.linear(x, self._buffers.get("weight_codes"), scales, self.output_dtype, ops._pool._fast or ops._pool.fast)
+        if type(y) is int:
+            _lib.check(y)
+        elif y is not None:
+            return y
+        return self._forward_checked(x)
 
     def _forward_trained(self, x: torch.Tensor, adapters, ids) -> torch.Tensor:
         ops.refuse_tangents(x)
@@ -140,16 +152,8 @@ class MXFP4Linear(torch.nn.Module):
         return y.reshape(*x.shape[:-1], self.out_features)
 
     def _base(self, x: torch.Tensor) -> torch.Tensor:
-        # a call whose tensors need no preparation; anything else comes back unhandled
-        native, scales = _native(), self._native_scales
-        if native is None or scales is None:
-            return self._forward_checked(x)
-        y = native.linear(x, self._buffers.get("weight_codes"), scales, self.output_dtype, ops._pool._fast or ops._pool.fast)
-        if type(y) is int:
-            _lib.check(y)
-        elif y is not None:
-            return y
-        return self._forward_checked(x)
+        """The layer's own output, without a graph."""
+        return MXFP4Linear.forward(self, x, None, _ALONE)
 
     def _forward_checked(self, x: torch.Tensor) -> torch.Tensor:
         lead = x.shape[:-1]
