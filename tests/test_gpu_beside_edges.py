@@ -164,3 +164,26 @@ def test_a_layer_without_adapters_is_called_as_directly_as_before():
     finally:
         sys.setprofile(None)
     assert seen == ["forward", "_native"] and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("tokens,cols,by_token", [(1, 4096, True), (1, 8192, False), (255, 8192, False), (256, 8192, True), (3, 16384, False), (512, 16384, True), (4, 512, False)])
+@pytest.mark.parametrize("top_k", [1, 6, 8])
+def test_few_tokens_of_wide_rows_are_combined_by_all_threads_at_once(tokens, cols, by_token, top_k):
+    """Which of its two kernels the sum of a token's rows takes, and that the result is the same on both sides of the border: f32 sums in slot order, at most
+    one rounding for each of top_k products and sums, and one to bf16."""
+    g = torch.Generator().manual_seed(tokens)
+    y = torch.randn(tokens * top_k + 3, cols, generator=g).to(BF16).to(DEV)
+    row_of = torch.randperm(tokens * top_k + 3, generator=g)[:tokens * top_k].reshape(tokens, top_k).to(torch.int32).to(DEV)
+    row_of[0, top_k // 2] = -1
+    weight = torch.rand(tokens, top_k, generator=g).to(DEV)
+    wb.combine_rows(y, row_of, weight)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        got = wb.combine_rows(y, row_of, weight)
+        torch.cuda.synchronize()
+    names = " ".join(e.key for e in prof.key_averages())
+    assert ("combine_token_kernel" in names) == by_token and ("moe_combine_kernel" in names) != by_token, names
+    rows = y.double()[row_of.clamp(min=0).long()] * (row_of >= 0).double()[:, :, None] * weight.double()[:, :, None]
+    want, size = rows.sum(1), rows.abs().sum(1)
+    tol = 2 * top_k * 2.0 ** -24 * size
+    tol = tol + 2.0 ** -8 * (want.abs() + tol) + 1e-38
+    assert bool(((got.double() - want).abs() <= tol).all())

@@ -1634,7 +1634,11 @@ int wb200_moe_combine(const void* y, long long ldy, int dtype, const int* row_of
   int rc = get_device(&dev);
   if (rc) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == WB200_BF16 && top_k <= 8 && cols % 8 == 0 && cols >= 1024 && rows_aligned(y, ldy, dtype) && rows_aligned(out, ldo, dtype)) {
+  // A CTA a token takes 2048 columns at a time, one round of loads after the other: where there are few tokens of wide rows, a thread for every 8 columns
+  // has all of them in flight. us, thread / CTA, top 6: 1 token of 4096 3.6 / 3.3, of 8192 3.6 / 4.5, of 16384 3.6 / 6.9; 64 of 8192 4.3 / 4.7; 256 of
+  // 8192 11.3 / 9.5, of 16384 17.3 / 15.2, of 32768 31.6 / 28.3 (top 1 13.7 / 16.0); 1024 of 32768, top 2, 55.6 / 34.4; 4096 of 4096 52 / 38.
+  const bool by_token = cols >= 1024 && (cols <= 4096 || 32ll * tokens >= cols);
+  if (dtype == WB200_BF16 && top_k <= 8 && cols % 8 == 0 && by_token && rows_aligned(y, ldy, dtype) && rows_aligned(out, ldo, dtype)) {
     WB_CUDA(wbhost::combine_tokens(y, ldy, row_of, weight, tokens, top_k, cols, out, ldo, s));
     return WB200_OK;
   }
