@@ -260,7 +260,9 @@ __device__ __forceinline__ void finish_hidden(const ShrinkParams& p, float* sums
 #pragma unroll
       for (int s = 0; s < 8; ++s) v += part[s];
     }
-    p.hidden[(long long)row_of(row) * p.Rp + n0 + col] = n0 + col < p.R ? v * scale_of(row) : 0.f;  // (an infinity of x would be a NaN in the ranks behind the last)
+    const int at_row = row_of(row);
+    if (WB_CHECK(at_row >= 0 && at_row < p.rows, kCheckOutputIndex, at_row))
+      p.hidden[(long long)at_row * p.Rp + n0 + col] = n0 + col < p.R ? v * scale_of(row) : 0.f;  // (an infinity of x would be a NaN in the ranks behind the last)
   }
   if (splits > 1) {  // nobody overwrites what others still read
     cluster_arrive();
@@ -387,7 +389,8 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
           if (n0 + col >= p.Rp) continue;
           float v = 0.f;
           for (int i = 0; i < splits; ++i) v += sums[i * share + mine][col];
-          p.hidden[(long long)(row0 + nth_bit(group.rows, first + row)) * p.Rp + n0 + col] = n0 + col < p.R ? v * scale : 0.f;
+          const int at_row = row0 + nth_bit(group.rows, first + row);
+          if (WB_CHECK(at_row >= row0 && at_row < p.rows, kCheckOutputIndex, at_row)) p.hidden[(long long)at_row * p.Rp + n0 + col] = n0 + col < p.R ? v * scale : 0.f;
         }
       }
     }
@@ -769,7 +772,7 @@ __device__ __forceinline__ void expand_rest(const ExpandParams& p, long long row
     const int valid = c_end - c;
     float v[8] = {};
     if (y) read8<T>(y + row * p.ldy + c, p.io_vec && valid >= 8, valid, v);
-    write8<T>(out + row * p.ldo + c, p.io_vec && valid >= 8, valid, v);
+    if (WB_CHECK(row < p.rows && c < p.C && c_end <= p.C, kCheckOutputIndex, row << 32 | c)) write8<T>(out + row * p.ldo + c, p.io_vec && valid >= 8, valid, v);
   }
 }
 
@@ -890,6 +893,7 @@ adapter_expand_few_kernel(const ExpandParams p) {
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         if (i >= count || c >= c_end) break;
+        if (!WB_CHECK(row[i] >= row0 && row[i] < p.rows && c + int(both) < p.C, kCheckOutputIndex, (long long)row[i] << 32 | c)) continue;
         T* at = out + row[i] * p.ldo + c;
         if (p.io_vec && both) {
           if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(at) = pack_bf16x2(acc[i][0], acc[i][1]);
@@ -966,7 +970,8 @@ adapter_expand_few_whole_kernel(const ExpandParams p) {
 #pragma unroll
         for (int k = 0; k < KEPT; ++k) {
           const int col = c + (k * PIECES + pc) * COLS;
-          if (col < c_end) out[row[i] * p.ldo + col] = as_out<T>(old[i][k]);
+          if (col < c_end && WB_CHECK(row[i] >= row0 && row[i] < p.rows && col < p.C, kCheckOutputIndex, (long long)row[i] << 32 | col))
+            out[row[i] * p.ldo + col] = as_out<T>(old[i][k]);
         }
       }
     }
@@ -1279,6 +1284,7 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               if (row[m][h] < 0 || c0 + 8 * t >= p.C) continue;
+              if (!WB_CHECK(row0 + row[m][h] < p.rows && c0 + 8 * t + 8 <= p.C, kCheckOutputIndex, (long long)(row0 + row[m][h]) << 32 | (c0 + 8 * t))) continue;
               float v[8];
 #pragma unroll
               for (int n = 0; n < 4; ++n)
@@ -1305,13 +1311,15 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
                   const uint32_t off = out_off[FAST ? 0 : m * 16 + 2 * r + lane_row];
-                  if (off != 0xffffffffu) *reinterpret_cast<uint32_t*>(out + (off + at)) = pack_bf16x2(v[2 * r], v[2 * r + 1]);
+                  if (off != 0xffffffffu && WB_CHECK(row0 + int(off / out_pitch) < p.rows && c0 + lane_col + 2 <= p.C, kCheckOutputIndex, off))
+                    *reinterpret_cast<uint32_t*>(out + (off + at)) = pack_bf16x2(v[2 * r], v[2 * r + 1]);
                 }
               } else {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                   const uint32_t off = out_off[FAST ? 0 : m * 16 + r];
-                  if (off != 0xffffffffu) *reinterpret_cast<T*>(out + (off + at)) = as_out<T>(v[r]);
+                  if (off != 0xffffffffu && WB_CHECK(row0 + int(off / out_pitch) < p.rows && c0 + lane_col < p.C, kCheckOutputIndex, off))
+                    *reinterpret_cast<T*>(out + (off + at)) = as_out<T>(v[r]);
                 }
               }
             }
@@ -1603,7 +1611,7 @@ __global__ void __launch_bounds__(256) adapter_align_kernel(const __nv_bfloat16*
     const int row = int(e / pieces), c = int(e - (long long)row * pieces) * 8;
     uint32_t r[4];
     load_bf16<8>(src + row * ld + c, false, cols - c, r);
-    *reinterpret_cast<uint4*>(dst + e * 8) = make_uint4(r[0], r[1], r[2], r[3]);
+    if (WB_CHECK(row < rows && c + 8 <= pitch, kCheckOutputIndex, (long long)row << 32 | c)) *reinterpret_cast<uint4*>(dst + e * 8) = make_uint4(r[0], r[1], r[2], r[3]);
   }
 }
 
@@ -1797,6 +1805,7 @@ adapter_outer_kernel(const OuterParams p) {
     }
     if (splits == 1 && !any) {  // an adapter without rows
       const int cols = min(kOuterCols, side.C - c0);
+      if (!WB_CHECK(l < p.L && cols > 0, kCheckOutputIndex, (long long)l << 32 | c0)) return;
       if (side.rank_major) {
         for (int r = warp; r < p.R; r += kAdapterWarps) zero_fill(side.out + ((long long)l * p.R + r) * side.C + c0, cols, lane, 32);
       } else {
@@ -1849,7 +1858,7 @@ adapter_outer_kernel(const OuterParams p) {
         for (int s = 0; s < 8; ++s) v = make_float4(v.x + part[s].x, v.y + part[s].y, v.z + part[s].z, v.w + part[s].w);
       }
       const int r = n0 + 4 * q, col = c0 + c;
-      if (col >= side.C || r >= p.R) continue;
+      if (col >= side.C || r >= p.R || !WB_CHECK(l < p.L && c >= 0 && c < kOuterCols, kCheckOutputIndex, (long long)l << 32 | col)) continue;
       const float f[4] = {v.x, v.y, v.z, v.w};
       if (side.rank_major) {
         __nv_bfloat16* to = side.out + ((long long)l * p.R + r) * side.C + col;

@@ -179,8 +179,9 @@ __device__ __forceinline__ void sum_slices(const InputGradParams& p, uint32_t sm
 #pragma unroll
         for (int s = 1; s < S; ++s) sum[j] += v[i][s][j];
       }
-      *reinterpret_cast<uint4*>(p.dx + (long long)row * p.ldd + col) = make_uint4(pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]),
-                                                                                  pack_bf16x2(sum[4], sum[5]), pack_bf16x2(sum[6], sum[7]));
+      if (WB_CHECK(row < p.M && col + 8 <= p.K, kCheckOutputIndex, (long long)row << 32 | col))
+        *reinterpret_cast<uint4*>(p.dx + (long long)row * p.ldd + col) = make_uint4(pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]),
+                                                                                    pack_bf16x2(sum[4], sum[5]), pack_bf16x2(sum[6], sum[7]));
     }
   }
 }
@@ -368,7 +369,7 @@ input_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_consta
         uint4* at = reinterpret_cast<uint4*>(dst + col);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (row + j < p.M) at[j * pitch] = make_uint4(q[j][0], q[j][1], q[j][2], q[j][3]);
+          if (row + j < p.M && WB_CHECK(col + (lane & 3) * 8 + 8 <= p.K, kCheckOutputIndex, (long long)(row + j) << 32 | col)) at[j * pitch] = make_uint4(q[j][0], q[j][1], q[j][2], q[j][3]);
       }
       tc_fence_before_sync();
       __syncwarp();

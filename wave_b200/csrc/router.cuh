@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(1024) router_finish_kernel(const RouterParams 
       count += counts[i][lane];
       n += rows[i];
     }
-    if (e < p.E) p.counts[e] = count;
+    if (e < p.E && WB_CHECK(count >= 0, kCheckOutputIndex, e)) p.counts[e] = count;
     double mine = e < p.E ? sum * count : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -244,7 +244,7 @@ router_kernel(const RouterParams p) {
     }
     float scale = inv;
     if (p.renormalize) scale = 1.f / warp_sum(chosen_x);
-    if (lane < p.top_k) {
+    if (lane < p.top_k && WB_CHECK(t < p.rows && chosen >= 0 && chosen < p.E, kCheckOutputIndex, (long long)t << 32 | unsigned(chosen))) {
       ids[lane] = chosen;
       weight[lane] = chosen_x * scale;
       atomicAdd(&sum_n[chosen], 1);
@@ -263,6 +263,7 @@ router_kernel(const RouterParams p) {
       p.counts[e] = sum_n[e];
       mine = double(sum) * sum_n[e];
     } else {
+      if (!WB_CHECK(blockIdx.x < kRouterMaxCtas, kCheckPartialSlot, blockIdx.x)) break;
       p.part_p[blockIdx.x * p.E + e] = sum;
       p.part_n[blockIdx.x * (p.E + 1) + e] = sum_n[e];
     }
@@ -351,13 +352,13 @@ router_grad_kernel(const RouterGradParams p) {
     }
     if constexpr (EV == 8) {
       if (p.vec) {
-        if (e0 < p.E) write8<T>(out + e0, true, 8, d);
+        if (e0 < p.E && WB_CHECK(t < p.rows && e0 + 8 <= p.E, kCheckOutputIndex, (long long)t << 32 | e0)) write8<T>(out + e0, true, 8, d);
         continue;
       }
     }
 #pragma unroll
     for (int i = 0; i < EV; ++i)
-      if (e0 + i < p.E) out[e0 + i] = T(d[i]);
+      if (e0 + i < p.E && WB_CHECK(t < p.rows, kCheckOutputIndex, (long long)t << 32 | (e0 + i))) out[e0 + i] = T(d[i]);
   }
 }
 
@@ -398,7 +399,7 @@ combine_token_kernel(const __nv_bfloat16* y, long long ldy, const int* row_of, c
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] += w[j] * v[i];
       }
-      write8<__nv_bfloat16>(out + t * ldo + c + u * 1024, true, 8, acc);
+      if (WB_CHECK(c + u * 1024 + 8 <= cols, kCheckOutputIndex, t << 32 | (c + u * 1024))) write8<__nv_bfloat16>(out + t * ldo + c + u * 1024, true, 8, acc);
     }
   }
 }
@@ -466,7 +467,7 @@ combine_grad_kernel(const T* g, long long ldg, const T* y, long long ldy, const 
       if (lane == 0) part[warp][j] = acc[j];
     }
     __syncthreads();
-    if (threadIdx.x < SLOTS && j0 + threadIdx.x < top_k)
+    if (threadIdx.x < SLOTS && j0 + threadIdx.x < top_k && WB_CHECK(t < gridDim.x, kCheckOutputIndex, t))
       g_weight[t * top_k + j0 + threadIdx.x] = part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
     __syncthreads();
   }
