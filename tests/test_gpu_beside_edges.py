@@ -2,6 +2,7 @@
 
 import ctypes
 import sys
+import threading
 
 import pytest
 import torch
@@ -187,3 +188,62 @@ def test_few_tokens_of_wide_rows_are_combined_by_all_threads_at_once(tokens, col
     tol = 2 * top_k * 2.0 ** -24 * size
     tol = tol + 2.0 ** -8 * (want.abs() + tol) + 1e-38
     assert bool(((got.double() - want).abs() <= tol).all())
+
+
+def training_call(seed):
+    """A call of every operator with its gradients, on inputs made from the seed: () -> the outputs and gradients."""
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g).to(DEV)  # noqa: E731
+    y, x, a, b = (t.to(BF16).requires_grad_() for t in (r(90, 40), r(90, 64), r(3, 8, 64), r(3, 40, 8)))
+    ids = torch.randint(-1, 3, (90,), generator=g).to(torch.int32).to(DEV)
+    logits, weight = r(90, 12).requires_grad_(), r(30, 3).requires_grad_()
+    row_of, rows = torch.randperm(90, generator=g).to(torch.int32).to(DEV).reshape(30, 3), r(90, 40).to(BF16)
+
+    def call():
+        routing = wb.router(logits, 2)
+        outs = [wb.apply_adapters(y, x, a, b, ids), routing.weight, routing.balance_loss, wb.combine_rows(rows, row_of, weight)]
+        grads = torch.autograd.grad(outs, (y, x, a, b, logits, weight), [torch.ones_like(o) for o in outs])
+        return [o.detach() for o in outs] + list(grads)
+
+    return call
+
+
+def test_saved_tensors_pass_through_hooks():
+    """Python functions that pack and unpack what is saved run while a native call builds its node."""
+    call = training_call(3)
+    want = call()
+    with torch.autograd.graph.save_on_cpu():
+        assert all(torch.equal(p, q) for p, q in zip(call(), want))
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (seen.append(tuple(t.shape)), t.clone())[1], lambda t: t):
+        assert all(torch.equal(p, q) for p, q in zip(call(), want))
+    assert (90, 64) in seen and (90, 12) in seen and (90, 40) in seen
+    with torch.autograd.set_detect_anomaly(True):
+        assert all(torch.equal(p, q) for p, q in zip(call(), want))
+
+
+def test_threads_call_at_once():
+    """Calls with gradients from several threads, each on a stream and on inputs of its own."""
+    calls = [training_call(seed) for seed in range(4)]
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(25):
+                    got = calls[i]()
+                stream.synchronize()
+            if not all(torch.equal(p, q) for p, q in zip(got, want[i])):
+                bad.append(i)
+        except Exception as e:  # noqa: BLE001
+            bad.append((i, e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not bad and not any(t.is_alive() for t in threads)
