@@ -1632,7 +1632,7 @@ struct OuterParams {
 // Grid (row splits = one cluster, blocks of 128 columns of both sides, adapters). A CTA picks the rows of its adapter out of its range of ids,
 // in order, and adds up their outer products with MMAs whose k runs over the rows, from a ring of 64 rows a stage. The splits are
 // added up through distributed shared memory, in their order. An MMA drops the bits of its f32 sum that do not fit, always towards zero, so that the
-// products of 16 rows are summed by it and added to the others with rounding: over thousands of rows the sums would shrink by 3e-6 of themselves, several
+// products of 32 rows are summed by it and added to the others with rounding: over thousands of rows the sums would shrink by 3e-6 of themselves, several
 // times what rounding costs. The warps stand side by side over the ranks first and over the columns where there are fewer ranks, so that a hidden number
 // is split into its bf16 parts by as few of them as possible. Both sums of a backward pass are one launch: 4096 rows, 4096 + 4096 columns, rank 16
 // 25 us (67 MB, 2.7 TB/s); bound by the start-up (ids, list, first loads), the barriers of the ring and the MMAs: a part takes 2 us of it.
@@ -1771,32 +1771,33 @@ adapter_outer_kernel(const OuterParams p) {
         if (step + STAGES - 1 < steps) load();
         else cp_async_commit();
         const int half = lane >> 4, in = lane & 15;
+        // the lane's four rows of a rank (a column of the second operand) for either half of 16 rows: 2 t, 2 t + 1 and the same eight rows on
+        uint32_t hf[2][OCTETS][2][kParts];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int r = 32 * wk + 16 * k;
-          // the lane's four rows of a rank (a column of the second operand): 2 t, 2 t + 1 and the same eight rows on
-          uint32_t hf[OCTETS][2][kParts];
-          const unsigned char* h_rows = smem + (from - base) + Cfg::Z_BYTES + (r + 2 * t) * (COLS * 4);
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int o = 0; o < OCTETS; ++o) {
             const int rank = (wr * OCTETS + o) * 8 + g;
-            const unsigned char* at = h_rows + (((rank >> 2) ^ ((2 * t) & (Cfg::H_PIECES - 1))) << 4) + (rank & 3) * 4;  // (hidden_piece of each of them)
+            const unsigned char* at = smem + (from - base) + Cfg::Z_BYTES + (32 * wk + 16 * k + 2 * t) * (COLS * 4) +
+                                      (((rank >> 2) ^ ((2 * t) & (Cfg::H_PIECES - 1))) << 4) + (rank & 3) * 4;  // (hidden_piece of each of them)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              split_pair(*reinterpret_cast<const float*>(at + h * (COLS * 32)), *reinterpret_cast<const float*>(at + h * (COLS * 32) + COLS * 4), hf[o][h]);
+              split_pair(*reinterpret_cast<const float*>(at + h * (COLS * 32)), *reinterpret_cast<const float*>(at + h * (COLS * 32) + COLS * 4), hf[k][o][h]);
           }
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            uint32_t za[4];  // matrices (k 0-7, c 0-7), (k 0-7, c 8-15), (k 8-15, c 0-7), (k 8-15, c 8-15)
-            ldsm4_trans(from + piece<16>(r + (in & 7) + half * 8, 2 * (wc * MT + m) + (in >> 3)), za);
+        for (int m = 0; m < MT; ++m) {
+          uint32_t za[2][4];  // matrices (k 0-7, c 0-7), (k 0-7, c 8-15), (k 8-15, c 0-7), (k 8-15, c 8-15)
 #pragma unroll
-            for (int o = 0; o < OCTETS; ++o) {
-              float sum[4] = {};
+          for (int k = 0; k < 2; ++k) ldsm4_trans(from + piece<16>(32 * wk + 16 * k + (in & 7) + half * 8, 2 * (wc * MT + m) + (in >> 3)), za[k]);
 #pragma unroll
-              for (int q = 0; q < kParts; ++q) mma_bf16(sum, za[0], za[1], za[2], za[3], hf[o][0][q], hf[o][1][q]);
+          for (int o = 0; o < OCTETS; ++o) {
+            float sum[4] = {};
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[m][o][e] += sum[e];
-            }
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int q = 0; q < kParts; ++q) mma_bf16(sum, za[k][0], za[k][1], za[k][2], za[k][3], hf[k][o][0][q], hf[k][o][1][q]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[m][o][e] += sum[e];
           }
         }
         from = from == base + (STAGES - 1) * Cfg::STAGE_BYTES ? base : from + Cfg::STAGE_BYTES;
