@@ -578,13 +578,13 @@ struct ShrinkWide {
   // Two CTAs to an SM, which share its columns, and beside them none of the library's other kernels that take tensor memory: a CTA holds its columns
   // while it waits for its cluster.
   static constexpr int SMEM_BYTES = 97 * 1024;           // the sums reuse the stages
-  // Accumulators of an adapter, taken in turn by the stages: an MMA drops the bits of its f32 sum that do not fit, always towards zero, and 2048 k in one
+  // Two accumulators to an adapter, taken in turn by the stages: an MMA drops the bits of its f32 sum that do not fit, always towards zero, and 2048 k in one
   // accumulator shrink by 1.8e-6 of themselves where an f32 sum with rounding is 1e-6 off at random.
-  static constexpr int ACCS = N == 64 ? 2 : 4;
-  static constexpr int TMEM_COLS = 256;
+  static constexpr int ACCS = 2;
+  static constexpr int TMEM_COLS = N < 32 ? 128 : 4 * N;  // (32 columns are read at a time)
   static_assert(STAGES * STAGE_BYTES + 1024 <= SMEM_BYTES && 2 * TMEM_COLS <= 512, "stages; columns of two CTAs");
   static_assert(SMEM_BYTES + kSmemOfTmemKernel > kSmemOfSm && 3 * SMEM_BYTES > kSmemOfSm, "no other kernel with tensor memory beside one CTA, no third CTA");
-  static_assert((2 * ACCS - 1) * N + (N < 32 ? 32 : N) <= TMEM_COLS, "accumulators of two adapters, of which 32 columns are read at a time");
+  static_assert((2 * ACCS - 1) * N + (N < 32 ? 32 : N) <= TMEM_COLS, "accumulators of two adapters");
   static_assert(ROWS * (N + 1) * 4 <= STAGES * STAGE_BYTES && ROWS <= kAdapterThreads, "sums; a thread per row where rows are grouped");
 };
 template <int N, bool TRANS>
