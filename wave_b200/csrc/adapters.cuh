@@ -1515,15 +1515,19 @@ adapter_expand_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
       const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane, id = groups.id[row];
       if (ngroups > 0) {  // the chunk's hidden vectors, pieces of 8 ranks (every MMA on those of the chunk before is complete: its sums were waited for)
         const int r = (int(threadIdx.x) - 64) >> 1;
+        float v[4][8] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // all loads in flight together
+          const int c = 2 * i + (threadIdx.x & 1);
+          if (c * 8 < p.Rp && row0 + r < p.rows) read8<float>(p.hidden + (long long)(row0 + r) * p.Rp + c * 8, true, 8, v[i]);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int c = 2 * i + (threadIdx.x & 1);
           if (c * 8 >= p.Rp) break;
-          float v[8] = {};
-          if (row0 + r < p.rows) read8<float>(p.hidden + (long long)(row0 + r) * p.Rp + c * 8, true, 8, v);
           uint32_t part[4][kParts];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) split_pair(v[2 * j], v[2 * j + 1], part[j]);
+          for (int j = 0; j < 4; ++j) split_pair(v[i][2 * j], v[i][2 * j + 1], part[j]);
 #pragma unroll
           for (int q = 0; q < kParts; ++q)
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + q * (Cfg::A_BYTES / kParts) + r * 128 + ((c ^ (r & 7)) << 4)), "r"(part[0][q]), "r"(part[1][q]),
