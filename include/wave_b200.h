@@ -450,7 +450,8 @@ int wb200_multi_gpu_time_end(wb200_multi_gpu_t* h, float* max_ms);
 /* Low-rank adapters of many requests: out[t] = y[t] + scale[l] * B_l (A_l x[t]) with l = ids[t]; rows whose id is outside
  * [0, num_adapters) have no adapter and keep y. x [rows, K] bf16 (pitch ldx), a [num_adapters, rank, K] and b [num_adapters, N, rank]
  * bf16, contiguous; ids int32 or int64; scale f32 [num_adapters], or null for ones; y and out [rows, N] of `dtype`, out may be y (in
- * place), otherwise they do not overlap. K is a multiple of 8, rank at most 256, N any. hidden: wb200_adapters_hidden_bytes(rows, rank, dtype)
+ * place), otherwise they do not overlap. K is a multiple of 8, rank at most 256, at most 4000000 rows, ceil(N / 128) + ceil(K / 128) at most 65535,
+ * row pitches of y and out below 2^24 elements; beyond that WB200_ERR_UNSUPPORTED. hidden: wb200_adapters_hidden_bytes(rows, rank, dtype)
  * bytes, 16-byte aligned, left with scale[l] * A_l x[t] in f32, which the backward call reads. Two launches, no order of the
  * ids needed. */
 size_t wb200_adapters_hidden_bytes(int rows, int rank, int dtype);
@@ -459,7 +460,8 @@ int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, c
                            int dtype, void* hidden, size_t hidden_bytes, void* stream);
 /* Its gradients for g = the gradient of a bf16 out [rows, N]: dx [rows, K] (the adapters' part, or with accumulate_dx != 0 added to what dx
  * holds), da and db laid out as a and b (zeros for an adapter without rows), all bf16; each may be null. hidden: as the forward call left it
- * (read for db). Sums over rows are made in a fixed order, which does not depend on which gradients are asked for. At most 65535 adapters.
+ * (read for db). Sums over rows are made in a fixed order, which does not depend on which gradients are asked for. At most 65535 adapters, and a row
+ * pitch of dx below 2^24 elements; for da and db the time grows with the adapters of the pool, used or not.
  * workspace: wb200_adapters_backward_workspace_bytes(rows, N, rank) bytes, 16-byte aligned. */
 size_t wb200_adapters_backward_workspace_bytes(int rows, int N, int rank);
 int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, const void* x, long long ldx, const void* a, const void* b,

@@ -152,8 +152,9 @@ def apply_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.T
 
     y [rows, N] f32 or bf16, x [rows, K] bf16, a [adapters, rank, K] and b [adapters, N, rank] bf16 (adapters of a lower rank are padded
     with zeros), ids [rows] int32 or int64, scale [adapters] f32 or None for ones. A row whose id is outside [0, adapters) has no adapter:
-    its y comes back. The sum is made in f32 and rounded once to y's type. out: where to write (may be y), not together with gradients.
-    Differentiable in y, x, a and b for a bf16 y and pools of at most 65535 adapters; sums over rows are made in a fixed order.
+    its y comes back. The sum is made in f32 and rounded once to y's type. out: where to write (y itself, or memory that does not overlap it), not together
+    with gradients. Differentiable in y, x, a and b for a bf16 y and pools of at most 65535 adapters; sums over rows are made in a fixed order.
+    Limits: rank 256, K a multiple of 8, 4000000 rows, N + K of some 8.3 million, rows of y and out less than 2^24 elements apart.
     """
     native = _lib.native_calls()
     if native is not None and _lib.unwatched("wb200_adapters_forward", "wb200_adapters_backward"):

@@ -24,8 +24,8 @@ int div_up(long long a, long long b) { return int((a + b - 1) / b); }
 int rank_pad(int R) { return (R + 15) / 16 * 16; }
 int chunks_of(int rows) { return div_up(rows, wb::kChunkRows); }
 // The kernels for few rows (taken 32 at a time) are those for groups of a few rows: a group's rows share the loads of its adapter but not its arithmetic.
-// us, few / many, K = N = 4096: rank 16, 1 row 5.0 / 6.6, 8 rows of one adapter 8.0 / 6.6, 32 rows of one 20.8 / 7.4, of eight 8.1 / 8.8, of 64
-// 8.8 / 12.2; rank 64, 4 rows of one adapter 9.1 / 9.2, 64 rows of 16 14.0 / 14.9.
+// us, few / many, K = N = 4096: rank 16, 1 row 5.2 / 6.4, 8 rows of one adapter 7.6 / 6.4, 32 rows of one 20.3 / 7.1, of eight 8.0 / 8.8, of 64
+// 8.9 / 12.8; rank 64, 4 rows of one adapter 8.8 / 8.6, 64 rows of 16 13.6 / 16.4.
 bool few_rows(int rows, int L) { return rows <= 64 && rows < 8ll * L; }
 
 template <typename... P, typename... A>
@@ -132,8 +132,8 @@ int launch_shrink_wide(const AdapterCall& c, wb::ShrinkParams p, int chunks) {
   return WB200_OK;
 }
 // The tensor cores take 2048 rows or more, and any number of more than 32 ranks. us of both products, ring of copies / tensor cores, K = N = 4096, three sequences:
-// rank 16, 1024 rows 15.7 / 18.3, 2048 rows 25.8 / 22.0, 8192 rows 44.5 / 44.3; rank 64, 256 rows 18.3 / 16.6, 2048 rows 36.4 / 27.9; 4096 rows of mixed
-// adapters at rank 16 102 / 77. Rows of few ranks are short pieces for the copy engine (trans): 4096 rows of rank 16 with gradients 68 / 71 with both.
+// rank 16, 1024 rows 15.8 / 18.4, 2048 rows 26.0 / 22.8, 8192 rows 45.0 / 46.3; rank 64, 256 rows 18.0 / 17.0, 2048 rows 37.6 / 28.2; 4096 rows of 64 mixed
+// adapters at rank 16 430 / 423. Rows of few ranks are short pieces for the copy engine (trans): 4096 rows of rank 16 with gradients 74 / 79 with both.
 bool wide_shrink(const AdapterCall& c, const wb::ShrinkParams& p, bool trans) {
   return p.x_vec && aligned_to(p.w, 16) && p.K % 64 == 0 && (!trans || p.R % 8 == 0) && (long long)p.L * std::max(p.K, p.R) < 0x7fffffff &&
          (c.Rp > 32 || (c.rows >= 2048 && !trans));
@@ -223,7 +223,7 @@ int launch_expand_wide(const AdapterCall& c, const wb::ExpandParams& e) {
   return WB200_OK;
 }
 // The tensor cores take more than 32 ranks where y and out are larger than L2. us of both products with the shrinking one on the tensor cores, rank 64:
-// 4096 x 4096 36.5 / 42.4, 8192 x 4096 61.7 / 56.5, 16384 x 8192 193 / 158; rank 32, 16384 x 8192 156 / 153, 8192 x 4096 49.3 / 53.3.
+// 4096 x 4096 41.1 / 44.6, 8192 x 4096 70.3 / 60.9, 16384 x 8192 230 / 165; rank 32, 16384 x 8192 169 / 156, 8192 x 8192 91.6 / 89.3, 8192 x 4096 53.6 / 56.7.
 bool wide_expand(const AdapterCall& c, const wb::ExpandParams& p, bool trans, bool f32) {
   return !f32 && p.io_vec && aligned_to(p.w, 16) && p.C % 8 == 0 && p.Rp <= 64 && p.R % (trans ? 16 : 8) == 0 && (long long)p.L * std::max(p.C, p.R) < 0x7fffff00 && p.Rp > 32 && (long long)c.rows * p.C >= 1 << 25;
 }

@@ -4,15 +4,17 @@
 //   u[t]   = s_l B_l^T g[t]      dx[t] = A_l^T u[t]      dA_l = sum_t u[t] x[t]^T      dB_l = s_l sum_t g[t] (A_l x[t])^T
 //
 // Three kernels: `shrink` (rows times a wide matrix onto the ranks: A_l x, B_l^T g), `expand` (ranks onto wide rows: B_l h, A_l^T u) and
-// `outer` (sums over the rows of an adapter). Each product is far below the tensor cores' rate at the ranks adapters have (2 R flops per
-// two bytes of x), so they are bound by HBM for many rows and by latency for few, and what counts is that every row of x, y and g moves
-// once, in whole 32-byte sectors, with enough of them in flight. mma.sync does for these products: at rank 64, 8192 rows and 8192 columns its share
-// is 2 x 15 us (576 TFLOP/s, two bf16 parts in `expand`) of 63 us of memory traffic.
+// `outer` (sums over the rows of an adapter). At the ranks adapters have (2 R flops per two bytes of x) they are bound by HBM for many rows and by latency
+// for few, and what counts is that every row of x, y and g moves once, in whole 32-byte sectors, with enough of them in flight.
 //
-// shrink and expand come in two forms each. Up to 64 rows with few rows to an adapter (`few`): operands from global memory straight to registers, every warp
-// finds the rows of its adapter itself by a vote, no barrier before the first load. Otherwise (`tile`): rows are taken in chunks of 64 neighbours,
-// every CTA sorts the chunk's rows by adapter itself (64 compares a thread; a chunk of one sequence is noticed and not sorted), so that no
-// launch precedes it and ids need no order.
+// shrink and expand come in three forms each, chosen by rules on rows, ranks, types and alignment (few_rows, wide_shrink and wide_expand in adapt.cu):
+//   few    up to 64 rows with few rows to an adapter: operands from global memory straight to registers, every warp finds the rows of its adapter itself
+//          by a vote, no barrier before the first load; f32 FMAs in the second product.
+//   tile   mma.sync, at any alignment and rank: rows are taken in chunks of 64 neighbours, every CTA sorts the chunk's rows by adapter itself (64 compares a
+//          thread; a chunk of one sequence is noticed and not sorted), so that no launch precedes it and ids need no order.
+//   wide   tcgen05 with tiles by TMA, for aligned bf16 rows: shrink from 2048 rows or above 32 ranks, expand at 33 to 64 ranks where y and out are larger
+//          than L2. mma.sync is slower there: `expand` with its three bf16 parts 97 against 57 us at rank 64, 8192 rows and 8192 columns.
+// outer is mma.sync at every size.
 //
 // Layouts for mma.sync m16n8k16: an MMA adds over its 16 k in any order, so a lane may hold any 8 consecutive k of a row (one 16-byte load, two
 // MMAs) as long as the other operand is permuted alike, and the columns of an output tile may be dealt to the lanes so that each has 8
@@ -400,8 +402,8 @@ adapter_shrink_few_kernel(const ShrinkParams p) {
 // Many rows: a ring of stages of 64 k in shared memory, rows of x gathered by their place in the group. Warp (m, q) takes rows 32 m .. and the
 // q-th 16 of the 64 k: x passes through ldmatrix once, w twice, and the four sums over k meet at the end. Two stages between barriers, so that the warps
 // wait for one another half as often. Bound by HBM on x at rank 16 and by shared memory and issue slots at rank 64, where each 64 rows x 64 k take as
-// many ldmatrix of w as of x: 8192 x 8192 at rank 64 50 us (134 MB of x, 2.7 TB/s; MMA pipe 39 %), where the tensor cores take 35;
-// 4096 x 4096 at rank 16 11 us.
+// many ldmatrix of w as of x: 8192 x 8192 at rank 64 48 us (134 MB of x, 2.8 TB/s; MMA pipe 39 %), where the tensor cores take 30 to 33;
+// 4096 x 4096 at rank 16 12.7 us.
 template <int RT>
 struct ShrinkTile {
   static constexpr int X_BYTES = kChunkRows * 128, W_BYTES = RT * 1024, STAGE_BYTES = X_BYTES + W_BYTES;
@@ -569,7 +571,7 @@ adapter_shrink_tile_kernel(const ShrinkParams p) {
 // of N columns for each; a row takes the sums of its own. Rows come as one tile, w as one a adapter: A_l's rows K-major, B_l's (TRANS) as they
 // lie, with the ranks in an MN-major operand. Ranks behind the last are the next adapter's or zeros and are not kept. No load passes through
 // registers, w is read once for 128 rows, and a chunk in which one sequence ends and another begins takes a third longer than others.
-// 8192 x 8192 at rank 64 35 us for seven sequences, 31 for one (134 MB, 4.3 TB/s). Bound by HBM, which 128 bytes of a row at a time do not bring to its full
+// 8192 x 8192 at rank 64 33 us for six sequences, 30 for one (134 MB, 4.1 and 4.5 TB/s). Bound by HBM, which 128 bytes of a row at a time do not bring to its full
 // rate; 256 bytes fetched into L2 at a time gained 2 us. Rows gathered by the copy engine, four to a request, took 55.
 template <int N, bool TRANS>
 struct ShrinkWide {
@@ -912,7 +914,7 @@ adapter_expand_few_kernel(const ExpandParams p) {
 
 // The same for ranks of 8 PIECES whose rows of B start on 16 bytes: PIECES lanes share a column, each with 8 of its ranks, so that a warp's load is 512
 // consecutive bytes, STEPS of them in flight; the lanes' sums meet by shuffles, and the u-th lane of a column keeps every so-manieth column.
-// Both products of 32 rows and some 25 of 64 adapters, K = 4096, N = 14336, rank 16: 12.2 us (17 MB; with two columns a thread 13.7), of one row
+// Both products of 32 rows and some 25 of 64 adapters, K = 4096, N = 14336, rank 16: 11.8 us (17 MB; with two columns a thread 13.7), of one row
 // with N = 4096 5.0 us (6.0).
 __host__ __device__ constexpr int few_whole_steps(int pieces) { return pieces > 4 ? pieces : 4; }
 template <typename T, int PIECES>
@@ -998,9 +1000,9 @@ __host__ __device__ constexpr int expand_ring_bytes(int esz, bool exact) { retur
 // they are the accumulators' first values. Otherwise the accumulators go through shared memory, so that 32 lanes share a row's 32 columns, and y a
 // row of 32 columns at a time, a tile of 16 rows ahead.
 // QN: steps of 16 ranks of w in registers at a time. EXACT: the rank is known when compiled.
-// Bound by its start-up and HBM at rank 16 (4096 x 4096 14 us); at rank 64 by shared memory (59 %) and the MMA pipe (51 %) between them, at two CTAs of
-// 128 registers a thread: 8192 x 8192 63 us (268 MB of y and out, 4.3 TB/s). With the batch ahead in registers instead of the ring 76 us; w of the
-// next columns through the ring too: no faster.
+// Bound by its start-up and HBM at rank 16 (4096 x 4096 18 us); at rank 64 by the MMA pipe and shared memory between them, at two CTAs of 128 registers a
+// thread: 8192 x 8192 97 us (268 MB of y and out, 2.8 TB/s), where the tensor cores take 57 to 61. With the batch ahead in registers instead of the
+// ring a fifth slower; w of the next columns through the ring too: no faster.
 template <typename T, int QN, bool TRANS, bool FAST, bool EXACT>
 __global__ void __launch_bounds__(kAdapterThreads, 2)
 adapter_expand_tile_kernel(const ExpandParams p) {
@@ -1337,9 +1339,10 @@ adapter_expand_tile_kernel(const ExpandParams p) {
 // The same for many aligned bf16 rows and ranks up to 64, on the tensor cores: 128 rows of a chunk x 128 columns, the three parts of the hidden vectors against
 // the same tile of w (A operand: the chunk's hidden vectors, split into parts once, by the warps that later read the sums; B: B_l's rows K-major, or
 // (TRANS) A_l's as they lie, MN-major). Two adapters at a time have accumulators, a row takes the sums of its own; y comes by the copy engine, is added to in shared memory and leaves from there.
-// One CTA per SM works through its share of all (chunk, 128 columns) in order. 8192 x 8192 at rank 64 50 us for one sequence (268 MB, 5.4 TB/s), 57 for
-// seven; the mma.sync form 63 to 70. Bound by HBM, and below 8192 x 4096 by the start-up of one large CTA per SM.
-//   warp 0: y and w by TMA; warp 1: tcgen05.mma; warps 2 .. 9: sums, thread = row, 64 columns; warp 10: out by TMA
+// One CTA per SM works through its share of all (chunk, 128 columns) in order. 8192 x 8192 at rank 64 57 us for one sequence (268 MB, 4.7 TB/s), 61 for six, of
+// which 3 are the third part and 3 the loads of the hidden vectors at the head of a chunk; the mma.sync form 97. Bound by HBM, and below 8192 x 4096
+// by the start-up of one large CTA per SM.
+//   warp 0: y and w by TMA; warp 1: tcgen05.mma; warps 2 .. 9: hidden vectors, then sums, thread = row, 64 columns; warp 10: out by TMA
 template <bool TRANS>
 struct ExpandWide {
   static constexpr int ROWS = 128, COLS = 128, A_BYTES = kParts * ROWS * 128, B_BYTES = COLS * 128, Y_BYTES = ROWS * COLS * 2;
@@ -1639,7 +1642,8 @@ struct OuterParams {
 // products of 32 rows are summed by it and added to the others with rounding: over thousands of rows the sums would shrink by 3e-6 of themselves, several
 // times what rounding costs. The warps stand side by side over the ranks first and over the columns where there are fewer ranks, so that a hidden number
 // is split into its bf16 parts by as few of them as possible. Both sums of a backward pass are one launch: 4096 rows, 4096 + 4096 columns, rank 16
-// 25 us (67 MB, 2.7 TB/s); bound by the start-up (ids, list, first loads), the barriers of the ring and the MMAs: a part takes 2 us of it.
+// 23 us (67 MB, 2.9 TB/s); bound by the start-up (ids, list, first loads), the barriers of the ring and the MMAs: a part takes 2 us of it. The CTAs of an
+// adapter without rows look through all ids too: a call has (N + K) / 128 of them for every adapter of the pool.
 constexpr int kOuterCols = 128;
 constexpr int kOuterSegment = 4096;  // ids looked through at a time
 template <int RT>

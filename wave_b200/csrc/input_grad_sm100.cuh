@@ -23,8 +23,8 @@
 // CG = 2: 256 x 256 tiles, each CTA holds 128 rows of g and expands 128 columns of W; CG = 1: 128 x 128 tiles. Both accumulators of
 // neighbouring tiles are in tensor memory, so an epilogue runs under the next tile's products.
 //
-// 8192^3 in a graph of launches: 793 us, 1386 TFLOP/s, at the board's power limit (the library's bf16 product sustains 1368); 600 x 4000 x 2048 24 us, of
-// which 13 are its 32 steps.
+// 8192^3 in a graph of launches: 793 to 832 us by board, 1322 to 1386 TFLOP/s, at the power limit (cuBLAS' bf16 product sustains 1368); a call among others
+// on changing inputs 911 to 926 us, about 1200 TFLOP/s. 600 x 4000 x 2048 24 us, of which 13 are its 32 steps.
 #pragma once
 #include "ptx.cuh"
 

@@ -365,7 +365,7 @@ router_grad_kernel(const RouterGradParams p) {
 // out[t] = sum_j weight[t, j] y[row_of[t, j]] in slot order, for bf16 rows that start on 16 bytes: a CTA takes a token, all its pairs (SLOTS at a time)
 // and two pieces of their rows are in flight behind the row numbers. The same sums as moe_combine_kernel, which has a thread per piece of 8
 // columns, in the same order. 4096 x 4096 in pairs 15 us (101 MB), where a thread per piece took 23; narrow rows stay with the other, whose CTAs
-// share tokens.
+// share tokens, and so do few tokens of wide rows, which it has in flight all at once (wb200_moe_combine has the rule).
 template <int SLOTS>
 __global__ void __launch_bounds__(128)
 combine_token_kernel(const __nv_bfloat16* y, long long ldy, const int* row_of, const float* weight, int top_k, int cols, __nv_bfloat16* out, long long ldo) {

@@ -416,7 +416,8 @@ class MXFP4ExpertMLP:
     def forward_routed(self, x: torch.Tensor, routing: Routing) -> torch.Tensor:
         """The expert MLP on choices and weights made by `router` (or put together by the caller): bf16 [tokens, K_out], differentiable in
         routing.weight. The experts are frozen and have no input gradient: an x that requires one is refused. Pairs with an id of -1 (padding)
-        add nothing. Never waits for the GPU."""
+        add nothing. Never waits for the GPU. These are the separate steps, a launch and a pass over memory each, in blocks of 256 rows: `forward` with
+        the logits is the single call with fused kernels, and the faster one where nothing is trained."""
         if torch.is_grad_enabled() and x.requires_grad:
             raise ValueError("frozen experts give no gradient for x: pass x.detach()")
         ops.refuse_tangents(x)
