@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <iterator>
 #include <mutex>
 
@@ -20,6 +21,9 @@ using wbhost::fail;
 constexpr int kTargetCtas = 296;  // two per SM of a B200
 
 bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool words_aligned(std::initializer_list<const void*> pointers) {  // to four bytes (a null pointer is)
+  return std::all_of(pointers.begin(), pointers.end(), [](const void* p) { return aligned_to(p, 4); });
+}
 int div_up(long long a, long long b) { return int((a + b - 1) / b); }
 int rank_pad(int R) { return (R + 15) / 16 * 16; }
 int chunks_of(int rows) { return div_up(rows, wb::kChunkRows); }
@@ -457,7 +461,7 @@ int wb200_adapters_forward(int rows, int K, int N, int rank, int num_adapters, c
   if (rows > 1 && (ldx < K || ldy < N || ldo < N)) return fail(WB200_ERR_INVALID_ARG, "adapters: a row pitch is smaller than a row");
   if (ldy >= 1 << 24 || ldo >= 1 << 24) return fail(WB200_ERR_UNSUPPORTED, "adapters: a row pitch of 2^24 elements or more");
   if (!aligned_to(x, 2) || !aligned_to(a, 2) || !aligned_to(b, 2) || !aligned_to(y, dtype == WB200_F32 ? 4 : 2) || !aligned_to(out, dtype == WB200_F32 ? 4 : 2) ||
-      !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(hidden, 16))
+      !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(scale, 4) || !aligned_to(hidden, 16))
     return fail(WB200_ERR_ALIGNMENT, "adapters: a tensor is not aligned to its element size, or hidden not to 16 bytes");
   const size_t need = wb200_adapters_hidden_bytes(rows, rank, dtype);
   if (hidden_bytes < need) return fail(WB200_ERR_WORKSPACE, "adapters: hidden of %zu bytes needed (got %zu)", need, hidden_bytes);
@@ -487,7 +491,7 @@ int wb200_adapters_backward(int rows, int K, int N, int rank, int num_adapters, 
   if (rows > 1 && (ldg < N || (da && ldx < K) || (dx && ldd < K))) return fail(WB200_ERR_INVALID_ARG, "adapters backward: a row pitch is smaller than a row");
   if (ldd >= 1 << 24) return fail(WB200_ERR_UNSUPPORTED, "adapters backward: a row pitch of 2^24 elements or more");
   if (!aligned_to(x, 2) || !aligned_to(a, 2) || !aligned_to(b, 2) || !aligned_to(g, 2) || !aligned_to(dx, 2) || !aligned_to(da, 2) || !aligned_to(db, 2) ||
-      !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(hidden, 16) || !aligned_to(workspace, 16))
+      !aligned_to(ids, ids_are_int64 ? 8 : 4) || !aligned_to(scale, 4) || !aligned_to(hidden, 16) || !aligned_to(workspace, 16))
     return fail(WB200_ERR_ALIGNMENT, "adapters backward: a tensor is not aligned to its element size, or hidden or the workspace not to 16 bytes");
   const size_t ws_need = wb200_adapters_backward_workspace_bytes(rows, N, rank);
   if (workspace_bytes < ws_need) return fail(WB200_ERR_WORKSPACE, "adapters backward: workspace of %zu bytes needed (got %zu)", ws_need, workspace_bytes);
@@ -560,6 +564,8 @@ int wb200_router(int rows, int num_experts, int top_k, const void* logits, int d
   const size_t need = wb200_router_workspace_bytes(rows, num_experts);
   if (workspace_bytes < need) return fail(WB200_ERR_WORKSPACE, "router: workspace of %zu bytes needed (got %zu)", need, workspace_bytes);
   if (!aligned_to(workspace, 4)) return fail(WB200_ERR_ALIGNMENT, "router: the workspace must be 4-byte aligned");
+  if (!words_aligned({weight, ids, counts, unit, loss}) || !aligned_to(given_ids, given_are_int64 ? 8 : 4))
+    return fail(WB200_ERR_ALIGNMENT, "router: a tensor is not aligned to its element size");
   if (int rc = wbhost::device(nullptr, nullptr)) return rc;
   wb::RouterParams p;
   p.logits = logits; p.mask = static_cast<const uint8_t*>(mask); p.given = given_ids; p.ld = ld;
@@ -584,6 +590,8 @@ int wb200_router_grad(int rows, int num_experts, int top_k, const void* logits, 
   if (g_weight && (top_k > num_experts || top_k > wb::kRouterMaxTopK))
     return fail(WB200_ERR_INVALID_ARG, "router gradient: top_k = %d with %d experts (at most %d)", top_k, num_experts, wb::kRouterMaxTopK);
   if (rows > 1 && ldg < num_experts) return fail(WB200_ERR_INVALID_ARG, "router gradient: row pitch %lld is smaller than %d experts", ldg, num_experts);
+  if (!words_aligned({ids, g_weight, g_loss, counts, unit}) || !aligned_to(g_logits, dtype == WB200_F32 ? 4 : 2))
+    return fail(WB200_ERR_ALIGNMENT, "router gradient: a tensor is not aligned to its element size");
   if (int rc = wbhost::device(nullptr, nullptr)) return rc;
   wb::RouterGradParams p;
   p.logits = logits; p.mask = static_cast<const uint8_t*>(mask); p.ids = ids; p.g_weight = g_weight; p.g_loss = g_loss; p.counts = counts;
@@ -603,6 +611,8 @@ int wb200_moe_combine_grad(const void* g, long long ldg, const void* y, long lon
   if (!g || !y || !row_of || !g_weight) return fail(WB200_ERR_INVALID_ARG, "moe_combine_grad: null pointer");
   if (dtype != WB200_F32 && dtype != WB200_BF16) return fail(WB200_ERR_INVALID_ARG, "moe_combine_grad: unknown dtype %d", dtype);
   if (ldy < cols || (tokens > 1 && ldg < cols)) return fail(WB200_ERR_INVALID_ARG, "moe_combine_grad: a row pitch is smaller than cols = %d", cols);
+  if (!words_aligned({row_of, g_weight}) || !aligned_to(g, dtype == WB200_F32 ? 4 : 2) || !aligned_to(y, dtype == WB200_F32 ? 4 : 2))
+    return fail(WB200_ERR_ALIGNMENT, "moe_combine_grad: a tensor is not aligned to its element size");
   if (int rc = wbhost::device(nullptr, nullptr)) return rc;
   const size_t esz = dtype == WB200_F32 ? 4 : 2;
   const bool vec = cols % 8 == 0 && aligned_to(g, 16) && aligned_to(y, 16) && ldg * esz % 16 == 0 && ldy * esz % 16 == 0;
